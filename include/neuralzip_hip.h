@@ -10,8 +10,9 @@
  *   - int results: 0 on success, a negative nz_status on failure, with a
  *     thread-local message from nz_last_error();
  *   - host functions are re-entrant; nz_decode_launch, nz_matvec_launch,
- *     nz_matvec_reduce and nz_matvec_rows are asynchronous and
- *     ordered on the given HIP stream.
+ *     nz_matvec_reduce, nz_matvec_rows and the serving-step operators
+ *     (nz_pages_*, nz_rotary_store, nz_attention_*, nz_adjust_logits) are
+ *     asynchronous and ordered on the given HIP stream.
  */
 #ifndef NEURALZIP_HIP_H
 #define NEURALZIP_HIP_H
@@ -23,7 +24,7 @@
 extern "C" {
 #endif
 
-#define NZ_ABI_VERSION 12
+#define NZ_ABI_VERSION 13
 
 enum nz_status {
     NZ_OK = 0,
@@ -497,6 +498,225 @@ void nz_clusterer_destroy(nz_clusterer* clusterer);
 int nz_clusterer_assign(nz_clusterer* clusterer, const uint32_t* field_counts, uint64_t n, int32_t kind,
                         const int64_t* labels, const uint64_t* weights, int32_t* assignment);
 int nz_clusterer_count(const nz_clusterer* clusterer, uint32_t* n_clusters);
+
+/* ---- operators of a serving step ---------------------------------------- */
+
+/* One step of many requests whose lengths differ, around the decoded
+ * weights: pages for the step's tokens, rotation of queries and keys with
+ * the store into the pages, attention over them, and the logits'
+ * adjustments. No counterpart in the reference, whose forwards keep
+ * Transformers' own cache and attention (gpu/inference.py:476-509).
+ *
+ * The key-value cache of a layer is two arrays (keys, values) of n_pages
+ * pages of page_size tokens, kv_heads heads and head_dim elements each, in
+ * any order of the first three axes (element strides; the last axis is
+ * contiguous). page_size is a power of two from 16 to 1024. A token's slot
+ * is page * page_size + place in the page. Request r's tokens are at the
+ * pages tables[r * max_pages + i], i = position / page_size.
+ *
+ * The kernels check every page, slot, request, position and token number
+ * that they read from device memory against the sizes given here, so wrong
+ * ones give wrong results (as said at each entry) but no access out of
+ * bounds. */
+
+enum nz_value_type { NZ_BF16 = 0, NZ_FP16 = 1, NZ_FP32 = 2 };
+
+/* All pointers are device pointers; arrays are dense. */
+typedef struct nz_pages_extend_args {
+    const int32_t* lengths;      /* n_requests: tokens of each request       */
+    const int32_t* new_tokens;   /* n_requests: tokens it gets in this step  */
+    int32_t* tables;             /* n_requests x max_pages page numbers      */
+    const int32_t* free_pages;   /* n_pages: a stack of unused pages         */
+    const int32_t* n_free;       /* its height                               */
+    int64_t* slots;              /* max_tokens (out): slot of each new token */
+    int32_t* positions;          /* max_tokens (out): position in its request */
+    int32_t* requests;           /* max_tokens (out): its request            */
+    int32_t* contexts;           /* max_tokens (out): position + 1           */
+    int32_t* starts;             /* n_requests + 1 (out): first new token    */
+    int32_t* status;             /* n_requests (out): enum nz_pages_status   */
+    int32_t* lengths_after;      /* n_requests (out)                         */
+    int32_t* n_free_after;       /* 1 (out)                                  */
+    uint32_t* ticket;            /* 1, zero before the first call; zero after each */
+    uint32_t n_requests;
+    uint32_t max_pages;
+    uint32_t page_size;
+    uint32_t n_pages;
+    uint32_t max_tokens;
+    uint32_t advance;            /* 1: also write lengths and n_free         */
+} nz_pages_extend_args;
+
+enum nz_pages_status {
+    NZ_PAGES_OK = 0,
+    NZ_PAGES_TOO_LONG = 1,       /* negative, or past max_pages * page_size  */
+    NZ_PAGES_NO_ROOM = 2,        /* past the step's max_tokens               */
+    NZ_PAGES_NO_PAGE = 3,        /* the free stack is too low                */
+};
+
+/* Takes in a step's new tokens. In request order, a request is refused
+ * (gets no token, and status says why) if its length would be negative or
+ * pass max_pages * page_size; else if it asks for tokens and the sum of what
+ * it and those before it that fitted ask for passes max_tokens; else if it needs pages and
+ * the sum of the pages that it and those before it not refused so far need passes *n_free. The others' pages come
+ * off the stack in order (from the top, free_pages[n_free - 1], downwards)
+ * and into their table rows; the new tokens are listed request by request.
+ * Entries past the last token hold slot -1, position 0, request -1 and
+ * context 0. Table entries past a request's pages mean nothing. Without
+ * `advance` lengths and *n_free stay, and the same call again gives the
+ * same results (tables' new entries are written either way); calls on one
+ * set of tables run one after another (they share the ticket). */
+int nz_pages_extend(const nz_pages_extend_args* args, void* stream);
+
+typedef struct nz_pages_release_args {
+    const int32_t* lengths;      /* n_requests                               */
+    const uint8_t* done;         /* n_requests: nonzero: the request ends    */
+    const int32_t* tables;       /* n_requests x max_pages                   */
+    int32_t* free_pages;         /* n_pages                                  */
+    const int32_t* n_free;
+    int32_t* lengths_after;      /* n_requests (out)                         */
+    int32_t* n_free_after;       /* 1 (out)                                  */
+    uint32_t* ticket;            /* as for nz_pages_extend                   */
+    uint32_t n_requests;
+    uint32_t max_pages;
+    uint32_t page_size;
+    uint32_t n_pages;
+    uint32_t advance;
+    uint32_t reserved;           /* 0 */
+} nz_pages_release_args;
+
+/* Puts the pages of the requests that are done back onto the stack, in
+ * request order and table order, and sets their lengths to 0. Pages past the
+ * stack's n_pages entries are dropped. `advance` as above; without it
+ * free_pages above *n_free is still written. */
+int nz_pages_release(const nz_pages_release_args* args, void* stream);
+
+typedef struct nz_rotary_args {
+    const void* q;               /* tokens x heads x head_dim                */
+    const void* k;               /* tokens x kv_heads x head_dim             */
+    const void* v;
+    void* out;                   /* rotated q (may be q itself)              */
+    void* key_cache;             /* NULL (both caches): store nothing        */
+    void* value_cache;
+    const float* cos;            /* n_positions x rotary_dim / 2             */
+    const float* sin;
+    const void* q_weight;        /* head_dim norm weights, or NULL: no norm  */
+    const void* k_weight;
+    const int32_t* positions;    /* tokens                                   */
+    const int64_t* slots;        /* tokens                                   */
+    /* element strides; the last axis is contiguous */
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
+    int64_t key_page, key_head, key_slot, value_page, value_head, value_slot;
+    uint32_t tokens;
+    uint32_t heads;
+    uint32_t kv_heads;
+    uint32_t head_dim;
+    uint32_t rotary_dim;
+    uint32_t interleaved;        /* pairs (2i, 2i + 1) instead of (i, i + rotary_dim / 2) */
+    uint32_t page_size;
+    uint32_t n_pages;
+    uint32_t n_positions;
+    uint32_t type;               /* enum nz_value_type of q, k, v, out and the caches */
+    uint32_t weight_type;        /* of the norm weights: `type` or NZ_FP32   */
+    float eps;
+} nz_rotary_args;
+
+/* For every token: q and k, each head divided by its root mean square
+ * (sqrt(mean x^2 + eps)) and multiplied by the weights where they are given,
+ * then the first rotary_dim elements rotated by the token's position; q goes
+ * to `out`, k and v to the token's slot of the caches. Held in 32 bits,
+ * rounded once. Tokens whose slot is outside the caches (-1 for padding)
+ * store no key and value; a position outside n_positions gives NaN.
+ * head_dim and rotary_dim are multiples of 16, head_dim at most 256, strides
+ * and addresses multiples of 16 bytes. Slots must differ. */
+int nz_rotary_store(const nz_rotary_args* args, void* stream);
+
+/* One workgroup's share of nz_attention: the keys begin .. end - 1 of a row. */
+typedef struct nz_attention_item {
+    int32_t row;                 /* -1: none                                 */
+    int32_t request;
+    int32_t begin;
+    int32_t end;
+    int32_t index;               /* among the row's items                    */
+    int32_t count;               /* the row's items                          */
+    int32_t first;               /* the row's first item                     */
+    int32_t reserved;
+} nz_attention_item;
+
+/* Cuts rows' contexts into items of about equal length, on the device:
+ * n_rows contexts (negative ones count as 0), requests[row] their requests
+ * (NULL: row i is request i). `items` has room for n_rows + target entries;
+ * rows are cut so that there are at most that many, of at least 128 keys
+ * (but for the last of a row), and the rest are marked unused. The plan
+ * serves the attention of every layer of a step. */
+int nz_attention_plan(const int32_t* contexts, const int32_t* requests, uint32_t n_rows, uint32_t target,
+                      nz_attention_item* items, void* stream);
+
+typedef struct nz_attention_args {
+    const void* q;               /* n_rows x heads x head_dim                */
+    const void* key_cache;
+    const void* value_cache;
+    void* out;                   /* n_rows x heads x head_dim                */
+    const int32_t* tables;       /* n_requests x max_pages                   */
+    const nz_attention_item* items;
+    float* partials;             /* nz_attention_partials(...) values        */
+    int64_t q_row, q_head, out_row, out_head;
+    int64_t key_page, key_head, key_slot, value_page, value_head, value_slot;
+    uint32_t n_rows;
+    uint32_t n_items;            /* capacity of `items`                      */
+    uint32_t heads;
+    uint32_t kv_heads;
+    uint32_t head_dim;
+    uint32_t n_requests;
+    uint32_t max_pages;
+    uint32_t page_size;
+    uint32_t n_pages;
+    uint32_t type;
+    float scale;
+    uint32_t reserved;           /* 0 */
+} nz_attention_args;
+
+/* 32-bit words of scratch that nz_attention needs for a plan of n_items. */
+uint64_t nz_attention_partials(uint32_t n_items, uint32_t heads, uint32_t head_dim);
+
+/* out[row] = softmax(scale * q[row] . keys) values, over the row's context in
+ * its request's pages; head h reads key-value head h / (heads / kv_heads). A
+ * row without keys gives zeros. Keys whose page or request is not in range
+ * count as masked. head_dim is a multiple of 16, at most 256; strides and
+ * addresses are multiples of 16 bytes. Two calls that may overlap need their
+ * own partials. */
+int nz_attention(const nz_attention_args* args, void* stream);
+
+typedef struct nz_logits_args {
+    const void* logits;          /* rows x vocab                             */
+    void* out;                   /* rows x vocab (may be logits itself)      */
+    const void* history;         /* rows x history_capacity token ids, or NULL */
+    const int32_t* lengths;      /* rows: ids of each row                    */
+    const int32_t* prompt_lengths; /* rows: how many of them are the prompt, or NULL: none */
+    const float* repetition;     /* rows, or NULL: 1                         */
+    const float* frequency;      /* rows, or NULL: 0                         */
+    const float* presence;       /* rows, or NULL: 0                         */
+    const int32_t* bias_starts;  /* rows + 1, or NULL: no biases             */
+    const int32_t* bias_tokens;  /* n_bias                                   */
+    const float* bias_values;    /* n_bias                                   */
+    const uint32_t* masks;       /* n_masks x ceil(vocab / 32), or NULL      */
+    const int32_t* mask_rows;    /* rows: each row's mask, -1 none; NULL: row i has mask i */
+    int64_t logits_row, out_row, history_row;
+    uint32_t rows;
+    uint32_t vocab;
+    uint32_t history_capacity;
+    uint32_t n_bias;
+    uint32_t n_masks;
+    uint32_t type;               /* of logits and out                        */
+    uint32_t history_bytes;      /* 4 or 8 per id                            */
+    uint32_t reserved;           /* 0 */
+} nz_logits_args;
+
+/* Per row and token: x / repetition (x * repetition for x <= 0) if the token
+ * is in the row's history; minus frequency times its count and presence
+ * (once) if it is in the history after the prompt; plus the row's bias for
+ * it (its last entry counts); -infinity where the row's mask has no bit (bit
+ * v % 32 of word v / 32). In 32 bits, rounded once. Ids outside the
+ * vocabulary are ignored. */
+int nz_adjust_logits(const nz_logits_args* args, void* stream);
 
 #ifdef __cplusplus
 }

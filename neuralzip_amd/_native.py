@@ -5,6 +5,7 @@ The library must be built in-tree (``python -m neuralzip_amd.build`` or
 """
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 import numpy as np
@@ -82,9 +83,21 @@ class _Totals(ctypes.Structure):
     _fields_ = [("packed_bytes", ctypes.c_uint64), ("n_fragments", ctypes.c_uint64), ("n_tiles", ctypes.c_uint64)]
 
 
+# The serving-step operators' argument structs (nz_*_args of the header, in
+# field order): packed into a bytes object per call, which costs the host a
+# fraction of filling a ctypes structure and is safe between threads.
+PAGES_EXTEND = struct.Struct("=14Q6I")
+PAGES_RELEASE = struct.Struct("=8Q6I")
+ROTARY = struct.Struct("=12Q14q11If")
+ATTENTION = struct.Struct("=7Q10q10IfI")
+LOGITS = struct.Struct("=13Q3q8I")
+ATTENTION_ITEM = np.dtype([(name, "<i4") for name in ("row", "request", "begin", "end", "index", "count", "first",
+                                                      "reserved")])
+VALUE_BF16, VALUE_FP16, VALUE_FP32 = 0, 1, 2   # enum nz_value_type
+
 _lib = None
 # The C ABI version (NZ_ABI_VERSION of include/neuralzip_hip.h) these bindings follow.
-ABI_VERSION = 12
+ABI_VERSION = 13
 # Activation rows one fused matrix-vector product takes (NZ_MATVEC_MAX_BATCH).
 MATVEC_MAX_BATCH = 4
 # Weights one fused product takes (NZ_MATVEC_MAX_WEIGHTS).
@@ -143,6 +156,11 @@ def lib():
         L.nz_clusterer_destroy.restype = None
         L.nz_clusterer_assign.argtypes = [vp, vp, u64, ctypes.c_int32, vp, vp, vp]
         L.nz_clusterer_count.argtypes = [vp, ctypes.POINTER(u32)]
+        for name in ("nz_pages_extend", "nz_pages_release", "nz_rotary_store", "nz_attention", "nz_adjust_logits"):
+            getattr(L, name).argtypes = [ctypes.c_char_p, vp]
+        L.nz_attention_plan.argtypes = [vp, vp, u32, u32, vp, vp]
+        L.nz_attention_partials.argtypes = [u32, u32, u32]
+        L.nz_attention_partials.restype = u64
         _lib = L
     return _lib
 

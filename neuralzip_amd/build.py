@@ -13,8 +13,10 @@ LIBRARY = HERE / "libneuralzip_hip.so"
 ARCH = os.environ.get("NZ_OFFLOAD_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
-HOST_SOURCES = ("codebook.cpp", "layout.cpp", "codec.cpp", "capi.cpp", "capi_storage.cpp", "survey.cpp")
-DEVICE_SOURCES = ("hip/decode_gfx950.hip", "hip/matvec_gfx950.hip")
+HOST_SOURCES = ("codebook.cpp", "layout.cpp", "codec.cpp", "capi.cpp", "capi_storage.cpp", "capi_serving.cpp",
+                "survey.cpp")
+DEVICE_SOURCES = ("hip/decode_gfx950.hip", "hip/matvec_gfx950.hip", "hip/serving_gfx950.hip",
+                  "hip/attention_gfx950.hip")
 COMMON = ["-O3", "-std=c++17", "-fPIC", "-Wall", "-I", str(CSRC), "-I", str(ROOT / "include")]
 # host float arithmetic (the setup's clustering) is evaluated as written: no fused multiply-add
 HOST_FLAGS = ["-ffp-contract=off"]

@@ -1,0 +1,400 @@
+// serving_gfx950.hip -- gfx950 kernels of a serving step around the decoded
+// weights: pages of the step's tokens (nz_pages_*), head norms, rotation and
+// the store into the pages (nz_rotary_store), and the logits' adjustments
+// (nz_adjust_logits). The attention over the pages is in attention_gfx950.hip.
+#include <hip/hip_runtime.h>
+
+#include <stdint.h>
+#include <stdio.h>
+
+#include "neuralzip_hip.h"
+#include "serving_types.h"
+
+namespace {
+
+// ------------------------------------------------------------------ pages
+
+constexpr uint32_t kPagesThreads = 1024, kPagesWaves = kPagesThreads / 64;
+
+// Saturating, so that a step's sum of absurd requests stays past every limit.
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
+
+// Inclusive saturating prefix sum over the workgroup; *total receives the sum.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* waves, uint32_t* total) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d <<= 1) {
+        const uint32_t below = __shfl_up(v, d);
+        if (lane >= d) v = add_sat(v, below);
+    }
+    __syncthreads();   // the last call's reads of `waves`
+    if (lane == 63) waves[wave] = v;
+    __syncthreads();
+    uint32_t before = 0, sum = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kPagesWaves; ++w) {
+        if (w < wave) before = add_sat(before, waves[w]);
+        sum = add_sat(sum, waves[w]);
+    }
+    *total = sum;
+    return add_sat(before, v);
+}
+
+// The last i in [0, n) with first[i] <= x, where first[0] <= x.
+__device__ __forceinline__ uint32_t owner(const uint32_t* first, uint32_t n, uint32_t x) {
+    uint32_t lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (first[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// Ends a call that may advance the state: the last workgroup to arrive
+// copies the new lengths and stack height over the old ones, which the
+// others may have been reading until then.
+__device__ __forceinline__ void advance_state(uint32_t* ticket, const int32_t* lengths_after, const int32_t* n_free_after,
+                                              int32_t* lengths, int32_t* n_free, uint32_t n) {
+    __shared__ uint32_t last;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0)
+        last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) + 1 == gridDim.x;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    for (uint32_t r = threadIdx.x; r < n; r += kPagesThreads)
+        lengths[r] = __hip_atomic_load(lengths_after + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (threadIdx.x == 0) {
+        n_free[0] = __hip_atomic_load(n_free_after, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *ticket = 0;
+    }
+}
+
+// Three prefix sums over the requests (tokens asked, pages wanted, tokens
+// granted), then the new pages and tokens, each found by a search in the
+// sums. Every workgroup computes the sums for itself and writes its share of
+// the tokens and pages.
+__global__ __launch_bounds__(kPagesThreads) void nz_pages_extend_kernel(nz_pages_extend_args a) {
+    __shared__ uint32_t waves[kPagesWaves];
+    __shared__ uint32_t page_first[kPagesThreads], token_first[kPagesThreads];
+    __shared__ int32_t lens[kPagesThreads];
+    const uint32_t page = a.page_size, shift = 31 - __clz(page);
+    const uint32_t stride = gridDim.x * kPagesThreads, at = blockIdx.x * kPagesThreads + threadIdx.x;
+    const uint64_t limit = static_cast<uint64_t>(a.max_pages) << shift;
+    const uint32_t n_free = min(static_cast<uint32_t>(max(a.n_free[0], 0)), a.n_pages);
+    uint32_t asked_before = 0, pages_before = 0, tokens_before = 0, taken = 0;
+    for (uint32_t r0 = 0; r0 < a.n_requests; r0 += kPagesThreads) {
+        const uint32_t r = r0 + threadIdx.x;
+        const bool live = r < a.n_requests;
+        const int32_t length = live ? a.lengths[r] : 0, asks = live ? a.new_tokens[r] : 0;
+        const bool fits = asks >= 0 && length >= 0 &&
+                          static_cast<uint64_t>(length) + static_cast<uint64_t>(asks) <= limit;
+        uint32_t n = fits ? asks : 0, total;
+        const uint32_t asked = add_sat(asked_before, block_scan(n, waves, &total));
+        asked_before = add_sat(asked_before, total);
+        const bool room = n == 0 || asked <= a.max_tokens;
+        if (!room) n = 0;
+        const uint32_t old = fits ? (static_cast<uint32_t>(length) + page - 1) >> shift : 0;
+        uint32_t want = fits ? ((static_cast<uint32_t>(length) + n + page - 1) >> shift) - old : 0;
+        const uint32_t wanted = pages_before + block_scan(want, waves, &total);
+        pages_before += total;
+        const bool have = want == 0 || wanted <= n_free;
+        if (!have) n = 0, want = 0;
+        const uint32_t tokens = tokens_before + block_scan(n, waves, &total);
+        const uint32_t strip_tokens = total;
+        // pages granted: those wanted up to the last request that has them
+        const uint32_t granted = taken + block_scan(want, waves, &total);
+        const uint32_t strip_pages = total;
+        page_first[threadIdx.x] = granted - want;
+        token_first[threadIdx.x] = tokens - n;
+        lens[threadIdx.x] = length;
+        if (live && blockIdx.x == 0) {
+            a.status[r] = !fits ? NZ_PAGES_TOO_LONG : !room ? NZ_PAGES_NO_ROOM : !have ? NZ_PAGES_NO_PAGE : NZ_PAGES_OK;
+            a.starts[r] = tokens - n;
+            a.lengths_after[r] = length + static_cast<int32_t>(n);
+        }
+        __syncthreads();
+        for (uint32_t j = at; j < strip_pages; j += stride) {
+            const uint32_t i = owner(page_first, kPagesThreads, taken + j);
+            const uint32_t entry = ((static_cast<uint32_t>(lens[i]) + page - 1) >> shift) + taken + j - page_first[i];
+            a.tables[static_cast<uint64_t>(r0 + i) * a.max_pages + entry] = a.free_pages[n_free - 1 - (taken + j)];
+        }
+        for (uint32_t j = at; j < strip_tokens; j += stride) {
+            const uint32_t t = tokens_before + j, i = owner(token_first, kPagesThreads, t);
+            const uint32_t len = lens[i], position = len + t - token_first[i], entry = position >> shift;
+            const uint32_t old_pages = (len + page - 1) >> shift;
+            const int32_t p = entry < old_pages ? a.tables[static_cast<uint64_t>(r0 + i) * a.max_pages + entry]
+                                                : a.free_pages[n_free - 1 - (page_first[i] + entry - old_pages)];
+            a.slots[t] = static_cast<uint32_t>(p) < a.n_pages
+                             ? (static_cast<int64_t>(p) << shift) + (position & (page - 1)) : -1;
+            a.positions[t] = static_cast<int32_t>(position);
+            a.requests[t] = static_cast<int32_t>(r0 + i);
+            a.contexts[t] = static_cast<int32_t>(position) + 1;
+        }
+        tokens_before += strip_tokens;
+        taken += strip_pages;
+        __syncthreads();   // the searches above, before the next strip's sums
+    }
+    for (uint32_t t = tokens_before + at; t < a.max_tokens; t += stride) {
+        a.slots[t] = -1;
+        a.positions[t] = 0;
+        a.requests[t] = -1;
+        a.contexts[t] = 0;
+    }
+    if (at == 0) {
+        a.starts[a.n_requests] = static_cast<int32_t>(tokens_before);
+        a.n_free_after[0] = static_cast<int32_t>(n_free - taken);
+    }
+    if (a.advance)
+        advance_state(a.ticket, a.lengths_after, a.n_free_after, const_cast<int32_t*>(a.lengths),
+                      const_cast<int32_t*>(a.n_free), a.n_requests);
+}
+
+__global__ __launch_bounds__(kPagesThreads) void nz_pages_release_kernel(nz_pages_release_args a) {
+    __shared__ uint32_t waves[kPagesWaves];
+    __shared__ uint32_t first[kPagesThreads];
+    const uint32_t page = a.page_size, shift = 31 - __clz(page);
+    const uint32_t stride = gridDim.x * kPagesThreads, at = blockIdx.x * kPagesThreads + threadIdx.x;
+    uint32_t top = min(static_cast<uint32_t>(max(a.n_free[0], 0)), a.n_pages);
+    for (uint32_t r0 = 0; r0 < a.n_requests; r0 += kPagesThreads) {
+        const uint32_t r = r0 + threadIdx.x;
+        const bool live = r < a.n_requests, done = live && a.done[r] != 0;
+        const int32_t length = live ? max(a.lengths[r], 0) : 0;
+        const uint32_t back = done ? min((static_cast<uint32_t>(length) + page - 1) >> shift, a.max_pages) : 0;
+        uint32_t total;
+        const uint32_t scanned = block_scan(back, waves, &total);
+        first[threadIdx.x] = scanned - back;
+        if (live && blockIdx.x == 0) a.lengths_after[r] = done ? 0 : length;
+        __syncthreads();
+        const uint32_t kept = min(total, a.n_pages - top);
+        for (uint32_t j = at; j < kept; j += stride) {
+            const uint32_t i = owner(first, kPagesThreads, j);
+            a.free_pages[top + j] = a.tables[static_cast<uint64_t>(r0 + i) * a.max_pages + j - first[i]];
+        }
+        top += kept;
+        __syncthreads();
+    }
+    if (at == 0) a.n_free_after[0] = static_cast<int32_t>(top);
+    if (a.advance)
+        advance_state(a.ticket, a.lengths_after, a.n_free_after, const_cast<int32_t*>(a.lengths),
+                      const_cast<int32_t*>(a.n_free), a.n_requests);
+}
+
+// ------------------------------------------------- norm, rotation and store
+
+constexpr uint32_t kRotaryThreads = 256;
+
+// A head is held by a group of `LANES` lanes (a power of two), 16 elements
+// each: two runs of 8, at a and b. Rotated lanes hold pairs (i, i + half), or
+// 16 neighbours where pairs are neighbours; the lanes after them hold the
+// elements that are only normed.
+template <typename T, uint32_t LANES>
+__global__ __launch_bounds__(kRotaryThreads) void nz_rotary_kernel(nz_rotary_args a) {
+    const uint32_t lane = threadIdx.x % LANES;
+    const uint64_t vec = (static_cast<uint64_t>(blockIdx.x) * kRotaryThreads + threadIdx.x) / LANES;
+    const uint32_t per_token = a.heads + 2 * a.kv_heads;
+    if (vec >= static_cast<uint64_t>(a.tokens) * per_token) return;   // whole groups leave together
+    const uint32_t token = static_cast<uint32_t>(vec / per_token), head = static_cast<uint32_t>(vec % per_token);
+    const uint32_t half = a.rotary_dim / 2, turned = a.rotary_dim / 16;
+    const bool live = lane < a.head_dim / 16, turns = lane < turned;
+    const uint32_t at = turns && !a.interleaved ? 8 * lane : 16 * lane;
+    const uint32_t bt = turns && !a.interleaved ? at + half : at + 8;
+    const bool is_q = head < a.heads, is_v = head >= a.heads + a.kv_heads;
+    const uint32_t h = is_q ? head : is_v ? head - a.heads - a.kv_heads : head - a.heads;
+    T* dst = nullptr;
+    if (is_q) {
+        dst = static_cast<T*>(a.out) + token * a.out_token + h * a.out_head;
+    } else if (a.key_cache != nullptr) {
+        const int64_t slot = a.slots[token];
+        const uint32_t shift = 31 - __clz(a.page_size);
+        if (static_cast<uint64_t>(slot) < static_cast<uint64_t>(a.n_pages) << shift) {
+            const int64_t p = slot >> shift, place = slot & (a.page_size - 1);
+            dst = is_v ? static_cast<T*>(a.value_cache) + p * a.value_page + place * a.value_slot + h * a.value_head
+                       : static_cast<T*>(a.key_cache) + p * a.key_page + place * a.key_slot + h * a.key_head;
+        }
+    }
+    const T* src = is_q   ? static_cast<const T*>(a.q) + token * a.q_token + h * a.q_head
+                   : is_v ? static_cast<const T*>(a.v) + token * a.v_token + h * a.v_head
+                          : static_cast<const T*>(a.k) + token * a.k_token + h * a.k_head;
+    if (!live || dst == nullptr) src = nullptr;
+    float x[8] = {}, y[8] = {};
+    if (src != nullptr) {
+        load8(src + at, x);
+        load8(src + bt, y);
+    }
+    if (!is_v) {
+        const void* weight = is_q ? a.q_weight : a.k_weight;
+        if (weight != nullptr) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += x[i] * x[i];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += y[i] * y[i];
+#pragma unroll
+            for (uint32_t d = 1; d < LANES; d <<= 1) sum += __shfl_xor(sum, d);
+            const float scale = rsqrtf(sum / static_cast<float>(a.head_dim) + a.eps);
+            if (live) {
+                float wx[8], wy[8];
+                if (a.weight_type == NZ_FP32) {
+                    load8(static_cast<const float*>(weight) + at, wx);
+                    load8(static_cast<const float*>(weight) + bt, wy);
+                } else {
+                    load8(static_cast<const T*>(weight) + at, wx);
+                    load8(static_cast<const T*>(weight) + bt, wy);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = x[i] * scale * wx[i], y[i] = y[i] * scale * wy[i];
+            }
+        }
+        if (turns) {
+            const uint32_t position = static_cast<uint32_t>(a.positions[token]);
+            float c[8], s[8];
+            if (position < a.n_positions) {
+                load8(a.cos + static_cast<uint64_t>(position) * half + 8 * lane, c);
+                load8(a.sin + static_cast<uint64_t>(position) * half + 8 * lane, s);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) c[i] = s[i] = __builtin_nanf("");
+            }
+            if (a.interleaved) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    turn(x[2 * i], x[2 * i + 1], c[i], s[i]);
+                    turn(y[2 * i], y[2 * i + 1], c[4 + i], s[4 + i]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) turn(x[i], y[i], c[i], s[i]);
+            }
+        }
+    }
+    if (src != nullptr) {
+        store8(dst + at, x);
+        store8(dst + bt, y);
+    }
+}
+
+// -------------------------------------------------------------- the logits
+
+constexpr uint32_t kLogitsThreads = 256;
+// Tokens of the vocabulary that a workgroup counts in LDS.
+constexpr uint32_t kLogitsChunk = 4096;
+
+__device__ __forceinline__ int64_t history_id(const nz_logits_args& a, uint32_t row, uint32_t i) {
+    const uint64_t at = static_cast<uint64_t>(row) * static_cast<uint64_t>(a.history_row) + i;
+    return a.history_bytes == 8 ? static_cast<const int64_t*>(a.history)[at]
+                                : static_cast<int64_t>(static_cast<const int32_t*>(a.history)[at]);
+}
+
+// One workgroup: a row's tokens v0 .. v0 + kLogitsChunk - 1. It counts the
+// row's history that falls into them (answer tokens in the low 31 bits, any
+// token in the top bit), notes each token's last bias entry and then passes
+// over the logits once. Integer LDS atomics only: the order of arrival does
+// not show.
+template <typename T>
+__global__ __launch_bounds__(kLogitsThreads) void nz_logits_kernel(nz_logits_args a) {
+    __shared__ uint32_t counts[kLogitsChunk], entries[kLogitsChunk];
+    const uint32_t row = blockIdx.y, v0 = blockIdx.x * kLogitsChunk, n = min(kLogitsChunk, a.vocab - v0);
+    for (uint32_t i = threadIdx.x; i < kLogitsChunk; i += kLogitsThreads) counts[i] = 0, entries[i] = 0;
+    __syncthreads();
+    if (a.history != nullptr) {
+        const uint32_t length = min(static_cast<uint32_t>(max(a.lengths[row], 0)), a.history_capacity);
+        const uint32_t prompt = a.prompt_lengths ? static_cast<uint32_t>(max(a.prompt_lengths[row], 0)) : 0;
+        for (uint32_t i = threadIdx.x; i < length; i += kLogitsThreads) {
+            const uint64_t v = static_cast<uint64_t>(history_id(a, row, i)) - v0;
+            if (v < n) {
+                atomicOr(&counts[v], 0x80000000u);
+                if (i >= prompt) atomicAdd(&counts[v], 1u);
+            }
+        }
+    }
+    if (a.bias_starts != nullptr) {
+        const uint32_t e0 = min(static_cast<uint32_t>(max(a.bias_starts[row], 0)), a.n_bias);
+        const uint32_t e1 = min(static_cast<uint32_t>(max(a.bias_starts[row + 1], 0)), a.n_bias);
+        for (uint32_t e = e0 + threadIdx.x; e < e1; e += kLogitsThreads) {
+            const uint64_t v = static_cast<uint64_t>(static_cast<int64_t>(a.bias_tokens[e])) - v0;
+            if (v < n) atomicMax(&entries[v], e + 1);
+        }
+    }
+    __syncthreads();
+    const float repetition = a.repetition ? a.repetition[row] : 1.0f, frequency = a.frequency ? a.frequency[row] : 0.0f;
+    const float presence = a.presence ? a.presence[row] : 0.0f;
+    const uint32_t* mask = nullptr;
+    if (a.masks != nullptr) {
+        const int64_t m = a.mask_rows ? a.mask_rows[row] : static_cast<int64_t>(row);
+        if (static_cast<uint64_t>(m) < a.n_masks) mask = a.masks + static_cast<uint64_t>(m) * ((a.vocab + 31) / 32);
+    }
+    const T* src = static_cast<const T*>(a.logits) + row * a.logits_row + v0;
+    T* dst = static_cast<T*>(a.out) + row * a.out_row + v0;
+    for (uint32_t i = threadIdx.x; i < n; i += kLogitsThreads) {
+        float x = to_float(src[i]);
+        const uint32_t count = counts[i], entry = entries[i];
+        if (count) {
+            x = x > 0.0f ? x / repetition : x * repetition;
+            const uint32_t answers = count & 0x7FFFFFFFu;
+            if (answers) x = x - frequency * static_cast<float>(answers) - presence;
+        }
+        if (entry) x += a.bias_values[entry - 1];
+        if (mask && !((mask[(v0 + i) >> 5] >> ((v0 + i) & 31)) & 1u)) x = -__builtin_inff();
+        dst[i] = from_float<T>(x);
+    }
+}
+
+int launched(const char* what, char* message, size_t message_size) {
+    const hipError_t rc = hipGetLastError();
+    if (rc == hipSuccess) return 0;
+    snprintf(message, message_size, "%s launch failed: %s", what, hipGetErrorString(rc));
+    return -6;
+}
+
+template <typename T>
+void launch_rotary(const nz_rotary_args& a, hipStream_t stream) {
+    uint32_t lanes = 1;
+    while (lanes * 16 < a.head_dim) lanes *= 2;
+    const uint64_t threads = static_cast<uint64_t>(a.tokens) * (a.heads + 2 * a.kv_heads) * lanes;
+    const dim3 grid(static_cast<uint32_t>((threads + kRotaryThreads - 1) / kRotaryThreads));
+#define NZ_ROTARY(L) hipLaunchKernelGGL((nz_rotary_kernel<T, L>), grid, dim3(kRotaryThreads), 0, stream, a)
+    switch (lanes) {
+        case 1: NZ_ROTARY(1); break;
+        case 2: NZ_ROTARY(2); break;
+        case 4: NZ_ROTARY(4); break;
+        case 8: NZ_ROTARY(8); break;
+        default: NZ_ROTARY(16); break;
+    }
+#undef NZ_ROTARY
+}
+
+}  // namespace
+
+// The callers (capi_serving.cpp) have checked the arguments.
+
+extern "C" int nz_hip_pages_extend(const nz_pages_extend_args* args, void* stream, char* message, size_t message_size) {
+    hipLaunchKernelGGL(nz_pages_extend_kernel, dim3(1), dim3(kPagesThreads), 0, static_cast<hipStream_t>(stream), *args);
+    return launched("pages extend", message, message_size);
+}
+
+extern "C" int nz_hip_pages_release(const nz_pages_release_args* args, void* stream, char* message,
+                                    size_t message_size) {
+    hipLaunchKernelGGL(nz_pages_release_kernel, dim3(1), dim3(kPagesThreads), 0, static_cast<hipStream_t>(stream),
+                       *args);
+    return launched("pages release", message, message_size);
+}
+
+extern "C" int nz_hip_rotary_store(const nz_rotary_args* args, void* stream, char* message, size_t message_size) {
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (args->type == NZ_BF16) launch_rotary<bf16_t>(*args, st);
+    else if (args->type == NZ_FP16) launch_rotary<_Float16>(*args, st);
+    else launch_rotary<float>(*args, st);
+    return launched("rotary", message, message_size);
+}
+
+extern "C" int nz_hip_adjust_logits(const nz_logits_args* args, void* stream, char* message, size_t message_size) {
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const dim3 grid((args->vocab + kLogitsChunk - 1) / kLogitsChunk, args->rows), block(kLogitsThreads);
+    if (args->type == NZ_BF16) hipLaunchKernelGGL(nz_logits_kernel<bf16_t>, grid, block, 0, st, *args);
+    else if (args->type == NZ_FP16) hipLaunchKernelGGL(nz_logits_kernel<_Float16>, grid, block, 0, st, *args);
+    else hipLaunchKernelGGL(nz_logits_kernel<float>, grid, block, 0, st, *args);
+    return launched("logits", message, message_size);
+}

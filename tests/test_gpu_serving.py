@@ -1,0 +1,746 @@
+"""The serving-step operators on the GPU against plain implementations in 64
+bits (whole numbers: in loops over the requests).
+
+Tolerances. u is half the type's epsilon (the one rounding of a result);
+2^-24 that of 32 bits, in which everything else is held. Each test says which
+errors add up to its bound; none was set from what the kernels give."""
+import math
+import random
+
+import pytest
+import torch
+
+from neuralzip_amd.gpu import serving
+
+pytestmark = pytest.mark.gpu
+
+DEVICE = "cuda:0"
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+F32 = 2.0 ** -24
+
+
+def unit(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def ints(values, dtype=torch.int32):
+    return torch.tensor(values, dtype=dtype, device=DEVICE)
+
+
+def randn(*shape, seed=0, dtype=torch.float32, scale=1.0):
+    g = torch.Generator(device=DEVICE).manual_seed(seed)
+    return (scale * torch.randn(*shape, generator=g, device=DEVICE)).to(dtype)
+
+
+# ------------------------------------------------------------------- tables
+
+def pages_of(tokens, page):
+    return -(-tokens // page)
+
+
+def plain_extend(lengths, new, tables, free, n_free, page, max_tokens):
+    """The rules of nz_pages_extend, request by request."""
+    tables, left = [list(row) for row in tables], n_free
+    tokens, starts, status, after = [], [0], [], []
+    asked = wanted = 0
+    for r, (length, n) in enumerate(zip(lengths, new)):
+        state, pages = 0, 0
+        if n < 0 or length + n > len(tables[r]) * page:
+            state = serving.PAGES_TOO_LONG
+        elif n:
+            asked += n
+            if asked > max_tokens:
+                state = serving.PAGES_NO_ROOM
+        if not state:
+            pages = pages_of(length + n, page) - pages_of(length, page)
+            wanted += pages
+            if pages and wanted > n_free:
+                state = serving.PAGES_NO_PAGE
+        n = 0 if state else n
+        for j in range(0 if state else pages):
+            left -= 1
+            tables[r][pages_of(length, page) + j] = free[left]
+        tokens += [(tables[r][p // page] * page + p % page, p, r, p + 1) for p in range(length, length + n)]
+        starts.append(starts[-1] + n)
+        status.append(state)
+        after.append(length + n)
+    tokens += [(-1, 0, -1, 0)] * (max_tokens - len(tokens))
+    return [list(x) for x in zip(*tokens)] or [[], [], [], []], starts, status, after, left, tables
+
+
+def filled_tables(lengths, page, width, spare, seed=0):
+    """A PageTables with the given lengths and `spare` free pages, in random order."""
+    total = sum(pages_of(n, page) for n in lengths) + spare
+    order = list(range(total))
+    random.Random(seed).shuffle(order)
+    book = serving.PageTables(len(lengths), width, page, total, device=DEVICE)
+    tables = [[-1] * width for _ in lengths]
+    for r, n in enumerate(lengths):
+        for i in range(pages_of(n, page)):
+            tables[r][i] = order.pop()
+    book.lengths.copy_(ints(lengths))
+    book.tables.copy_(ints(tables))
+    free = order + [-1] * (total - len(order))
+    book.free.copy_(ints(free))
+    book.n_free.fill_(len(order))
+    return book, tables, free, len(order)
+
+
+def check_step(step, expected, book):
+    columns, starts, status, after, left, tables = expected
+    for name, want in zip(("slots", "positions", "requests", "contexts"), columns):
+        assert getattr(step, name).tolist() == want, name
+    assert step.starts.tolist() == starts and step.status.tolist() == status
+    assert step.lengths.tolist() == after and step.n_free.tolist() == [left]
+    assert book.tables.tolist() == tables
+
+
+EXTENDS = {
+    # lengths, new tokens, page, table width, spare pages, max tokens
+    "one token each": ([0, 1, 15, 16, 17, 31, 32], [1] * 7, 16, 4, 9, 7),
+    "no request has any": ([5, 0], [0, 0], 16, 2, 1, 3),
+    "nothing to fill": ([5, 0], [0, 0], 16, 2, 1, 0),
+    "page ends": ([15, 16, 0, 31], [1, 16, 33, 2], 16, 4, 9, 60),
+    "too long and negative": ([30, 5, 63, 64], [3, -1, 1, 1], 32, 2, 9, 20),
+    "no room": ([0, 0, 0, 0], [4, 9, 0, 1], 16, 4, 9, 10),
+    "no pages": ([16, 16, 5, 16, 16], [16, 17, 2, 1, 0], 16, 4, 2, 60),
+    "no pages at all": ([16, 3], [1, 1], 16, 4, 0, 4),
+    "padding": ([7], [2], 64, 1, 3, 9),
+    "large page": ([1000, 1023, 0], [25, 1, 1500], 1024, 3, 9, 2000),
+    "absurd": ([5, 6, 7], [2 ** 31 - 1, 2 ** 30, 3], 16, 1000, 9, 10),
+}
+
+
+@pytest.mark.parametrize("case", EXTENDS)
+@pytest.mark.parametrize("advance", [False, True])
+def test_extend_follows_the_rules(case, advance):
+    lengths, new, page, width, spare, most = EXTENDS[case]
+    book, tables, free, n_free = filled_tables(lengths, page, width, spare)
+    expected = plain_extend(lengths, new, tables, free, n_free, page, most)
+    step = book.extend(ints(new), most, advance=advance)
+    check_step(step, expected, book)
+    assert book.lengths.tolist() == (expected[3] if advance else lengths)
+    assert book.n_free.tolist() == [expected[4] if advance else n_free]
+    if not advance:   # the same again, into the same step
+        assert book.extend(ints(new), most, advance=False, out=step) is step
+        check_step(step, expected, book)
+
+
+@pytest.mark.parametrize("requests", [1, 63, 1023, 1024, 1025, 2600])
+def test_extend_and_release_over_many_requests(requests):
+    """More requests than a workgroup has threads, prompts among single
+    tokens, refusals of every kind, then half of them released."""
+    rng = random.Random(requests)
+    lengths = [rng.choice((0, 1, 16, rng.randrange(200))) for _ in range(requests)]
+    new = [rng.choice((0, 1, 1, rng.randrange(100), -1 if rng.random() < 0.1 else 2)) for _ in range(requests)]
+    total = sum(max(n, 0) for n in new)
+    book, tables, free, n_free = filled_tables(lengths, 16, 18, max(1, requests * 2), seed=requests)
+    for most in (total + 5, max(total // 2, 1)):
+        expected = plain_extend(lengths, new, tables, free, n_free, 16, most)
+        step = book.extend(ints(new), most, advance=False)
+        check_step(step, expected, book)
+        tables = expected[5]
+    book.extend(ints(new), most)
+    lengths, left = expected[3], expected[4]
+    done = [rng.random() < 0.5 for _ in range(requests)]
+    for r, gone in enumerate(done):
+        if gone:
+            for page in tables[r][:pages_of(lengths[r], 16)]:
+                free[left] = page
+                left += 1
+    after = book.release(torch.tensor(done, device=DEVICE))
+    want = [0 if gone else n for n, gone in zip(lengths, done)]
+    assert after.lengths.tolist() == book.lengths.tolist() == want
+    assert after.n_free.tolist() == book.n_free.tolist() == [left]
+    assert book.free.tolist() == free
+
+
+def test_a_pool_lives_through_many_steps():
+    """Requests come, grow and go; no page is ever held twice."""
+    rng = random.Random(3)
+    book = serving.PageTables(7, 6, 16, 20, device=DEVICE)
+    lengths = [0] * 7
+    for _ in range(40):
+        new = [rng.choice((0, 1, 1, 20)) for _ in range(7)]
+        step = book.extend(ints(new), 64)
+        lengths = [n + (g if s == 0 else 0) for n, g, s in zip(lengths, new, step.status.tolist())]
+        assert book.lengths.tolist() == lengths
+        done = [n > 60 or rng.random() < 0.1 for n in lengths]
+        book.release(torch.tensor(done, device=DEVICE))
+        lengths = [0 if d else n for n, d in zip(lengths, done)]
+        held = [p for row, n in zip(book.tables.tolist(), lengths) for p in row[:pages_of(n, 16)]]
+        stack = book.free.tolist()[:book.n_free.item()]
+        assert sorted(held + stack) == list(range(20))
+
+
+def test_release_without_advance_and_of_nothing():
+    book, tables, free, n_free = filled_tables([33, 0, 16], 16, 4, 2)
+    after = book.release(torch.tensor([True, True, False], device=DEVICE), advance=False)
+    assert after.lengths.tolist() == [0, 0, 16] and after.n_free.tolist() == [n_free + 3]
+    assert book.lengths.tolist() == [33, 0, 16] and book.n_free.tolist() == [n_free]
+    assert book.free.tolist()[n_free:n_free + 3] == tables[0][:3]
+    after = book.release(torch.zeros(3, dtype=torch.bool, device=DEVICE))
+    assert after.lengths.tolist() == [33, 0, 16] and after.n_free.tolist() == [n_free]
+
+
+# ------------------------------------------------------------------- rotary
+
+def angles(positions, half, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    a = torch.rand(positions, half, generator=g, dtype=torch.float64) * 2 * math.pi
+    return a.cos().float().to(DEVICE), a.sin().float().to(DEVICE)
+
+
+def plain_rotary(x, cos, sin, positions, weight, eps, interleaved):
+    x, rotary = x.double(), 2 * cos.shape[1]
+    if weight is not None:
+        x = x / (x.square().mean(-1, keepdim=True) + eps).sqrt() * weight.double()
+    c, s = cos.double()[positions.long()][:, None], sin.double()[positions.long()][:, None]
+    y = x.clone()
+    a, b = (slice(0, rotary, 2), slice(1, rotary, 2)) if interleaved else (slice(0, rotary // 2),
+                                                                           slice(rotary // 2, rotary))
+    y[..., a], y[..., b] = x[..., a] * c - x[..., b] * s, x[..., b] * c + x[..., a] * s
+    return y
+
+
+def rotary_bound(want, x, weight, dtype):
+    """One rounding of the result; before it, in 32 bits: the norm's sum (dim
+    terms, the mean, the root and two products: dim + 6 roundings, halved by
+    the root) and the rotation's three. Both products of a pair are at most
+    the pair's length."""
+    size = plain_rotary(x, *(torch.ones(1, x.shape[-1] // 2, device=DEVICE) * f for f in (1.0, 0.0)),
+                        torch.zeros(x.shape[0], device=DEVICE), weight, 1e-6, False).abs().amax(-1, keepdim=True)
+    return unit(dtype) * want.abs() + F32 * (x.shape[-1] + 12) * 2 * size + torch.finfo(dtype).tiny
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim, rotary", [(16, 16), (32, 16), (48, 48), (64, 64), (80, 32), (96, 96), (128, 128),
+                                         (128, 0), (192, 64), (256, 256)])
+@pytest.mark.parametrize("norm", ["none", "both", "keys", "fp32"])
+def test_rotary_against_64_bits(dtype, dim, rotary, norm):
+    for tokens, heads, kv_heads, interleaved in ((1, 3, 1, False), (37, 4, 2, True), (5, 7, 7, False)):
+        q, k, v = (randn(tokens, h, dim, seed=h, dtype=dtype) for h in (heads, kv_heads, kv_heads + 100))
+        v = v[:, :kv_heads].contiguous()
+        cos, sin = angles(50, rotary // 2)
+        g = torch.Generator().manual_seed(tokens)
+        positions = torch.randint(0, 50, (tokens,), generator=g).int().to(DEVICE)
+        weight = randn(dim, seed=9, dtype=torch.float32 if norm == "fp32" else dtype)
+        qw, kw = (weight if norm in ("both", "fp32") else None), (weight if norm != "none" else None)
+        rotary_op = serving.Rotary(cos, sin, interleaved=interleaved, q_weight=qw, k_weight=kw, eps=1e-6)
+        pages, page = 4, 16
+        caches = [torch.full((pages, kv_heads, page, dim), 7.0, dtype=dtype, device=DEVICE) for _ in range(2)]
+        slots = torch.randperm(pages * page, generator=g)[:tokens].to(DEVICE)
+        if tokens > 2:
+            slots[1], slots[2] = -1, pages * page      # padding, and a slot past the cache
+        out = rotary_op(q, k, v, positions, slots, *caches)
+        want = plain_rotary(q, cos, sin, positions, qw, 1e-6, interleaved)
+        assert ((out.double() - want).abs() <= rotary_bound(want, q, qw, dtype)).all()
+        want_k = plain_rotary(k, cos, sin, positions, kw, 1e-6, interleaved)
+        bound_k = rotary_bound(want_k, k, kw, dtype)
+        untouched = torch.ones(pages * page, dtype=torch.bool)
+        for t, slot in enumerate(slots.tolist()):
+            if 0 <= slot < pages * page:
+                untouched[slot] = False
+                got = caches[0][slot // page, :, slot % page].double()
+                assert ((got - want_k[t]).abs() <= bound_k[t]).all()
+                assert torch.equal(caches[1][slot // page, :, slot % page], v[t])
+        for cache in caches:
+            rest = cache.transpose(1, 2).reshape(pages * page, -1)[untouched.to(DEVICE)]
+            assert (rest == 7.0).all()
+
+
+def test_rotary_takes_views_in_place_and_caches_in_other_orders():
+    """q, k and v as views of one product, q rotated in place, caches whose
+    tokens come before their heads, as layers of one tensor: the same bits as
+    from copies."""
+    tokens, heads, kv_heads, dim, page = 19, 6, 2, 64, 32
+    rows = randn(tokens, (heads + 2 * kv_heads) * dim + 64, dtype=torch.bfloat16)
+    q, k, v, _ = (x.view(tokens, -1, dim) for x in
+                  rows.split((heads * dim, kv_heads * dim, kv_heads * dim, 64), dim=1))
+    cos, sin = angles(20, 32)
+    positions, slots = torch.arange(tokens, device=DEVICE).int(), torch.arange(tokens, device=DEVICE) + 5
+    op = serving.Rotary(cos, sin, q_weight=randn(dim, seed=1), k_weight=randn(dim, seed=2))
+    plain = [torch.zeros(2, kv_heads, page, dim, dtype=torch.bfloat16, device=DEVICE) for _ in range(2)]
+    want = op(q.contiguous(), k.contiguous(), v.contiguous(), positions, slots, *plain)
+    layers = torch.zeros(2, 3, 2, page, kv_heads, dim, dtype=torch.bfloat16, device=DEVICE)
+    caches = [layers[i, 1].transpose(1, 2) for i in range(2)]
+    rest = rows[:, heads * dim:].clone()
+    assert op(q, k, v, positions, slots, *caches, out=q) is q
+    assert torch.equal(q, want) and all(torch.equal(a, b) for a, b in zip(caches, plain))
+    assert torch.equal(rows[:, heads * dim:], rest) and not layers[:, 0].any() and not layers[:, 2].any()
+    # without a store
+    assert torch.equal(op(k, k, v, positions), op(k, k, v, positions, slots, *plain))
+
+
+def test_rotary_positions_outside_the_tables_give_nan():
+    cos, sin = angles(4, 16)
+    q = randn(3, 1, 64)
+    out = serving.Rotary(cos, sin)(q, q, q, ints([3, 4, -1]))
+    assert torch.isfinite(out[0]).all() and out[1:, :, :32].isnan().all() and torch.equal(out[1:, :, 32:], q[1:, :, 32:])
+
+
+def test_rotary_norm_of_extreme_heads():
+    """A head of zeros, one whose squares are small against eps, and one of
+    large fp16 values, whose squares pass fp16's range."""
+    cos, sin = angles(1, 32)
+    q = torch.cat([torch.zeros(1, 64), torch.full((1, 64), 2.0 ** -14), torch.full((1, 64), 60000.0)]).half().to(DEVICE)[None]
+    out = serving.Rotary(cos, sin, q_weight=torch.ones(64, device=DEVICE))(q, q, q, ints([0]))
+    want = plain_rotary(q, cos, sin, ints([0]), torch.ones(64, device=DEVICE), 1e-6, False)
+    assert ((out.double() - want).abs() <= 2 * unit(torch.float16) * want.abs().clamp(min=2.0 ** -14)).all()
+
+
+# ---------------------------------------------------------------- attention
+
+def plain_attention(q, keys, values, tables, contexts, requests, scale):
+    """(result, |q| . |k| at most, |v| at most) per row and head, in 64 bits."""
+    rows, heads, dim = q.shape
+    kv_heads, page = keys.shape[1], keys.shape[2]
+    group = heads // kv_heads
+    out = torch.zeros(rows, heads, dim, dtype=torch.float64, device=DEVICE)
+    size, most = (torch.zeros(rows, heads, 1, dtype=torch.float64, device=DEVICE) for _ in range(2))
+    for row, (n, request) in enumerate(zip(contexts, requests)):
+        at = [(int(tables[request][i // page]), i % page) for i in range(n)] if 0 <= request < len(tables) else []
+        at = [(p, i) for p, i in at if 0 <= p < keys.shape[0]]
+        if not at:
+            continue
+        page_index, place = (torch.tensor(x, device=DEVICE) for x in zip(*at))
+        k = keys[page_index, :, place].double().repeat_interleave(group, 1)
+        v = values[page_index, :, place].double().repeat_interleave(group, 1)
+        x = q[row].double()
+        out[row] = ((scale * (k * x).sum(-1)).softmax(0)[..., None] * v).sum(0)
+        size[row] = (k.abs() * x.abs()).sum(-1).amax(0)[:, None] * abs(scale)
+        most[row] = v.abs().amax((0, 2))[:, None]
+    return out, size, most
+
+
+def attention_bound(want, size, most, contexts, dim, dtype):
+    """One rounding of the result. Before it, relative to the largest value:
+    a score's dot product (dim + 2 roundings of what its terms add up to) and
+    its exponential (4) err a weight by so much, numerator and denominator
+    alike; the sums over the keys and the joined parts round once a key; and
+    16-bit types split a weight in two halves, which keep it to u^2 (and to
+    2^-39 of the largest weight in fp16, at most once a key)."""
+    n = max(contexts)
+    weight = F32 * (2 * (dim + 2) * size + 8 + 2 * n)
+    split = 2 * unit(dtype) ** 2 + n * 2.0 ** -39 if dtype != torch.float32 else 0.0
+    return unit(dtype) * want.abs() + most * (weight + split) + torch.finfo(dtype).tiny
+
+
+def attention_case(dtype, heads, kv_heads, dim, page, contexts, seed=0, sharp=1.0, extra=2):
+    """q, caches and tables; every place of the caches that no context
+    reaches holds NaN, as memory that was never written may."""
+    rng = random.Random(seed)
+    used = [pages_of(n, page) for n in contexts]
+    order = list(range(sum(used) + extra))
+    rng.shuffle(order)
+    width = max(1, max(used)) + 1
+    tables = [[-1] * width for _ in contexts]
+    shape = (len(order), kv_heads, page, dim)
+    keys, values = (torch.full(shape, float("nan"), dtype=dtype, device=DEVICE) for _ in range(2))
+    for r, n in enumerate(contexts):
+        for i in range(used[r]):
+            p = tables[r][i] = order.pop()
+            live = min(page, n - i * page)
+            keys[p, :, :live] = randn(kv_heads, live, dim, seed=seed + 17 * p, dtype=dtype)
+            values[p, :, :live] = randn(kv_heads, live, dim, seed=seed + 17 * p + 1, dtype=dtype)
+    q = randn(len(contexts), heads, dim, seed=seed + 1, dtype=dtype, scale=sharp)
+    return q, keys, values, ints(tables), tables
+
+
+def check_attention(dtype, heads, kv_heads, dim, page, contexts, seed=0, sharp=1.0, scale=None):
+    q, keys, values, tables, host = attention_case(dtype, heads, kv_heads, dim, page, contexts, seed, sharp)
+    plan = serving.AttentionPlan(ints(contexts), heads=heads, kv_heads=kv_heads)
+    out = serving.paged_attention(q, keys, values, tables, plan, scale=scale)
+    want, size, most = plain_attention(q, keys, values, host, contexts, range(len(contexts)),
+                                       dim ** -0.5 if scale is None else scale)
+    bound = attention_bound(want, size, most, contexts, dim, dtype)
+    assert ((out.double() - want).abs() <= bound).all(), ((out.double() - want).abs() / bound).max()
+    again = serving.paged_attention(q, keys, values, tables, plan, scale=scale, out=torch.empty_like(q))
+    assert torch.equal(out, again)
+    return out
+
+
+EDGES = [0, 1, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 0, 300]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [16, 32, 48, 64, 80, 96, 128, 160, 192, 256])
+def test_attention_of_every_head_size(dtype, dim):
+    check_attention(dtype, 4, 2, dim, 16, EDGES, seed=dim)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads, kv_heads", [(1, 1), (3, 3), (8, 1), (14, 2), (32, 8), (16, 1), (17, 1), (71, 1), (40, 2)])
+def test_attention_of_shared_heads(dtype, heads, kv_heads):
+    check_attention(dtype, heads, kv_heads, 64, 32, [40, 0, 7, 100], seed=heads)
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256, 512, 1024])
+def test_attention_of_every_page_size(page):
+    check_attention(torch.bfloat16, 4, 2, 128, page, [1, page - 1, page, page + 1, 2 * page + 5, 0], seed=page)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("contexts", [[5000], [0, 0, 0], [1], [4097, 3, 0, 2049, 1000] * 3, [1] * 130, [9000, 12000]])
+def test_attention_split_over_long_contexts(dtype, contexts):
+    check_attention(dtype, 8, 2, 64, 16, contexts, seed=len(contexts))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_of_sharp_and_flat_scores(dtype):
+    check_attention(dtype, 4, 1, 64, 16, [700, 33], sharp=30.0)
+    check_attention(dtype, 4, 1, 64, 16, [700, 33], sharp=1e-3)
+    check_attention(dtype, 4, 1, 64, 16, [700, 33], scale=0.0)
+    check_attention(dtype, 4, 1, 64, 16, [700, 33], scale=-0.3)
+
+
+def test_attention_of_rows_of_one_request():
+    """Several rows of one request with contexts of their own (a prompt's
+    last tokens), rows of unknown requests, rows without one."""
+    contexts, requests = [50, 51, 52, 9, 0, 20], [1, 1, 1, 0, -1, 7]
+    q, keys, values, tables, host = attention_case(torch.float16, 4, 2, 64, 16, [9, 52])
+    q = randn(6, 4, 64, seed=5, dtype=torch.float16)
+    plan = serving.AttentionPlan(ints(contexts), heads=4, kv_heads=2, requests=ints(requests))
+    out = serving.paged_attention(q, keys, values, tables, plan)
+    want, size, most = plain_attention(q, keys, values, host, contexts, requests, 0.125)
+    assert ((out.double() - want).abs() <= attention_bound(want, size, most, contexts, 64, torch.float16)).all()
+    assert not out[4:].any()
+
+
+def test_attention_masks_pages_outside_the_cache():
+    """Table entries of -1 or past the pages, and contexts past the table's
+    width: their keys count as masked."""
+    q, keys, values, tables, host = attention_case(torch.bfloat16, 4, 2, 64, 16, [100, 100, 64])
+    host[0][2], host[0][3], host[1][:7], host[2][3] = -1, 10 ** 6, [keys.shape[0]] * 7, -(2 ** 31)
+    contexts = [100, 100, 64]
+    plan = serving.AttentionPlan(ints(contexts), heads=4, kv_heads=2)
+    out = serving.paged_attention(q, keys, values, ints(host), plan)
+    want, size, most = plain_attention(q, keys, values, host, contexts, range(3), 0.125)
+    assert ((out.double() - want).abs() <= attention_bound(want, size, most, contexts, 64, torch.bfloat16)).all()
+    assert not out[1].any()
+    narrow = ints(host)[:, :2].contiguous()   # contexts of 100 over two pages: 32 keys
+    plan = serving.AttentionPlan(ints([10 ** 6, -5, 64]), heads=4, kv_heads=2)
+    out = serving.paged_attention(q, keys, values, narrow, plan)
+    want, size, most = plain_attention(q, keys, values, host, [32, 0, 32], range(3), 0.125)
+    assert ((out.double() - want).abs() <= attention_bound(want, size, most, [32], 64, torch.bfloat16)).all()
+
+
+def test_attention_passes_on_what_is_not_finite():
+    """NaN or infinity in a key or value that counts shows in the rows and
+    heads that see it, and nowhere else."""
+    contexts = [40, 40, 40]
+    q, keys, values, tables, host = attention_case(torch.bfloat16, 4, 2, 64, 16, contexts)
+    values[host[0][1], 0, 3, 5] = float("nan")
+    values[host[1][0], 1, 2, 7] = float("inf")
+    out = serving.paged_attention(q, keys, values, tables, serving.AttentionPlan(ints(contexts), heads=4, kv_heads=2))
+    assert out[0, :2, 5].isnan().all() and out[1, 2:, 7].isinf().all()
+    clean = out.clone()
+    clean[0, :2, 5] = clean[1, 2:, 7] = 0
+    assert torch.isfinite(clean).all()
+
+
+def test_attention_of_small_fp16_values():
+    """Values below fp16's normal range keep their bits."""
+    q, keys, values, tables, host = attention_case(torch.float16, 2, 2, 64, 16, [50])
+    values *= 2.0 ** -18
+    plan = serving.AttentionPlan(ints([50]), heads=2, kv_heads=2)
+    out = serving.paged_attention(q, keys, values, tables, plan)
+    want, size, most = plain_attention(q, keys, values, host, [50], [0], 0.125)
+    # results below the normal range round to multiples of 2^-24
+    bound = attention_bound(want, size, most, [50], 64, torch.float16).clamp(max=1.0) - torch.finfo(torch.float16).tiny
+    assert ((out.double() - want).abs() <= bound + 2.0 ** -25).all()
+
+
+def test_attention_over_strided_caches_and_outputs():
+    """Caches whose tokens come before their heads, as layers of one tensor;
+    q as a view of a wider product; an output with gaps: the same bits."""
+    contexts = [70, 3, 0, 33]
+    q, keys, values, tables, _ = attention_case(torch.bfloat16, 6, 2, 96, 16, contexts)
+    plan = serving.AttentionPlan(ints(contexts), heads=6, kv_heads=2)
+    want = serving.paged_attention(q, keys, values, tables, plan)
+    layers = torch.full((3, 2, keys.shape[0], 16, 2, 96), float("nan"), dtype=torch.bfloat16, device=DEVICE)
+    layers[1, 0], layers[1, 1] = keys.transpose(1, 2), values.transpose(1, 2)
+    wide = torch.zeros(4, 10, 96, dtype=torch.bfloat16, device=DEVICE)
+    wide[:, 2:8] = q
+    out = torch.zeros(4, 8, 96, dtype=torch.bfloat16, device=DEVICE)
+    serving.paged_attention(wide[:, 2:8], layers[1, 0].transpose(1, 2), layers[1, 1].transpose(1, 2), tables, plan,
+                            out=out[:, 1:7])
+    assert torch.equal(out[:, 1:7], want) and not out[:, 0].any() and not out[:, 7].any()
+
+
+def test_attention_and_store_beyond_32_bits_of_offset():
+    """Pages that lie more than 2^32 elements into the cache."""
+    pages, kv_heads, page, dim = 70_000, 4, 256, 64
+    assert (pages - 1) * kv_heads * page * dim > 1 << 32
+    keys, values = (torch.empty(pages, kv_heads, page, dim, dtype=torch.bfloat16, device=DEVICE) for _ in range(2))
+    used = [pages - 1, 0, pages - 2]
+    n = 2 * page + 17
+    k, v = (randn(n, kv_heads, dim, seed=s, dtype=torch.bfloat16) for s in (1, 2))
+    slots = torch.tensor([used[i // page] * page + i % page for i in range(n)], device=DEVICE)
+    cos, sin = torch.empty(1, 0, device=DEVICE), torch.empty(1, 0, device=DEVICE)
+    serving.Rotary(cos, sin)(k, k, v, torch.zeros(n, dtype=torch.int32, device=DEVICE), slots, keys, values)
+    small = [torch.zeros(3, kv_heads, page, dim, dtype=torch.bfloat16, device=DEVICE) for _ in range(2)]
+    for cache, x in zip(small, (k, v)):
+        for i in range(3):
+            cache[i, :, :min(page, n - i * page)] = x[i * page:(i + 1) * page].transpose(0, 1)
+    q = randn(1, 8, dim, seed=3, dtype=torch.bfloat16)
+    plan = serving.AttentionPlan(ints([n]), heads=8, kv_heads=kv_heads)
+    got = serving.paged_attention(q, keys, values, ints([used]), plan)
+    assert torch.equal(got, serving.paged_attention(q, *small, ints([[0, 1, 2]]), plan))
+    del keys, values
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("contexts", [[0], [1], [128], [129], [5000], [0, 10 ** 6, 3], [200] * 1500, [100_000, 7] * 40,
+                                      [2 ** 31 - 1, 2 ** 31 - 1, 5], [-4, 33]])
+def test_plans_cover_every_key_once(contexts):
+    plan = serving.AttentionPlan(ints(contexts), heads=32, kv_heads=8)
+    items = plan.items.tolist()
+    assert len(items) == plan.capacity
+    count = sum(1 for item in items if item[0] >= 0)
+    assert all(item[0] >= 0 for item in items[:count]) and all(item[0] == -1 for item in items[count:])
+    at = 0
+    for row, context in enumerate(contexts):
+        context = max(context, 0)
+        n, position = items[at][5], 0
+        for i in range(n):
+            r, request, begin, end, index, of, first, _ = items[at + i]
+            assert (r, request, begin, index, of, first) == (row, row, position, i, n, at)
+            assert begin % 32 == 0 and (begin < end or (context == 0 and n == 1)) and end <= context
+            assert end - begin >= min(context, 32)  or i == n - 1
+            position = end
+        assert position == context
+        at += n
+    assert at == count
+
+
+# ------------------------------------------------------------------- logits
+
+def plain_logits(logits, history, lengths, prompt, repetition, frequency, presence, bias, masks, mask_rows):
+    x = logits.double().cpu()
+    size = x.abs()
+    vocab = x.shape[1]
+    for r in range(x.shape[0]):
+        if history is not None:
+            ids = [int(t) for t in history[r][:max(lengths[r], 0)]]
+            first = max(prompt[r], 0) if prompt is not None else 0
+            inside = [t for t in ids if 0 <= t < vocab]
+            answer = [t for t in ids[first:] if 0 <= t < vocab]
+            for t in set(inside):
+                rep = repetition[r] if repetition is not None else 1.0
+                x[r, t] = x[r, t] / rep if x[r, t] > 0 else x[r, t] * rep
+                size[r, t] = x[r, t].abs()
+            for t in set(answer):
+                f = (frequency[r] if frequency is not None else 0.0) * answer.count(t)
+                p = presence[r] if presence is not None else 0.0
+                x[r, t] += -f - p
+                size[r, t] += abs(f) + abs(p)
+        if bias is not None:
+            starts, tokens, values = bias
+            for t, value in dict(zip(tokens[starts[r]:starts[r + 1]], values[starts[r]:starts[r + 1]])).items():
+                if 0 <= t < vocab:
+                    x[r, t] += value
+                    size[r, t] += abs(value)
+        if masks is not None:
+            m = mask_rows[r] if mask_rows is not None else r
+            if 0 <= m < len(masks):
+                for t in range(vocab):
+                    if not masks[m][t // 32] >> (t % 32) & 1:
+                        x[r, t], size[r, t] = -math.inf, 0.0
+    return x, size
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [1, 31, 32, 33, 1000, 4095, 4096, 4097, 9001])
+@pytest.mark.parametrize("parts", ["history", "bias", "masks", "all", "none"])
+def test_logits_against_64_bits(dtype, vocab, parts):
+    rng = random.Random(vocab)
+    rows, capacity = 4, 90
+    logits = randn(rows, vocab, seed=vocab, dtype=dtype, scale=3.0)
+    f32 = lambda values: torch.tensor(values, dtype=torch.float32).tolist()
+    history = lengths = prompt = repetition = frequency = presence = bias = masks = mask_rows = None
+    if parts in ("history", "all"):
+        top = min(vocab, 40)
+        history = [[rng.randrange(-1, top) if rng.random() < 0.9 else vocab - 1 + rng.randrange(3)
+                    for _ in range(capacity)] for _ in range(rows)]
+        lengths, prompt = [capacity, 0, 1, 57], [30, 5, 0, 100]
+        repetition, frequency, presence = f32([1.3, 2.0, 0.7, 1.0]), f32([0.1, 0.0, -0.2, 0.5]), f32([0.3, 1.0, 0.0, -0.4])
+    if parts in ("bias", "all"):
+        starts = [0, 0, 3, 10, 17]
+        bias = (starts, [rng.choice((0, vocab - 1, rng.randrange(vocab), vocab, -3)) for _ in range(17)],
+                f32([rng.uniform(-9, 9) for _ in range(17)]))
+    if parts in ("masks", "all"):
+        masks = [[rng.randrange(1 << 32) for _ in range((vocab + 31) // 32)] for _ in range(3)]
+        masks[1] = [0] * len(masks[1])                  # a grammar that allows nothing
+        mask_rows = [0, -1, 1, 2]
+    signed = lambda rows: [[w - (1 << 32) if w >> 31 else w for w in row] for row in rows]
+    kwargs = {}
+    if history is not None:
+        kwargs.update(history=ints(history, torch.int64 if vocab % 2 else torch.int32), lengths=ints(lengths),
+                      prompt_lengths=ints(prompt), repetition=torch.tensor(repetition, device=DEVICE),
+                      frequency=torch.tensor(frequency, device=DEVICE), presence=torch.tensor(presence, device=DEVICE))
+    if bias is not None:
+        kwargs["bias"] = (ints(bias[0]), ints(bias[1]), torch.tensor(bias[2], device=DEVICE))
+    if masks is not None:
+        kwargs.update(masks=ints(signed(masks)), mask_rows=ints(mask_rows))
+    got = serving.adjust_logits(logits, **kwargs)
+    want, size = plain_logits(logits, history, lengths, prompt, repetition, frequency, presence, bias, masks, mask_rows)
+    got = got.double().cpu()
+    gone = want.isinf()
+    assert torch.equal(got[gone], want[gone])
+    # one rounding of the result; before it at most six in 32 bits, of sums no larger than `size`
+    assert ((got - want).abs() <= unit(dtype) * want.abs() + 6 * F32 * size)[~gone].all()
+    if parts == "none":
+        assert torch.equal(got, logits.double().cpu())
+    wide = torch.full((rows, vocab + 7), 5.0, dtype=dtype, device=DEVICE)
+    wide[:, 3:3 + vocab] = logits
+    view = wide[:, 3:3 + vocab]
+    assert serving.adjust_logits(view, out=view, **kwargs) is view
+    assert torch.equal(view.double().cpu(), got) and (wide[:, :3] == 5).all() and (wide[:, 3 + vocab:] == 5).all()
+
+
+def test_logits_that_are_not_finite():
+    """Infinities and the type's lowest value stay what they are; NaN stays
+    where no mask covers it."""
+    low = torch.finfo(torch.bfloat16).min
+    logits = torch.tensor([[math.inf, -math.inf, math.nan, low, math.nan, 1.0]], dtype=torch.bfloat16, device=DEVICE)
+    got = serving.adjust_logits(logits, history=ints([[0, 1, 3]]), lengths=ints([3]), masks=ints([[0b101111]]),
+                                repetition=torch.tensor([1.5], device=DEVICE))[0].tolist()
+    assert got[0] == math.inf and got[1] == -math.inf and math.isnan(got[2]) and got[3] == -math.inf
+    assert got[4] == -math.inf and got[5] == 1.0
+
+
+def test_logits_of_long_histories():
+    """More tokens than threads, counts above 2^15, int64 ids past 32 bits."""
+    vocab, n = 5000, 70_001
+    ids = torch.full((2, n), 17, dtype=torch.int64, device=DEVICE)
+    ids[1, ::2] = (1 << 32) + 17
+    logits = torch.zeros(2, vocab, device=DEVICE)
+    got = serving.adjust_logits(logits, history=ids, lengths=ints([n, n]), prompt_lengths=ints([1, 0]),
+                                frequency=torch.tensor([1.0, 1.0], device=DEVICE))
+    assert got[:, 17].tolist() == [-(n - 1.0), -float(n // 2)]
+    got[:, 17] = 0
+    assert not got.any()
+
+
+# --------------------------------------------------- streams, graphs, a step
+
+def small_step(book, caches, op, new, most, seed):
+    """One step of three requests through all operators."""
+    step = book.extend(new, most)
+    tokens = randn(most, 8, 64, seed=seed, dtype=torch.bfloat16)
+    plan = serving.AttentionPlan(step.contexts, heads=4, kv_heads=2, requests=step.requests)
+    q = op(tokens[:, :4], tokens[:, 4:6], tokens[:, 6:], step.positions, step.slots, *caches)
+    return serving.paged_attention(q, *caches, book.tables, plan)
+
+
+def serving_state():
+    cos, sin = angles(64, 32)
+    book = serving.PageTables(3, 4, 16, 9, device=DEVICE)
+    caches = [torch.full((9, 2, 16, 64), float("nan"), dtype=torch.bfloat16, device=DEVICE) for _ in range(2)]
+    return book, caches, serving.Rotary(cos, sin)
+
+
+def test_operators_on_a_side_stream():
+    """`stream` runs everything there; results are those of the current one."""
+    book, caches, op = serving_state()
+    want = [small_step(book, caches, op, ints(new), 40, i) for i, new in enumerate(([17, 0, 5], [1, 1, 1]))]
+    book, caches, op = serving_state()
+    news = [ints(new) for new in ([17, 0, 5], [1, 1, 1])]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = []
+    for i, new in enumerate(news):
+        tokens = randn(40, 8, 64, seed=i, dtype=torch.bfloat16)
+        side.wait_stream(torch.cuda.current_stream())
+        step = book.extend(new, 40, stream=side)
+        plan = serving.AttentionPlan(step.contexts, heads=4, kv_heads=2, requests=step.requests, stream=side)
+        q = op(tokens[:, :4], tokens[:, 4:6], tokens[:, 6:], step.positions, step.slots, *caches, stream=side)
+        got.append(serving.paged_attention(q, *caches, book.tables, plan, stream=side))
+        side.synchronize()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_captured_step_is_replayed_while_requests_grow():
+    """extend, plan, rotation, attention and logits in one graph: every
+    replay gives the eager step's bits, with eager work between replays."""
+    most, vocab = 3, 500
+    def build():
+        book, caches, op = serving_state()
+        inputs = dict(new=ints([1, 1, 1]), rows=torch.zeros(most, 8, 64, dtype=torch.bfloat16, device=DEVICE),
+                      logits=torch.zeros(most, vocab, device=DEVICE), history=ints([[0] * 30] * most))
+        factor = torch.full((most,), 0.5, device=DEVICE)
+        step = serving.Step(3, most, DEVICE)
+        plan = serving.AttentionPlan(torch.zeros(most, dtype=torch.int32, device=DEVICE), heads=4, kv_heads=2)
+        def run():
+            book.extend(inputs["new"], most, out=step)
+            plan.update(step.contexts, requests=step.requests)
+            rows = inputs["rows"]
+            q = op(rows[:, :4], rows[:, 4:6], rows[:, 6:], step.positions, step.slots, *caches)
+            out = serving.paged_attention(q, *caches, book.tables, plan)
+            return out, serving.adjust_logits(inputs["logits"], history=inputs["history"], lengths=step.contexts,
+                                              frequency=factor), step.status, step.lengths
+        return inputs, run
+    eager_inputs, eager = build()
+    inputs, run = build()
+    def feed(target, i):
+        target["new"].copy_(ints([1, i % 2, 1]))
+        target["rows"].copy_(randn(most, 8, 64, seed=i, dtype=torch.bfloat16))
+        target["logits"].copy_(randn(most, vocab, seed=i))
+        target["history"].copy_(ints([[(i * j) % vocab for j in range(30)]] * most))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for i in range(2):
+            feed(inputs, i), feed(eager_inputs, i)
+            run()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outputs = run()
+    for i in range(2):
+        feed(eager_inputs, i)
+        eager()
+    for i in range(2, 30):
+        feed(inputs, i), feed(eager_inputs, i)
+        graph.replay()
+        want = eager()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outputs, want)), i
+    assert want[3].tolist() == [30, 15, 30]
+
+
+def test_refusals_that_need_the_device():
+    q, keys, values, tables, _ = attention_case(torch.float16, 4, 2, 64, 16, [20, 5])
+    plan = serving.AttentionPlan(ints([20, 5]), heads=4, kv_heads=2)
+    for bad in (q[:1], q[:, :2], q.double()):
+        with pytest.raises(ValueError, match="q must be"):
+            serving.paged_attention(bad, keys, values, tables, plan)
+    with pytest.raises(ValueError, match="Caches"):
+        serving.paged_attention(q, keys, values[:, :1], tables, plan)
+    with pytest.raises(ValueError, match="dtype and device"):
+        serving.paged_attention(q, keys.float(), values.float(), tables, plan)
+    with pytest.raises(ValueError, match="tables"):
+        serving.paged_attention(q, keys, values, tables.long(), plan)
+    with pytest.raises(ValueError, match="contiguous"):
+        serving.paged_attention(torch.zeros(2, 4, 128, dtype=q.dtype, device=DEVICE)[..., ::2], keys, values, tables, plan)
+    with pytest.raises(ValueError, match="no backward"):
+        serving.paged_attention(q.clone().requires_grad_(), keys, values, tables, plan)
+    with pytest.raises(ValueError, match="16 bytes"):
+        serving.paged_attention(torch.zeros(2, 4, 65, dtype=q.dtype, device=DEVICE)[..., :64], keys, values, tables, plan)
+    with pytest.raises(ValueError, match="power of two"):
+        serving.paged_attention(q, *(torch.zeros(3, 2, 24, 64, dtype=q.dtype, device=DEVICE) for _ in range(2)), tables,
+                                plan)
+    with pytest.raises(ValueError, match="contexts"):
+        plan.update(ints([1, 2, 3]))
+    logits = torch.zeros(2, 40, device=DEVICE)
+    for kwargs, message in ((dict(history=ints([[1], [2]])), "lengths"),
+                            (dict(repetition=torch.ones(2, device=DEVICE)), "history"),
+                            (dict(masks=ints([[0, 0]])), "one mask per row"),
+                            (dict(masks=ints([[0], [0]])), "masks must"),
+                            (dict(mask_rows=ints([0, 0])), "need masks"),
+                            (dict(bias=(ints([0, 1]), ints([3]), torch.ones(1, device=DEVICE))), "bias starts"),
+                            (dict(history=ints([[1.0], [2.0]], torch.float32), lengths=ints([1, 1])), "history must")):
+        with pytest.raises(ValueError, match=message):
+            serving.adjust_logits(logits, **kwargs)
