@@ -657,7 +657,7 @@ typedef struct nz_attention_args {
     void* out;                   /* n_rows x heads x head_dim                */
     const int32_t* tables;       /* n_requests x max_pages                   */
     const nz_attention_item* items;
-    float* partials;             /* nz_attention_partials(...) values        */
+    float* partials;             /* nz_attention_partials(...) words         */
     int64_t q_row, q_head, out_row, out_head;
     int64_t key_page, key_head, key_slot, value_page, value_head, value_slot;
     uint32_t n_rows;
@@ -674,7 +674,9 @@ typedef struct nz_attention_args {
     uint32_t reserved;           /* 0 */
 } nz_attention_args;
 
-/* 32-bit words of scratch that nz_attention needs for a plan of n_items. */
+/* 32-bit words of scratch that nz_attention needs for a plan of n_items:
+ * zero before the first call (a fill kernel's work; each call leaves the
+ * words that need it zero), 16-byte aligned. */
 uint64_t nz_attention_partials(uint32_t n_items, uint32_t heads, uint32_t head_dim);
 
 /* out[row] = softmax(scale * q[row] . keys) values, over the row's context in

@@ -137,7 +137,9 @@ int nz_attention_plan(const int32_t* contexts, const int32_t* requests, uint32_t
 }
 
 uint64_t nz_attention_partials(uint32_t n_items, uint32_t heads, uint32_t head_dim) {
-    return static_cast<uint64_t>(n_items) * heads * (head_dim + 2ull);
+    // a counter, the sums, their maximum and weight per item and head (hip/attention_gfx950.hip)
+    const uint64_t slots = static_cast<uint64_t>(n_items) * heads;
+    return (slots + 3) / 4 * 4 + slots * (head_dim + 2ull);
 }
 
 int nz_attention(const nz_attention_args* args, void* stream) {
@@ -156,6 +158,7 @@ int nz_attention(const nz_attention_args* args, void* stream) {
         check_alignment(size, a.out, a.out_row, a.out_head);
         check_alignment(size, a.key_cache, a.key_page, a.key_head, a.key_slot);
         check_alignment(size, a.value_cache, a.value_page, a.value_head, a.value_slot);
+        check_alignment(4, a.partials, 0);
         if (a.n_items < a.n_rows) refuse("The plan has fewer items than rows.");
         if (static_cast<uint64_t>(a.n_items) * a.heads > kMaxGrid) refuse("Too many items and heads in one call.");
         return false;

@@ -154,13 +154,52 @@ __device__ __forceinline__ float column_sum(float v) {
     return v + __shfl_xor(v, 32);
 }
 
+// What a maximum's scores are measured from: 0 where every key is masked.
+__device__ __forceinline__ float finite_base(float top) { return top == -__builtin_inff() ? 0.0f : top; }
+
+// Four elements of a row; zeros where it has no keys.
+template <typename T>
+__device__ __forceinline__ void store_row(T* dst, f32x4 sum, float weight) {
+    vec<T, 4> x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = from_float<T>(weight == 0.0f ? 0.0f : sum[i] / weight);
+    *reinterpret_cast<vec<T, 4>*>(dst) = x;
+}
+
+// Sums that another workgroup, maybe of another XCD, will read: stores and
+// loads of device scope go past the caches that only one XCD sees. A release
+// fence would write back all of the XCD's L2 instead.
+__device__ __forceinline__ void put_pair(float* dst, float x, float y) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(dst),
+                       static_cast<uint64_t>(__float_as_uint(y)) << 32 | __float_as_uint(x), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__device__ __forceinline__ float2 get_pair(const float* src) {
+    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(src), __ATOMIC_RELAXED,
+                                         __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32)));
+}
+
+// The scratch: a counter per item and head, which is 0 between calls, then
+// the items' sums, then their maxima and weights (32-bit words).
+__device__ __forceinline__ uint64_t partials_sums(uint64_t n_items, uint64_t heads) {
+    return (n_items * heads + 3) / 4 * 4;
+}
+__device__ __forceinline__ uint64_t sums_words(uint64_t n_items, uint64_t heads, uint64_t head_dim) {
+    return n_items * heads * head_dim;
+}
+
 template <typename T, uint32_t DP>
 struct Shape {
     static constexpr uint32_t kRun = Piece<T>::kRun;
     static constexpr uint32_t kKeySteps = DP / (4 * kRun);              // pieces of a key row per lane
     static constexpr uint32_t kValueRun = DP / 16 < kRun ? DP / 16 : kRun;   // neighbours a lane loads of a value row
     static constexpr uint32_t kValueSteps = DP / (16 * kValueRun);
-    static constexpr uint32_t kGroups = kTile / (4 * kRun);             // value products per tile
+    // keys a wavefront takes at a time, in runs of 16: fewer where a tile's
+    // keys and values would not fit the registers
+    static constexpr uint32_t kHalves = sizeof(T) == 4 && DP > 64 ? 1 : 2, kKeys = 16 * kHalves;
+    static constexpr uint32_t kGroups = kKeys / (4 * kRun);             // value products per tile
 };
 
 // One item: 16 query heads' softmax over the keys begin .. end - 1 of one
@@ -172,13 +211,14 @@ struct Shape {
 // scores belong to, and transposed in registers; no LDS until the
 // wavefronts' sums are joined.
 template <typename T, uint32_t DP, bool FULL>
-__global__ __launch_bounds__(kThreads) void nz_attention_kernel(nz_attention_args a) {
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 128 && sizeof(T) == 2 ? 3 : 1))) void nz_attention_kernel(nz_attention_args a) {
     using S = Shape<T, DP>;
     using P = Piece<T>;
     using piece = typename P::type;
     using value_run = vec<T, S::kValueRun>;
     __shared__ float lds_m[kWaves][kHeads], lds_l[kWaves][kHeads];
     __shared__ __align__(16) float lds_o[kWaves][kHeads][DP + 4];
+    __shared__ uint32_t last;
 
     const uint32_t group = a.heads / a.kv_heads, blocks = (group + kHeads - 1) / kHeads;
     const uint32_t per_item = a.kv_heads * blocks;
@@ -205,44 +245,91 @@ __global__ __launch_bounds__(kThreads) void nz_attention_kernel(nz_attention_arg
         }
     }
     const float scale = a.scale * kLog2e;
+    const T* const key_base = static_cast<const T*>(a.key_cache) + kv_head * a.key_head;
+    const T* const value_base = static_cast<const T*>(a.value_cache) + kv_head * a.value_head;
     f32x4 o[S::kValueSteps][S::kValueRun] = {};
     float m = -__builtin_inff(), l = 0.0f;
 
-    for (uint32_t t0 = static_cast<uint32_t>(item.begin) + wave * kTile; t0 < end; t0 += kWaves * kTile) {
-        float score[2][4];
-        const T* values[2];
-        uint32_t limit[2];
+    // The pages of a tile's runs of 16 keys (a run lies in one page).
+    // Entries are read a tile ahead of the keys, and keys a tile ahead of
+    // their products. Past the end, and where there is no page, page 0
+    // is read and everything masked.
+    auto entries = [&](uint32_t t0, int32_t (&page)[S::kHalves]) {
 #pragma unroll
-        for (uint32_t h = 0; h < 2; ++h) {
-            // 16 keys of one page; where there is none, page 0 is read and everything masked
+        for (uint32_t h = 0; h < S::kHalves; ++h) {
             const uint32_t t = t0 + 16 * h, entry = t >> shift;
-            const int32_t p = known && t < end && entry < a.max_pages ? table[entry] : -1;
-            const bool valid = static_cast<uint32_t>(p) < a.n_pages;
-            const int64_t page = valid ? p : 0;
-            limit[h] = valid ? end : 0;
-            const T* keys = static_cast<const T*>(a.key_cache) + page * a.key_page + kv_head * a.key_head
-                            + static_cast<int64_t>(t & place_mask) * a.key_slot;
-            values[h] = static_cast<const T*>(a.value_cache) + page * a.value_page + kv_head * a.value_head
-                        + static_cast<int64_t>(t & place_mask) * a.value_slot;
-            f32x4 acc = {};
+            page[h] = table[min(entry, a.max_pages - 1)];
+            if (!known || t >= end || entry >= a.max_pages) page[h] = -1;
+        }
+    };
+    piece keys[S::kHalves][S::kKeySteps];
+    auto load_keys = [&](uint32_t t0, const int32_t (&page)[S::kHalves]) {
+#pragma unroll
+        for (uint32_t h = 0; h < S::kHalves; ++h) {
+            const int64_t p = static_cast<uint32_t>(page[h]) < a.n_pages ? page[h] : 0;
+            const T* src = key_base + p * a.key_page + static_cast<int64_t>((t0 + 16 * h) & place_mask) * a.key_slot;
 #pragma unroll
             for (uint32_t s = 0; s < S::kKeySteps; ++s) {
                 const uint32_t d = s * 4 * S::kRun + quad * S::kRun;
-                piece k = {};
-                if (FULL || d < a.head_dim) k = *reinterpret_cast<const piece*>(keys + col * a.key_slot + d);
-                acc = P::mma(k, q[s], acc);
+                keys[h][s] = piece{};
+                if (FULL || d < a.head_dim) keys[h][s] = *reinterpret_cast<const piece*>(src + col * a.key_slot + d);
             }
+        }
+    };
+    constexpr uint32_t kStep = kWaves * S::kKeys;
+    uint32_t t0 = static_cast<uint32_t>(item.begin) + wave * S::kKeys;
+    int32_t page[S::kHalves], next[S::kHalves];
+    if (t0 < end) {
+        entries(t0, page);
+        load_keys(t0, page);
+        entries(t0 + kStep, next);
+    }
+    for (; t0 < end; t0 += kStep) {
+        const T* values[S::kHalves];
+        uint32_t limit[S::kHalves];
+#pragma unroll
+        for (uint32_t h = 0; h < S::kHalves; ++h) {
+            const bool valid = static_cast<uint32_t>(page[h]) < a.n_pages;
+            const int64_t p = valid ? page[h] : 0;
+            limit[h] = valid ? end : 0;
+            values[h] = value_base + p * a.value_page + static_cast<int64_t>((t0 + 16 * h) & place_mask) * a.value_slot;
+        }
+        value_run v[S::kGroups][S::kValueSteps][S::kRun];
+#pragma unroll
+        for (uint32_t w = 0; w < S::kGroups; ++w)
+#pragma unroll
+            for (uint32_t s = 0; s < S::kValueSteps; ++s)
+#pragma unroll
+                for (uint32_t k = 0; k < S::kRun; ++k) {
+                    const uint32_t d = (s * 16 + col) * S::kValueRun;
+                    const uint32_t h = S::kRun == 8 ? k / 4 : w, place = 4 * quad + k % 4;
+                    v[w][s][k] = value_run{};
+                    if (FULL || d < a.head_dim)
+                        v[w][s][k] = *reinterpret_cast<const value_run*>(values[h] + place * a.value_slot + d);
+                }
+        float score[S::kHalves][4];
+#pragma unroll
+        for (uint32_t h = 0; h < S::kHalves; ++h) {
+            f32x4 acc = {};
+#pragma unroll
+            for (uint32_t s = 0; s < S::kKeySteps; ++s) acc = P::mma(keys[h][s], q[s], acc);
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i)
-                score[h][i] = t + 4 * quad + i < limit[h] ? acc[i] * scale : -__builtin_inff();
+                score[h][i] = t0 + 16 * h + 4 * quad + i < limit[h] ? acc[i] * scale : -__builtin_inff();
+        }
+        if (t0 + kStep < end) {
+            load_keys(t0 + kStep, next);
+#pragma unroll
+            for (uint32_t h = 0; h < S::kHalves; ++h) page[h] = next[h];
+            entries(t0 + 2 * kStep, next);
         }
         float top = m;
 #pragma unroll
-        for (uint32_t h = 0; h < 2; ++h)
+        for (uint32_t h = 0; h < S::kHalves; ++h)
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) top = fmaxf(top, score[h][i]);
         top = column_max(top);
-        const float base = top == -__builtin_inff() ? 0.0f : top;
+        const float base = finite_base(top);
         const float fade = __builtin_amdgcn_exp2f(m - base);
         m = top;
         l *= fade;
@@ -251,12 +338,24 @@ __global__ __launch_bounds__(kThreads) void nz_attention_kernel(nz_attention_arg
 #pragma unroll
             for (uint32_t e = 0; e < S::kValueRun; ++e) o[s][e] *= fade;
 #pragma unroll
-        for (uint32_t h = 0; h < 2; ++h)
+        for (uint32_t h = 0; h < S::kHalves; ++h)
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) {
                 score[h][i] = __builtin_amdgcn_exp2f(score[h][i] - (base - P::kLift));
                 l += score[h][i];
             }
+        // values of masked keys may be anything, NaN among it
+        if (t0 + S::kKeys > min(limit[0], limit[S::kHalves - 1])) {
+#pragma unroll
+            for (uint32_t w = 0; w < S::kGroups; ++w)
+#pragma unroll
+                for (uint32_t s = 0; s < S::kValueSteps; ++s)
+#pragma unroll
+                    for (uint32_t k = 0; k < S::kRun; ++k) {
+                        const uint32_t h = S::kRun == 8 ? k / 4 : w;
+                        if (t0 + 16 * h + 4 * quad + k % 4 >= limit[h]) v[w][s][k] = value_run{};
+                    }
+        }
         // the products with the values, 4 * kRun keys at a time
 #pragma unroll
         for (uint32_t w = 0; w < S::kGroups; ++w) {
@@ -268,25 +367,15 @@ __global__ __launch_bounds__(kThreads) void nz_attention_kernel(nz_attention_arg
                 p_lo[k] = static_cast<T>(fmaxf(p - static_cast<float>(p_hi[k]), P::kLeast));
             }
 #pragma unroll
-            for (uint32_t s = 0; s < S::kValueSteps; ++s) {
-                const uint32_t d = (s * 16 + col) * S::kValueRun;
-                value_run v[S::kRun];
-#pragma unroll
-                for (uint32_t k = 0; k < S::kRun; ++k) {
-                    const uint32_t h = S::kRun == 8 ? k / 4 : w, place = 4 * quad + k % 4;
-                    v[k] = value_run{};
-                    if ((FULL || d < a.head_dim) && t0 + 16 * h + place < limit[h])
-                        v[k] = *reinterpret_cast<const value_run*>(values[h] + place * a.value_slot + d);
-                }
+            for (uint32_t s = 0; s < S::kValueSteps; ++s)
 #pragma unroll
                 for (uint32_t e = 0; e < S::kValueRun; ++e) {
                     piece x;
 #pragma unroll
-                    for (uint32_t k = 0; k < S::kRun; ++k) x[k] = v[k][e];
+                    for (uint32_t k = 0; k < S::kRun; ++k) x[k] = v[w][s][k][e];
                     o[s][e] = P::mma(x, p_hi, o[s][e]);
                     if (S::kRun == 8) o[s][e] = P::mma(x, p_lo, o[s][e]);
                 }
-            }
         }
     }
 
@@ -295,64 +384,105 @@ __global__ __launch_bounds__(kThreads) void nz_attention_kernel(nz_attention_arg
         lds_m[wave][col] = m;
         lds_l[wave][col] = l;
     }
+    if (col < heads) {
 #pragma unroll
-    for (uint32_t s = 0; s < S::kValueSteps; ++s)
+        for (uint32_t s = 0; s < S::kValueSteps; ++s)
 #pragma unroll
-        for (uint32_t e = 0; e < S::kValueRun; ++e)
+            for (uint32_t e = 0; e < S::kValueRun; ++e)
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                const uint32_t d = (s * 16 + 4 * quad + i) * S::kValueRun + e;
-                lds_o[wave][col][d] = o[s][e][i];
-            }
+                for (uint32_t i = 0; i < 4; ++i)
+                    lds_o[wave][col][(s * 16 + 4 * quad + i) * S::kValueRun + e] = o[s][e][i];
+    }
     __syncthreads();
-    // the item's sums: unnormalised, with their maximum and weight, or the row itself
+    // The item's sums over its wavefronts: the row itself, or, unnormalised
+    // and with their maximum and weight, a part of it.
     const bool whole = item.count == 1;
-    for (uint32_t i = threadIdx.x; i < heads * DP; i += kThreads) {
-        const uint32_t h = i / DP, d = i % DP;
+    const uint64_t slot = static_cast<uint64_t>(which) * a.heads + head0;
+    float* const part_o = a.partials + partials_sums(a.n_items, a.heads);
+    float* const part_ml = part_o + sums_words(a.n_items, a.heads, a.head_dim);
+    T* const out = static_cast<T*>(a.out) + item.row * a.out_row + head0 * a.out_head;
+    const uint32_t quads = a.head_dim / 4;   // runs of 4 elements of a head
+    for (uint32_t i = threadIdx.x; i < heads * quads; i += kThreads) {
+        const uint32_t h = i / quads, d = i % quads * 4;
         float top = -__builtin_inff();
 #pragma unroll
         for (uint32_t w = 0; w < kWaves; ++w) top = fmaxf(top, lds_m[w][h]);
-        const float base = top == -__builtin_inff() ? 0.0f : top;
-        float sum = 0.0f, weight = 0.0f;
+        const float base = finite_base(top);
+        float weight = 0.0f;
+        f32x4 sum = {};
 #pragma unroll
         for (uint32_t w = 0; w < kWaves; ++w) {
             const float share = __builtin_amdgcn_exp2f(lds_m[w][h] - base);
             weight += share * lds_l[w][h];
-            sum += share * lds_o[w][h][d];
+            sum += share * *reinterpret_cast<const f32x4*>(&lds_o[w][h][d]);
         }
-        if (d >= a.head_dim) continue;
         if (whole) {
-            static_cast<T*>(a.out)[item.row * a.out_row + (head0 + h) * a.out_head + d] =
-                from_float<T>(weight == 0.0f ? 0.0f : sum / weight);
+            store_row(out + h * a.out_head + d, sum, weight);
         } else {
-            float* dst = a.partials + (static_cast<uint64_t>(which) * a.heads + head0 + h) * (a.head_dim + 2);
-            if (d == 0) dst[0] = top, dst[1] = weight;
-            dst[2 + d] = sum;
+            if (d == 0) put_pair(part_ml + 2 * (slot + h), top, weight);
+            float* const dst = part_o + (slot + h) * a.head_dim + d;
+            put_pair(dst, sum[0], sum[1]);
+            put_pair(dst + 2, sum[2], sum[3]);
         }
     }
-}
-
-// Rows of several items: the items' sums joined in their order.
-template <typename T>
-__global__ __launch_bounds__(256) void nz_attention_join_kernel(nz_attention_args a) {
-    const nz_attention_item item = a.items[blockIdx.x];
-    if (static_cast<uint32_t>(item.row) >= a.n_rows || item.index != 0 || item.count <= 1) return;
-    const uint32_t step = a.head_dim + 2;
-    for (uint32_t i = threadIdx.x; i < a.heads * a.head_dim; i += 256) {
-        const uint32_t h = i / a.head_dim, d = i % a.head_dim;
-        const float* src = a.partials + (static_cast<uint64_t>(blockIdx.x) * a.heads + h) * step;
-        const uint64_t stride = static_cast<uint64_t>(a.heads) * step;
-        float top = -__builtin_inff();
-        for (int32_t k = 0; k < item.count; ++k) top = fmaxf(top, src[k * stride]);
-        const float base = top == -__builtin_inff() ? 0.0f : top;
-        float sum = 0.0f, weight = 0.0f;
-        for (int32_t k = 0; k < item.count; ++k) {
-            const float share = __builtin_amdgcn_exp2f(src[k * stride] - base);
-            weight += share * src[k * stride + 1];
-            sum += share * src[k * stride + 2 + d];
+    if (whole) return;
+    // The last of the row's items to arrive joins them all, in their order.
+    uint32_t* const counter = reinterpret_cast<uint32_t*>(a.partials) + static_cast<uint64_t>(item.first) * per_item + part;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wavefront's stores have arrived
+    __syncthreads();
+    if (threadIdx.x == 0)
+        last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 ==
+               static_cast<uint32_t>(item.count);
+    __syncthreads();
+    if (!last) return;
+    if (threadIdx.x == 0) *counter = 0;   // for the next call
+    const uint32_t n = static_cast<uint32_t>(item.count);
+    const uint64_t step = a.heads, slot0 = static_cast<uint64_t>(item.first) * a.heads + head0;
+    {   // 16 threads a head: its maximum and weight over the items
+        const uint32_t h = threadIdx.x >> 4, sub = threadIdx.x & 15;
+        float top = -__builtin_inff(), weight = 0.0f;
+        if (h < heads)
+            for (uint32_t k = sub; k < n; k += 16) top = fmaxf(top, get_pair(part_ml + 2 * (slot0 + k * step + h)).x);
+#pragma unroll
+        for (uint32_t d = 1; d < 16; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+        const float base = finite_base(top);
+        if (h < heads)
+            for (uint32_t k = sub; k < n; k += 16) {
+                const float2 ml = get_pair(part_ml + 2 * (slot0 + k * step + h));
+                weight += __builtin_amdgcn_exp2f(ml.x - base) * ml.y;
+            }
+#pragma unroll
+        for (uint32_t d = 1; d < 16; d <<= 1) weight += __shfl_xor(weight, d);
+        if (sub == 0) lds_m[0][h] = base, lds_l[0][h] = weight;
+    }
+    __syncthreads();
+    // Each run of 4 elements is summed by `subs` threads over a share of the
+    // items, where there are fewer runs than threads.
+    const uint32_t runs = heads * quads, subs = max(kThreads / runs, 1u);
+    float* const lds_sum = &lds_o[0][0][0];
+    for (uint32_t i = threadIdx.x; i < runs * subs; i += kThreads) {
+        const uint32_t run = i % runs, sub = i / runs, h = run / quads, d = run % quads * 4;
+        const float base = lds_m[0][h];
+        const uint32_t k0 = sub * n / subs, k1 = (sub + 1) * n / subs;
+        f32x4 sum = {};
+#pragma unroll 8
+        for (uint32_t k = k0; k < k1; ++k) {
+            const uint64_t at = slot0 + k * step + h;
+            const float share = __builtin_amdgcn_exp2f(get_pair(part_ml + 2 * at).x - base);
+            const float2 lo = get_pair(part_o + at * a.head_dim + d), hi = get_pair(part_o + at * a.head_dim + d + 2);
+            sum += share * f32x4{lo.x, lo.y, hi.x, hi.y};
         }
-        static_cast<T*>(a.out)[item.row * a.out_row + h * a.out_head + d] =
-            from_float<T>(weight == 0.0f ? 0.0f : sum / weight);
+        if (subs == 1) store_row(out + h * a.out_head + d, sum, lds_l[0][h]);
+        else *reinterpret_cast<f32x4*>(lds_sum + i * 4) = sum;
+    }
+    if (subs == 1) return;
+    __syncthreads();
+    if (threadIdx.x < runs) {
+        const uint32_t h = threadIdx.x / quads, d = threadIdx.x % quads * 4;
+        f32x4 sum = {};
+        for (uint32_t sub = 0; sub < subs; ++sub)
+            sum += *reinterpret_cast<const f32x4*>(lds_sum + (sub * runs + threadIdx.x) * 4);
+        store_row(out + h * a.out_head + d, sum, lds_l[0][h]);
     }
 }
 
@@ -369,7 +499,6 @@ void launch_attention(const nz_attention_args& a, hipStream_t stream) {
     if (a.head_dim <= 64) launch_attention_dim<T, 64>(a, grid, stream);
     else if (a.head_dim <= 128) launch_attention_dim<T, 128>(a, grid, stream);
     else launch_attention_dim<T, 256>(a, grid, stream);
-    hipLaunchKernelGGL(nz_attention_join_kernel<T>, dim3(a.n_items), dim3(256), 0, stream, a);
 }
 
 int launched(const char* what, char* message, size_t message_size) {

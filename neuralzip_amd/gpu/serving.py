@@ -29,7 +29,7 @@ from neuralzip_amd.gpu.decoder import _CURRENT, _stream_handle
 
 _TYPES = {torch.bfloat16: _native.VALUE_BF16, torch.float16: _native.VALUE_FP16, torch.float32: _native.VALUE_FP32}
 # Workgroups that an attention's items are cut into, over all key-value heads.
-ATTENTION_WORKGROUPS = 1024
+ATTENTION_WORKGROUPS = 512
 # Query heads of one workgroup (the columns of a matrix instruction).
 _HEADS = 16
 # PageTables.extend's status of a request (enum nz_pages_status).
@@ -292,7 +292,7 @@ class AttentionPlan:
         scratch = self._scratch.get(handle)
         if scratch is None or scratch.numel() < words:
             with _on(stream):
-                scratch = self._scratch[handle] = torch.empty(words, dtype=torch.float32, device=self.device)
+                scratch = self._scratch[handle] = torch.zeros(words, dtype=torch.float32, device=self.device)
         return scratch
 
 

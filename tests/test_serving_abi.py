@@ -148,7 +148,7 @@ def test_null_argument_structs_and_plans_are_refused():
     assert lib.nz_attention_plan(None, None, 1, 1, 4096, None) == -1
     assert lib.nz_attention_plan(4096, None, 1, 0, 4096, None) == -1
     assert lib.nz_attention_plan(4096, None, 1 << 31, 1, 4096, None) == -1
-    assert lib.nz_attention_partials(10, 32, 128) == 10 * 32 * 130
+    assert lib.nz_attention_partials(10, 32, 128) == 10 * 32 * (1 + 130)
 
 
 def test_calls_without_work_return_without_a_device():
