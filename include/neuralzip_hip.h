@@ -643,10 +643,13 @@ typedef struct nz_attention_item {
 
 /* Cuts rows' contexts into items of about equal length, on the device:
  * n_rows contexts (negative ones count as 0), requests[row] their requests
- * (NULL: row i is request i). `items` has room for n_rows + target entries;
- * rows are cut so that there are at most that many, of at least 128 keys
- * (but for the last of a row), and the rest are marked unused. The plan
- * serves the attention of every layer of a step. */
+ * (NULL: row i is request i). Let n be n_rows, rounded up to a multiple of
+ * target (target for none): `items` has room for n + target. There are at
+ * most n items, as short as that allows but of at least 128 keys (512 from
+ * contexts of 8192 on; except for a row's last); or at most n + target, where
+ * the longest would else be more than half longer than the n-th part of all
+ * keys and than half their target-th part. The rest are marked unused. The
+ * plan serves the attention of every layer of a step. */
 int nz_attention_plan(const int32_t* contexts, const int32_t* requests, uint32_t n_rows, uint32_t target,
                       nz_attention_item* items, void* stream);
 
@@ -684,7 +687,7 @@ uint64_t nz_attention_partials(uint32_t n_items, uint32_t heads, uint32_t head_d
  * row without keys gives zeros. Keys whose page or request is not in range
  * count as masked. head_dim is a multiple of 16, at most 256; strides and
  * addresses are multiples of 16 bytes. Two calls that may overlap need their
- * own partials. */
+ * own partials; n_items * heads * head_dim is below 2^30. */
 int nz_attention(const nz_attention_args* args, void* stream);
 
 typedef struct nz_logits_args {

@@ -127,8 +127,8 @@ int nz_attention_plan(const int32_t* contexts, const int32_t* requests, uint32_t
                       nz_attention_item* items, void* stream) {
     const int bad = guarded([&] {
         if (!items || (!contexts && n_rows)) refuse("Null attention plan argument.");
-        if (target == 0 || static_cast<uint64_t>(n_rows) + target > kMaxGrid)
-            refuse("The plan's target must be positive, and rows plus target below 2^31.");
+        if (target == 0 || target > kMaxGrid / 2 || n_rows > kMaxGrid / 2)
+            refuse("The plan's target must be positive, and rows and target below 2^30.");
     });
     if (bad) return bad;
     char message[256] = {0};
@@ -160,7 +160,9 @@ int nz_attention(const nz_attention_args* args, void* stream) {
         check_alignment(size, a.value_cache, a.value_page, a.value_head, a.value_slot);
         check_alignment(4, a.partials, 0);
         if (a.n_items < a.n_rows) refuse("The plan has fewer items than rows.");
-        if (static_cast<uint64_t>(a.n_items) * a.heads > kMaxGrid) refuse("Too many items and heads in one call.");
+        if (a.n_items > kMaxGrid || a.heads > kMaxGrid ||
+            static_cast<uint64_t>(a.n_items) * a.heads > (1ull << 30) / a.head_dim)
+            refuse("Too many items and heads in one call.");
         return false;
     });
 }

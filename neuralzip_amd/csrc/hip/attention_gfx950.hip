@@ -14,40 +14,99 @@ namespace {
 // ------------------------------------------------------------------- plan
 
 constexpr uint32_t kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
-// Items start at multiples of the keys a wavefront takes at a time, and are
-// cut no smaller than gives each wavefront of a workgroup one such tile.
-constexpr uint32_t kTile = 32, kLeastItem = 128;
+// Items start at multiples of kTile keys, and are cut no shorter than gives
+// each wavefront of a workgroup one such tile, or, up to kLeastLong, than a
+// sixteenth of the longest context: more items than that take longer to join
+// than they save (one row over 8 heads of 8000 keys 13.2 us with items of
+// 512 keys and 14.6 of 256; of 2001 keys 11.1 of 512 and 8.8 of 128).
+constexpr uint32_t kTile = 32, kLeastItem = 128, kLeastLong = 512;
 
-__device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
-    return v;
+struct PlanLds {
+    uint64_t keys[kPlanWaves];
+    uint32_t most[kPlanWaves], counts[kPlanWaves];
+};
+
+__device__ __forceinline__ uint32_t context_of(const int32_t* contexts, uint32_t r) {
+    return static_cast<uint32_t>(max(contexts[r], 0));
 }
 
+// Items of all rows when none is longer than `share` (a wavefront's sum).
+__device__ __forceinline__ uint32_t count_items(const int32_t* contexts, uint32_t n_rows, uint32_t share) {
+    uint32_t n = 0;
+    for (uint32_t r = threadIdx.x & 63; r < n_rows; r += 64)
+        n += max((context_of(contexts, r) + share - 1) / share, 1u);
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d <<= 1) n += __shfl_xor(n, d);
+    return n;
+}
+
+// The shortest item length (in tiles, from `lo` to `hi`) of which there are
+// at most `limit` items; `hi` is one. Every wavefront tries another length.
+__device__ uint32_t shortest_share(const int32_t* contexts, uint32_t n_rows, uint32_t limit, uint32_t lo, uint32_t hi,
+                                   PlanLds& lds) {
+    const uint32_t wave = threadIdx.x >> 6;
+    while (lo < hi) {
+        const uint32_t step = (hi - lo + kPlanWaves) / (kPlanWaves + 1);
+        const uint32_t tried = min(lo + wave * step, hi);
+        const uint32_t n = count_items(contexts, n_rows, tried * kTile);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) lds.counts[wave] = n;
+        __syncthreads();
+        uint32_t below = lo, found = hi;
+#pragma unroll
+        for (uint32_t w = 0; w < kPlanWaves; ++w) {
+            const uint32_t length = min(lo + w * step, hi);
+            if (lds.counts[w] <= limit) found = min(found, length);
+            else below = max(below, length + 1);
+        }
+        lo = below;
+        hi = max(found, below);
+    }
+    return lo;
+}
+
+// One workgroup. Items are as short as the number wanted allows, so that they
+// take about the same time: one per compute unit and row's heads while that
+// cuts no row far shorter than its share, since rows of one item need no
+// join; twice as many where some rows are much longer than others.
 __global__ __launch_bounds__(kPlanThreads) void nz_attention_plan_kernel(const int32_t* __restrict__ contexts,
                                                                          const int32_t* __restrict__ requests,
                                                                          uint32_t n_rows, uint32_t target,
                                                                          nz_attention_item* __restrict__ items) {
-    __shared__ uint64_t sums[kPlanWaves];
-    __shared__ uint32_t counts[kPlanWaves];
+    __shared__ PlanLds lds;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint64_t keys = 0;
-    for (uint32_t r = threadIdx.x; r < n_rows; r += kPlanThreads) keys += static_cast<uint32_t>(max(contexts[r], 0));
-    keys = wave_sum(keys);
-    if (lane == 0) sums[wave] = keys;
+    uint32_t longest = 0;
+    for (uint32_t r = threadIdx.x; r < n_rows; r += kPlanThreads) {
+        const uint32_t context = context_of(contexts, r);
+        keys += context;
+        longest = max(longest, context);
+    }
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d <<= 1) {
+        keys += __shfl_xor(keys, d);
+        longest = max(longest, static_cast<uint32_t>(__shfl_xor(longest, d)));
+    }
+    if (lane == 0) lds.keys[wave] = keys, lds.most[wave] = longest;
     __syncthreads();
     keys = 0;
 #pragma unroll
-    for (uint32_t w = 0; w < kPlanWaves; ++w) keys += sums[w];
-    // the items' length: the sum of ceil(context / most) over the rows is at most n_rows + target
-    uint64_t share = (keys + target - 1) / target;
-    share = share < kLeastItem ? kLeastItem : (share + kTile - 1) / kTile * kTile;
-    const uint32_t most = static_cast<uint32_t>(share < 0x80000000ull ? share : 0x80000000ull);
+    for (uint32_t w = 0; w < kPlanWaves; ++w) keys += lds.keys[w], longest = max(longest, lds.most[w]);
+    const uint32_t fewest = (max(target, n_rows) + target - 1) / target * target, tiles = (longest + kTile - 1) / kTile;
+    const uint32_t least = min(max((tiles + 15) / 16, kLeastItem / kTile), kLeastLong / kTile);
+    uint32_t share = least;
+    if (tiles > least) {
+        share = shortest_share(contexts, n_rows, fewest, least, tiles, lds);
+        const uint64_t length = static_cast<uint64_t>(share) * kTile;
+        if (length * fewest * 2 > keys * 3 && length * target * 2 > keys)
+            share = shortest_share(contexts, n_rows, fewest + target, least, share, lds);
+    }
+    const uint32_t most = share * kTile;
     uint32_t first = 0;
     for (uint32_t r0 = 0; r0 < n_rows; r0 += kPlanThreads) {
         const uint32_t r = r0 + threadIdx.x;
         const bool live = r < n_rows;
-        const uint32_t context = live ? static_cast<uint32_t>(max(contexts[r], 0)) : 0;
+        const uint32_t context = live ? context_of(contexts, r) : 0;
         // a row's items are of equal length, in whole tiles
         uint32_t n = max((context + most - 1) / most, 1u);
         const uint32_t each = max(((context + n - 1) / n + kTile - 1) / kTile * kTile, kTile);
@@ -58,14 +117,14 @@ __global__ __launch_bounds__(kPlanThreads) void nz_attention_plan_kernel(const i
             const uint32_t below = __shfl_up(scan, d);
             if (lane >= d) scan += below;
         }
-        __syncthreads();   // the last strip's reads of `counts`
-        if (lane == 63) counts[wave] = scan;
+        __syncthreads();   // the last reads of `counts`
+        if (lane == 63) lds.counts[wave] = scan;
         __syncthreads();
         uint32_t before = first, total = 0;
 #pragma unroll
         for (uint32_t w = 0; w < kPlanWaves; ++w) {
-            if (w < wave) before += counts[w];
-            total += counts[w];
+            if (w < wave) before += lds.counts[w];
+            total += lds.counts[w];
         }
         const uint32_t base = before + scan - n;
         for (uint32_t i = 0; i < n; ++i) {
@@ -83,7 +142,7 @@ __global__ __launch_bounds__(kPlanThreads) void nz_attention_plan_kernel(const i
         first += total;
     }
     const nz_attention_item none = {-1, -1, 0, 0, 0, 0, 0, 0};
-    for (uint32_t i = first + threadIdx.x; i < n_rows + target; i += kPlanThreads) items[i] = none;
+    for (uint32_t i = first + threadIdx.x; i < fewest + target; i += kPlanThreads) items[i] = none;
 }
 
 // -------------------------------------------------------------- attention
@@ -168,17 +227,30 @@ __device__ __forceinline__ void store_row(T* dst, f32x4 sum, float weight) {
 
 // Sums that another workgroup, maybe of another XCD, will read: stores and
 // loads of device scope go past the caches that only one XCD sees. A release
-// fence would write back all of the XCD's L2 instead.
-__device__ __forceinline__ void put_pair(float* dst, float x, float y) {
-    __hip_atomic_store(reinterpret_cast<uint64_t*>(dst),
-                       static_cast<uint64_t>(__float_as_uint(y)) << 32 | __float_as_uint(x), __ATOMIC_RELAXED,
-                       __HIP_MEMORY_SCOPE_AGENT);
+// fence would write back all of the XCD's L2 instead. (The buffer forms, for
+// 16 bytes at a time; offsets are in bytes from a row's first item.)
+constexpr int kDeviceScope = 16;   // sc1
+using rsrc_t = __amdgpu_buffer_rsrc_t;
+
+__device__ __forceinline__ rsrc_t device_buffer(float* base) {
+    return __builtin_amdgcn_make_buffer_rsrc(base, 0, 0xFFFFFFFFu, 0x00020000u);
 }
 
-__device__ __forceinline__ float2 get_pair(const float* src) {
-    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(src), __ATOMIC_RELAXED,
-                                         __HIP_MEMORY_SCOPE_AGENT);
-    return make_float2(__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32)));
+__device__ __forceinline__ void put_four(rsrc_t buffer, uint32_t offset, f32x4 x) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(vec<uint32_t, 4>, x), buffer, offset, 0, kDeviceScope);
+}
+
+__device__ __forceinline__ f32x4 get_four(rsrc_t buffer, uint32_t offset) {
+    return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer, offset, 0, kDeviceScope));
+}
+
+__device__ __forceinline__ void put_pair(rsrc_t buffer, uint32_t offset, float x, float y) {
+    __builtin_amdgcn_raw_buffer_store_b64(vec<uint32_t, 2>{__float_as_uint(x), __float_as_uint(y)}, buffer, offset, 0,
+                                          kDeviceScope);
+}
+
+__device__ __forceinline__ vec<float, 2> get_pair(rsrc_t buffer, uint32_t offset) {
+    return __builtin_bit_cast(vec<float, 2>, __builtin_amdgcn_raw_buffer_load_b64(buffer, offset, 0, kDeviceScope));
 }
 
 // The scratch: a counter per item and head, which is 0 between calls, then
@@ -397,9 +469,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 
     // The item's sums over its wavefronts: the row itself, or, unnormalised
     // and with their maximum and weight, a part of it.
     const bool whole = item.count == 1;
-    const uint64_t slot = static_cast<uint64_t>(which) * a.heads + head0;
-    float* const part_o = a.partials + partials_sums(a.n_items, a.heads);
-    float* const part_ml = part_o + sums_words(a.n_items, a.heads, a.head_dim);
+    const uint64_t slot0 = static_cast<uint64_t>(item.first) * a.heads + head0;
+    float* const sums = a.partials + partials_sums(a.n_items, a.heads);
+    const rsrc_t part_o = device_buffer(sums + slot0 * a.head_dim);
+    const rsrc_t part_ml = device_buffer(sums + sums_words(a.n_items, a.heads, a.head_dim) + 2 * slot0);
+    const uint32_t step = a.heads;   // of an item's heads among the slots
     T* const out = static_cast<T*>(a.out) + item.row * a.out_row + head0 * a.out_head;
     const uint32_t quads = a.head_dim / 4;   // runs of 4 elements of a head
     for (uint32_t i = threadIdx.x; i < heads * quads; i += kThreads) {
@@ -419,10 +493,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 
         if (whole) {
             store_row(out + h * a.out_head + d, sum, weight);
         } else {
-            if (d == 0) put_pair(part_ml + 2 * (slot + h), top, weight);
-            float* const dst = part_o + (slot + h) * a.head_dim + d;
-            put_pair(dst, sum[0], sum[1]);
-            put_pair(dst + 2, sum[2], sum[3]);
+            const uint32_t slot = static_cast<uint32_t>(item.index) * step + h;
+            if (d == 0) put_pair(part_ml, 8 * slot, top, weight);
+            put_four(part_o, 4 * (slot * a.head_dim + d), sum);
         }
     }
     if (whole) return;
@@ -436,53 +509,65 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 
     __syncthreads();
     if (!last) return;
     if (threadIdx.x == 0) *counter = 0;   // for the next call
+    // Each run of 4 elements of a head is joined by `subs` threads, each over
+    // a share of the items, kBatch of them in flight at a time.
     const uint32_t n = static_cast<uint32_t>(item.count);
-    const uint64_t step = a.heads, slot0 = static_cast<uint64_t>(item.first) * a.heads + head0;
-    {   // 16 threads a head: its maximum and weight over the items
-        const uint32_t h = threadIdx.x >> 4, sub = threadIdx.x & 15;
-        float top = -__builtin_inff(), weight = 0.0f;
-        if (h < heads)
-            for (uint32_t k = sub; k < n; k += 16) top = fmaxf(top, get_pair(part_ml + 2 * (slot0 + k * step + h)).x);
-#pragma unroll
-        for (uint32_t d = 1; d < 16; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-        const float base = finite_base(top);
-        if (h < heads)
-            for (uint32_t k = sub; k < n; k += 16) {
-                const float2 ml = get_pair(part_ml + 2 * (slot0 + k * step + h));
-                weight += __builtin_amdgcn_exp2f(ml.x - base) * ml.y;
-            }
-#pragma unroll
-        for (uint32_t d = 1; d < 16; d <<= 1) weight += __shfl_xor(weight, d);
-        if (sub == 0) lds_m[0][h] = base, lds_l[0][h] = weight;
-    }
-    __syncthreads();
-    // Each run of 4 elements is summed by `subs` threads over a share of the
-    // items, where there are fewer runs than threads.
     const uint32_t runs = heads * quads, subs = max(kThreads / runs, 1u);
     float* const lds_sum = &lds_o[0][0][0];
     for (uint32_t i = threadIdx.x; i < runs * subs; i += kThreads) {
         const uint32_t run = i % runs, sub = i / runs, h = run / quads, d = run % quads * 4;
-        const float base = lds_m[0][h];
         const uint32_t k0 = sub * n / subs, k1 = (sub + 1) * n / subs;
+        float top = -__builtin_inff(), weight = 0.0f;
         f32x4 sum = {};
-#pragma unroll 8
-        for (uint32_t k = k0; k < k1; ++k) {
-            const uint64_t at = slot0 + k * step + h;
-            const float share = __builtin_amdgcn_exp2f(get_pair(part_ml + 2 * at).x - base);
-            const float2 lo = get_pair(part_o + at * a.head_dim + d), hi = get_pair(part_o + at * a.head_dim + d + 2);
-            sum += share * f32x4{lo.x, lo.y, hi.x, hi.y};
+        constexpr uint32_t kBatch = 8;
+        for (uint32_t k = k0; k < k1; k += kBatch) {
+            vec<float, 2> ml[kBatch];
+            f32x4 x[kBatch];
+#pragma unroll
+            for (uint32_t j = 0; j < kBatch; ++j) {
+                const uint32_t slot = min(k + j, k1 - 1) * step + h;
+                ml[j] = get_pair(part_ml, 8 * slot);
+                x[j] = get_four(part_o, 4 * (slot * a.head_dim + d));
+            }
+            float higher = top;
+#pragma unroll
+            for (uint32_t j = 0; j < kBatch; ++j) higher = fmaxf(higher, ml[j].x);
+            const float base = finite_base(higher), fade = __builtin_amdgcn_exp2f(top - base);
+            top = higher;
+            weight *= fade;
+            sum *= fade;
+#pragma unroll
+            for (uint32_t j = 0; j < kBatch; ++j) {
+                const float share = __builtin_amdgcn_exp2f(ml[j].x - base);
+                if (k + j < k1) {
+                    weight += share * ml[j].y;
+                    sum += share * x[j];
+                }
+            }
         }
-        if (subs == 1) store_row(out + h * a.out_head + d, sum, lds_l[0][h]);
-        else *reinterpret_cast<f32x4*>(lds_sum + i * 4) = sum;
+        if (subs == 1) {
+            store_row(out + h * a.out_head + d, sum, weight);
+        } else {
+            *reinterpret_cast<f32x4*>(lds_sum + i * 8) = sum;
+            lds_sum[i * 8 + 4] = top;
+            lds_sum[i * 8 + 5] = weight;
+        }
     }
     if (subs == 1) return;
     __syncthreads();
     if (threadIdx.x < runs) {
         const uint32_t h = threadIdx.x / quads, d = threadIdx.x % quads * 4;
+        float top = -__builtin_inff(), weight = 0.0f;
+        for (uint32_t sub = 0; sub < subs; ++sub) top = fmaxf(top, lds_sum[(sub * runs + threadIdx.x) * 8 + 4]);
+        const float base = finite_base(top);
         f32x4 sum = {};
-        for (uint32_t sub = 0; sub < subs; ++sub)
-            sum += *reinterpret_cast<const f32x4*>(lds_sum + (sub * runs + threadIdx.x) * 4);
-        store_row(out + h * a.out_head + d, sum, lds_l[0][h]);
+        for (uint32_t sub = 0; sub < subs; ++sub) {
+            const float* src = lds_sum + (sub * runs + threadIdx.x) * 8;
+            const float share = __builtin_amdgcn_exp2f(src[4] - base);
+            weight += share * src[5];
+            sum += share * *reinterpret_cast<const f32x4*>(src);
+        }
+        store_row(out + h * a.out_head + d, sum, weight);
     }
 }
 

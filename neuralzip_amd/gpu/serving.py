@@ -28,8 +28,9 @@ from neuralzip_amd import _native
 from neuralzip_amd.gpu.decoder import _CURRENT, _stream_handle
 
 _TYPES = {torch.bfloat16: _native.VALUE_BF16, torch.float16: _native.VALUE_FP16, torch.float32: _native.VALUE_FP32}
-# Workgroups that an attention's items are cut into, over all key-value heads.
-ATTENTION_WORKGROUPS = 512
+# Workgroups that an attention's items are cut into, over all key-value heads,
+# if there are not more rows.
+ATTENTION_WORKGROUPS = 256
 # Query heads of one workgroup (the columns of a matrix instruction).
 _HEADS = 16
 # PageTables.extend's status of a request (enum nz_pages_status).
@@ -270,7 +271,7 @@ class AttentionPlan:
         self.rows, self.heads, self.kv_heads, self.device = contexts.shape[0], heads, kv_heads, contexts.device
         per_item = kv_heads * -(-(heads // kv_heads) // _HEADS)
         self._target = max(1, ATTENTION_WORKGROUPS // per_item)
-        self.capacity = self.rows + self._target
+        self.capacity = (max(1, -(-self.rows // self._target)) + 1) * self._target
         with _on(stream):
             self.items = torch.empty((self.capacity, 8), dtype=torch.int32, device=self.device)
         self._scratch = {}
