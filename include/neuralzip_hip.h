@@ -536,7 +536,6 @@ typedef struct nz_pages_extend_args {
     int32_t* status;             /* n_requests (out): enum nz_pages_status   */
     int32_t* lengths_after;      /* n_requests (out)                         */
     int32_t* n_free_after;       /* 1 (out)                                  */
-    uint32_t* ticket;            /* 1, zero before the first call; zero after each */
     uint32_t n_requests;
     uint32_t max_pages;
     uint32_t page_size;
@@ -562,8 +561,7 @@ enum nz_pages_status {
  * Entries past the last token hold slot -1, position 0, request -1 and
  * context 0. Table entries past a request's pages mean nothing. Without
  * `advance` lengths and *n_free stay, and the same call again gives the
- * same results (tables' new entries are written either way); calls on one
- * set of tables run one after another (they share the ticket). */
+ * same results (tables' new entries are written either way). */
 int nz_pages_extend(const nz_pages_extend_args* args, void* stream);
 
 typedef struct nz_pages_release_args {
@@ -574,7 +572,6 @@ typedef struct nz_pages_release_args {
     const int32_t* n_free;
     int32_t* lengths_after;      /* n_requests (out)                         */
     int32_t* n_free_after;       /* 1 (out)                                  */
-    uint32_t* ticket;            /* as for nz_pages_extend                   */
     uint32_t n_requests;
     uint32_t max_pages;
     uint32_t page_size;

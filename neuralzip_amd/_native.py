@@ -86,8 +86,8 @@ class _Totals(ctypes.Structure):
 # The serving-step operators' argument structs (nz_*_args of the header, in
 # field order): packed into a bytes object per call, which costs the host a
 # fraction of filling a ctypes structure and is safe between threads.
-PAGES_EXTEND = struct.Struct("=14Q6I")
-PAGES_RELEASE = struct.Struct("=8Q6I")
+PAGES_EXTEND = struct.Struct("=13Q6I")
+PAGES_RELEASE = struct.Struct("=7Q6I")
 ROTARY = struct.Struct("=12Q14q11If")
 ATTENTION = struct.Struct("=7Q10q10IfI")
 LOGITS = struct.Struct("=13Q3q8I")

@@ -70,7 +70,7 @@ extern "C" {
 int nz_pages_extend(const nz_pages_extend_args* args, void* stream) {
     return run(args, stream, nz_hip_pages_extend, [](const nz_pages_extend_args& a) {
         if (!a.lengths || !a.new_tokens || !a.tables || !a.free_pages || !a.n_free || !a.starts || !a.status ||
-            !a.lengths_after || !a.n_free_after || !a.ticket ||
+            !a.lengths_after || !a.n_free_after ||
             (a.max_tokens && (!a.slots || !a.positions || !a.requests || !a.contexts)))
             refuse("Null pages argument.");
         check_pages(a.n_requests, a.max_pages, a.page_size, a.n_pages);
@@ -82,8 +82,7 @@ int nz_pages_extend(const nz_pages_extend_args* args, void* stream) {
 
 int nz_pages_release(const nz_pages_release_args* args, void* stream) {
     return run(args, stream, nz_hip_pages_release, [](const nz_pages_release_args& a) {
-        if (!a.lengths || !a.done || !a.tables || !a.free_pages || !a.n_free || !a.lengths_after || !a.n_free_after ||
-            !a.ticket)
+        if (!a.lengths || !a.done || !a.tables || !a.free_pages || !a.n_free || !a.lengths_after || !a.n_free_after)
             refuse("Null pages argument.");
         check_pages(a.n_requests, a.max_pages, a.page_size, a.n_pages);
         if (a.advance > 1 || a.reserved) refuse("advance is 0 or 1 and reserved is 0.");

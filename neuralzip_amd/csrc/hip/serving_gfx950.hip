@@ -4,6 +4,7 @@
 // (nz_adjust_logits). The attention over the pages is in attention_gfx950.hip.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <stdint.h>
 #include <stdio.h>
 
@@ -14,30 +15,49 @@ namespace {
 
 // ------------------------------------------------------------------ pages
 
-constexpr uint32_t kPagesThreads = 1024, kPagesWaves = kPagesThreads / 64;
+// Workgroups are as wide as a step of so many requests needs (a strip of
+// requests at a time): one wavefront needs no barriers between wavefronts.
+constexpr uint32_t kPagesThreads = 1024;
+// Tokens (or pages to release) that one workgroup writes before the work is
+// shared among several.
+constexpr uint32_t kPagesShare = 2048, kPagesGroups = 128;
 
 // Saturating, so that a step's sum of absurd requests stays past every limit.
 __device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
 
-// Inclusive saturating prefix sum over the workgroup; *total receives the sum.
-__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* waves, uint32_t* total) {
+// Inclusive saturating prefix sums over the workgroup of N values at once;
+// total receives the sums.
+template <uint32_t THREADS, int N>
+__device__ __forceinline__ void block_scan(uint32_t (&v)[N], uint32_t (&total)[N], uint32_t (*lds)[THREADS / 64]) {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-    for (uint32_t d = 1; d < 64; d <<= 1) {
-        const uint32_t below = __shfl_up(v, d);
-        if (lane >= d) v = add_sat(v, below);
-    }
-    __syncthreads();   // the last call's reads of `waves`
-    if (lane == 63) waves[wave] = v;
-    __syncthreads();
-    uint32_t before = 0, sum = 0;
+    for (uint32_t d = 1; d < 64; d <<= 1)
 #pragma unroll
-    for (uint32_t w = 0; w < kPagesWaves; ++w) {
-        if (w < wave) before = add_sat(before, waves[w]);
-        sum = add_sat(sum, waves[w]);
+        for (int i = 0; i < N; ++i) {
+            const uint32_t below = __shfl_up(v[i], d);
+            if (lane >= d) v[i] = add_sat(v[i], below);
+        }
+    if (THREADS == 64) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) total[i] = __shfl(v[i], 63);
+        return;
     }
-    *total = sum;
-    return add_sat(before, v);
+    __syncthreads();   // the last call's reads
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (lane == 63) lds[i][wave] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        uint32_t before = 0, sum = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < THREADS / 64; ++w) {
+            if (w < wave) before = add_sat(before, lds[i][w]);
+            sum = add_sat(sum, lds[i][w]);
+        }
+        v[i] = add_sat(before, v[i]);
+        total[i] = sum;
+    }
 }
 
 // The last i in [0, n) with first[i] <= x, where first[0] <= x.
@@ -51,78 +71,68 @@ __device__ __forceinline__ uint32_t owner(const uint32_t* first, uint32_t n, uin
     return lo;
 }
 
-// Ends a call that may advance the state: the last workgroup to arrive
-// copies the new lengths and stack height over the old ones, which the
-// others may have been reading until then.
-__device__ __forceinline__ void advance_state(uint32_t* ticket, const int32_t* lengths_after, const int32_t* n_free_after,
-                                              int32_t* lengths, int32_t* n_free, uint32_t n) {
-    __shared__ uint32_t last;
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0)
-        last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) + 1 == gridDim.x;
-    __syncthreads();
-    if (!last) return;
-    __threadfence();
-    for (uint32_t r = threadIdx.x; r < n; r += kPagesThreads)
-        lengths[r] = __hip_atomic_load(lengths_after + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (threadIdx.x == 0) {
-        n_free[0] = __hip_atomic_load(n_free_after, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        *ticket = 0;
-    }
-}
-
-// Three prefix sums over the requests (tokens asked, pages wanted, tokens
-// granted), then the new pages and tokens, each found by a search in the
-// sums. Every workgroup computes the sums for itself and writes its share of
-// the tokens and pages.
-__global__ __launch_bounds__(kPagesThreads) void nz_pages_extend_kernel(nz_pages_extend_args a) {
-    __shared__ uint32_t waves[kPagesWaves];
-    __shared__ uint32_t page_first[kPagesThreads], token_first[kPagesThreads];
-    __shared__ int32_t lens[kPagesThreads];
+// Prefix sums over the requests of the tokens asked and the pages wanted; if
+// that refuses some, of the pages wanted by the rest, the tokens granted and
+// the pages granted; then the new pages and tokens, each found by a search in
+// the sums. Every workgroup computes the sums for itself and writes its share of the
+// tokens and pages. Bound by the latency of two dependent reads: 7 kinds of
+// arrays are written, 20 bytes a token.
+template <uint32_t THREADS>
+__global__ __launch_bounds__(THREADS) void nz_pages_extend_kernel(nz_pages_extend_args a) {
+    __shared__ uint32_t waves[2][THREADS / 64];
+    __shared__ uint32_t page_first[THREADS], token_first[THREADS];
+    __shared__ int32_t lens[THREADS];
     const uint32_t page = a.page_size, shift = 31 - __clz(page);
-    const uint32_t stride = gridDim.x * kPagesThreads, at = blockIdx.x * kPagesThreads + threadIdx.x;
+    const uint32_t stride = gridDim.x * THREADS, at = blockIdx.x * THREADS + threadIdx.x;
     const uint64_t limit = static_cast<uint64_t>(a.max_pages) << shift;
     const uint32_t n_free = min(static_cast<uint32_t>(max(a.n_free[0], 0)), a.n_pages);
     uint32_t asked_before = 0, pages_before = 0, tokens_before = 0, taken = 0;
-    for (uint32_t r0 = 0; r0 < a.n_requests; r0 += kPagesThreads) {
+    for (uint32_t r0 = 0; r0 < a.n_requests; r0 += THREADS) {
         const uint32_t r = r0 + threadIdx.x;
         const bool live = r < a.n_requests;
         const int32_t length = live ? a.lengths[r] : 0, asks = live ? a.new_tokens[r] : 0;
         const bool fits = asks >= 0 && length >= 0 &&
                           static_cast<uint64_t>(length) + static_cast<uint64_t>(asks) <= limit;
-        uint32_t n = fits ? asks : 0, total;
-        const uint32_t asked = add_sat(asked_before, block_scan(n, waves, &total));
-        asked_before = add_sat(asked_before, total);
-        const bool room = n == 0 || asked <= a.max_tokens;
-        if (!room) n = 0;
         const uint32_t old = fits ? (static_cast<uint32_t>(length) + page - 1) >> shift : 0;
+        uint32_t n = fits ? asks : 0;
         uint32_t want = fits ? ((static_cast<uint32_t>(length) + n + page - 1) >> shift) - old : 0;
-        const uint32_t wanted = pages_before + block_scan(want, waves, &total);
-        pages_before += total;
-        const bool have = want == 0 || wanted <= n_free;
-        if (!have) n = 0, want = 0;
-        const uint32_t tokens = tokens_before + block_scan(n, waves, &total);
-        const uint32_t strip_tokens = total;
-        // pages granted: those wanted up to the last request that has them
-        const uint32_t granted = taken + block_scan(want, waves, &total);
-        const uint32_t strip_pages = total;
-        page_first[threadIdx.x] = granted - want;
-        token_first[threadIdx.x] = tokens - n;
+        uint32_t sums[2] = {n, want}, totals[2];
+        block_scan<THREADS, 2>(sums, totals, waves);
+        bool room = true, have = true;
+        if (add_sat(asked_before, totals[0]) > a.max_tokens || add_sat(pages_before, totals[1]) > n_free) {
+            room = n == 0 || add_sat(asked_before, sums[0]) <= a.max_tokens;
+            if (!room) n = 0, want = 0;
+            uint32_t wanted[1] = {want}, total[1];
+            block_scan<THREADS, 1>(wanted, total, waves);
+            have = want == 0 || add_sat(pages_before, wanted[0]) <= n_free;
+            asked_before = add_sat(asked_before, totals[0]);
+            pages_before = add_sat(pages_before, total[0]);
+            if (!have) n = 0, want = 0;
+            sums[0] = n, sums[1] = want;
+            block_scan<THREADS, 2>(sums, totals, waves);
+        } else {
+            asked_before = add_sat(asked_before, totals[0]);
+            pages_before = add_sat(pages_before, totals[1]);
+        }
+        const uint32_t tokens = tokens_before + sums[0] - n;
+        page_first[threadIdx.x] = taken + sums[1] - want;
+        token_first[threadIdx.x] = tokens;
         lens[threadIdx.x] = length;
         if (live && blockIdx.x == 0) {
             a.status[r] = !fits ? NZ_PAGES_TOO_LONG : !room ? NZ_PAGES_NO_ROOM : !have ? NZ_PAGES_NO_PAGE : NZ_PAGES_OK;
-            a.starts[r] = tokens - n;
+            a.starts[r] = static_cast<int32_t>(tokens);
             a.lengths_after[r] = length + static_cast<int32_t>(n);
+            // a single workgroup advances the state itself: no other reads it
+            if (a.advance && gridDim.x == 1) const_cast<int32_t*>(a.lengths)[r] = length + static_cast<int32_t>(n);
         }
         __syncthreads();
-        for (uint32_t j = at; j < strip_pages; j += stride) {
-            const uint32_t i = owner(page_first, kPagesThreads, taken + j);
+        for (uint32_t j = at; j < totals[1]; j += stride) {
+            const uint32_t i = owner(page_first, THREADS, taken + j);
             const uint32_t entry = ((static_cast<uint32_t>(lens[i]) + page - 1) >> shift) + taken + j - page_first[i];
             a.tables[static_cast<uint64_t>(r0 + i) * a.max_pages + entry] = a.free_pages[n_free - 1 - (taken + j)];
         }
-        for (uint32_t j = at; j < strip_tokens; j += stride) {
-            const uint32_t t = tokens_before + j, i = owner(token_first, kPagesThreads, t);
+        for (uint32_t j = at; j < totals[0]; j += stride) {
+            const uint32_t t = tokens_before + j, i = owner(token_first, THREADS, t);
             const uint32_t len = lens[i], position = len + t - token_first[i], entry = position >> shift;
             const uint32_t old_pages = (len + page - 1) >> shift;
             const int32_t p = entry < old_pages ? a.tables[static_cast<uint64_t>(r0 + i) * a.max_pages + entry]
@@ -133,8 +143,8 @@ __global__ __launch_bounds__(kPagesThreads) void nz_pages_extend_kernel(nz_pages
             a.requests[t] = static_cast<int32_t>(r0 + i);
             a.contexts[t] = static_cast<int32_t>(position) + 1;
         }
-        tokens_before += strip_tokens;
-        taken += strip_pages;
+        tokens_before += totals[0];
+        taken += totals[1];
         __syncthreads();   // the searches above, before the next strip's sums
     }
     for (uint32_t t = tokens_before + at; t < a.max_tokens; t += stride) {
@@ -146,40 +156,54 @@ __global__ __launch_bounds__(kPagesThreads) void nz_pages_extend_kernel(nz_pages
     if (at == 0) {
         a.starts[a.n_requests] = static_cast<int32_t>(tokens_before);
         a.n_free_after[0] = static_cast<int32_t>(n_free - taken);
+        if (a.advance && gridDim.x == 1) const_cast<int32_t*>(a.n_free)[0] = static_cast<int32_t>(n_free - taken);
     }
-    if (a.advance)
-        advance_state(a.ticket, a.lengths_after, a.n_free_after, const_cast<int32_t*>(a.lengths),
-                      const_cast<int32_t*>(a.n_free), a.n_requests);
 }
 
-__global__ __launch_bounds__(kPagesThreads) void nz_pages_release_kernel(nz_pages_release_args a) {
-    __shared__ uint32_t waves[kPagesWaves];
-    __shared__ uint32_t first[kPagesThreads];
+// Prefix sums over the requests of the pages they give back, then the pages,
+// each found by a search in the sums.
+template <uint32_t THREADS>
+__global__ __launch_bounds__(THREADS) void nz_pages_release_kernel(nz_pages_release_args a) {
+    __shared__ uint32_t waves[1][THREADS / 64];
+    __shared__ uint32_t first[THREADS];
     const uint32_t page = a.page_size, shift = 31 - __clz(page);
-    const uint32_t stride = gridDim.x * kPagesThreads, at = blockIdx.x * kPagesThreads + threadIdx.x;
+    const uint32_t stride = gridDim.x * THREADS, at = blockIdx.x * THREADS + threadIdx.x;
     uint32_t top = min(static_cast<uint32_t>(max(a.n_free[0], 0)), a.n_pages);
-    for (uint32_t r0 = 0; r0 < a.n_requests; r0 += kPagesThreads) {
+    for (uint32_t r0 = 0; r0 < a.n_requests; r0 += THREADS) {
         const uint32_t r = r0 + threadIdx.x;
         const bool live = r < a.n_requests, done = live && a.done[r] != 0;
         const int32_t length = live ? max(a.lengths[r], 0) : 0;
         const uint32_t back = done ? min((static_cast<uint32_t>(length) + page - 1) >> shift, a.max_pages) : 0;
-        uint32_t total;
-        const uint32_t scanned = block_scan(back, waves, &total);
-        first[threadIdx.x] = scanned - back;
-        if (live && blockIdx.x == 0) a.lengths_after[r] = done ? 0 : length;
+        uint32_t sum[1] = {back}, total[1];
+        block_scan<THREADS, 1>(sum, total, waves);
+        first[threadIdx.x] = sum[0] - back;
+        if (live && blockIdx.x == 0) {
+            a.lengths_after[r] = done ? 0 : length;
+            if (a.advance && gridDim.x == 1) const_cast<int32_t*>(a.lengths)[r] = done ? 0 : length;
+        }
         __syncthreads();
-        const uint32_t kept = min(total, a.n_pages - top);
+        const uint32_t kept = min(total[0], a.n_pages - top);
         for (uint32_t j = at; j < kept; j += stride) {
-            const uint32_t i = owner(first, kPagesThreads, j);
+            const uint32_t i = owner(first, THREADS, j);
             a.free_pages[top + j] = a.tables[static_cast<uint64_t>(r0 + i) * a.max_pages + j - first[i]];
         }
         top += kept;
         __syncthreads();
     }
-    if (at == 0) a.n_free_after[0] = static_cast<int32_t>(top);
-    if (a.advance)
-        advance_state(a.ticket, a.lengths_after, a.n_free_after, const_cast<int32_t*>(a.lengths),
-                      const_cast<int32_t*>(a.n_free), a.n_requests);
+    if (at == 0) {
+        a.n_free_after[0] = static_cast<int32_t>(top);
+        if (a.advance && gridDim.x == 1) const_cast<int32_t*>(a.n_free)[0] = static_cast<int32_t>(top);
+    }
+}
+
+// The state after a call of several workgroups, which read the old one until
+// the last of them ends.
+__global__ __launch_bounds__(kPagesThreads) void nz_pages_advance_kernel(const int32_t* __restrict__ lengths_after,
+                                                                         const int32_t* __restrict__ n_free_after,
+                                                                         int32_t* lengths, int32_t* n_free, uint32_t n) {
+    const uint32_t r = blockIdx.x * kPagesThreads + threadIdx.x;
+    if (r < n) lengths[r] = lengths_after[r];
+    if (r == 0) n_free[0] = n_free_after[0];
 }
 
 // ------------------------------------------------- norm, rotation and store
@@ -279,8 +303,8 @@ __global__ __launch_bounds__(kRotaryThreads) void nz_rotary_kernel(nz_rotary_arg
 // -------------------------------------------------------------- the logits
 
 constexpr uint32_t kLogitsThreads = 256;
-// Tokens of the vocabulary that a workgroup counts in LDS.
-constexpr uint32_t kLogitsChunk = 4096;
+// Tokens of the vocabulary that a workgroup takes and counts in LDS.
+constexpr uint32_t kLogitsChunk = 2048;
 
 __device__ __forceinline__ int64_t history_id(const nz_logits_args& a, uint32_t row, uint32_t i) {
     const uint64_t at = static_cast<uint64_t>(row) * static_cast<uint64_t>(a.history_row) + i;
@@ -288,23 +312,49 @@ __device__ __forceinline__ int64_t history_id(const nz_logits_args& a, uint32_t 
                                 : static_cast<int64_t>(static_cast<const int32_t*>(a.history)[at]);
 }
 
-// One workgroup: a row's tokens v0 .. v0 + kLogitsChunk - 1. It counts the
-// row's history that falls into them (answer tokens in the low 31 bits, any
-// token in the top bit), notes each token's last bias entry and then passes
-// over the logits once. Integer LDS atomics only: the order of arrival does
-// not show.
-template <typename T>
+// One workgroup: kLogitsChunk neighbouring tokens of a row, the first on a
+// 16-byte boundary of the row's memory (in the row's first chunk that may lie
+// before the row). It requests its logits, counts the row's history that
+// falls into the chunk meanwhile (answer tokens in the low 31 bits, any token
+// in the top bit) and notes each token's last bias entry, and then adjusts
+// and stores the logits. Integer LDS atomics only: the order of arrival does
+// not show. Every chunk's workgroup reads the row's whole history, out of the
+// L2. VECTOR: logits and out lie alike on 16-byte boundaries.
+template <typename T, bool VECTOR>
 __global__ __launch_bounds__(kLogitsThreads) void nz_logits_kernel(nz_logits_args a) {
+    constexpr uint32_t kRun = VECTOR ? 16 / sizeof(T) : 1, kRuns = kLogitsChunk / (kLogitsThreads * kRun);
+    using run = vec<T, kRun>;
     __shared__ uint32_t counts[kLogitsChunk], entries[kLogitsChunk];
-    const uint32_t row = blockIdx.y, v0 = blockIdx.x * kLogitsChunk, n = min(kLogitsChunk, a.vocab - v0);
-    for (uint32_t i = threadIdx.x; i < kLogitsChunk; i += kLogitsThreads) counts[i] = 0, entries[i] = 0;
+    const uint32_t row = blockIdx.y;
+    const T* const src = static_cast<const T*>(a.logits) + row * a.logits_row;
+    T* const dst = static_cast<T*>(a.out) + row * a.out_row;
+    const uint32_t before = VECTOR ? static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src) % 16 / sizeof(T)) : 0;
+    const int64_t v0 = static_cast<int64_t>(blockIdx.x) * kLogitsChunk - before;
+    if (v0 >= static_cast<int64_t>(a.vocab)) return;
+    // a run inside the row as one access, one at its ends by elements
+    run x[kRuns];
+#pragma unroll
+    for (uint32_t k = 0; k < kRuns; ++k) {
+        const int64_t v = v0 + (k * kLogitsThreads + threadIdx.x) * kRun;
+        if (v >= 0 && v + kRun <= a.vocab) {
+            x[k] = *reinterpret_cast<const run*>(src + v);
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < kRun; ++i)
+                x[k][i] = v + i >= 0 && v + i < a.vocab ? src[v + i] : static_cast<T>(0.0f);
+        }
+    }
+    for (uint32_t i = threadIdx.x; i < kLogitsChunk; i += kLogitsThreads) counts[i] = 0;
+    if (a.bias_starts != nullptr)
+        for (uint32_t i = threadIdx.x; i < kLogitsChunk; i += kLogitsThreads) entries[i] = 0;
     __syncthreads();
     if (a.history != nullptr) {
         const uint32_t length = min(static_cast<uint32_t>(max(a.lengths[row], 0)), a.history_capacity);
         const uint32_t prompt = a.prompt_lengths ? static_cast<uint32_t>(max(a.prompt_lengths[row], 0)) : 0;
+#pragma unroll 4
         for (uint32_t i = threadIdx.x; i < length; i += kLogitsThreads) {
-            const uint64_t v = static_cast<uint64_t>(history_id(a, row, i)) - v0;
-            if (v < n) {
+            const uint64_t v = static_cast<uint64_t>(history_id(a, row, i) - v0);
+            if (v < kLogitsChunk) {
                 atomicOr(&counts[v], 0x80000000u);
                 if (i >= prompt) atomicAdd(&counts[v], 1u);
             }
@@ -314,8 +364,8 @@ __global__ __launch_bounds__(kLogitsThreads) void nz_logits_kernel(nz_logits_arg
         const uint32_t e0 = min(static_cast<uint32_t>(max(a.bias_starts[row], 0)), a.n_bias);
         const uint32_t e1 = min(static_cast<uint32_t>(max(a.bias_starts[row + 1], 0)), a.n_bias);
         for (uint32_t e = e0 + threadIdx.x; e < e1; e += kLogitsThreads) {
-            const uint64_t v = static_cast<uint64_t>(static_cast<int64_t>(a.bias_tokens[e])) - v0;
-            if (v < n) atomicMax(&entries[v], e + 1);
+            const uint64_t v = static_cast<uint64_t>(static_cast<int64_t>(a.bias_tokens[e]) - v0);
+            if (v < kLogitsChunk) atomicMax(&entries[v], e + 1);
         }
     }
     __syncthreads();
@@ -326,19 +376,31 @@ __global__ __launch_bounds__(kLogitsThreads) void nz_logits_kernel(nz_logits_arg
         const int64_t m = a.mask_rows ? a.mask_rows[row] : static_cast<int64_t>(row);
         if (static_cast<uint64_t>(m) < a.n_masks) mask = a.masks + static_cast<uint64_t>(m) * ((a.vocab + 31) / 32);
     }
-    const T* src = static_cast<const T*>(a.logits) + row * a.logits_row + v0;
-    T* dst = static_cast<T*>(a.out) + row * a.out_row + v0;
-    for (uint32_t i = threadIdx.x; i < n; i += kLogitsThreads) {
-        float x = to_float(src[i]);
-        const uint32_t count = counts[i], entry = entries[i];
-        if (count) {
-            x = x > 0.0f ? x / repetition : x * repetition;
-            const uint32_t answers = count & 0x7FFFFFFFu;
-            if (answers) x = x - frequency * static_cast<float>(answers) - presence;
+#pragma unroll
+    for (uint32_t k = 0; k < kRuns; ++k) {
+        const uint32_t at = (k * kLogitsThreads + threadIdx.x) * kRun;
+        const int64_t v = v0 + at;
+#pragma unroll
+        for (uint32_t i = 0; i < kRun; ++i) {
+            float y = to_float(static_cast<T>(x[k][i]));
+            const uint32_t count = counts[at + i], entry = a.bias_starts != nullptr ? entries[at + i] : 0;
+            if (count) {
+                y = y > 0.0f ? y / repetition : y * repetition;
+                const uint32_t answers = count & 0x7FFFFFFFu;
+                if (answers) y = y - frequency * static_cast<float>(answers) - presence;
+            }
+            if (entry) y += a.bias_values[entry - 1];
+            if (mask && v + i >= 0 && v + i < a.vocab && !((mask[(v + i) >> 5] >> ((v + i) & 31)) & 1u))
+                y = -__builtin_inff();
+            x[k][i] = from_float<T>(y);
         }
-        if (entry) x += a.bias_values[entry - 1];
-        if (mask && !((mask[(v0 + i) >> 5] >> ((v0 + i) & 31)) & 1u)) x = -__builtin_inff();
-        dst[i] = from_float<T>(x);
+        if (v >= 0 && v + kRun <= a.vocab) {
+            *reinterpret_cast<run*>(dst + v) = x[k];
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < kRun; ++i)
+                if (v + i >= 0 && v + i < a.vocab) dst[v + i] = x[k][i];
+        }
     }
 }
 
@@ -370,15 +432,34 @@ void launch_rotary(const nz_rotary_args& a, hipStream_t stream) {
 
 // The callers (capi_serving.cpp) have checked the arguments.
 
+// `work` tokens or pages by workgroups of 64, 256 or 1024 threads, several
+// where one would write more than kPagesShare; then the state's advance.
+#define NZ_PAGES(kernel, work)                                                                                    \
+    const hipStream_t st = static_cast<hipStream_t>(stream);                                                      \
+    const uint64_t amount = (work);                                                                               \
+    const uint32_t groups = amount <= kPagesShare                                                                 \
+                                ? 1 : static_cast<uint32_t>(std::min<uint64_t>((amount + 1023) / 1024, kPagesGroups)); \
+    if (groups == 1 && args->n_requests <= 64 && amount <= 128)                                                   \
+        hipLaunchKernelGGL(kernel<64>, dim3(1), dim3(64), 0, st, *args);                                          \
+    else if (groups == 1 && args->n_requests <= 256 && amount <= 1024)                                            \
+        hipLaunchKernelGGL(kernel<256>, dim3(1), dim3(256), 0, st, *args);                                        \
+    else                                                                                                          \
+        hipLaunchKernelGGL(kernel<kPagesThreads>, dim3(groups), dim3(kPagesThreads), 0, st, *args);               \
+    if (args->advance && groups > 1)                                                                              \
+        hipLaunchKernelGGL(nz_pages_advance_kernel, dim3((args->n_requests + kPagesThreads) / kPagesThreads),     \
+                           dim3(kPagesThreads), 0, st, args->lengths_after, args->n_free_after,                   \
+                           const_cast<int32_t*>(args->lengths), const_cast<int32_t*>(args->n_free), args->n_requests)
+
 extern "C" int nz_hip_pages_extend(const nz_pages_extend_args* args, void* stream, char* message, size_t message_size) {
-    hipLaunchKernelGGL(nz_pages_extend_kernel, dim3(1), dim3(kPagesThreads), 0, static_cast<hipStream_t>(stream), *args);
+    NZ_PAGES(nz_pages_extend_kernel, args->max_tokens);
     return launched("pages extend", message, message_size);
 }
 
 extern "C" int nz_hip_pages_release(const nz_pages_release_args* args, void* stream, char* message,
                                     size_t message_size) {
-    hipLaunchKernelGGL(nz_pages_release_kernel, dim3(1), dim3(kPagesThreads), 0, static_cast<hipStream_t>(stream),
-                       *args);
+    // no more pages come back than there are, or than the tables hold
+    NZ_PAGES(nz_pages_release_kernel,
+             std::min<uint64_t>(args->n_pages, static_cast<uint64_t>(args->n_requests) * args->max_pages));
     return launched("pages release", message, message_size);
 }
 
@@ -392,9 +473,20 @@ extern "C" int nz_hip_rotary_store(const nz_rotary_args* args, void* stream, cha
 
 extern "C" int nz_hip_adjust_logits(const nz_logits_args* args, void* stream, char* message, size_t message_size) {
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const dim3 grid((args->vocab + kLogitsChunk - 1) / kLogitsChunk, args->rows), block(kLogitsThreads);
-    if (args->type == NZ_BF16) hipLaunchKernelGGL(nz_logits_kernel<bf16_t>, grid, block, 0, st, *args);
-    else if (args->type == NZ_FP16) hipLaunchKernelGGL(nz_logits_kernel<_Float16>, grid, block, 0, st, *args);
-    else hipLaunchKernelGGL(nz_logits_kernel<float>, grid, block, 0, st, *args);
+    // every row of the two must start alike on 16-byte boundaries; one more
+    // chunk holds what the first one's tokens before the row push out
+    const uint32_t size = args->type == NZ_FP32 ? 4 : 2;
+    const bool vector = (reinterpret_cast<uintptr_t>(args->logits) - reinterpret_cast<uintptr_t>(args->out)) % 16 == 0 &&
+                        (args->rows == 1 || (args->logits_row - args->out_row) * size % 16 == 0);
+    const dim3 grid((args->vocab + 16 / size - 1 + kLogitsChunk - 1) / kLogitsChunk, args->rows), block(kLogitsThreads);
+#define NZ_LOGITS(T)                                                                                   \
+    do {                                                                                               \
+        if (vector) hipLaunchKernelGGL((nz_logits_kernel<T, true>), grid, block, 0, st, *args);        \
+        else hipLaunchKernelGGL((nz_logits_kernel<T, false>), grid, block, 0, st, *args);              \
+    } while (0)
+    if (args->type == NZ_BF16) NZ_LOGITS(bf16_t);
+    else if (args->type == NZ_FP16) NZ_LOGITS(_Float16);
+    else NZ_LOGITS(float);
+#undef NZ_LOGITS
     return launched("logits", message, message_size);
 }

@@ -124,7 +124,6 @@ class PageTables:
         self.tables = torch.full((requests, max_pages), -1, dtype=torch.int32, device=device)
         self.free = torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=device)
         self.n_free = torch.full((1,), num_pages, dtype=torch.int32, device=device)
-        self._ticket = torch.zeros(1, dtype=torch.int32, device=device)
 
     def extend(self, new_tokens, max_tokens, *, advance=True, out=None, stream=None):
         """Gives every request its `new_tokens` (int32, one per request) new
@@ -149,7 +148,7 @@ class PageTables:
             self.lengths.data_ptr(), new_tokens.data_ptr(), self.tables.data_ptr(), self.free.data_ptr(),
             self.n_free.data_ptr(), out.slots.data_ptr(), out.positions.data_ptr(), out.requests.data_ptr(),
             out.contexts.data_ptr(), out.starts.data_ptr(), out.status.data_ptr(), out.lengths.data_ptr(),
-            out.n_free.data_ptr(), self._ticket.data_ptr(), self.requests, self.max_pages, self.page_size,
+            out.n_free.data_ptr(), self.requests, self.max_pages, self.page_size,
             self.num_pages, max_tokens, bool(advance))
         _call(_native.lib().nz_pages_extend, self.device, args, stream)
         return out
@@ -163,8 +162,8 @@ class PageTables:
             out = Released(self.requests, self.device)
         args = _native.PAGES_RELEASE.pack(
             self.lengths.data_ptr(), done.data_ptr(), self.tables.data_ptr(), self.free.data_ptr(),
-            self.n_free.data_ptr(), out.lengths.data_ptr(), out.n_free.data_ptr(), self._ticket.data_ptr(),
-            self.requests, self.max_pages, self.page_size, self.num_pages, bool(advance), 0)
+            self.n_free.data_ptr(), out.lengths.data_ptr(), out.n_free.data_ptr(), self.requests, self.max_pages,
+            self.page_size, self.num_pages, bool(advance), 0)
         _call(_native.lib().nz_pages_release, self.device, args, stream)
         return out
 

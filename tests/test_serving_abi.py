@@ -72,9 +72,9 @@ def packed(name, **values):
 
 EXTEND = dict(lengths=True, new_tokens=True, tables=True, free_pages=True, n_free=True, slots=True, positions=True,
               requests=True, contexts=True, starts=True, status=True, lengths_after=True, n_free_after=True,
-              ticket=True, n_requests=4, max_pages=8, page_size=16, n_pages=32, max_tokens=4)
+              n_requests=4, max_pages=8, page_size=16, n_pages=32, max_tokens=4)
 RELEASE = dict(lengths=True, done=True, tables=True, free_pages=True, n_free=True, lengths_after=True,
-               n_free_after=True, ticket=True, n_requests=4, max_pages=8, page_size=16, n_pages=32)
+               n_free_after=True, n_requests=4, max_pages=8, page_size=16, n_pages=32)
 ROTARY = dict(q=True, k=True, v=True, out=True, key_cache=True, value_cache=True, cos=True, sin=True, positions=True,
               slots=True, q_token=128, q_head=64, k_token=128, k_head=64, v_token=128, v_head=64, out_token=128,
               out_head=64, key_page=2048, key_head=1024, key_slot=64, value_page=2048, value_head=1024, value_slot=64,
