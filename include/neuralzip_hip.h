@@ -645,10 +645,11 @@ typedef struct nz_attention_item {
  * most n items, as short as that allows but of at least 128 keys (512 from
  * contexts of 8192 on; except for a row's last); or at most n + target, where
  * the longest would else be more than half longer than the n-th part of all
- * keys and than half their target-th part. The rest are marked unused. The
- * plan serves the attention of every layer of a step. */
+ * keys and than half their target-th part. The rest are marked unused.
+ * `counters` has room for as many entries times `parts`, kv_heads * ceil(heads
+ * / kv_heads / 16). The plan serves the attention of every layer of a step. */
 int nz_attention_plan(const int32_t* contexts, const int32_t* requests, uint32_t n_rows, uint32_t target,
-                      nz_attention_item* items, void* stream);
+                      uint32_t parts, nz_attention_item* items, uint32_t* counters, void* stream);
 
 typedef struct nz_attention_args {
     const void* q;               /* n_rows x heads x head_dim                */
@@ -657,6 +658,7 @@ typedef struct nz_attention_args {
     void* out;                   /* n_rows x heads x head_dim                */
     const int32_t* tables;       /* n_requests x max_pages                   */
     const nz_attention_item* items;
+    uint32_t* counters;          /* the plan's                               */
     float* partials;             /* nz_attention_partials(...) words         */
     int64_t q_row, q_head, out_row, out_head;
     int64_t key_page, key_head, key_slot, value_page, value_head, value_slot;
@@ -674,17 +676,16 @@ typedef struct nz_attention_args {
     uint32_t reserved;           /* 0 */
 } nz_attention_args;
 
-/* 32-bit words of scratch that nz_attention needs for a plan of n_items:
- * zero before the first call (a fill kernel's work; each call leaves the
- * words that need it zero), 16-byte aligned. */
+/* 32-bit words of scratch that nz_attention needs for a plan of n_items. */
 uint64_t nz_attention_partials(uint32_t n_items, uint32_t heads, uint32_t head_dim);
 
 /* out[row] = softmax(scale * q[row] . keys) values, over the row's context in
  * its request's pages; head h reads key-value head h / (heads / kv_heads). A
  * row without keys gives zeros. Keys whose page or request is not in range
  * count as masked. head_dim is a multiple of 16, at most 256; strides and
- * addresses are multiples of 16 bytes. Two calls that may overlap need their
- * own partials; n_items * heads * head_dim is below 2^30. */
+ * addresses are multiples of 16 bytes. Calls with one plan must not
+ * overlap: they share its counters, which each call leaves as it found them.
+ * n_items * heads * head_dim is below 2^30. */
 int nz_attention(const nz_attention_args* args, void* stream);
 
 typedef struct nz_logits_args {

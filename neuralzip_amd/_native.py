@@ -89,7 +89,7 @@ class _Totals(ctypes.Structure):
 PAGES_EXTEND = struct.Struct("=13Q6I")
 PAGES_RELEASE = struct.Struct("=7Q6I")
 ROTARY = struct.Struct("=12Q14q11If")
-ATTENTION = struct.Struct("=7Q10q10IfI")
+ATTENTION = struct.Struct("=8Q10q10IfI")
 LOGITS = struct.Struct("=13Q3q8I")
 ATTENTION_ITEM = np.dtype([(name, "<i4") for name in ("row", "request", "begin", "end", "index", "count", "first",
                                                       "reserved")])
@@ -158,7 +158,7 @@ def lib():
         L.nz_clusterer_count.argtypes = [vp, ctypes.POINTER(u32)]
         for name in ("nz_pages_extend", "nz_pages_release", "nz_rotary_store", "nz_attention", "nz_adjust_logits"):
             getattr(L, name).argtypes = [ctypes.c_char_p, vp]
-        L.nz_attention_plan.argtypes = [vp, vp, u32, u32, vp, vp]
+        L.nz_attention_plan.argtypes = [vp, vp, u32, u32, u32, vp, vp, vp]
         L.nz_attention_partials.argtypes = [u32, u32, u32]
         L.nz_attention_partials.restype = u64
         _lib = L

@@ -15,7 +15,8 @@ extern "C" int nz_hip_pages_release(const nz_pages_release_args* args, void* str
                                     size_t message_size);
 extern "C" int nz_hip_rotary_store(const nz_rotary_args* args, void* stream, char* message, size_t message_size);
 extern "C" int nz_hip_attention_plan(const int32_t* contexts, const int32_t* requests, uint32_t n_rows, uint32_t target,
-                                     nz_attention_item* items, void* stream, char* message, size_t message_size);
+                                     uint32_t parts, nz_attention_item* items, uint32_t* counters, void* stream,
+                                     char* message, size_t message_size);
 extern "C" int nz_hip_attention(const nz_attention_args* args, void* stream, char* message, size_t message_size);
 extern "C" int nz_hip_adjust_logits(const nz_logits_args* args, void* stream, char* message, size_t message_size);
 
@@ -123,22 +124,21 @@ int nz_rotary_store(const nz_rotary_args* args, void* stream) {
 }
 
 int nz_attention_plan(const int32_t* contexts, const int32_t* requests, uint32_t n_rows, uint32_t target,
-                      nz_attention_item* items, void* stream) {
+                      uint32_t parts, nz_attention_item* items, uint32_t* counters, void* stream) {
     const int bad = guarded([&] {
-        if (!items || (!contexts && n_rows)) refuse("Null attention plan argument.");
-        if (target == 0 || target > kMaxGrid / 2 || n_rows > kMaxGrid / 2)
-            refuse("The plan's target must be positive, and rows and target below 2^30.");
+        if (!items || !counters || (!contexts && n_rows)) refuse("Null attention plan argument.");
+        if (target == 0 || target > kMaxGrid / 4 || n_rows > kMaxGrid / 4 || parts == 0)
+            refuse("The plan's target and parts must be positive, and rows and target below 2^29.");
     });
     if (bad) return bad;
     char message[256] = {0};
-    const int rc = nz_hip_attention_plan(contexts, requests, n_rows, target, items, stream, message, sizeof message);
+    const int rc = nz_hip_attention_plan(contexts, requests, n_rows, target, parts, items, counters, stream, message,
+                                         sizeof message);
     return rc ? set_error(rc, message) : 0;
 }
 
 uint64_t nz_attention_partials(uint32_t n_items, uint32_t heads, uint32_t head_dim) {
-    // a counter, the sums, their maximum and weight per item and head (hip/attention_gfx950.hip)
-    const uint64_t slots = static_cast<uint64_t>(n_items) * heads;
-    return (slots + 3) / 4 * 4 + slots * (head_dim + 2ull);
+    return static_cast<uint64_t>(n_items) * heads * (head_dim + 2ull);
 }
 
 int nz_attention(const nz_attention_args* args, void* stream) {
@@ -149,7 +149,7 @@ int nz_attention(const nz_attention_args* args, void* stream) {
             refuse("heads must be a positive multiple of kv_heads.");
         if (a.reserved) refuse("reserved is 0.");
         if (a.n_rows == 0) return true;
-        if (!a.q || !a.key_cache || !a.value_cache || !a.out || !a.tables || !a.items || !a.partials)
+        if (!a.q || !a.key_cache || !a.value_cache || !a.out || !a.tables || !a.items || !a.counters || !a.partials)
             refuse("Null attention argument.");
         check_pages(a.n_requests, a.max_pages, a.page_size, a.n_pages);
         if (a.n_pages == 0 || a.n_requests == 0) refuse("There must be pages and requests.");

@@ -71,8 +71,9 @@ __device__ uint32_t shortest_share(const int32_t* contexts, uint32_t n_rows, uin
 // join; twice as many where some rows are much longer than others.
 __global__ __launch_bounds__(kPlanThreads) void nz_attention_plan_kernel(const int32_t* __restrict__ contexts,
                                                                          const int32_t* __restrict__ requests,
-                                                                         uint32_t n_rows, uint32_t target,
-                                                                         nz_attention_item* __restrict__ items) {
+                                                                         uint32_t n_rows, uint32_t target, uint32_t parts,
+                                                                         nz_attention_item* __restrict__ items,
+                                                                         uint32_t* __restrict__ counters) {
     __shared__ PlanLds lds;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint64_t keys = 0;
@@ -143,6 +144,7 @@ __global__ __launch_bounds__(kPlanThreads) void nz_attention_plan_kernel(const i
     }
     const nz_attention_item none = {-1, -1, 0, 0, 0, 0, 0, 0};
     for (uint32_t i = first + threadIdx.x; i < fewest + target; i += kPlanThreads) items[i] = none;
+    for (uint64_t i = threadIdx.x; i < static_cast<uint64_t>(first) * parts; i += kPlanThreads) counters[i] = 0;
 }
 
 // -------------------------------------------------------------- attention
@@ -251,15 +253,6 @@ __device__ __forceinline__ void put_pair(rsrc_t buffer, uint32_t offset, float x
 
 __device__ __forceinline__ vec<float, 2> get_pair(rsrc_t buffer, uint32_t offset) {
     return __builtin_bit_cast(vec<float, 2>, __builtin_amdgcn_raw_buffer_load_b64(buffer, offset, 0, kDeviceScope));
-}
-
-// The scratch: a counter per item and head, which is 0 between calls, then
-// the items' sums, then their maxima and weights (32-bit words).
-__device__ __forceinline__ uint64_t partials_sums(uint64_t n_items, uint64_t heads) {
-    return (n_items * heads + 3) / 4 * 4;
-}
-__device__ __forceinline__ uint64_t sums_words(uint64_t n_items, uint64_t heads, uint64_t head_dim) {
-    return n_items * heads * head_dim;
 }
 
 template <typename T, uint32_t DP>
@@ -470,9 +463,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 
     // and with their maximum and weight, a part of it.
     const bool whole = item.count == 1;
     const uint64_t slot0 = static_cast<uint64_t>(item.first) * a.heads + head0;
-    float* const sums = a.partials + partials_sums(a.n_items, a.heads);
-    const rsrc_t part_o = device_buffer(sums + slot0 * a.head_dim);
-    const rsrc_t part_ml = device_buffer(sums + sums_words(a.n_items, a.heads, a.head_dim) + 2 * slot0);
+    // the scratch: every item's and head's sums, then their maxima and weights
+    const rsrc_t part_o = device_buffer(a.partials + slot0 * a.head_dim);
+    const rsrc_t part_ml =
+        device_buffer(a.partials + static_cast<uint64_t>(a.n_items) * a.heads * a.head_dim + 2 * slot0);
     const uint32_t step = a.heads;   // of an item's heads among the slots
     T* const out = static_cast<T*>(a.out) + item.row * a.out_row + head0 * a.out_head;
     const uint32_t quads = a.head_dim / 4;   // runs of 4 elements of a head
@@ -500,7 +494,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 
     }
     if (whole) return;
     // The last of the row's items to arrive joins them all, in their order.
-    uint32_t* const counter = reinterpret_cast<uint32_t*>(a.partials) + static_cast<uint64_t>(item.first) * per_item + part;
+    uint32_t* const counter = a.counters + static_cast<uint64_t>(item.first) * per_item + part;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wavefront's stores have arrived
     __syncthreads();
     if (threadIdx.x == 0)
@@ -598,9 +592,10 @@ int launched(const char* what, char* message, size_t message_size) {
 // The callers (capi_serving.cpp) have checked the arguments.
 
 extern "C" int nz_hip_attention_plan(const int32_t* contexts, const int32_t* requests, uint32_t n_rows, uint32_t target,
-                                     nz_attention_item* items, void* stream, char* message, size_t message_size) {
+                                     uint32_t parts, nz_attention_item* items, uint32_t* counters, void* stream,
+                                     char* message, size_t message_size) {
     hipLaunchKernelGGL(nz_attention_plan_kernel, dim3(1), dim3(kPlanThreads), 0, static_cast<hipStream_t>(stream),
-                       contexts, requests, n_rows, target, items);
+                       contexts, requests, n_rows, target, parts, items, counters);
     return launched("attention plan", message, message_size);
 }
 

@@ -302,9 +302,9 @@ __global__ __launch_bounds__(kRotaryThreads) void nz_rotary_kernel(nz_rotary_arg
 
 // -------------------------------------------------------------- the logits
 
-constexpr uint32_t kLogitsThreads = 256;
+constexpr uint32_t kLogitsThreads = 1024;
 // Tokens of the vocabulary that a workgroup takes and counts in LDS.
-constexpr uint32_t kLogitsChunk = 2048;
+constexpr uint32_t kLogitsChunk = 8192;
 
 __device__ __forceinline__ int64_t history_id(const nz_logits_args& a, uint32_t row, uint32_t i) {
     const uint64_t at = static_cast<uint64_t>(row) * static_cast<uint64_t>(a.history_row) + i;
@@ -315,8 +315,8 @@ __device__ __forceinline__ int64_t history_id(const nz_logits_args& a, uint32_t 
 // One workgroup: kLogitsChunk neighbouring tokens of a row, the first on a
 // 16-byte boundary of the row's memory (in the row's first chunk that may lie
 // before the row). It requests its logits, counts the row's history that
-// falls into the chunk meanwhile (answer tokens in the low 31 bits, any token
-// in the top bit) and notes each token's last bias entry, and then adjusts
+// falls into the chunk meanwhile (answer tokens in the low 31 bits, a prompt
+// token in the top bit) and notes each token's last bias entry, and then adjusts
 // and stores the logits. Integer LDS atomics only: the order of arrival does
 // not show. Every chunk's workgroup reads the row's whole history, out of the
 // L2. VECTOR: logits and out lie alike on 16-byte boundaries.
@@ -355,8 +355,8 @@ __global__ __launch_bounds__(kLogitsThreads) void nz_logits_kernel(nz_logits_arg
         for (uint32_t i = threadIdx.x; i < length; i += kLogitsThreads) {
             const uint64_t v = static_cast<uint64_t>(history_id(a, row, i) - v0);
             if (v < kLogitsChunk) {
-                atomicOr(&counts[v], 0x80000000u);
-                if (i >= prompt) atomicAdd(&counts[v], 1u);
+                if (i < prompt) atomicOr(&counts[v], 0x80000000u);
+                else atomicAdd(&counts[v], 1u);
             }
         }
     }

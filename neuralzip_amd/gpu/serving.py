@@ -55,22 +55,24 @@ def _refuse_gradients(*tensors):
 
 
 def _check_vector(name, t, dtype, n, device):
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or t.device != device or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != (n,) or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} vector of {n} on {device}; "
                          f"got {t.dtype} {tuple(t.shape)} on {t.device}.")
 
 
-def _pool_strides(keys, values, kv_heads, head_dim, dtype, device):
-    """Strides of a layer's two caches, (pages, kv_heads, page_size, head_dim)."""
-    if keys.dim() != 4 or keys.shape != values.shape or keys.shape[1] != kv_heads or keys.shape[3] != head_dim:
+def _pool_layout(keys, values, kv_heads, head_dim, dtype, device):
+    """Strides of a layer's two caches, (pages, kv_heads, page size, head_dim),
+    their pages and page size."""
+    shape = keys.shape
+    if len(shape) != 4 or shape != values.shape or shape[1] != kv_heads or shape[3] != head_dim:
         raise ValueError(f"Caches must both be (pages, {kv_heads}, page size, {head_dim}); "
                          f"got {tuple(keys.shape)} and {tuple(values.shape)}.")
-    if keys.dtype != dtype or values.dtype != dtype or keys.device != device or values.device != device:
+    if keys.dtype is not dtype or values.dtype is not dtype or keys.device != device or values.device != device:
         raise ValueError("Caches must have the queries' dtype and device.")
     ks, vs = keys.stride(), values.stride()
     if ks[3] != 1 or vs[3] != 1:
         raise ValueError("A head's elements must be contiguous in the caches.")
-    return ks, vs
+    return ks[:3] + vs[:3], shape[0], shape[2]
 
 
 class Step:
@@ -191,6 +193,7 @@ class Rotary:
                 raise ValueError("Norm weights must be contiguous vectors on cos's device.")
         self.cos, self.sin, self.q_weight, self.k_weight = cos, sin, q_weight, k_weight
         self.rotary_dim, self.interleaved, self.eps = 2 * cos.shape[1], bool(interleaved), float(eps)
+        self._device, self._positions = cos.device, cos.shape[0]
         self._weight_type = _TYPES[weights[0].dtype] if weights else None
         self._weight_dim = weights[0].shape[0] if weights else None
         self._tables = (cos.data_ptr(), sin.data_ptr(), q_weight.data_ptr() if q_weight is not None else 0,
@@ -206,49 +209,47 @@ class Rotary:
         32 bits and rounded once. Tokens' slots must differ. A slot outside
         the caches stores nothing, a position outside the tables gives NaN."""
         _refuse_gradients(q, k, v, self.q_weight, self.k_weight)
-        dtype, device = q.dtype, q.device
-        if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape:
+        dtype, device, shape, kv_shape = q.dtype, q.device, q.shape, k.shape
+        if len(shape) != 3 or len(kv_shape) != 3 or kv_shape != v.shape:
             raise ValueError("q, k and v must be (tokens, heads, head_dim), k and v alike.")
-        tokens, heads, dim = q.shape
-        kv_heads = k.shape[1]
-        if dtype not in _TYPES or k.shape[0] != tokens or k.shape[2] != dim or self.rotary_dim > dim:
-            raise ValueError(f"q {tuple(q.shape)} {dtype} and k {tuple(k.shape)} do not fit one another or the "
+        tokens, heads, dim = shape
+        kv_heads, kind = kv_shape[1], _TYPES.get(dtype)
+        if kind is None or kv_shape[0] != tokens or kv_shape[2] != dim or self.rotary_dim > dim:
+            raise ValueError(f"q {tuple(shape)} {dtype} and k {tuple(kv_shape)} do not fit one another or the "
                              f"rotation of {self.rotary_dim} elements.")
-        if k.dtype != dtype or v.dtype != dtype or k.device != device or v.device != device or device != self.cos.device:
+        if k.dtype is not dtype or v.dtype is not dtype or k.device != device or v.device != device \
+                or device != self._device:
             raise ValueError("q, k, v and the tables must match in dtype and device.")
-        if self._weight_dim is not None and (self._weight_dim != dim or self._weight_type not in
-                                             (_TYPES[dtype], _native.VALUE_FP32)):
+        weight_type = self._weight_type
+        if weight_type is None:
+            weight_type = kind
+        elif self._weight_dim != dim or weight_type not in (kind, _native.VALUE_FP32):
             raise ValueError("Norm weights must be head_dim values of q's dtype or float32.")
         _check_vector("positions", positions, torch.int32, tokens, device)
         qs, ks, vs = q.stride(), k.stride(), v.stride()
         if qs[2] != 1 or ks[2] != 1 or vs[2] != 1:
             raise ValueError("A head's elements must be contiguous.")
-        if (key_cache is None) != (value_cache is None) or (key_cache is None) != (slots is None):
+        if key_cache is None and value_cache is None and slots is None:
+            pool, key_ptr, value_ptr, slots_ptr, page_size, pages = (0, 0, 0, 0, 0, 0), 0, 0, 0, 0, 0
+        elif key_cache is None or value_cache is None or slots is None:
             raise ValueError("The two caches and the slots go together.")
-        if key_cache is None:
-            pool = (0, 0, 0, 0, 0, 0)
-            key_ptr = value_ptr = slots_ptr = page_size = pages = 0
         else:
             _check_vector("slots", slots, torch.int64, tokens, device)
-            c, d = _pool_strides(key_cache, value_cache, kv_heads, dim, dtype, device)
-            pool = (c[0], c[1], c[2], d[0], d[1], d[2])
+            pool, pages, page_size = _pool_layout(key_cache, value_cache, kv_heads, dim, dtype, device)
             key_ptr, value_ptr, slots_ptr = key_cache.data_ptr(), value_cache.data_ptr(), slots.data_ptr()
-            pages, page_size = key_cache.shape[0], key_cache.shape[2]
         if out is None:
             with _on(stream):
-                out = torch.empty((tokens, heads, dim), dtype=dtype, device=device)
+                out = torch.empty_like(q, memory_format=torch.contiguous_format)
             os = (heads * dim, dim, 1)
         else:
             os = out.stride()
-            if out.shape != q.shape or out.dtype != dtype or out.device != device or os[2] != 1:
+            if out.shape != shape or out.dtype is not dtype or out.device != device or os[2] != 1:
                 raise ValueError("`out` must be like q, with contiguous heads.")
-        cos_ptr, sin_ptr, qw_ptr, kw_ptr = self._tables
-        kind = _TYPES[dtype]
         args = _native.ROTARY.pack(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), key_ptr, value_ptr, cos_ptr, sin_ptr, qw_ptr,
-            kw_ptr, positions.data_ptr(), slots_ptr, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1], *pool,
-            tokens, heads, kv_heads, dim, self.rotary_dim, self.interleaved, page_size, pages, self.cos.shape[0], kind,
-            kind if self._weight_type is None else self._weight_type, self.eps)
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), key_ptr, value_ptr, *self._tables,
+            positions.data_ptr(), slots_ptr, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1], *pool,
+            tokens, heads, kv_heads, dim, self.rotary_dim, self.interleaved, page_size, pages, self._positions, kind,
+            weight_type, self.eps)
         _call(_native.lib().nz_rotary_store, device, args, stream)
         return out
 
@@ -259,8 +260,8 @@ class AttentionPlan:
     heads over `kv_heads`. Row i belongs to request requests[i] (int32), or
     to request i. Made on the device, so it follows lengths that the host
     does not know; update() makes it anew in the same memory, also inside a
-    captured graph. One plan serves all layers of the step. It keeps their
-    scratch too, per stream: calls with one plan on one stream share it."""
+    captured graph. One plan serves all layers of the step, whose calls run
+    one after another, on one stream or ordered by events."""
 
     def __init__(self, contexts, *, heads, kv_heads, requests=None, stream=None):
         if kv_heads < 1 or heads < 1 or heads % kv_heads:
@@ -268,32 +269,40 @@ class AttentionPlan:
         if contexts.dim() != 1 or contexts.dtype != torch.int32 or not contexts.is_cuda:
             raise ValueError("contexts must be an int32 vector on the GPU.")
         self.rows, self.heads, self.kv_heads, self.device = contexts.shape[0], heads, kv_heads, contexts.device
-        per_item = kv_heads * -(-(heads // kv_heads) // _HEADS)
-        self._target = max(1, ATTENTION_WORKGROUPS // per_item)
+        self._parts = kv_heads * -(-(heads // kv_heads) // _HEADS)
+        self._target = max(1, ATTENTION_WORKGROUPS // self._parts)
         self.capacity = (max(1, -(-self.rows // self._target)) + 1) * self._target
         with _on(stream):
-            self.items = torch.empty((self.capacity, 8), dtype=torch.int32, device=self.device)
-        self._scratch = {}
+            words = torch.empty(self.capacity * (8 + self._parts), dtype=torch.int32, device=self.device)
+        items, self._counters = words.split((8 * self.capacity, self.capacity * self._parts))
+        self.items = items.view(self.capacity, 8)
+        self._pointers = items.data_ptr(), self._counters.data_ptr()
+        self._stream, self._scratch = _stream_handle(self.device, stream), {}
         self.update(contexts, requests=requests, stream=stream)
 
     def update(self, contexts, *, requests=None, stream=None):
+        """Plans the same number of rows anew."""
         _check_vector("contexts", contexts, torch.int32, self.rows, self.device)
         if requests is not None:
             _check_vector("requests", requests, torch.int32, self.rows, self.device)
         rc = _native.lib().nz_attention_plan(contexts.data_ptr(), requests.data_ptr() if requests is not None else None,
-                                             self.rows, self._target, self.items.data_ptr(),
+                                             self.rows, self._target, self._parts, *self._pointers,
                                              _stream_handle(self.device, stream))
         if rc:
             _native.check(rc)
         return self
 
     def _partials(self, head_dim, handle, stream):
-        words = _native.lib().nz_attention_partials(self.capacity, self.heads, head_dim)
-        scratch = self._scratch.get(handle)
-        if scratch is None or scratch.numel() < words:
+        """Address of the scratch for calls of `head_dim` on one stream."""
+        scratch = self._scratch.get((handle, head_dim))
+        if scratch is None:
+            words = _native.lib().nz_attention_partials(self.capacity, self.heads, head_dim)
             with _on(stream):
-                scratch = self._scratch[handle] = torch.zeros(words, dtype=torch.float32, device=self.device)
-        return scratch
+                scratch = torch.empty(words, dtype=torch.float32, device=self.device)
+                if handle != self._stream:   # the plan's memory must outlive what runs there
+                    self.items.record_stream(torch.cuda.current_stream(self.device))
+            self._scratch[handle, head_dim] = scratch
+        return scratch.data_ptr()
 
 
 def paged_attention(q, key_cache, value_cache, tables, plan, *, scale=None, out=None, stream=None):
@@ -307,34 +316,35 @@ def paged_attention(q, key_cache, value_cache, tables, plan, *, scale=None, out=
     decides. head_dim is a multiple of 16 up to 256; strides may be any that
     keep heads, tokens and pages on 16-byte boundaries."""
     _refuse_gradients(q, key_cache, value_cache)
-    dtype, device = q.dtype, q.device
-    if q.dim() != 3 or q.shape[0] != plan.rows or q.shape[1] != plan.heads or dtype not in _TYPES:
+    dtype, device, shape = q.dtype, q.device, q.shape
+    kind = _TYPES.get(dtype)
+    if len(shape) != 3 or shape[0] != plan.rows or shape[1] != plan.heads or kind is None:
         raise ValueError(f"q must be ({plan.rows}, {plan.heads}, head_dim) in bfloat16, float16 or float32; "
-                         f"got {tuple(q.shape)} {dtype}.")
-    rows, heads, dim = q.shape
+                         f"got {tuple(shape)} {dtype}.")
+    rows, heads, dim = shape
     if device != plan.device or tables.device != device:
         raise ValueError("q, the tables and the plan must be on one device.")
-    if tables.dim() != 2 or tables.dtype != torch.int32 or not tables.is_contiguous():
+    table_shape = tables.shape
+    if len(table_shape) != 2 or tables.dtype is not torch.int32 or not tables.is_contiguous():
         raise ValueError("tables must be a contiguous int32 (requests, max_pages).")
-    ks, vs = _pool_strides(key_cache, value_cache, plan.kv_heads, dim, dtype, device)
+    pool, pages, page_size = _pool_layout(key_cache, value_cache, plan.kv_heads, dim, dtype, device)
     qs = q.stride()
     if out is None:
         with _on(stream):
-            out = torch.empty((rows, heads, dim), dtype=dtype, device=device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         os = (heads * dim, dim, 1)
     else:
         os = out.stride()
-        if out.shape != q.shape or out.dtype != dtype or out.device != device:
+        if out.shape != shape or out.dtype is not dtype or out.device != device:
             raise ValueError("`out` must be like q.")
     if qs[2] != 1 or os[2] != 1:
         raise ValueError("A head's elements must be contiguous.")
     handle = _stream_handle(device, stream)
-    partials = plan._partials(dim, handle, stream)
     args = _native.ATTENTION.pack(
         q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), out.data_ptr(), tables.data_ptr(),
-        plan.items.data_ptr(), partials.data_ptr(), qs[0], qs[1], os[0], os[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-        rows, plan.capacity, heads, plan.kv_heads, dim, tables.shape[0], tables.shape[1], key_cache.shape[2],
-        key_cache.shape[0], _TYPES[dtype], dim ** -0.5 if scale is None else scale, 0)
+        *plan._pointers, plan._partials(dim, handle, stream), qs[0], qs[1], os[0], os[1], *pool, rows,
+        plan.capacity, heads, plan.kv_heads, dim, table_shape[0], table_shape[1], page_size, pages, kind,
+        dim ** -0.5 if scale is None else scale, 0)
     rc = _native.lib().nz_attention(args, handle)
     if rc:
         _native.check(rc)
@@ -406,7 +416,7 @@ def adjust_logits(logits, *, history=None, lengths=None, prompt_lengths=None, re
         raise ValueError("mask_rows need masks.")
     if out is None:
         with _on(stream):
-            out = torch.empty((rows, vocab), dtype=logits.dtype, device=device)
+            out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != device or out.stride(1) != 1:
         raise ValueError("`out` must be like logits, rows contiguous.")
     args = _native.LOGITS.pack(

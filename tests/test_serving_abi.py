@@ -79,7 +79,7 @@ ROTARY = dict(q=True, k=True, v=True, out=True, key_cache=True, value_cache=True
               slots=True, q_token=128, q_head=64, k_token=128, k_head=64, v_token=128, v_head=64, out_token=128,
               out_head=64, key_page=2048, key_head=1024, key_slot=64, value_page=2048, value_head=1024, value_slot=64,
               tokens=3, heads=2, kv_heads=2, head_dim=64, rotary_dim=64, page_size=16, n_pages=4, n_positions=10)
-ATTENTION = dict(q=True, key_cache=True, value_cache=True, out=True, tables=True, items=True, partials=True, q_row=128,
+ATTENTION = dict(q=True, key_cache=True, value_cache=True, out=True, tables=True, items=True, counters=True, partials=True, q_row=128,
                  q_head=64, out_row=128, out_head=64, key_page=2048, key_head=1024, key_slot=64, value_page=2048,
                  value_head=1024, value_slot=64, n_rows=2, n_items=4, heads=2, kv_heads=2, head_dim=64, n_requests=2,
                  max_pages=3, page_size=16, n_pages=4)
@@ -116,6 +116,7 @@ LOGITS = dict(logits=True, out=True, rows=2, vocab=100, logits_row=100, out_row=
     ("nz_rotary_store", ROTARY, dict(page_size=100), b"power of two"),
     ("nz_rotary_store", ROTARY, dict(tokens=1 << 30), b"Too many"),
     ("nz_attention", ATTENTION, dict(partials=0), b"Null"),
+    ("nz_attention", ATTENTION, dict(counters=0), b"Null"),
     ("nz_attention", ATTENTION, dict(heads=3), b"multiple of kv_heads"),
     ("nz_attention", ATTENTION, dict(kv_heads=0), b"multiple of kv_heads"),
     ("nz_attention", ATTENTION, dict(head_dim=8), b"head_dim"),
@@ -145,10 +146,11 @@ def test_null_argument_structs_and_plans_are_refused():
     lib = _native.lib()
     for function in ("nz_pages_extend", "nz_pages_release", "nz_rotary_store", "nz_attention", "nz_adjust_logits"):
         assert getattr(lib, function)(None, None) == -1 and b"Null" in lib.nz_last_error()
-    assert lib.nz_attention_plan(None, None, 1, 1, 4096, None) == -1
-    assert lib.nz_attention_plan(4096, None, 1, 0, 4096, None) == -1
-    assert lib.nz_attention_plan(4096, None, 1 << 31, 1, 4096, None) == -1
-    assert lib.nz_attention_partials(10, 32, 128) == 10 * 32 * (1 + 130)
+    for wrong in ((None, None, 1, 1, 8, 4096, 4096), (4096, None, 1, 1, 8, None, 4096), (4096, None, 1, 1, 8, 4096, None),
+                  (4096, None, 1, 0, 8, 4096, 4096), (4096, None, 1, 1, 0, 4096, 4096),
+                  (4096, None, 1 << 31, 1, 8, 4096, 4096)):
+        assert lib.nz_attention_plan(*wrong, None) == -1
+    assert lib.nz_attention_partials(10, 32, 128) == 10 * 32 * 130
 
 
 def test_calls_without_work_return_without_a_device():
