@@ -153,6 +153,8 @@ constexpr uint32_t kWaves = 4, kThreads = 64 * kWaves;
 // Query heads of one key-value head that a workgroup takes: the columns of a
 // matrix instruction.
 constexpr uint32_t kHeads = 16;
+// Workgroups are placed on the XCDs in turn.
+constexpr uint32_t kXcds = 8;
 constexpr float kLog2e = 1.44269504088896340736f;
 
 using f32x4 = vec<float, 4>;
@@ -286,11 +288,15 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 
     __shared__ uint32_t last;
 
     const uint32_t group = a.heads / a.kv_heads, blocks = (group + kHeads - 1) / kHeads;
-    const uint32_t per_item = a.kv_heads * blocks;
-    const uint32_t which = blockIdx.x / per_item, part = blockIdx.x % per_item;
+    // Workgroups that read the same keys, for different blocks of heads, lie
+    // kXcds apart: they run on one XCD and share its L2.
+    const uint32_t turn = blockIdx.x / kXcds, unit = turn / blocks * kXcds + blockIdx.x % kXcds, block = turn % blocks;
+    const uint32_t which = unit / a.kv_heads, kv_head = unit % a.kv_heads;
+    if (which >= a.n_items) return;
     const nz_attention_item item = a.items[which];
     if (static_cast<uint32_t>(item.row) >= a.n_rows) return;
-    const uint32_t kv_head = part / blocks, head0 = kv_head * group + part % blocks * kHeads;
+    const uint32_t per_item = a.kv_heads * blocks, part = kv_head * blocks + block;
+    const uint32_t head0 = kv_head * group + block * kHeads;
     const uint32_t heads = min(kHeads, (kv_head + 1) * group - head0);
     const uint32_t lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -342,7 +348,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 
         }
     };
     constexpr uint32_t kStep = kWaves * S::kKeys;
-    uint32_t t0 = static_cast<uint32_t>(item.begin) + wave * S::kKeys;
+    uint32_t t0 = static_cast<uint32_t>(item.begin) / 16 * 16 + wave * S::kKeys;
     int32_t page[S::kHalves], next[S::kHalves];
     if (t0 < end) {
         entries(t0, page);
@@ -574,8 +580,10 @@ void launch_attention_dim(const nz_attention_args& a, dim3 grid, hipStream_t str
 template <typename T>
 void launch_attention(const nz_attention_args& a, hipStream_t stream) {
     const uint32_t group = a.heads / a.kv_heads;
-    const dim3 grid(a.n_items * a.kv_heads * ((group + kHeads - 1) / kHeads));
-    if (a.head_dim <= 64) launch_attention_dim<T, 64>(a, grid, stream);
+    const uint32_t units = a.n_items * a.kv_heads;
+    const dim3 grid((units + kXcds - 1) / kXcds * kXcds * ((group + kHeads - 1) / kHeads));
+    if (a.head_dim <= 32) launch_attention_dim<T, 32>(a, grid, stream);
+    else if (a.head_dim <= 64) launch_attention_dim<T, 64>(a, grid, stream);
     else if (a.head_dim <= 128) launch_attention_dim<T, 128>(a, grid, stream);
     else launch_attention_dim<T, 256>(a, grid, stream);
 }

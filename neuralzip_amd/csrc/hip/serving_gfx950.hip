@@ -217,10 +217,11 @@ constexpr uint32_t kRotaryThreads = 256;
 template <typename T, uint32_t LANES>
 __global__ __launch_bounds__(kRotaryThreads) void nz_rotary_kernel(nz_rotary_args a) {
     const uint32_t lane = threadIdx.x % LANES;
-    const uint64_t vec = (static_cast<uint64_t>(blockIdx.x) * kRotaryThreads + threadIdx.x) / LANES;
+    // (the caller keeps the heads of a call below 2^31)
+    const uint32_t index = blockIdx.x * (kRotaryThreads / LANES) + threadIdx.x / LANES;
     const uint32_t per_token = a.heads + 2 * a.kv_heads;
-    if (vec >= static_cast<uint64_t>(a.tokens) * per_token) return;   // whole groups leave together
-    const uint32_t token = static_cast<uint32_t>(vec / per_token), head = static_cast<uint32_t>(vec % per_token);
+    if (index >= a.tokens * per_token) return;   // whole groups leave together
+    const uint32_t token = index / per_token, head = index % per_token;
     const uint32_t half = a.rotary_dim / 2, turned = a.rotary_dim / 16;
     const bool live = lane < a.head_dim / 16, turns = lane < turned;
     const uint32_t at = turns && !a.interleaved ? 8 * lane : 16 * lane;
@@ -331,8 +332,16 @@ __global__ __launch_bounds__(kLogitsThreads) void nz_logits_kernel(nz_logits_arg
     const uint32_t before = VECTOR ? static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src) % 16 / sizeof(T)) : 0;
     const int64_t v0 = static_cast<int64_t>(blockIdx.x) * kLogitsChunk - before;
     if (v0 >= static_cast<int64_t>(a.vocab)) return;
-    // a run inside the row as one access, one at its ends by elements
+    const uint32_t* mask = nullptr;
+    const uint32_t words = (a.vocab + 31) / 32;
+    if (a.masks != nullptr) {
+        const int64_t m = a.mask_rows ? a.mask_rows[row] : static_cast<int64_t>(row);
+        if (static_cast<uint64_t>(m) < a.n_masks) mask = a.masks + static_cast<uint64_t>(m) * words;
+    }
+    // a run inside the row as one access, one at its ends by elements; its
+    // mask bits are in one word or two
     run x[kRuns];
+    uint32_t bits[kRuns];
 #pragma unroll
     for (uint32_t k = 0; k < kRuns; ++k) {
         const int64_t v = v0 + (k * kLogitsThreads + threadIdx.x) * kRun;
@@ -343,7 +352,16 @@ __global__ __launch_bounds__(kLogitsThreads) void nz_logits_kernel(nz_logits_arg
             for (uint32_t i = 0; i < kRun; ++i)
                 x[k][i] = v + i >= 0 && v + i < a.vocab ? src[v + i] : static_cast<T>(0.0f);
         }
+        bits[k] = ~0u;
+        if (mask != nullptr && v + kRun > 0 && v < a.vocab) {
+            const uint32_t first = v > 0 ? static_cast<uint32_t>(v) : 0, word = first >> 5;
+            uint64_t two = mask[word];
+            if (kRun > 1 && (first & 31) + kRun > 32 && word + 1 < words) two |= static_cast<uint64_t>(mask[word + 1]) << 32;
+            bits[k] = static_cast<uint32_t>(two >> (first & 31)) << (first - v);
+        }
     }
+    const float repetition = a.repetition ? a.repetition[row] : 1.0f, frequency = a.frequency ? a.frequency[row] : 0.0f;
+    const float presence = a.presence ? a.presence[row] : 0.0f;
     for (uint32_t i = threadIdx.x; i < kLogitsChunk; i += kLogitsThreads) counts[i] = 0;
     if (a.bias_starts != nullptr)
         for (uint32_t i = threadIdx.x; i < kLogitsChunk; i += kLogitsThreads) entries[i] = 0;
@@ -369,13 +387,6 @@ __global__ __launch_bounds__(kLogitsThreads) void nz_logits_kernel(nz_logits_arg
         }
     }
     __syncthreads();
-    const float repetition = a.repetition ? a.repetition[row] : 1.0f, frequency = a.frequency ? a.frequency[row] : 0.0f;
-    const float presence = a.presence ? a.presence[row] : 0.0f;
-    const uint32_t* mask = nullptr;
-    if (a.masks != nullptr) {
-        const int64_t m = a.mask_rows ? a.mask_rows[row] : static_cast<int64_t>(row);
-        if (static_cast<uint64_t>(m) < a.n_masks) mask = a.masks + static_cast<uint64_t>(m) * ((a.vocab + 31) / 32);
-    }
 #pragma unroll
     for (uint32_t k = 0; k < kRuns; ++k) {
         const uint32_t at = (k * kLogitsThreads + threadIdx.x) * kRun;
@@ -390,8 +401,7 @@ __global__ __launch_bounds__(kLogitsThreads) void nz_logits_kernel(nz_logits_arg
                 if (answers) y = y - frequency * static_cast<float>(answers) - presence;
             }
             if (entry) y += a.bias_values[entry - 1];
-            if (mask && v + i >= 0 && v + i < a.vocab && !((mask[(v + i) >> 5] >> ((v + i) & 31)) & 1u))
-                y = -__builtin_inff();
+            if (!(bits[k] >> i & 1u)) y = -__builtin_inff();
             x[k][i] = from_float<T>(y);
         }
         if (v >= 0 && v + kRun <= a.vocab) {
