@@ -635,7 +635,7 @@ typedef struct nz_attention_item {
     int32_t index;               /* among the row's items                    */
     int32_t count;               /* the row's items                          */
     int32_t first;               /* the row's first item                     */
-    int32_t reserved;
+    int32_t keys;                /* of all rows, in 1024                     */
 } nz_attention_item;
 
 /* Cuts rows' contexts into items of about equal length, on the device:

@@ -92,7 +92,7 @@ ROTARY = struct.Struct("=12Q14q11If")
 ATTENTION = struct.Struct("=8Q10q10IfI")
 LOGITS = struct.Struct("=13Q3q8I")
 ATTENTION_ITEM = np.dtype([(name, "<i4") for name in ("row", "request", "begin", "end", "index", "count", "first",
-                                                      "reserved")])
+                                                      "keys")])
 VALUE_BF16, VALUE_FP16, VALUE_FP32 = 0, 1, 2   # enum nz_value_type
 
 _lib = None

@@ -6,6 +6,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <type_traits>
+
 #include "neuralzip_hip.h"
 #include "serving_types.h"
 
@@ -103,6 +105,7 @@ __global__ __launch_bounds__(kPlanThreads) void nz_attention_plan_kernel(const i
             share = shortest_share(contexts, n_rows, fewest + target, least, share, lds);
     }
     const uint32_t most = share * kTile;
+    const int32_t total_keys = static_cast<int32_t>(min<uint64_t>((keys + 1023) / 1024, 0x7FFFFFFFu));
     uint32_t first = 0;
     for (uint32_t r0 = 0; r0 < n_rows; r0 += kPlanThreads) {
         const uint32_t r = r0 + threadIdx.x;
@@ -137,7 +140,7 @@ __global__ __launch_bounds__(kPlanThreads) void nz_attention_plan_kernel(const i
             item.index = static_cast<int32_t>(i);
             item.count = static_cast<int32_t>(n);
             item.first = static_cast<int32_t>(base);
-            item.reserved = 0;
+            item.keys = total_keys;
             items[base + i] = item;
         }
         first += total;
@@ -153,6 +156,8 @@ constexpr uint32_t kWaves = 4, kThreads = 64 * kWaves;
 // Query heads of one key-value head that a workgroup takes: the columns of a
 // matrix instruction.
 constexpr uint32_t kHeads = 16;
+// What the Infinity Cache holds.
+constexpr uint64_t kCacheBytes = 256ull << 20;
 // Workgroups are placed on the XCDs in turn.
 constexpr uint32_t kXcds = 8;
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -205,6 +210,12 @@ template <> struct Piece<float> {
         return c;
     }
 };
+
+template <bool PAST, typename V, typename T>
+__device__ __forceinline__ V fetch(const T* src) {
+    const V* const p = reinterpret_cast<const V*>(src);
+    return PAST ? __builtin_nontemporal_load(p) : *p;
+}
 
 // Largest of a column's values over the four lanes that hold it.
 __device__ __forceinline__ float column_max(float v) {
@@ -333,122 +344,131 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 
             if (!known || t >= end || entry >= a.max_pages) page[h] = -1;
         }
     };
-    piece keys[S::kHalves][S::kKeySteps];
-    auto load_keys = [&](uint32_t t0, const int32_t (&page)[S::kHalves]) {
+    auto run_tiles = [&](auto past) {
+        constexpr bool PAST = decltype(past)::value;
+        piece keys[S::kHalves][S::kKeySteps];
+        auto load_keys = [&](uint32_t t0, const int32_t (&page)[S::kHalves]) {
 #pragma unroll
-        for (uint32_t h = 0; h < S::kHalves; ++h) {
-            const int64_t p = static_cast<uint32_t>(page[h]) < a.n_pages ? page[h] : 0;
-            const T* src = key_base + p * a.key_page + static_cast<int64_t>((t0 + 16 * h) & place_mask) * a.key_slot;
+            for (uint32_t h = 0; h < S::kHalves; ++h) {
+                const int64_t p = static_cast<uint32_t>(page[h]) < a.n_pages ? page[h] : 0;
+                const T* src = key_base + p * a.key_page + static_cast<int64_t>((t0 + 16 * h) & place_mask) * a.key_slot;
 #pragma unroll
-            for (uint32_t s = 0; s < S::kKeySteps; ++s) {
-                const uint32_t d = s * 4 * S::kRun + quad * S::kRun;
-                keys[h][s] = piece{};
-                if (FULL || d < a.head_dim) keys[h][s] = *reinterpret_cast<const piece*>(src + col * a.key_slot + d);
-            }
-        }
-    };
-    constexpr uint32_t kStep = kWaves * S::kKeys;
-    uint32_t t0 = static_cast<uint32_t>(item.begin) / 16 * 16 + wave * S::kKeys;
-    int32_t page[S::kHalves], next[S::kHalves];
-    if (t0 < end) {
-        entries(t0, page);
-        load_keys(t0, page);
-        entries(t0 + kStep, next);
-    }
-    for (; t0 < end; t0 += kStep) {
-        const T* values[S::kHalves];
-        uint32_t limit[S::kHalves];
-#pragma unroll
-        for (uint32_t h = 0; h < S::kHalves; ++h) {
-            const bool valid = static_cast<uint32_t>(page[h]) < a.n_pages;
-            const int64_t p = valid ? page[h] : 0;
-            limit[h] = valid ? end : 0;
-            values[h] = value_base + p * a.value_page + static_cast<int64_t>((t0 + 16 * h) & place_mask) * a.value_slot;
-        }
-        value_run v[S::kGroups][S::kValueSteps][S::kRun];
-#pragma unroll
-        for (uint32_t w = 0; w < S::kGroups; ++w)
-#pragma unroll
-            for (uint32_t s = 0; s < S::kValueSteps; ++s)
-#pragma unroll
-                for (uint32_t k = 0; k < S::kRun; ++k) {
-                    const uint32_t d = (s * 16 + col) * S::kValueRun;
-                    const uint32_t h = S::kRun == 8 ? k / 4 : w, place = 4 * quad + k % 4;
-                    v[w][s][k] = value_run{};
-                    if (FULL || d < a.head_dim)
-                        v[w][s][k] = *reinterpret_cast<const value_run*>(values[h] + place * a.value_slot + d);
+                for (uint32_t s = 0; s < S::kKeySteps; ++s) {
+                    const uint32_t d = s * 4 * S::kRun + quad * S::kRun;
+                    keys[h][s] = piece{};
+                    if (FULL || d < a.head_dim) keys[h][s] = fetch<PAST, piece>(src + col * a.key_slot + d);
                 }
-        float score[S::kHalves][4];
-#pragma unroll
-        for (uint32_t h = 0; h < S::kHalves; ++h) {
-            f32x4 acc = {};
-#pragma unroll
-            for (uint32_t s = 0; s < S::kKeySteps; ++s) acc = P::mma(keys[h][s], q[s], acc);
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i)
-                score[h][i] = t0 + 16 * h + 4 * quad + i < limit[h] ? acc[i] * scale : -__builtin_inff();
-        }
-        if (t0 + kStep < end) {
-            load_keys(t0 + kStep, next);
-#pragma unroll
-            for (uint32_t h = 0; h < S::kHalves; ++h) page[h] = next[h];
-            entries(t0 + 2 * kStep, next);
-        }
-        float top = m;
-#pragma unroll
-        for (uint32_t h = 0; h < S::kHalves; ++h)
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) top = fmaxf(top, score[h][i]);
-        top = column_max(top);
-        const float base = finite_base(top);
-        const float fade = __builtin_amdgcn_exp2f(m - base);
-        m = top;
-        l *= fade;
-#pragma unroll
-        for (uint32_t s = 0; s < S::kValueSteps; ++s)
-#pragma unroll
-            for (uint32_t e = 0; e < S::kValueRun; ++e) o[s][e] *= fade;
-#pragma unroll
-        for (uint32_t h = 0; h < S::kHalves; ++h)
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                score[h][i] = __builtin_amdgcn_exp2f(score[h][i] - (base - P::kLift));
-                l += score[h][i];
             }
-        // values of masked keys may be anything, NaN among it
-        if (t0 + S::kKeys > min(limit[0], limit[S::kHalves - 1])) {
+        };
+        constexpr uint32_t kStep = kWaves * S::kKeys;
+        uint32_t t0 = static_cast<uint32_t>(item.begin) / 16 * 16 + wave * S::kKeys;
+        int32_t page[S::kHalves], next[S::kHalves];
+        if (t0 < end) {
+            entries(t0, page);
+            load_keys(t0, page);
+            entries(t0 + kStep, next);
+        }
+        for (; t0 < end; t0 += kStep) {
+            const T* values[S::kHalves];
+            uint32_t limit[S::kHalves];
+#pragma unroll
+            for (uint32_t h = 0; h < S::kHalves; ++h) {
+                const bool valid = static_cast<uint32_t>(page[h]) < a.n_pages;
+                const int64_t p = valid ? page[h] : 0;
+                limit[h] = valid ? end : 0;
+                values[h] = value_base + p * a.value_page + static_cast<int64_t>((t0 + 16 * h) & place_mask) * a.value_slot;
+            }
+            value_run v[S::kGroups][S::kValueSteps][S::kRun];
 #pragma unroll
             for (uint32_t w = 0; w < S::kGroups; ++w)
 #pragma unroll
                 for (uint32_t s = 0; s < S::kValueSteps; ++s)
 #pragma unroll
                     for (uint32_t k = 0; k < S::kRun; ++k) {
-                        const uint32_t h = S::kRun == 8 ? k / 4 : w;
-                        if (t0 + 16 * h + 4 * quad + k % 4 >= limit[h]) v[w][s][k] = value_run{};
+                        const uint32_t d = (s * 16 + col) * S::kValueRun;
+                        const uint32_t h = S::kRun == 8 ? k / 4 : w, place = 4 * quad + k % 4;
+                        v[w][s][k] = value_run{};
+                        if (FULL || d < a.head_dim)
+                            v[w][s][k] = fetch<PAST, value_run>(values[h] + place * a.value_slot + d);
                     }
-        }
-        // the products with the values, 4 * kRun keys at a time
+            float score[S::kHalves][4];
 #pragma unroll
-        for (uint32_t w = 0; w < S::kGroups; ++w) {
-            piece p_hi, p_lo;
+            for (uint32_t h = 0; h < S::kHalves; ++h) {
+                f32x4 acc = {};
 #pragma unroll
-            for (uint32_t k = 0; k < S::kRun; ++k) {
-                const float p = S::kRun == 8 ? score[k / 4][k % 4] : score[w][k];
-                p_hi[k] = P::head(p);
-                p_lo[k] = static_cast<T>(fmaxf(p - static_cast<float>(p_hi[k]), P::kLeast));
+                for (uint32_t s = 0; s < S::kKeySteps; ++s) acc = P::mma(keys[h][s], q[s], acc);
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i)
+                    score[h][i] = t0 + 16 * h + 4 * quad + i < limit[h] ? acc[i] * scale : -__builtin_inff();
             }
+            if (t0 + kStep < end) {
+                load_keys(t0 + kStep, next);
+#pragma unroll
+                for (uint32_t h = 0; h < S::kHalves; ++h) page[h] = next[h];
+                entries(t0 + 2 * kStep, next);
+            }
+            float top = m;
+#pragma unroll
+            for (uint32_t h = 0; h < S::kHalves; ++h)
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) top = fmaxf(top, score[h][i]);
+            top = column_max(top);
+            const float base = finite_base(top);
+            const float fade = __builtin_amdgcn_exp2f(m - base);
+            m = top;
+            l *= fade;
 #pragma unroll
             for (uint32_t s = 0; s < S::kValueSteps; ++s)
 #pragma unroll
-                for (uint32_t e = 0; e < S::kValueRun; ++e) {
-                    piece x;
+                for (uint32_t e = 0; e < S::kValueRun; ++e) o[s][e] *= fade;
 #pragma unroll
-                    for (uint32_t k = 0; k < S::kRun; ++k) x[k] = v[w][s][k][e];
-                    o[s][e] = P::mma(x, p_hi, o[s][e]);
-                    if (S::kRun == 8) o[s][e] = P::mma(x, p_lo, o[s][e]);
+            for (uint32_t h = 0; h < S::kHalves; ++h)
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    score[h][i] = __builtin_amdgcn_exp2f(score[h][i] - (base - P::kLift));
+                    l += score[h][i];
                 }
+            // values of masked keys may be anything, NaN among it
+            if (t0 + S::kKeys > min(limit[0], limit[S::kHalves - 1])) {
+#pragma unroll
+                for (uint32_t w = 0; w < S::kGroups; ++w)
+#pragma unroll
+                    for (uint32_t s = 0; s < S::kValueSteps; ++s)
+#pragma unroll
+                        for (uint32_t k = 0; k < S::kRun; ++k) {
+                            const uint32_t h = S::kRun == 8 ? k / 4 : w;
+                            if (t0 + 16 * h + 4 * quad + k % 4 >= limit[h]) v[w][s][k] = value_run{};
+                        }
+            }
+            // the products with the values, 4 * kRun keys at a time
+#pragma unroll
+            for (uint32_t w = 0; w < S::kGroups; ++w) {
+                piece p_hi, p_lo;
+#pragma unroll
+                for (uint32_t k = 0; k < S::kRun; ++k) {
+                    const float p = S::kRun == 8 ? score[k / 4][k % 4] : score[w][k];
+                    p_hi[k] = P::head(p);
+                    p_lo[k] = static_cast<T>(fmaxf(p - static_cast<float>(p_hi[k]), P::kLeast));
+                }
+#pragma unroll
+                for (uint32_t s = 0; s < S::kValueSteps; ++s)
+#pragma unroll
+                    for (uint32_t e = 0; e < S::kValueRun; ++e) {
+                        piece x;
+#pragma unroll
+                        for (uint32_t k = 0; k < S::kRun; ++k) x[k] = v[w][s][k][e];
+                        o[s][e] = P::mma(x, p_hi, o[s][e]);
+                        if (S::kRun == 8) o[s][e] = P::mma(x, p_lo, o[s][e]);
+                    }
+            }
         }
-    }
+    };
+    // Keys and values that no cache holds until the next step, and that no
+    // other workgroup reads, are streamed (64 rows of 70B's heads over up to
+    // 16384 keys: 378 us, 391 without).
+    const uint64_t cache_bytes = static_cast<uint64_t>(item.keys) * 1024 * a.kv_heads * a.head_dim * 2 * sizeof(T);
+    if (FULL && blocks == 1 && cache_bytes > kCacheBytes) run_tiles(std::true_type());
+    else run_tiles(std::false_type());
 
     l = column_sum(l);
     if (quad == 0) {

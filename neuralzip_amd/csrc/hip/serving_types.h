@@ -21,27 +21,43 @@ __device__ __forceinline__ T from_float(float x) { return static_cast<T>(x); }
 template <typename T, int N>
 using vec = T __attribute__((ext_vector_type(N)));
 
-// Eight neighbours, in 16-byte accesses.
+// Elements of a 16-byte access.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float* x) {
-    constexpr int kRun = 16 / sizeof(T);
+constexpr uint32_t run_of() { return 16 / sizeof(T); }
+
+// Eight elements as 16-byte runs `apart` elements from one another.
+template <typename T>
+__device__ __forceinline__ void load_runs(const T* p, uint32_t apart, float* x) {
+    constexpr uint32_t kRun = run_of<T>();
 #pragma unroll
-    for (int r = 0; r < 8 / kRun; ++r) {
-        const vec<T, kRun> v = *reinterpret_cast<const vec<T, kRun>*>(p + r * kRun);
+    for (uint32_t r = 0; r < 8 / kRun; ++r) {
+        const vec<T, kRun> v = *reinterpret_cast<const vec<T, kRun>*>(p + r * apart);
 #pragma unroll
-        for (int i = 0; i < kRun; ++i) x[r * kRun + i] = to_float(static_cast<T>(v[i]));
+        for (uint32_t i = 0; i < kRun; ++i) x[r * kRun + i] = to_float(static_cast<T>(v[i]));
     }
 }
 
+// Streaming stores.
 template <typename T>
-__device__ __forceinline__ void store8(T* p, const float* x) {
-    constexpr int kRun = 16 / sizeof(T);
+__device__ __forceinline__ void store_runs(T* p, uint32_t apart, const float* x) {
+    constexpr uint32_t kRun = run_of<T>();
 #pragma unroll
-    for (int r = 0; r < 8 / kRun; ++r) {
+    for (uint32_t r = 0; r < 8 / kRun; ++r) {
         vec<T, kRun> v;
 #pragma unroll
-        for (int i = 0; i < kRun; ++i) v[i] = from_float<T>(x[r * kRun + i]);
-        *reinterpret_cast<vec<T, kRun>*>(p + r * kRun) = v;
+        for (uint32_t i = 0; i < kRun; ++i) v[i] = from_float<T>(x[r * kRun + i]);
+        __builtin_nontemporal_store(v, reinterpret_cast<vec<T, kRun>*>(p + r * apart));
+    }
+}
+
+// N neighbouring 32-bit floats, on a 16-byte boundary.
+template <uint32_t N>
+__device__ __forceinline__ void load_floats(const float* p, float* x) {
+#pragma unroll
+    for (uint32_t i = 0; i < N; i += 4) {
+        const vec<float, 4> v = *reinterpret_cast<const vec<float, 4>*>(p + i);
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) x[i + j] = v[j];
     }
 }
 

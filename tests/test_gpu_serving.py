@@ -491,6 +491,32 @@ def test_attention_and_store_beyond_32_bits_of_offset():
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("dtype, dim", [(torch.bfloat16, 32), (torch.float16, 64), (torch.bfloat16, 128),
+                                        (torch.float32, 128), (torch.bfloat16, 256), (torch.float32, 256),
+                                        (torch.bfloat16, 96)])
+def test_attention_of_more_keys_than_caches_hold(dtype, dim):
+    """Rows whose keys come to more than 256 MiB, which are read past the
+    caches (the rows share their pages, so that the test stays small)."""
+    kv_heads, heads, page, n = 4, 8, 64, 3000
+    rows = (256 << 20) // (n * kv_heads * dim * 2 * dtype.itemsize) + 3
+    keys, values = (randn(pages_of(n, page) + 1, kv_heads, page, dim, seed=s, dtype=dtype) for s in (1, 2))
+    order = torch.randperm(pages_of(n, page), device=DEVICE).int()
+    contexts = [n - 7 * (i % 40) for i in range(rows)]
+    q = randn(rows, heads, dim, seed=3, dtype=dtype)
+    plan = serving.AttentionPlan(ints(contexts), heads=heads, kv_heads=kv_heads)
+    out = serving.paged_attention(q, keys, values, order[None].expand(rows, -1).contiguous(), plan)
+    k, v = (c[order.long()].transpose(0, 1).reshape(kv_heads, -1, dim).double() for c in (keys, values))
+    seen = torch.arange(k.shape[1], device=DEVICE) < ints(contexts)[:, None]
+    x = q.double().view(rows, kv_heads, heads // kv_heads, dim).transpose(0, 1).reshape(kv_heads, -1, dim)
+    scores = torch.matmul(x, k.transpose(1, 2)) * dim ** -0.5
+    scores = scores.view(kv_heads, rows, heads // kv_heads, -1).masked_fill(~seen[None, :, None], -math.inf)
+    want = torch.matmul(scores.softmax(-1).view(kv_heads, -1, k.shape[1]), v).view(kv_heads, rows, -1, dim)
+    want = want.transpose(0, 1).reshape(rows, heads, dim)
+    size = (torch.matmul(x.abs(), k.abs().transpose(1, 2)).amax() * dim ** -0.5)
+    bound = attention_bound(want, size, v.abs().amax(), contexts, dim, dtype)
+    assert ((out.double() - want).abs() <= bound).all()
+
+
 @pytest.mark.parametrize("contexts", [[0], [1], [128], [129], [5000], [0, 10 ** 6, 3], [200] * 1500, [100_000, 7] * 40,
                                       [2 ** 31 - 1, 2 ** 31 - 1, 5], [-4, 33]])
 def test_plans_cover_every_key_once(contexts):
