@@ -1,0 +1,237 @@
+"""Greedy decoding of many requests with lengths of their own over a paged
+key-value cache, on a Transformers decoder model, compressed or not.
+
+PagedDecoder runs every new token of a step through the operators of
+neuralzip_amd.gpu.serving: PageTables gives the tokens their pages, Rotary
+norms, rotates and stores each layer's queries and keys, paged_attention
+reads the pages and adjust_logits applies penalties and grammar masks. The
+model's own Linears, norms and blocks do the rest, so a NeuralZipRuntime's
+hooks decode the weights as in any forward. Prompts run through the model's
+own forward, one at a time, and their keys and values are then stored into
+the request's pages. A step never asks the device for anything, so that it
+can be captured in a HIP graph (capture()) and replayed while requests grow.
+
+Models are Llama-like: model.model.{embed_tokens, layers, norm, rotary_emb}
+and model.lm_head, layers with self_attn.{q,k,v,o}_proj and, optionally, RMS
+norms q_norm and k_norm over a head. The reference has no counterpart (its
+forwards keep Transformers' cache, neuralzip/gpu/inference.py:476-509).
+"""
+import contextlib
+
+import torch
+
+from neuralzip_amd.gpu import serving
+from neuralzip_amd.gpu.inference import RUNTIME_ATTRIBUTE
+
+# Rotary tables that depend on the length they are asked for.
+_GROWING_ROPES = ("dynamic", "longrope")
+
+
+class PagedDecoder:
+    """`requests` places for requests of at most `max_length` tokens, prompt
+    and answer together, on pages of `page_size` tokens: `num_pages` of them
+    for all requests, or enough for all at full length.
+
+    `repetition`, `frequency` and `presence` are adjust_logits' penalties,
+    for all requests. With `grammar`, `masks` (int32, requests x ceil(vocab /
+    32), all bits set at first) holds the tokens that each request may answer
+    with next; it may be written between steps."""
+
+    def __init__(self, model, *, requests, max_length, page_size=16, num_pages=None, repetition=1.0, frequency=0.0,
+                 presence=0.0, grammar=False):
+        body = model.model
+        self.model, self.layers = model, list(body.layers)
+        self._attentions = [layer.self_attn for layer in self.layers]
+        first = self._attentions[0]
+        for attention in self._attentions:
+            for name in ("q_proj", "k_proj", "v_proj", "o_proj", "head_dim"):
+                if not hasattr(attention, name):
+                    raise ValueError(f"PagedDecoder needs Llama-like attention modules; {type(attention).__name__} "
+                                     f"has no {name}.")
+            if getattr(attention, "sliding_window", None) is not None:
+                raise ValueError("PagedDecoder attends to whole contexts; this model's layers have a sliding window.")
+        if getattr(body.rotary_emb, "rope_type", "default") in _GROWING_ROPES:
+            raise ValueError("PagedDecoder needs rotary tables that do not depend on the length.")
+        embedding = body.embed_tokens.weight
+        self.device, dtype = embedding.device, embedding.dtype
+        self.dim = first.head_dim
+        self.kv_heads = model.config.num_key_value_heads
+        self.heads = model.config.num_attention_heads
+        self.requests, self.max_length, self.vocab = requests, max_length, model.config.vocab_size
+        width = -(-max_length // page_size)
+        self.tables = serving.PageTables(requests, width, page_size, num_pages or requests * width, device=self.device)
+        # one allocation for all layers: (layers, keys and values, pages, heads, places, elements)
+        self.cache = torch.zeros((len(self.layers), 2, self.tables.num_pages, self.kv_heads, page_size, self.dim),
+                                 dtype=dtype, device=self.device)
+        positions = torch.arange(max_length, device=self.device)[None]
+        cos, sin = body.rotary_emb(torch.zeros(1, dtype=torch.float32, device=self.device), positions)
+        half = cos.shape[-1] // 2
+        cos, sin = (t[0, :, :half].float().contiguous() for t in (cos, sin))
+        self._rotaries = []
+        for attention in self._attentions:
+            q_norm, k_norm = getattr(attention, "q_norm", None), getattr(attention, "k_norm", None)
+            weights = {} if q_norm is None else dict(q_weight=q_norm.weight.detach(), k_weight=k_norm.weight.detach(),
+                                                     eps=q_norm.variance_epsilon)
+            self._rotaries.append(serving.Rotary(cos, sin, **weights))
+        # prompts' keys are rotated already: a rotation of no elements stores them
+        self._store = serving.Rotary(cos[:, :0].contiguous(), sin[:, :0].contiguous())
+
+        def filled(value, dtype=torch.float32):
+            return torch.full((requests,), value, dtype=dtype, device=self.device)
+        self._step = serving.Step(requests, requests, self.device)
+        self._plan = serving.AttentionPlan(filled(0, torch.int32), heads=self.heads, kv_heads=self.kv_heads)
+        self._live = filled(0, torch.int32)           # 1: the request gets a token in a step
+        # row `requests` of what is written by request takes what a step's unused rows write
+        self._last = torch.zeros(requests + 1, dtype=torch.int64, device=self.device)
+        self._history = torch.zeros((requests + 1, max_length + 1), dtype=torch.int32, device=self.device)
+        self._prompts = filled(0, torch.int32)
+        self._penalties = {}
+        if (repetition, frequency, presence) != (1.0, 0.0, 0.0):
+            self._penalties = dict(repetition=filled(repetition), frequency=filled(frequency), presence=filled(presence))
+        self.masks = torch.full((requests, (self.vocab + 31) // 32), -1, dtype=torch.int32,
+                                device=self.device) if grammar else None
+        self.logits = None                            # of the last step, in token order, as adjusted
+        self._graph = None
+        self._taken = [False] * requests
+
+    # --------------------------------------------------------------- requests
+
+    @torch.no_grad()
+    def add(self, ids):
+        """Takes in a prompt (1-D token ids), picks its first answer token
+        and returns the request's place."""
+        ids = torch.as_tensor(ids, dtype=torch.int64, device=self.device)
+        n = ids.shape[0]
+        if ids.dim() != 1 or not 0 < n <= self.max_length:
+            raise ValueError(f"A prompt is a vector of 1 to {self.max_length} token ids.")
+        if all(self._taken):
+            raise RuntimeError("All requests' places are taken.")
+        place = self._taken.index(False)
+        new = torch.zeros(self.requests, dtype=torch.int32, device=self.device)
+        new[place] = n
+        step = self.tables.extend(new, n)
+        if int(step.status[place]) != serving.PAGES_OK:
+            raise RuntimeError("There are not enough free pages for the prompt.")
+        out = self.model(input_ids=ids[None], use_cache=True)
+        for layer, prompt in enumerate(out.past_key_values.layers):
+            k, v = (t[0].transpose(0, 1) for t in (prompt.keys, prompt.values))
+            self._store(k, k, v, step.positions, step.slots, *self.cache[layer])
+        self._history[place, :n] = ids.int()
+        self._prompts[place] = n
+        self._live[place] = 1
+        self._taken[place] = True
+        rows = torch.full((1,), place, dtype=torch.int32, device=self.device)
+        contexts = torch.full((1,), n, dtype=torch.int32, device=self.device)
+        self._pick(out.logits[0, -1:], rows, contexts)
+        return place
+
+    def finish(self, *places):
+        """Ends requests: their pages and places are free again."""
+        done = torch.zeros(self.requests, dtype=torch.bool, device=self.device)
+        for place in places:
+            if not self._taken[place]:
+                raise ValueError(f"Place {place} holds no request.")
+            done[place] = True
+            self._taken[place] = False
+        self.tables.release(done)
+        self._live.masked_fill_(done, 0)
+
+    # ------------------------------------------------------------------ steps
+
+    def _attend(self, layer, attention, hidden, *args, **kwargs):
+        """The attention module's forward during a step: hidden is (1, tokens, size)."""
+        tokens = hidden.shape[1]
+        q, k, v = (proj(hidden)[0].view(tokens, -1, self.dim) for proj in
+                   (attention.q_proj, attention.k_proj, attention.v_proj))
+        cache = self.cache[layer]
+        q = self._rotaries[layer](q, k, v, self._step.positions, self._step.slots, *cache)
+        scale = getattr(attention, "scaling", None)
+        out = serving.paged_attention(q, *cache, self.tables.tables, self._plan, scale=scale)
+        return attention.o_proj(out.view(1, tokens, -1)), None
+
+    @contextlib.contextmanager
+    def _paged(self):
+        """Attention over the pages while a step runs."""
+        def forward(layer, attention):
+            return lambda hidden_states, *args, **kwargs: self._attend(layer, attention, hidden_states, *args, **kwargs)
+        for layer, attention in enumerate(self._attentions):
+            attention.forward = forward(layer, attention)
+        try:
+            yield
+        finally:
+            for attention in self._attentions:
+                del attention.forward
+
+    def _run(self):
+        """One step, all of it on the device."""
+        self.tables.extend(self._live, self.requests, out=self._step)
+        step = self._step
+        self._plan.update(step.contexts, requests=step.requests)
+        body, rows = self.model.model, self._rows(step.requests)
+        hidden = body.embed_tokens(self._last[rows])[None]
+        with self._paged():
+            for layer in self.layers:
+                hidden = layer(hidden)
+                if isinstance(hidden, tuple):
+                    hidden = hidden[0]
+        logits = self.model.lm_head(body.norm(hidden))[0]
+        self._pick(logits, step.requests, step.contexts)
+
+    def _rows(self, requests):
+        return torch.where(requests < 0, self.requests, requests).long()
+
+    def _pick(self, logits, requests, contexts):
+        """Adjusts the logits of tokens that make their requests `contexts`
+        long, and notes the likeliest next ones."""
+        rows = self._rows(requests)
+        adjust = {}
+        if self._penalties:
+            inside = rows.clamp(max=self.requests - 1)
+            adjust.update({name: t[inside] for name, t in self._penalties.items()}, history=self._history[rows],
+                          lengths=contexts, prompt_lengths=self._prompts[inside])
+        if self.masks is not None:
+            adjust.update(masks=self.masks, mask_rows=requests)
+        if adjust:
+            logits = serving.adjust_logits(logits, **adjust)
+        self.logits = logits
+        best = logits.argmax(-1)
+        self._last.index_copy_(0, rows, best)
+        place = rows * self._history.shape[1] + contexts.long()
+        self._history.view(-1).index_copy_(0, place, best.int())
+
+    @torch.no_grad()
+    def step(self):
+        """One new token for every request; returns the tokens (int64, by
+        place; those of free places mean nothing). Requests at max_length, or
+        for which no page is free, stay as they are."""
+        if self._graph is not None:
+            self._graph.replay()
+        else:
+            self._run()
+        return self._last[:self.requests]
+
+    @torch.no_grad()
+    def capture(self):
+        """Captures the step in a HIP graph, which step() replays from then
+        on. A step should have run eagerly before."""
+        runtime = getattr(self.model, RUNTIME_ATTRIBUTE, None)
+        graph = torch.cuda.CUDAGraph()
+        with runtime.graph_capture() if runtime is not None else contextlib.nullcontext(), torch.cuda.graph(graph):
+            self._run()
+        self._graph = graph
+
+    def generate(self, prompts, new_tokens, *, capture=False):
+        """`new_tokens` greedy tokens for each prompt (as many prompts as
+        there are free places); lists of token ids. `capture` replays the
+        steps after the second from a HIP graph."""
+        if new_tokens < 1 or any(len(p) + new_tokens - 1 > self.max_length for p in prompts):
+            raise ValueError("Prompts and answers must fit max_length.")
+        places = [self.add(p) for p in prompts]
+        tokens = [self._last[:self.requests].clone()]
+        for i in range(new_tokens - 1):
+            if capture and i == 2 and self._graph is None:
+                self.capture()
+            tokens.append(self.step().clone())
+        answers = torch.stack(tokens, 1)[places].tolist()
+        self.finish(*places)
+        return answers
