@@ -26,6 +26,8 @@ constexpr uint32_t kTile = 32, kLeastItem = 128, kLeastLong = 512;
 struct PlanLds {
     uint64_t keys[kPlanWaves];
     uint32_t most[kPlanWaves], counts[kPlanWaves];
+    uint32_t contexts[kPlanThreads];                     // of up to as many rows
+    uint32_t first[kPlanThreads], each[kPlanThreads];    // per row of a strip: first item, its items' length
 };
 
 __device__ __forceinline__ uint32_t context_of(const int32_t* contexts, uint32_t r) {
@@ -33,36 +35,46 @@ __device__ __forceinline__ uint32_t context_of(const int32_t* contexts, uint32_t
 }
 
 // Items of all rows when none is longer than `share` (a wavefront's sum).
-__device__ __forceinline__ uint32_t count_items(const int32_t* contexts, uint32_t n_rows, uint32_t share) {
+__device__ __forceinline__ uint32_t count_items(const int32_t* contexts, uint32_t n_rows, uint32_t share,
+                                                const PlanLds& lds) {
     uint32_t n = 0;
-    for (uint32_t r = threadIdx.x & 63; r < n_rows; r += 64)
-        n += max((context_of(contexts, r) + share - 1) / share, 1u);
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d <<= 1) n += __shfl_xor(n, d);
-    return n;
+    if (n_rows <= kPlanThreads) {
+        for (uint32_t r = threadIdx.x & 63; r < n_rows; r += 64) n += max((lds.contexts[r] + share - 1) / share, 1u);
+    } else {
+#pragma unroll 4
+        for (uint32_t r = threadIdx.x & 63; r < n_rows; r += 64)
+            n += max((context_of(contexts, r) + share - 1) / share, 1u);
+    }
+    return last_lane(wave_scan(n));
 }
 
-// The shortest item length (in tiles, from `lo` to `hi`) of which there are
-// at most `limit` items; `hi` is one. Every wavefront tries another length.
-__device__ uint32_t shortest_share(const int32_t* contexts, uint32_t n_rows, uint32_t limit, uint32_t lo, uint32_t hi,
-                                   PlanLds& lds) {
+// The shortest item length, in tiles and from `least` on, of which there are
+// at most `limit` (n_rows or more) items; `longest` tiles is one. Every
+// wavefront tries another length.
+__device__ uint32_t shortest_share(const int32_t* contexts, uint32_t n_rows, uint32_t limit, uint64_t keys,
+                                   uint32_t least, uint32_t longest, PlanLds& lds) {
     const uint32_t wave = threadIdx.x >> 6;
+    // keys / share <= items < n_rows + keys / share
+    const uint64_t below_all = keys / (static_cast<uint64_t>(limit) * kTile);
+    uint32_t lo = static_cast<uint32_t>(std::max<uint64_t>(least, std::min<uint64_t>(below_all, longest))), hi = max(longest, lo);
+    if (limit > n_rows) {
+        const uint64_t enough = keys / (static_cast<uint64_t>(limit - n_rows) * kTile) + 1;
+        hi = max(static_cast<uint32_t>(min<uint64_t>(enough, hi)), lo);
+    }
     while (lo < hi) {
         const uint32_t step = (hi - lo + kPlanWaves) / (kPlanWaves + 1);
         const uint32_t tried = min(lo + wave * step, hi);
-        const uint32_t n = count_items(contexts, n_rows, tried * kTile);
+        const uint32_t n = count_items(contexts, n_rows, tried * kTile, lds);
         __syncthreads();
         if ((threadIdx.x & 63) == 0) lds.counts[wave] = n;
         __syncthreads();
-        uint32_t below = lo, found = hi;
-#pragma unroll
-        for (uint32_t w = 0; w < kPlanWaves; ++w) {
-            const uint32_t length = min(lo + w * step, hi);
-            if (lds.counts[w] <= limit) found = min(found, length);
-            else below = max(below, length + 1);
-        }
-        lo = below;
-        hi = max(found, below);
+        // longer items are fewer: the first length tried that gives few enough
+        const uint32_t lane = threadIdx.x & 63;
+        const uint64_t few = __ballot(lane < kPlanWaves && lds.counts[min(lane, kPlanWaves - 1)] <= limit);
+        const uint32_t at = few ? __builtin_ctzll(few) : kPlanWaves;
+        const uint32_t below = lo + at * step;   // the length itself, or one past those tried
+        if (at > 0) lo = min(below - step, hi) + 1;
+        if (few) hi = min(below, hi);
     }
     return lo;
 }
@@ -70,7 +82,10 @@ __device__ uint32_t shortest_share(const int32_t* contexts, uint32_t n_rows, uin
 // One workgroup. Items are as short as the number wanted allows, so that they
 // take about the same time: one per compute unit and row's heads while that
 // cuts no row far shorter than its share, since rows of one item need no
-// join; twice as many where some rows are much longer than others.
+// join; one more per compute unit where some rows are much longer than others
+// (in whole rounds of the units: 32 rows of up to 8191 keys over 8 heads 98 us
+// with 64 items and 111 with 48). Latency bound: 5 us for one row of 2001
+// keys, 9 for 64 ragged rows, once a step.
 __global__ __launch_bounds__(kPlanThreads) void nz_attention_plan_kernel(const int32_t* __restrict__ contexts,
                                                                          const int32_t* __restrict__ requests,
                                                                          uint32_t n_rows, uint32_t target, uint32_t parts,
@@ -82,6 +97,7 @@ __global__ __launch_bounds__(kPlanThreads) void nz_attention_plan_kernel(const i
     uint32_t longest = 0;
     for (uint32_t r = threadIdx.x; r < n_rows; r += kPlanThreads) {
         const uint32_t context = context_of(contexts, r);
+        if (r < kPlanThreads) lds.contexts[r] = context;
         keys += context;
         longest = max(longest, context);
     }
@@ -99,10 +115,10 @@ __global__ __launch_bounds__(kPlanThreads) void nz_attention_plan_kernel(const i
     const uint32_t least = min(max((tiles + 15) / 16, kLeastItem / kTile), kLeastLong / kTile);
     uint32_t share = least;
     if (tiles > least) {
-        share = shortest_share(contexts, n_rows, fewest, least, tiles, lds);
+        share = shortest_share(contexts, n_rows, fewest, keys, least, tiles, lds);
         const uint64_t length = static_cast<uint64_t>(share) * kTile;
         if (length * fewest * 2 > keys * 3 && length * target * 2 > keys)
-            share = shortest_share(contexts, n_rows, fewest + target, least, share, lds);
+            share = shortest_share(contexts, n_rows, fewest + target, keys, least, share, lds);
     }
     const uint32_t most = share * kTile;
     const int32_t total_keys = static_cast<int32_t>(min<uint64_t>((keys + 1023) / 1024, 0x7FFFFFFFu));
@@ -115,33 +131,33 @@ __global__ __launch_bounds__(kPlanThreads) void nz_attention_plan_kernel(const i
         uint32_t n = max((context + most - 1) / most, 1u);
         const uint32_t each = max(((context + n - 1) / n + kTile - 1) / kTile * kTile, kTile);
         n = live ? max((context + each - 1) / each, 1u) : 0;
-        uint32_t scan = n;
-#pragma unroll
-        for (uint32_t d = 1; d < 64; d <<= 1) {
-            const uint32_t below = __shfl_up(scan, d);
-            if (lane >= d) scan += below;
-        }
-        __syncthreads();   // the last reads of `counts`
+        const uint32_t scan = wave_scan(n);
+        __syncthreads();   // the last reads of `counts`, `first` and `each`
         if (lane == 63) lds.counts[wave] = scan;
         __syncthreads();
-        uint32_t before = first, total = 0;
+        uint32_t before = 0, total = 0;
 #pragma unroll
         for (uint32_t w = 0; w < kPlanWaves; ++w) {
             if (w < wave) before += lds.counts[w];
             total += lds.counts[w];
         }
-        const uint32_t base = before + scan - n;
-        for (uint32_t i = 0; i < n; ++i) {
+        lds.first[threadIdx.x] = before + scan - n;
+        lds.each[threadIdx.x] = each;
+        __syncthreads();
+        for (uint32_t j = threadIdx.x; j < total; j += kPlanThreads) {
+            const uint32_t i = owner(lds.first, min(n_rows - r0, kPlanThreads), j), index = j - lds.first[i];
+            const uint32_t end_of_row = i + 1 < min(n_rows - r0, kPlanThreads) ? lds.first[i + 1] : total;
+            const uint32_t length = n_rows <= kPlanThreads ? lds.contexts[i] : context_of(contexts, r0 + i);
             nz_attention_item item;
-            item.row = static_cast<int32_t>(r);
-            item.request = requests ? requests[r] : static_cast<int32_t>(r);
-            item.begin = static_cast<int32_t>(i * each);
-            item.end = static_cast<int32_t>(min(context, (i + 1) * each));
-            item.index = static_cast<int32_t>(i);
-            item.count = static_cast<int32_t>(n);
-            item.first = static_cast<int32_t>(base);
+            item.row = static_cast<int32_t>(r0 + i);
+            item.request = requests ? requests[r0 + i] : static_cast<int32_t>(r0 + i);
+            item.begin = static_cast<int32_t>(index * lds.each[i]);
+            item.end = static_cast<int32_t>(min(length, (index + 1) * lds.each[i]));
+            item.index = static_cast<int32_t>(index);
+            item.count = static_cast<int32_t>(end_of_row - lds.first[i]);
+            item.first = static_cast<int32_t>(first + lds.first[i]);
             item.keys = total_keys;
-            items[base + i] = item;
+            items[first + j] = item;
         }
         first += total;
     }

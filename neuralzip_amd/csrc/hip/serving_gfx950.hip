@@ -22,24 +22,16 @@ constexpr uint32_t kPagesThreads = 1024;
 // shared among several.
 constexpr uint32_t kPagesShare = 2048, kPagesGroups = 128;
 
-// Saturating, so that a step's sum of absurd requests stays past every limit.
-__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
-
 // Inclusive saturating prefix sums over the workgroup of N values at once;
 // total receives the sums.
 template <uint32_t THREADS, int N>
 __device__ __forceinline__ void block_scan(uint32_t (&v)[N], uint32_t (&total)[N], uint32_t (*lds)[THREADS / 64]) {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-    for (uint32_t d = 1; d < 64; d <<= 1)
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const uint32_t below = __shfl_up(v[i], d);
-            if (lane >= d) v[i] = add_sat(v[i], below);
-        }
+    for (int i = 0; i < N; ++i) v[i] = wave_scan(v[i]);
     if (THREADS == 64) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) total[i] = __shfl(v[i], 63);
+        for (int i = 0; i < N; ++i) total[i] = last_lane(v[i]);
         return;
     }
     __syncthreads();   // the last call's reads
@@ -58,17 +50,6 @@ __device__ __forceinline__ void block_scan(uint32_t (&v)[N], uint32_t (&total)[N
         v[i] = add_sat(before, v[i]);
         total[i] = sum;
     }
-}
-
-// The last i in [0, n) with first[i] <= x, where first[0] <= x.
-__device__ __forceinline__ uint32_t owner(const uint32_t* first, uint32_t n, uint32_t x) {
-    uint32_t lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) >> 1;
-        if (first[mid] <= x) lo = mid;
-        else hi = mid;
-    }
-    return lo;
 }
 
 // Prefix sums over the requests of the tokens asked and the pages wanted; if

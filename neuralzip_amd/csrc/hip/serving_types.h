@@ -1,5 +1,6 @@
-// serving_types.h -- value types of the serving-step kernels: loads to and
-// stores from 32-bit floats. Device code only.
+// serving_types.h -- shared by the serving-step kernels: value types, their
+// loads to and stores from 32-bit floats, a search in prefix sums. Device code
+// only.
 #ifndef NZ_SERVING_TYPES_H
 #define NZ_SERVING_TYPES_H
 
@@ -66,6 +67,41 @@ __device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
     const float x = a * c - b * s;
     b = b * c + a * s;
     a = x;
+}
+
+// Saturating, so that sums of absurd requests stay past every limit.
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
+    return add_sat(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false)));
+}
+
+// Inclusive saturating prefix sum over the wavefront: shifts of 1, 2, 4 and 8
+// lanes inside each row of 16, then the rows' carries.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v = dpp_add<0x111, 0xF>(v);
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);
+    return dpp_add<0x143, 0xC>(v);
+}
+
+// The wavefront's last lane's value.
+__device__ __forceinline__ uint32_t last_lane(uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
+}
+
+// The last i in [0, n) with first[i] <= x, where first[0] <= x.
+__device__ __forceinline__ uint32_t owner(const uint32_t* first, uint32_t n, uint32_t x) {
+    uint32_t lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (first[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
 }
 
 }  // namespace
