@@ -41,6 +41,14 @@ def _on(stream):
     return torch.cuda.stream(stream) if stream is not None else _CURRENT
 
 
+def _like(t, stream):
+    """A dense new tensor like t, allocated on `stream`."""
+    if stream is None:
+        return torch.empty_like(t, memory_format=torch.contiguous_format)
+    with torch.cuda.stream(stream):
+        return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _call(function, device, args, stream):
     rc = function(args, _stream_handle(device, stream))
     if rc:
@@ -48,31 +56,34 @@ def _call(function, device, args, stream):
 
 
 def _refuse_gradients(*tensors):
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise ValueError("The serving operators have no backward: call them under torch.no_grad().")
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise ValueError("The serving operators have no backward: call them under torch.no_grad().")
 
 
-def _check_vector(name, t, dtype, n, device):
-    if t.dtype is not dtype or t.shape != (n,) or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} vector of {n} on {device}; "
+# (Devices are compared by their index, -1 for the CPU: a call makes a dozen
+# comparisons, and those of torch.device take twice as long.)
+def _check_vector(name, t, dtype, n, index):
+    if t.dtype is not dtype or t.shape != (n,) or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} vector of {n} on device {index}; "
                          f"got {t.dtype} {tuple(t.shape)} on {t.device}.")
 
 
-def _pool_layout(keys, values, kv_heads, head_dim, dtype, device):
+def _pool_layout(keys, values, kv_heads, head_dim, dtype, index):
     """Strides of a layer's two caches, (pages, kv_heads, page size, head_dim),
     their pages and page size."""
     shape = keys.shape
-    if len(shape) != 4 or shape != values.shape or shape[1] != kv_heads or shape[3] != head_dim:
+    if shape != values.shape or len(shape) != 4 or shape[1] != kv_heads or shape[3] != head_dim:
         raise ValueError(f"Caches must both be (pages, {kv_heads}, page size, {head_dim}); "
                          f"got {tuple(keys.shape)} and {tuple(values.shape)}.")
-    if keys.dtype is not dtype or values.dtype is not dtype or keys.device != device or values.device != device:
+    if keys.dtype is not dtype or values.dtype is not dtype or keys.get_device() != index \
+            or values.get_device() != index:
         raise ValueError("Caches must have the queries' dtype and device.")
-    ks, vs = keys.stride(), values.stride()
-    if ks[3] != 1 or vs[3] != 1:
+    k0, k1, k2, k3 = keys.stride()
+    v0, v1, v2, v3 = values.stride()
+    if k3 != 1 or v3 != 1:
         raise ValueError("A head's elements must be contiguous in the caches.")
-    return ks[:3] + vs[:3], shape[0], shape[2]
+    return (k0, k1, k2, v0, v1, v2), shape[0], shape[2]
 
 
 class Step:
@@ -91,8 +102,8 @@ class Step:
         # one allocation: 8-byte slots first, then the 4-byte arrays
         words = torch.empty(5 * max_tokens + 3 * n_requests + 2, dtype=torch.int32, device=device)
         (slots, self.positions, self.requests, self.contexts, self.starts, self.status, self.lengths,
-         self.n_free) = words.split((2 * max_tokens, max_tokens, max_tokens, max_tokens, n_requests + 1, n_requests,
-                                     n_requests, 1))
+         self.n_free) = torch.split_with_sizes(words, (2 * max_tokens, max_tokens, max_tokens, max_tokens,
+                                                       n_requests + 1, n_requests, n_requests, 1))
         self.slots = slots.view(torch.int64)
 
 
@@ -101,7 +112,8 @@ class Released:
     __slots__ = ("lengths", "n_free")
 
     def __init__(self, n_requests, device):
-        self.lengths, self.n_free = torch.empty(n_requests + 1, dtype=torch.int32, device=device).split((n_requests, 1))
+        words = torch.empty(n_requests + 1, dtype=torch.int32, device=device)
+        self.lengths, self.n_free = torch.split_with_sizes(words, (n_requests, 1))
 
 
 class PageTables:
@@ -122,7 +134,7 @@ class PageTables:
             raise ValueError("There must be requests and pages, and a request's tokens must be below 2**31.")
         self.requests, self.max_pages, self.page_size, self.num_pages = requests, max_pages, page_size, num_pages
         self.lengths = torch.zeros(requests, dtype=torch.int32, device=device)
-        self.device = self.lengths.device
+        self.device, self._index = self.lengths.device, self.lengths.get_device()
         self.tables = torch.full((requests, max_pages), -1, dtype=torch.int32, device=device)
         self.free = torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=device)
         self.n_free = torch.full((1,), num_pages, dtype=torch.int32, device=device)
@@ -138,7 +150,7 @@ class PageTables:
         free. Without `advance` the state stays (but for table entries past
         the requests' pages): the step can be dropped, as after speculation.
         `out` is an earlier Step of the same sizes to write into."""
-        _check_vector("new_tokens", new_tokens, torch.int32, self.requests, self.device)
+        _check_vector("new_tokens", new_tokens, torch.int32, self.requests, self._index)
         if max_tokens < 0:
             raise ValueError("max_tokens must not be negative.")
         if out is None:
@@ -159,7 +171,7 @@ class PageTables:
         """Puts the pages of the requests whose `done` (bool) is set back
         onto the free stack and sets their lengths to 0; returns the state
         after it. Without `advance` lengths and n_free stay."""
-        _check_vector("done", done, torch.bool, self.requests, self.device)
+        _check_vector("done", done, torch.bool, self.requests, self._index)
         with _on(stream):
             out = Released(self.requests, self.device)
         args = _native.PAGES_RELEASE.pack(
@@ -193,7 +205,7 @@ class Rotary:
                 raise ValueError("Norm weights must be contiguous vectors on cos's device.")
         self.cos, self.sin, self.q_weight, self.k_weight = cos, sin, q_weight, k_weight
         self.rotary_dim, self.interleaved, self.eps = 2 * cos.shape[1], bool(interleaved), float(eps)
-        self._device, self._positions = cos.device, cos.shape[0]
+        self._device, self._index, self._positions = cos.device, cos.get_device(), cos.shape[0]
         self._weight_type = _TYPES[weights[0].dtype] if weights else None
         self._weight_dim = weights[0].shape[0] if weights else None
         self._tables = (cos.data_ptr(), sin.data_ptr(), q_weight.data_ptr() if q_weight is not None else 0,
@@ -208,49 +220,52 @@ class Rotary:
         any strides whose tokens and heads lie on 16-byte boundaries. Held in
         32 bits and rounded once. Tokens' slots must differ. A slot outside
         the caches stores nothing, a position outside the tables gives NaN."""
-        _refuse_gradients(q, k, v, self.q_weight, self.k_weight)
-        dtype, device, shape, kv_shape = q.dtype, q.device, q.shape, k.shape
+        if torch.is_grad_enabled():
+            _refuse_gradients(q, k, v, self.q_weight, self.k_weight)
+        dtype, index, shape, kv_shape = q.dtype, q.get_device(), q.shape, k.shape
         if len(shape) != 3 or len(kv_shape) != 3 or kv_shape != v.shape:
             raise ValueError("q, k and v must be (tokens, heads, head_dim), k and v alike.")
         tokens, heads, dim = shape
-        kv_heads, kind = kv_shape[1], _TYPES.get(dtype)
-        if kind is None or kv_shape[0] != tokens or kv_shape[2] != dim or self.rotary_dim > dim:
+        kv_tokens, kv_heads, kv_dim = kv_shape
+        kind = _TYPES.get(dtype)
+        if kind is None or kv_tokens != tokens or kv_dim != dim or self.rotary_dim > dim:
             raise ValueError(f"q {tuple(shape)} {dtype} and k {tuple(kv_shape)} do not fit one another or the "
                              f"rotation of {self.rotary_dim} elements.")
-        if k.dtype is not dtype or v.dtype is not dtype or k.device != device or v.device != device \
-                or device != self._device:
+        if k.dtype is not dtype or v.dtype is not dtype or k.get_device() != index or v.get_device() != index \
+                or index != self._index:
             raise ValueError("q, k, v and the tables must match in dtype and device.")
         weight_type = self._weight_type
         if weight_type is None:
             weight_type = kind
         elif self._weight_dim != dim or weight_type not in (kind, _native.VALUE_FP32):
             raise ValueError("Norm weights must be head_dim values of q's dtype or float32.")
-        _check_vector("positions", positions, torch.int32, tokens, device)
-        qs, ks, vs = q.stride(), k.stride(), v.stride()
-        if qs[2] != 1 or ks[2] != 1 or vs[2] != 1:
+        _check_vector("positions", positions, torch.int32, tokens, index)
+        q0, q1, q2 = q.stride()
+        k0, k1, k2 = k.stride()
+        v0, v1, v2 = v.stride()
+        if q2 != 1 or k2 != 1 or v2 != 1:
             raise ValueError("A head's elements must be contiguous.")
         if key_cache is None and value_cache is None and slots is None:
             pool, key_ptr, value_ptr, slots_ptr, page_size, pages = (0, 0, 0, 0, 0, 0), 0, 0, 0, 0, 0
         elif key_cache is None or value_cache is None or slots is None:
             raise ValueError("The two caches and the slots go together.")
         else:
-            _check_vector("slots", slots, torch.int64, tokens, device)
-            pool, pages, page_size = _pool_layout(key_cache, value_cache, kv_heads, dim, dtype, device)
+            _check_vector("slots", slots, torch.int64, tokens, index)
+            pool, pages, page_size = _pool_layout(key_cache, value_cache, kv_heads, dim, dtype, index)
             key_ptr, value_ptr, slots_ptr = key_cache.data_ptr(), value_cache.data_ptr(), slots.data_ptr()
         if out is None:
-            with _on(stream):
-                out = torch.empty_like(q, memory_format=torch.contiguous_format)
-            os = (heads * dim, dim, 1)
+            out = _like(q, stream)
+            o0, o1 = heads * dim, dim
         else:
-            os = out.stride()
-            if out.shape != shape or out.dtype is not dtype or out.device != device or os[2] != 1:
+            o0, o1, o2 = out.stride() if out.dim() == 3 else (0, 0, 0)
+            if out.shape != shape or out.dtype is not dtype or out.get_device() != index or o2 != 1:
                 raise ValueError("`out` must be like q, with contiguous heads.")
         args = _native.ROTARY.pack(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), key_ptr, value_ptr, *self._tables,
-            positions.data_ptr(), slots_ptr, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1], *pool,
-            tokens, heads, kv_heads, dim, self.rotary_dim, self.interleaved, page_size, pages, self._positions, kind,
-            weight_type, self.eps)
-        _call(_native.lib().nz_rotary_store, device, args, stream)
+            positions.data_ptr(), slots_ptr, q0, q1, k0, k1, v0, v1, o0, o1, *pool, tokens, heads,
+            kv_heads, dim, self.rotary_dim, self.interleaved, page_size, pages, self._positions, kind, weight_type,
+            self.eps)
+        _call(_native.lib().nz_rotary_store, self._device, args, stream)
         return out
 
 
@@ -268,7 +283,8 @@ class AttentionPlan:
             raise ValueError("heads must be a positive multiple of kv_heads.")
         if contexts.dim() != 1 or contexts.dtype != torch.int32 or not contexts.is_cuda:
             raise ValueError("contexts must be an int32 vector on the GPU.")
-        self.rows, self.heads, self.kv_heads, self.device = contexts.shape[0], heads, kv_heads, contexts.device
+        self.rows, self.heads, self.kv_heads = contexts.shape[0], heads, kv_heads
+        self.device, self._index = contexts.device, contexts.get_device()
         self._parts = kv_heads * -(-(heads // kv_heads) // _HEADS)
         self._target = max(1, ATTENTION_WORKGROUPS // self._parts)
         self.capacity = (max(1, -(-self.rows // self._target)) + 1) * self._target
@@ -282,9 +298,9 @@ class AttentionPlan:
 
     def update(self, contexts, *, requests=None, stream=None):
         """Plans the same number of rows anew."""
-        _check_vector("contexts", contexts, torch.int32, self.rows, self.device)
+        _check_vector("contexts", contexts, torch.int32, self.rows, self._index)
         if requests is not None:
-            _check_vector("requests", requests, torch.int32, self.rows, self.device)
+            _check_vector("requests", requests, torch.int32, self.rows, self._index)
         rc = _native.lib().nz_attention_plan(contexts.data_ptr(), requests.data_ptr() if requests is not None else None,
                                              self.rows, self._target, self._parts, *self._pointers,
                                              _stream_handle(self.device, stream))
@@ -315,36 +331,35 @@ def paged_attention(q, key_cache, value_cache, tables, plan, *, scale=None, out=
     masked. Sums and softmax in 32 bits, in an order that only the plan
     decides. head_dim is a multiple of 16 up to 256; strides may be any that
     keep heads, tokens and pages on 16-byte boundaries."""
-    _refuse_gradients(q, key_cache, value_cache)
-    dtype, device, shape = q.dtype, q.device, q.shape
+    if torch.is_grad_enabled():
+        _refuse_gradients(q, key_cache, value_cache)
+    dtype, index, shape = q.dtype, q.get_device(), q.shape
     kind = _TYPES.get(dtype)
     if len(shape) != 3 or shape[0] != plan.rows or shape[1] != plan.heads or kind is None:
         raise ValueError(f"q must be ({plan.rows}, {plan.heads}, head_dim) in bfloat16, float16 or float32; "
                          f"got {tuple(shape)} {dtype}.")
     rows, heads, dim = shape
-    if device != plan.device or tables.device != device:
+    if index != plan._index or tables.get_device() != index:
         raise ValueError("q, the tables and the plan must be on one device.")
     table_shape = tables.shape
     if len(table_shape) != 2 or tables.dtype is not torch.int32 or not tables.is_contiguous():
         raise ValueError("tables must be a contiguous int32 (requests, max_pages).")
-    pool, pages, page_size = _pool_layout(key_cache, value_cache, plan.kv_heads, dim, dtype, device)
-    qs = q.stride()
+    pool, pages, page_size = _pool_layout(key_cache, value_cache, plan.kv_heads, dim, dtype, index)
+    q0, q1, q2 = q.stride()
     if out is None:
-        with _on(stream):
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        os = (heads * dim, dim, 1)
+        out = _like(q, stream)
+        o0, o1, o2 = heads * dim, dim, 1
     else:
-        os = out.stride()
-        if out.shape != shape or out.dtype is not dtype or out.device != device:
+        if out.shape != shape or out.dtype is not dtype or out.get_device() != index:
             raise ValueError("`out` must be like q.")
-    if qs[2] != 1 or os[2] != 1:
+        o0, o1, o2 = out.stride()
+    if q2 != 1 or o2 != 1:
         raise ValueError("A head's elements must be contiguous.")
-    handle = _stream_handle(device, stream)
+    handle = _stream_handle(plan.device, stream)
     args = _native.ATTENTION.pack(
         q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), out.data_ptr(), tables.data_ptr(),
-        *plan._pointers, plan._partials(dim, handle, stream), qs[0], qs[1], os[0], os[1], *pool, rows,
-        plan.capacity, heads, plan.kv_heads, dim, table_shape[0], table_shape[1], page_size, pages, kind,
-        dim ** -0.5 if scale is None else scale, 0)
+        *plan._pointers, plan._partials(dim, handle, stream), q0, q1, o0, o1, *pool, rows, plan.capacity, heads,
+        plan.kv_heads, dim, *table_shape, page_size, pages, kind, dim ** -0.5 if scale is None else scale, 0)
     rc = _native.lib().nz_attention(args, handle)
     if rc:
         _native.check(rc)
@@ -368,22 +383,23 @@ def adjust_logits(logits, *, history=None, lengths=None, prompt_lengths=None, re
     32)), token v's bit is bit v % 32 of word v // 32; mask_rows: int32 per
     row, the row's mask, -1 for none (row i has mask i by default). In 32
     bits, rounded once. `out` may be logits itself."""
-    _refuse_gradients(logits)
+    if torch.is_grad_enabled():
+        _refuse_gradients(logits)
     if logits.dim() != 2 or logits.dtype not in _TYPES or not logits.is_cuda or logits.stride(1) != 1:
         raise ValueError("logits must be (rows, vocab) in bfloat16, float16 or float32 on the GPU, rows contiguous.")
-    (rows, vocab), device = logits.shape, logits.device
+    (rows, vocab), index = logits.shape, logits.get_device()
     history_ptr = lengths_ptr = prompt_ptr = history_row = capacity = id_bytes = 0
     if history is not None:
         if history.dim() != 2 or history.shape[0] != rows or history.dtype not in (torch.int32, torch.int64) \
-                or history.device != device or (history.stride(1) != 1 and history.shape[1] > 1):
+                or history.get_device() != index or (history.stride(1) != 1 and history.shape[1] > 1):
             raise ValueError("history must be int32 or int64 (rows, capacity), rows contiguous, on the logits' device.")
         if lengths is None:
             raise ValueError("A history needs its lengths.")
-        _check_vector("lengths", lengths, torch.int32, rows, device)
+        _check_vector("lengths", lengths, torch.int32, rows, index)
         history_ptr, lengths_ptr = history.data_ptr(), lengths.data_ptr()
         capacity, history_row, id_bytes = history.shape[1], history.stride(0), history.element_size()
         if prompt_lengths is not None:
-            _check_vector("prompt_lengths", prompt_lengths, torch.int32, rows, device)
+            _check_vector("prompt_lengths", prompt_lengths, torch.int32, rows, index)
             prompt_ptr = prompt_lengths.data_ptr()
     elif lengths is not None or prompt_lengths is not None or repetition is not None or frequency is not None \
             or presence is not None:
@@ -391,37 +407,36 @@ def adjust_logits(logits, *, history=None, lengths=None, prompt_lengths=None, re
     factors = []
     for name, t in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
         if t is not None:
-            _check_vector(name, t, torch.float32, rows, device)
+            _check_vector(name, t, torch.float32, rows, index)
         factors.append(t.data_ptr() if t is not None else 0)
     bias_ptrs, n_bias = (0, 0, 0), 0
     if bias is not None:
         starts, tokens, values = bias
         n_bias = tokens.shape[0]
-        _check_vector("bias starts", starts, torch.int32, rows + 1, device)
-        _check_vector("bias tokens", tokens, torch.int32, n_bias, device)
-        _check_vector("bias values", values, torch.float32, n_bias, device)
+        _check_vector("bias starts", starts, torch.int32, rows + 1, index)
+        _check_vector("bias tokens", tokens, torch.int32, n_bias, index)
+        _check_vector("bias values", values, torch.float32, n_bias, index)
         bias_ptrs = (starts.data_ptr(), tokens.data_ptr(), values.data_ptr())
     masks_ptr = mask_rows_ptr = n_masks = 0
     if masks is not None:
         if masks.dim() != 2 or masks.dtype != torch.int32 or masks.shape[1] != (vocab + 31) // 32 \
-                or masks.device != device or not masks.is_contiguous():
+                or masks.get_device() != index or not masks.is_contiguous():
             raise ValueError(f"masks must be contiguous int32 (masks, {(vocab + 31) // 32}) on the logits' device.")
         masks_ptr, n_masks = masks.data_ptr(), masks.shape[0]
         if mask_rows is not None:
-            _check_vector("mask_rows", mask_rows, torch.int32, rows, device)
+            _check_vector("mask_rows", mask_rows, torch.int32, rows, index)
             mask_rows_ptr = mask_rows.data_ptr()
         elif n_masks != rows:
             raise ValueError("Without mask_rows there must be one mask per row.")
     elif mask_rows is not None:
         raise ValueError("mask_rows need masks.")
     if out is None:
-        with _on(stream):
-            out = torch.empty_like(logits, memory_format=torch.contiguous_format)
-    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != device or out.stride(1) != 1:
+        out = _like(logits, stream)
+    elif out.shape != logits.shape or out.dtype != logits.dtype or out.get_device() != index or out.stride(1) != 1:
         raise ValueError("`out` must be like logits, rows contiguous.")
     args = _native.LOGITS.pack(
         logits.data_ptr(), out.data_ptr(), history_ptr, lengths_ptr, prompt_ptr, *factors, *bias_ptrs, masks_ptr,
         mask_rows_ptr, logits.stride(0), out.stride(0), history_row, rows, vocab, capacity, n_bias, n_masks,
         _TYPES[logits.dtype], id_bytes, 0)
-    _call(_native.lib().nz_adjust_logits, device, args, stream)
+    _call(_native.lib().nz_adjust_logits, logits.device, args, stream)
     return out
