@@ -517,11 +517,11 @@ int nz_clusterer_count(const nz_clusterer* clusterer, uint32_t* n_clusters);
  * The kernels check every page, slot, request, position and token number
  * that they read from device memory against the sizes given here, so wrong
  * ones give wrong results (as said at each entry) but no access out of
- * bounds. */
+ * bounds. Structs hold device pointers to dense arrays but for the strides
+ * given. */
 
 enum nz_value_type { NZ_BF16 = 0, NZ_FP16 = 1, NZ_FP32 = 2 };
 
-/* All pointers are device pointers; arrays are dense. */
 typedef struct nz_pages_extend_args {
     const int32_t* lengths;      /* n_requests: tokens of each request       */
     const int32_t* new_tokens;   /* n_requests: tokens it gets in this step  */
@@ -553,9 +553,10 @@ enum nz_pages_status {
 
 /* Takes in a step's new tokens. In request order, a request is refused
  * (gets no token, and status says why) if its length would be negative or
- * pass max_pages * page_size; else if it asks for tokens and the sum of what
- * it and those before it that fitted ask for passes max_tokens; else if it needs pages and
- * the sum of the pages that it and those before it not refused so far need passes *n_free. The others' pages come
+ * pass max_pages * page_size; else if it asks for tokens and what it and
+ * those before it that passed the first test ask for comes to more than
+ * max_tokens; else if it needs pages and what it and those before it that
+ * passed both tests need comes to more than *n_free. The others' pages come
  * off the stack in order (from the top, free_pages[n_free - 1], downwards)
  * and into their table rows; the new tokens are listed request by request.
  * Entries past the last token hold slot -1, position 0, request -1 and
@@ -683,9 +684,10 @@ uint64_t nz_attention_partials(uint32_t n_items, uint32_t heads, uint32_t head_d
  * its request's pages; head h reads key-value head h / (heads / kv_heads). A
  * row without keys gives zeros. Keys whose page or request is not in range
  * count as masked. head_dim is a multiple of 16, at most 256; strides and
- * addresses are multiples of 16 bytes. Calls with one plan must not
- * overlap: they share its counters, which each call leaves as it found them.
- * n_items * heads * head_dim is below 2^30. */
+ * addresses are multiples of 16 bytes. Items and counters are taken as
+ * nz_attention_plan wrote them, for the same heads. Calls with one plan must
+ * not overlap: they share its counters, which each call leaves as it found
+ * them. n_items * heads * head_dim is below 2^30. */
 int nz_attention(const nz_attention_args* args, void* stream);
 
 typedef struct nz_logits_args {
@@ -717,8 +719,8 @@ typedef struct nz_logits_args {
  * is in the row's history; minus frequency times its count and presence
  * (once) if it is in the history after the prompt; plus the row's bias for
  * it (its last entry counts); -infinity where the row's mask has no bit (bit
- * v % 32 of word v / 32). In 32 bits, rounded once. Ids outside the
- * vocabulary are ignored. */
+ * v % 32 of word v / 32; a mask outside n_masks masks nothing). In 32 bits,
+ * rounded once. Ids outside the vocabulary are ignored. */
 int nz_adjust_logits(const nz_logits_args* args, void* stream);
 
 #ifdef __cplusplus

@@ -171,7 +171,8 @@ int nz_adjust_logits(const nz_logits_args* args, void* stream) {
         type_size(a.type);
         if (a.reserved) refuse("reserved is 0.");
         if (a.rows == 0 || a.vocab == 0) return true;
-        if (!a.logits || !a.out || (a.history && !a.lengths) || (a.bias_starts && a.n_bias && (!a.bias_tokens || !a.bias_values)))
+        if (!a.logits || !a.out || (a.history && !a.lengths) ||
+            (a.bias_starts && a.n_bias && (!a.bias_tokens || !a.bias_values)))
             refuse("Null logits argument.");
         if (a.history && a.history_bytes != 4 && a.history_bytes != 8) refuse("Token ids are of 4 or 8 bytes.");
         if (a.vocab > kMaxGrid || a.rows > 65535) refuse("Too many rows or tokens in one call.");

@@ -56,7 +56,8 @@ __device__ uint32_t shortest_share(const int32_t* contexts, uint32_t n_rows, uin
     const uint32_t wave = threadIdx.x >> 6;
     // keys / share <= items < n_rows + keys / share
     const uint64_t below_all = keys / (static_cast<uint64_t>(limit) * kTile);
-    uint32_t lo = static_cast<uint32_t>(std::max<uint64_t>(least, std::min<uint64_t>(below_all, longest))), hi = max(longest, lo);
+    uint32_t lo = static_cast<uint32_t>(std::max<uint64_t>(least, std::min<uint64_t>(below_all, longest)));
+    uint32_t hi = max(longest, lo);
     if (limit > n_rows) {
         const uint64_t enough = keys / (static_cast<uint64_t>(limit - n_rows) * kTile) + 1;
         hi = max(static_cast<uint32_t>(min<uint64_t>(enough, hi)), lo);
@@ -86,11 +87,10 @@ __device__ uint32_t shortest_share(const int32_t* contexts, uint32_t n_rows, uin
 // (in whole rounds of the units: 32 rows of up to 8191 keys over 8 heads 98 us
 // with 64 items and 111 with 48). Latency bound: 5 us for one row of 2001
 // keys, 9 for 64 ragged rows, once a step.
-__global__ __launch_bounds__(kPlanThreads) void nz_attention_plan_kernel(const int32_t* __restrict__ contexts,
-                                                                         const int32_t* __restrict__ requests,
-                                                                         uint32_t n_rows, uint32_t target, uint32_t parts,
-                                                                         nz_attention_item* __restrict__ items,
-                                                                         uint32_t* __restrict__ counters) {
+__global__ __launch_bounds__(kPlanThreads)
+void nz_attention_plan_kernel(const int32_t* __restrict__ contexts, const int32_t* __restrict__ requests,
+                              uint32_t n_rows, uint32_t target, uint32_t parts, nz_attention_item* __restrict__ items,
+                              uint32_t* __restrict__ counters) {
     __shared__ PlanLds lds;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint64_t keys = 0;
@@ -297,15 +297,30 @@ struct Shape {
 };
 
 // One item: 16 query heads' softmax over the keys begin .. end - 1 of one
-// key-value head, tile by tile with a running maximum and sum. Scores are
-// computed transposed (keys are rows, heads columns), so that a lane's
-// scores of a tile are the very elements it needs as the second operand of
-// the product with the values: its four rows of each 16 keys. The values are
-// loaded whole rows at a time, each lane some neighbours of the keys its
-// scores belong to, and transposed in registers; no LDS until the
-// wavefronts' sums are joined.
+// key-value head, tile by tile with a running maximum and sum:
+//   m' = max(m, s_j), l' = l 2^(m - m') + sum_j 2^(s_j - m'),
+//   o' = o 2^(m - m') + sum_j 2^(s_j - m') v_j, s_j = scale log2(e) q . k_j.
+// Bound by HBM: 4 or 8 query heads read each key, a sixteenth of what the
+// matrix instructions could do with it, so they may have idle columns and
+// multiply by split weights. 64 rows of 100 to 16384 keys, 64 heads over 8 of
+// 128 fp16 elements (2.16 GB), take 370 to 394 us by the rows' order, 5.5 to
+// 5.8 TB/s; 32 rows of up to 8191 keys, 32 heads over 8 in bf16 (488 MB), 93
+// us; one row of 2001 keys 8.7 us, of which starting takes 2.7 and the join
+// of the items 2.7.
+// Scores are computed transposed (keys are rows, heads columns), so that a
+// lane's scores of a tile are the very elements it needs as the second
+// operand of the product with the values: its four rows of each 16 keys. The
+// values are loaded whole rows at a time, each lane some neighbours of the
+// keys its scores belong to, and transposed in registers; no LDS until the
+// wavefronts' sums are joined. Four wavefronts take every fourth tile of 32
+// keys, each with the next tile's keys under way: three such workgroups a
+// compute unit (two-byte types, up to 128 elements) keep 190 KB in flight.
+// 16-bit types of up to 128 elements are held to the registers of three
+// wavefronts a SIMD: 483 us for the 2.16 GB, 491 without, before the join
+// was part of this kernel.
 template <typename T, uint32_t DP, bool FULL>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 128 && sizeof(T) == 2 ? 3 : 1))) void nz_attention_kernel(nz_attention_args a) {
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 128 && sizeof(T) == 2 ? 3 : 1)))
+void nz_attention_kernel(nz_attention_args a) {
     using S = Shape<T, DP>;
     using P = Piece<T>;
     using piece = typename P::type;
@@ -367,7 +382,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 
 #pragma unroll
             for (uint32_t h = 0; h < S::kHalves; ++h) {
                 const int64_t p = static_cast<uint32_t>(page[h]) < a.n_pages ? page[h] : 0;
-                const T* src = key_base + p * a.key_page + static_cast<int64_t>((t0 + 16 * h) & place_mask) * a.key_slot;
+                const int64_t place = (t0 + 16 * h) & place_mask;
+                const T* src = key_base + p * a.key_page + place * a.key_slot;
 #pragma unroll
                 for (uint32_t s = 0; s < S::kKeySteps; ++s) {
                     const uint32_t d = s * 4 * S::kRun + quad * S::kRun;
@@ -392,7 +408,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 
                 const bool valid = static_cast<uint32_t>(page[h]) < a.n_pages;
                 const int64_t p = valid ? page[h] : 0;
                 limit[h] = valid ? end : 0;
-                values[h] = value_base + p * a.value_page + static_cast<int64_t>((t0 + 16 * h) & place_mask) * a.value_slot;
+                const int64_t place = (t0 + 16 * h) & place_mask;
+                values[h] = value_base + p * a.value_page + place * a.value_slot;
             }
             value_run v[S::kGroups][S::kValueSteps][S::kRun];
 #pragma unroll
@@ -535,7 +552,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 
         }
     }
     if (whole) return;
-    // The last of the row's items to arrive joins them all, in their order.
+    // The last of the row's items to arrive joins them all, in their order (a
+    // launch of its own for that took 118 us in all where one row's 2001 keys
+    // now take 8.7, and an arrival with a release fence 19).
     uint32_t* const counter = a.counters + static_cast<uint64_t>(item.first) * per_item + part;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wavefront's stores have arrived
     __syncthreads();

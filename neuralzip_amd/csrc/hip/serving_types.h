@@ -74,7 +74,8 @@ __device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __b
 
 template <int CTRL, int ROWS>
 __device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
-    return add_sat(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false)));
+    const int below = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false);
+    return add_sat(v, static_cast<uint32_t>(below));
 }
 
 // Inclusive saturating prefix sum over the wavefront: shifts of 1, 2, 4 and 8

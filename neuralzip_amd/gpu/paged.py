@@ -87,7 +87,8 @@ class PagedDecoder:
         self._prompts = filled(0, torch.int32)
         self._penalties = {}
         if (repetition, frequency, presence) != (1.0, 0.0, 0.0):
-            self._penalties = dict(repetition=filled(repetition), frequency=filled(frequency), presence=filled(presence))
+            self._penalties = dict(repetition=filled(repetition), frequency=filled(frequency),
+                                   presence=filled(presence))
         self.masks = torch.full((requests, (self.vocab + 31) // 32), -1, dtype=torch.int32,
                                 device=self.device) if grammar else None
         self.logits = None                            # of the last step, in token order, as adjusted

@@ -50,6 +50,8 @@ def _like(t, stream):
 
 
 def _call(function, device, args, stream):
+    if device.type != "cuda":
+        raise ValueError("The serving operators run on the GPU.")
     rc = function(args, _stream_handle(device, stream))
     if rc:
         _native.check(rc)

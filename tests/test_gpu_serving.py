@@ -276,14 +276,15 @@ def test_rotary_positions_outside_the_tables_give_nan():
     cos, sin = angles(4, 16)
     q = randn(3, 1, 64)
     out = serving.Rotary(cos, sin)(q, q, q, ints([3, 4, -1]))
-    assert torch.isfinite(out[0]).all() and out[1:, :, :32].isnan().all() and torch.equal(out[1:, :, 32:], q[1:, :, 32:])
+    assert torch.isfinite(out[0]).all() and out[1:, :, :32].isnan().all()
+    assert torch.equal(out[1:, :, 32:], q[1:, :, 32:])
 
 
 def test_rotary_norm_of_extreme_heads():
     """A head of zeros, one whose squares are small against eps, and one of
     large fp16 values, whose squares pass fp16's range."""
     cos, sin = angles(1, 32)
-    q = torch.cat([torch.zeros(1, 64), torch.full((1, 64), 2.0 ** -14), torch.full((1, 64), 60000.0)]).half().to(DEVICE)[None]
+    q = torch.tensor([0.0, 2.0 ** -14, 60000.0], dtype=torch.float16, device=DEVICE)[None, :, None].repeat(1, 1, 64)
     out = serving.Rotary(cos, sin, q_weight=torch.ones(64, device=DEVICE))(q, q, q, ints([0]))
     want = plain_rotary(q, cos, sin, ints([0]), torch.ones(64, device=DEVICE), 1e-6, False)
     assert ((out.double() - want).abs() <= 2 * unit(torch.float16) * want.abs().clamp(min=2.0 ** -14)).all()
@@ -370,7 +371,8 @@ def test_attention_of_every_head_size(dtype, dim):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("heads, kv_heads", [(1, 1), (3, 3), (8, 1), (14, 2), (32, 8), (16, 1), (17, 1), (71, 1), (40, 2)])
+@pytest.mark.parametrize("heads, kv_heads", [(1, 1), (3, 3), (8, 1), (14, 2), (32, 8), (16, 1), (17, 1), (71, 1),
+                                             (40, 2)])
 def test_attention_of_shared_heads(dtype, heads, kv_heads):
     check_attention(dtype, heads, kv_heads, 64, 32, [40, 0, 7, 100], seed=heads)
 
@@ -590,7 +592,8 @@ def test_logits_against_64_bits(dtype, vocab, parts):
         history = [[rng.randrange(-1, top) if rng.random() < 0.9 else vocab - 1 + rng.randrange(3)
                     for _ in range(capacity)] for _ in range(rows)]
         lengths, prompt = [capacity, 0, 1, 57], [30, 5, 0, 100]
-        repetition, frequency, presence = f32([1.3, 2.0, 0.7, 1.0]), f32([0.1, 0.0, -0.2, 0.5]), f32([0.3, 1.0, 0.0, -0.4])
+        repetition, frequency = f32([1.3, 2.0, 0.7, 1.0]), f32([0.1, 0.0, -0.2, 0.5])
+        presence = f32([0.3, 1.0, 0.0, -0.4])
     if parts in ("bias", "all"):
         starts = [0, 0, 3, 10, 17]
         bias = (starts, [rng.choice((0, vocab - 1, rng.randrange(vocab), vocab, -3)) for _ in range(17)],
@@ -750,11 +753,13 @@ def test_refusals_that_need_the_device():
     with pytest.raises(ValueError, match="tables"):
         serving.paged_attention(q, keys, values, tables.long(), plan)
     with pytest.raises(ValueError, match="contiguous"):
-        serving.paged_attention(torch.zeros(2, 4, 128, dtype=q.dtype, device=DEVICE)[..., ::2], keys, values, tables, plan)
+        serving.paged_attention(torch.zeros(2, 4, 128, dtype=q.dtype, device=DEVICE)[..., ::2], keys, values, tables,
+                                plan)
     with pytest.raises(ValueError, match="no backward"):
         serving.paged_attention(q.clone().requires_grad_(), keys, values, tables, plan)
     with pytest.raises(ValueError, match="16 bytes"):
-        serving.paged_attention(torch.zeros(2, 4, 65, dtype=q.dtype, device=DEVICE)[..., :64], keys, values, tables, plan)
+        serving.paged_attention(torch.zeros(2, 4, 65, dtype=q.dtype, device=DEVICE)[..., :64], keys, values, tables,
+                                plan)
     with pytest.raises(ValueError, match="power of two"):
         serving.paged_attention(q, *(torch.zeros(3, 2, 24, 64, dtype=q.dtype, device=DEVICE) for _ in range(2)), tables,
                                 plan)

@@ -43,8 +43,8 @@ def test_packed_arguments_match_the_header(name, tmp_path):
     expanded = "".join(c * int(n or 1) for n, c in re.findall(r"(\d*)([A-Za-z])", codes))
     assert [8 if c in "qQ" else 4 for c in expanded] == sizes
     probe = tmp_path / "size.c"
-    probe.write_text(f'#include <stdio.h>\n#include "neuralzip_hip.h"\nint main(void) {{ printf("%zu", sizeof({name})); '
-                     "return 0; }\n")
+    probe.write_text('#include <stdio.h>\n#include "neuralzip_hip.h"\n'
+                     f'int main(void) {{ printf("%zu", sizeof({name})); return 0; }}\n')
     subprocess.run(["gcc", "-std=c99", "-I", str(HEADER.parent), str(probe), "-o", str(tmp_path / "size")], check=True)
     size = int(subprocess.run([str(tmp_path / "size")], check=True, capture_output=True, text=True).stdout)
     assert size == STRUCTS[name].size == sum(sizes)
@@ -79,9 +79,9 @@ ROTARY = dict(q=True, k=True, v=True, out=True, key_cache=True, value_cache=True
               slots=True, q_token=128, q_head=64, k_token=128, k_head=64, v_token=128, v_head=64, out_token=128,
               out_head=64, key_page=2048, key_head=1024, key_slot=64, value_page=2048, value_head=1024, value_slot=64,
               tokens=3, heads=2, kv_heads=2, head_dim=64, rotary_dim=64, page_size=16, n_pages=4, n_positions=10)
-ATTENTION = dict(q=True, key_cache=True, value_cache=True, out=True, tables=True, items=True, counters=True, partials=True, q_row=128,
-                 q_head=64, out_row=128, out_head=64, key_page=2048, key_head=1024, key_slot=64, value_page=2048,
-                 value_head=1024, value_slot=64, n_rows=2, n_items=4, heads=2, kv_heads=2, head_dim=64, n_requests=2,
+ATTENTION = dict(q=True, key_cache=True, value_cache=True, out=True, tables=True, items=True, counters=True,
+                 partials=True, q_row=128, q_head=64, out_row=128, out_head=64, key_page=2048, key_head=1024, key_slot=64,
+                 value_page=2048, value_head=1024, value_slot=64, n_rows=2, n_items=4, heads=2, kv_heads=2, head_dim=64, n_requests=2,
                  max_pages=3, page_size=16, n_pages=4)
 LOGITS = dict(logits=True, out=True, rows=2, vocab=100, logits_row=100, out_row=100)
 
@@ -146,9 +146,9 @@ def test_null_argument_structs_and_plans_are_refused():
     lib = _native.lib()
     for function in ("nz_pages_extend", "nz_pages_release", "nz_rotary_store", "nz_attention", "nz_adjust_logits"):
         assert getattr(lib, function)(None, None) == -1 and b"Null" in lib.nz_last_error()
-    for wrong in ((None, None, 1, 1, 8, 4096, 4096), (4096, None, 1, 1, 8, None, 4096), (4096, None, 1, 1, 8, 4096, None),
-                  (4096, None, 1, 0, 8, 4096, 4096), (4096, None, 1, 1, 0, 4096, 4096),
-                  (4096, None, 1 << 31, 1, 8, 4096, 4096)):
+    for wrong in ((None, None, 1, 1, 8, 4096, 4096), (4096, None, 1, 1, 8, None, 4096),
+                  (4096, None, 1, 1, 8, 4096, None), (4096, None, 1, 0, 8, 4096, 4096),
+                  (4096, None, 1, 1, 0, 4096, 4096), (4096, None, 1 << 31, 1, 8, 4096, 4096)):
         assert lib.nz_attention_plan(*wrong, None) == -1
     assert lib.nz_attention_partials(10, 32, 128) == 10 * 32 * 130
 
@@ -177,6 +177,10 @@ def test_python_entries_refuse_wrong_tensors():
         book.extend(f(3, dtype=torch.int32), 4, out=serving.Step(3, 5, "cpu"))
     with pytest.raises(ValueError, match="done"):
         book.release(f(3))
+    with pytest.raises(ValueError, match="on the GPU"):
+        book.extend(f(3, dtype=torch.int32), 4)
+    with pytest.raises(ValueError, match="on the GPU"):
+        book.release(f(3, dtype=torch.bool))
     with pytest.raises(ValueError, match="rotary_dim"):
         serving.Rotary(f(4, 12), f(4, 12))
     with pytest.raises(ValueError, match="cos and sin"):
@@ -203,6 +207,9 @@ def test_python_entries_refuse_wrong_tensors():
         rotary(q, k, k, at, slots=at.long())
     with pytest.raises(ValueError, match="Caches"):
         rotary(q, k, k, at, at.long(), f(4, 3, 16, 16), f(4, 3, 16, 16))
+    for extra in ((), (at.long(), f(4, 2, 16, 16), f(4, 2, 16, 16))):
+        with pytest.raises(ValueError, match="on the GPU"):
+            rotary(q, k, k, at, *extra)
     with pytest.raises(ValueError, match="contexts"):
         serving.AttentionPlan(at, heads=4, kv_heads=2)   # not on the GPU
     with pytest.raises(ValueError, match="multiple of kv_heads"):
