@@ -652,6 +652,59 @@ def test_logits_of_long_histories():
     assert not got.any()
 
 
+# ------------------------------------------------ strides beyond 32 bits
+
+def test_rows_that_lie_more_than_32_bits_apart():
+    """Queries, outputs, logits and histories whose rows are over 2^31
+    elements from one another: the same bits as from dense rows."""
+    far, dim = (1 << 31) + 64, 64
+    memory = torch.empty(2 * far + 4096, dtype=torch.bfloat16, device=DEVICE)
+    outside = torch.empty(2 * far + 4096, dtype=torch.bfloat16, device=DEVICE)
+    contexts = [40, 3, 17]
+    q, keys, values, tables, _ = attention_case(torch.bfloat16, 4, 2, dim, 16, contexts)
+    wide, out = (m.as_strided((3, 4, dim), (far, dim, 1)) for m in (memory, outside))
+    wide.copy_(q)
+    plan = serving.AttentionPlan(ints(contexts), heads=4, kv_heads=2)
+    want = serving.paged_attention(q, keys, values, tables, plan)
+    assert torch.equal(serving.paged_attention(wide, keys, values, tables, plan, out=out), want)
+    cos, sin = angles(9, 16)
+    op, positions = serving.Rotary(cos, sin), ints([3, 8, 0])
+    k = randn(3, 2, dim, seed=4, dtype=torch.bfloat16)
+    assert torch.equal(op(wide, k, k, positions, out=out), op(q, k, k, positions))
+    wide, out = (m.as_strided((3, 1000), (far, 1)) for m in (memory, outside))
+    logits = randn(3, 1000, seed=6, dtype=torch.bfloat16)
+    wide.copy_(logits)
+    history = torch.arange(60, device=DEVICE).view(3, 20).int()
+    penalty = dict(lengths=ints([20, 7, 20]), repetition=torch.tensor([1.5, 2.0, 3.0], device=DEVICE))
+    want = serving.adjust_logits(logits, history=history, **penalty)
+    assert torch.equal(serving.adjust_logits(wide, history=history, out=out, **penalty), want)
+    apart = outside.view(torch.int32).as_strided((3, 20), (far // 2, 1))
+    apart.copy_(history)
+    assert torch.equal(serving.adjust_logits(logits, history=apart, **penalty), want)
+    del memory, outside, wide, out, apart
+    torch.cuda.empty_cache()
+
+
+def test_rotary_of_many_tokens():
+    """More heads than one round of workgroups, every token's place checked."""
+    tokens, heads, kv_heads, dim, page = 5000, 8, 4, 128, 32
+    q, k, v = (randn(tokens, h, dim, seed=h, dtype=torch.float16) for h in (heads, kv_heads, kv_heads + 1))
+    v = v[:, :kv_heads]
+    cos, sin = angles(5000, 64)
+    positions = torch.randperm(tokens, device=DEVICE).int()
+    pages = pages_of(tokens, page) + 1
+    slots = torch.randperm(pages * page, device=DEVICE)[:tokens]
+    caches = [torch.zeros(pages, kv_heads, page, dim, dtype=torch.float16, device=DEVICE) for _ in range(2)]
+    weight = randn(dim, seed=9)
+    out = serving.Rotary(cos, sin, q_weight=weight, k_weight=weight)(q, k, v, positions, slots, *caches)
+    want = plain_rotary(q, cos, sin, positions, weight, 1e-6, False)
+    assert ((out.double() - want).abs() <= rotary_bound(want, q, weight, torch.float16)).all()
+    want = plain_rotary(k, cos, sin, positions, weight, 1e-6, False)
+    got = caches[0].transpose(1, 2).reshape(-1, kv_heads, dim)[slots].double()
+    assert ((got - want).abs() <= rotary_bound(want, k, weight, torch.float16)).all()
+    assert torch.equal(caches[1].transpose(1, 2).reshape(-1, kv_heads, dim)[slots], v)
+
+
 # --------------------------------------------------- streams, graphs, a step
 
 def small_step(book, caches, op, new, most, seed):
