@@ -311,10 +311,23 @@ constexpr uint32_t kLogitsThreads = 1024;
 // Tokens of the vocabulary that a workgroup takes and counts in LDS.
 constexpr uint32_t kLogitsChunk = 8192;
 
-__device__ __forceinline__ int64_t history_id(const nz_logits_args& a, uint32_t row, uint32_t i) {
-    const uint64_t at = static_cast<uint64_t>(row) * static_cast<uint64_t>(a.history_row) + i;
-    return a.history_bytes == 8 ? static_cast<const int64_t*>(a.history)[at]
-                                : static_cast<int64_t>(static_cast<const int32_t*>(a.history)[at]);
+// Calls note(i, id) for the ids 0 .. length - 1 at `ids`: 16 bytes at a time
+// where they lie on such boundaries, one by one at the ends.
+template <typename ID, typename Note>
+__device__ __forceinline__ void for_history(const ID* ids, uint32_t length, const Note& note) {
+    constexpr uint32_t kRun = run_of<ID>();
+    const uint32_t skip = min(static_cast<uint32_t>(-reinterpret_cast<uintptr_t>(ids) % 16 / sizeof(ID)), length);
+    const uint32_t runs = (length - skip) / kRun, rest = length - runs * kRun;
+#pragma unroll 4
+    for (uint32_t j = threadIdx.x; j < runs; j += kLogitsThreads) {
+        const vec<ID, kRun> v = *reinterpret_cast<const vec<ID, kRun>*>(ids + skip + j * kRun);
+#pragma unroll
+        for (uint32_t e = 0; e < kRun; ++e) note(skip + j * kRun + e, static_cast<int64_t>(v[e]));
+    }
+    for (uint32_t e = threadIdx.x; e < rest; e += kLogitsThreads) {
+        const uint32_t i = e < skip ? e : e + runs * kRun;
+        note(i, static_cast<int64_t>(ids[i]));
+    }
 }
 
 // One workgroup: kLogitsChunk neighbouring tokens of a row, the first on a
@@ -327,7 +340,8 @@ __device__ __forceinline__ int64_t history_id(const nz_logits_args& a, uint32_t 
 // L2. Bound by memory, once the history is short against the vocabulary: 32
 // rows of 128256 fp32 logits with everything on (33 MB) take 9.7 us, one row of
 // 151936 bf16 logits 4.0; the first were 12.8 us with chunks of 2048, 11.3 of
-// 4096 and 10.6 of 8192 tokens (a history of 8000: 27, 21 and 18 for 64 rows).
+// 4096 and 10.6 of 8192 tokens (64 rows with up to 8000 ids 27, 21 and 18, and
+// 16 with ids read 16 bytes at a time).
 // VECTOR: logits and out lie alike on 16-byte boundaries.
 template <typename T, bool VECTOR>
 __global__ __launch_bounds__(kLogitsThreads) void nz_logits_kernel(nz_logits_args a) {
@@ -378,14 +392,16 @@ __global__ __launch_bounds__(kLogitsThreads) void nz_logits_kernel(nz_logits_arg
     if (a.history != nullptr) {
         const uint32_t length = min(static_cast<uint32_t>(max(a.lengths[row], 0)), a.history_capacity);
         const uint32_t prompt = a.prompt_lengths ? static_cast<uint32_t>(max(a.prompt_lengths[row], 0)) : 0;
-#pragma unroll 4
-        for (uint32_t i = threadIdx.x; i < length; i += kLogitsThreads) {
-            const uint64_t v = static_cast<uint64_t>(history_id(a, row, i) - v0);
+        const uint64_t first = static_cast<uint64_t>(row) * static_cast<uint64_t>(a.history_row);
+        const auto note = [&](uint32_t i, int64_t id) {
+            const uint64_t v = static_cast<uint64_t>(id - v0);
             if (v < kLogitsChunk) {
                 if (i < prompt) atomicOr(&counts[v], 0x80000000u);
                 else atomicAdd(&counts[v], 1u);
             }
-        }
+        };
+        if (a.history_bytes == 8) for_history(static_cast<const int64_t*>(a.history) + first, length, note);
+        else for_history(static_cast<const int32_t*>(a.history) + first, length, note);
     }
     if (a.bias_starts != nullptr) {
         const uint32_t e0 = min(static_cast<uint32_t>(max(a.bias_starts[row], 0)), a.n_bias);

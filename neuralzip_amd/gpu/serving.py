@@ -97,12 +97,18 @@ class Step:
     first token; one more entry ends the last), `status` (PAGES_OK, or why it
     got no token) and `lengths` after the step; `n_free`, the free stack's
     height after it."""
-    __slots__ = ("slots", "positions", "requests", "contexts", "starts", "status", "lengths", "n_free", "max_tokens")
+    __slots__ = ("slots", "positions", "requests", "contexts", "starts", "status", "lengths", "n_free", "max_tokens",
+                 "_sizes", "_pointers")
 
     def __init__(self, n_requests, max_tokens, device):
         self.max_tokens = max_tokens
         # one allocation: 8-byte slots first, then the 4-byte arrays
         words = torch.empty(5 * max_tokens + 3 * n_requests + 2, dtype=torch.int32, device=device)
+        self._sizes = n_requests, max_tokens, words.get_device()
+        at, starts = words.data_ptr(), words.data_ptr() + 20 * max_tokens
+        self._pointers = (at, at + 8 * max_tokens, at + 12 * max_tokens, at + 16 * max_tokens, starts,
+                          starts + 4 * (n_requests + 1), starts + 4 * (2 * n_requests + 1),
+                          starts + 4 * (3 * n_requests + 1))
         (slots, self.positions, self.requests, self.contexts, self.starts, self.status, self.lengths,
          self.n_free) = torch.split_with_sizes(words, (2 * max_tokens, max_tokens, max_tokens, max_tokens,
                                                        n_requests + 1, n_requests, n_requests, 1))
@@ -125,7 +131,7 @@ class PageTables:
     `lengths` (int32, one per request), `tables` (int32, requests x
     max_pages; entries past a request's pages mean nothing), `free` and
     `n_free` (the stack of unused pages and its height) are the state, on the
-    device; they may be set by hand. All requests start empty and all pages
+    device; they may be written by hand. All requests start empty and all pages
     free, the lowest on top. Calls that change one PageTables run one after
     another, on one stream or ordered by events."""
 
@@ -135,11 +141,17 @@ class PageTables:
         if requests < 1 or max_pages < 1 or num_pages < 1 or max_pages * page_size >= 1 << 31:
             raise ValueError("There must be requests and pages, and a request's tokens must be below 2**31.")
         self.requests, self.max_pages, self.page_size, self.num_pages = requests, max_pages, page_size, num_pages
-        self.lengths = torch.zeros(requests, dtype=torch.int32, device=device)
+        self._state = (torch.zeros(requests, dtype=torch.int32, device=device),
+                       torch.full((requests, max_pages), -1, dtype=torch.int32, device=device),
+                       torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=device),
+                       torch.full((1,), num_pages, dtype=torch.int32, device=device))
+        self._pointers = tuple(t.data_ptr() for t in self._state)
         self.device, self._index = self.lengths.device, self.lengths.get_device()
-        self.tables = torch.full((requests, max_pages), -1, dtype=torch.int32, device=device)
-        self.free = torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=device)
-        self.n_free = torch.full((1,), num_pages, dtype=torch.int32, device=device)
+
+    lengths = property(lambda self: self._state[0])
+    tables = property(lambda self: self._state[1])
+    free = property(lambda self: self._state[2])
+    n_free = property(lambda self: self._state[3])
 
     def extend(self, new_tokens, max_tokens, *, advance=True, out=None, stream=None):
         """Gives every request its `new_tokens` (int32, one per request) new
@@ -158,14 +170,12 @@ class PageTables:
         if out is None:
             with _on(stream):
                 out = Step(self.requests, max_tokens, self.device)
-        elif out.max_tokens != max_tokens or out.lengths.shape != self.lengths.shape:
+        elif out._sizes != (self.requests, max_tokens, self._index):
             raise ValueError("`out` is a Step of other sizes.")
-        args = _native.PAGES_EXTEND.pack(
-            self.lengths.data_ptr(), new_tokens.data_ptr(), self.tables.data_ptr(), self.free.data_ptr(),
-            self.n_free.data_ptr(), out.slots.data_ptr(), out.positions.data_ptr(), out.requests.data_ptr(),
-            out.contexts.data_ptr(), out.starts.data_ptr(), out.status.data_ptr(), out.lengths.data_ptr(),
-            out.n_free.data_ptr(), self.requests, self.max_pages, self.page_size,
-            self.num_pages, max_tokens, bool(advance))
+        lengths, tables, free, n_free = self._pointers
+        args = _native.PAGES_EXTEND.pack(lengths, new_tokens.data_ptr(), tables, free, n_free, *out._pointers,
+                                         self.requests, self.max_pages, self.page_size, self.num_pages, max_tokens,
+                                         bool(advance))
         _call(_native.lib().nz_pages_extend, self.device, args, stream)
         return out
 
@@ -176,10 +186,10 @@ class PageTables:
         _check_vector("done", done, torch.bool, self.requests, self._index)
         with _on(stream):
             out = Released(self.requests, self.device)
-        args = _native.PAGES_RELEASE.pack(
-            self.lengths.data_ptr(), done.data_ptr(), self.tables.data_ptr(), self.free.data_ptr(),
-            self.n_free.data_ptr(), out.lengths.data_ptr(), out.n_free.data_ptr(), self.requests, self.max_pages,
-            self.page_size, self.num_pages, bool(advance), 0)
+        lengths, tables, free, n_free = self._pointers
+        args = _native.PAGES_RELEASE.pack(lengths, done.data_ptr(), tables, free, n_free, out.lengths.data_ptr(),
+                                          out.n_free.data_ptr(), self.requests, self.max_pages, self.page_size,
+                                          self.num_pages, bool(advance), 0)
         _call(_native.lib().nz_pages_release, self.device, args, stream)
         return out
 
