@@ -101,10 +101,11 @@ class PagedDecoder:
     def add(self, ids):
         """Takes in a prompt (1-D token ids), picks its first answer token
         and returns the request's place."""
-        ids = torch.as_tensor(ids, dtype=torch.int64, device=self.device)
-        n = ids.shape[0]
-        if ids.dim() != 1 or not 0 < n <= self.max_length:
-            raise ValueError(f"A prompt is a vector of 1 to {self.max_length} token ids.")
+        ids = torch.as_tensor(ids, dtype=torch.int64)
+        if ids.dim() != 1 or not 0 < ids.shape[0] <= self.max_length or int(ids.min()) < 0 \
+                or int(ids.max()) >= self.vocab:
+            raise ValueError(f"A prompt is a vector of 1 to {self.max_length} token ids below {self.vocab}.")
+        ids, n = ids.to(self.device), ids.shape[0]
         if all(self._taken):
             raise RuntimeError("All requests' places are taken.")
         place = self._taken.index(False)
@@ -113,10 +114,14 @@ class PagedDecoder:
         step = self.tables.extend(new, n)
         if int(step.status[place]) != serving.PAGES_OK:
             raise RuntimeError("There are not enough free pages for the prompt.")
-        out = self.model(input_ids=ids[None], use_cache=True)
-        for layer, prompt in enumerate(out.past_key_values.layers):
-            k, v = (t[0].transpose(0, 1) for t in (prompt.keys, prompt.values))
-            self._store(k, k, v, step.positions, step.slots, *self.cache[layer])
+        try:
+            out = self.model(input_ids=ids[None], use_cache=True)
+            for layer, prompt in enumerate(out.past_key_values.layers):
+                k, v = (t[0].transpose(0, 1) for t in (prompt.keys, prompt.values))
+                self._store(k, k, v, step.positions, step.slots, *self.cache[layer])
+        except Exception:
+            self.tables.release(new > 0)   # a prompt that fails leaves no pages behind
+            raise
         self._history[place, :n] = ids.int()
         self._prompts[place] = n
         self._live[place] = 1
@@ -224,15 +229,21 @@ class PagedDecoder:
     def generate(self, prompts, new_tokens, *, capture=False):
         """`new_tokens` greedy tokens for each prompt (as many prompts as
         there are free places); lists of token ids. `capture` replays the
-        steps after the second from a HIP graph."""
+        steps after the second from a HIP graph. Raises where the pages did
+        not suffice for all."""
         if new_tokens < 1 or any(len(p) + new_tokens - 1 > self.max_length for p in prompts):
             raise ValueError("Prompts and answers must fit max_length.")
+        if len(prompts) > self._taken.count(False):
+            raise RuntimeError("There are more prompts than free places.")
         places = [self.add(p) for p in prompts]
         tokens = [self._last[:self.requests].clone()]
         for i in range(new_tokens - 1):
             if capture and i == 2 and self._graph is None:
                 self.capture()
             tokens.append(self.step().clone())
+        lengths = self.tables.lengths[places].tolist()
         answers = torch.stack(tokens, 1)[places].tolist()
         self.finish(*places)
+        if lengths != [len(p) + new_tokens - 1 for p in prompts]:
+            raise RuntimeError("The pages ran out before all requests had their tokens.")
         return answers

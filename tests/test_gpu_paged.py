@@ -146,6 +146,21 @@ def test_requests_come_and_go():
     assert decoder.tables.n_free.item() == 6
     with pytest.raises(RuntimeError, match="pages"):
         PagedDecoder(model, requests=2, max_length=64, num_pages=1).add(prompts(17)[0])
+    tight = PagedDecoder(model, requests=2, max_length=64, num_pages=3)
+    with pytest.raises(RuntimeError, match="ran out"):
+        tight.generate(prompts(16, 16), 20)
+    assert tight.tables.n_free.item() == 3 and not any(tight._taken)
+    with pytest.raises(RuntimeError, match="more prompts"):
+        tight.generate(prompts(1, 1, 1), 2)
+    for ids in ([], [3, 1000], [-1], 5, [[1, 2]]):
+        with pytest.raises(ValueError, match="token ids"):
+            tight.add(ids)
+    model.lm_head, head = None, model.lm_head     # a forward that fails
+    with pytest.raises(TypeError):
+        tight.add(prompts(20)[0])
+    model.lm_head = head
+    assert tight.tables.n_free.item() == 3 and tight.tables.lengths.tolist() == [0, 0]
+    assert len(tight.generate(prompts(20), 5)[0]) == 5
     with pytest.raises(ValueError, match="holds no request"):
         decoder.finish(0)
     with pytest.raises(ValueError, match="token ids"):
