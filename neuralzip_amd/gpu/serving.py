@@ -81,7 +81,7 @@ def _check_vector(name, t, dtype, n, index):
 
 
 # Parts of one allocation. (The form that keeps no record of them as views of
-# each other takes 2 us less for a step's eight arrays.)
+# each other takes 0.7 us less for a step's eight arrays.)
 _split = torch.unsafe_split_with_sizes
 
 
