@@ -170,7 +170,9 @@ class PagedDecoder:
 
     def _run(self):
         """One step, all of it on the device."""
-        self.tables.extend(self._live, self.requests, out=self._step)
+        # pages may reach past max_length; the rotary tables and the histories do not
+        asked = torch.where(self.tables.lengths < self.max_length, self._live, 0)
+        self.tables.extend(asked, self.requests, out=self._step)
         step = self._step
         self._plan.update(step.contexts, requests=step.requests)
         body, rows = self.model.model, self._rows(step.requests)
