@@ -11,9 +11,11 @@ own forward, one at a time, and their keys and values are then stored into
 the request's pages. A step never asks the device for anything, so that it
 can be captured in a HIP graph (capture()) and replayed while requests grow.
 
-Models are Llama-like: model.model.{embed_tokens, layers, norm, rotary_emb}
-and model.lm_head, layers with self_attn.{q,k,v,o}_proj and, optionally, RMS
-norms q_norm and k_norm over a head. The reference has no counterpart (its
+Models are Llama-like, of the types in MODEL_TYPES:
+model.model.{embed_tokens, layers, norm, rotary_emb} and model.lm_head, layers
+with self_attn.{q,k,v,o}_proj and, optionally, RMS norms q_norm and k_norm over
+a head, without a sliding window shorter than max_length. Others are refused.
+The reference has no counterpart (its
 forwards keep Transformers' cache, neuralzip/gpu/inference.py:476-509).
 """
 import contextlib
@@ -25,6 +27,35 @@ from neuralzip_amd.gpu.inference import RUNTIME_ATTRIBUTE
 
 # Rotary tables that depend on the length they are asked for.
 _GROWING_ROPES = ("dynamic", "longrope")
+# Model types whose forward is what a step here computes: layers over the
+# embeddings as they are, pairs (i, i + rotary_dim / 2) rotated in every layer,
+# lm_head's products as logits. Each is compared with its own forward by
+# tests/test_paged_decoder.py. Others may have the same modules and differ
+# (neighbouring pairs, layers without rotation, scaled logits).
+MODEL_TYPES = frozenset((
+    "apertus", "arcee", "aria_text", "dots1", "exaone4", "gemma", "glm4_moe", "granite", "granitemoe",
+    "granitemoeshared", "hy_v3", "hyperclovax", "jais2", "llama", "mistral", "mixtral", "nemotron", "olmo", "phimoe",
+    "qwen2", "qwen2_moe", "qwen3", "qwen3_moe", "seed_oss", "solar_open", "stablelm", "starcoder2"))
+# Settings of theirs that a step does not follow, with the values that change nothing.
+_PLAIN_SETTINGS = {"embedding_multiplier": (None, 1), "logits_scaling": (None, 1), "clip_qkv": (None,),
+                   "qk_layernorm": (None, False)}
+
+
+def _check_model(config, max_length):
+    """Refuses models that a step would compute otherwise than they do."""
+    kind = getattr(config, "model_type", None)
+    if kind not in MODEL_TYPES:
+        raise ValueError(f"PagedDecoder runs models of the types {', '.join(sorted(MODEL_TYPES))}; this one is "
+                         f"{kind!r}, whose forward may differ.")
+    for name, plain in _PLAIN_SETTINGS.items():
+        if getattr(config, name, None) not in plain:
+            raise ValueError(f"PagedDecoder does not follow {name}={getattr(config, name)!r} of this {kind} model.")
+    # (where layers differ, as layer_types says, their attention modules have the windows)
+    window = getattr(config, "sliding_window", None)
+    if window is not None and getattr(config, "use_sliding_window", True) and window < max_length \
+            and getattr(config, "layer_types", None) is None:
+        raise ValueError(f"PagedDecoder attends to whole contexts; this model has a sliding window of {window} tokens, "
+                         f"less than max_length.")
 
 
 class PagedDecoder:
@@ -39,6 +70,7 @@ class PagedDecoder:
 
     def __init__(self, model, *, requests, max_length, page_size=16, num_pages=None, repetition=1.0, frequency=0.0,
                  presence=0.0, grammar=False):
+        _check_model(model.config, max_length)
         body = model.model
         self.model, self.layers = model, list(body.layers)
         self._attentions = [layer.self_attn for layer in self.layers]

@@ -70,3 +70,76 @@ def test_requests_at_max_length_stay_as_they_are(device, most):
     assert torch.equal(decoder.cache[:, :, pages], keys[:, :, pages]) and torch.isfinite(decoder.cache).all()
     assert torch.equal(decoder._history[first], history)
     assert decoder._history[second, :3].tolist() == short.tolist()
+
+
+MOE = dict(num_experts=4, num_local_experts=4, n_routed_experts=4, num_experts_per_tok=2, moe_intermediate_size=48,
+           shared_expert_intermediate_size=48, n_shared_experts=1, n_group=1, topk_group=1)
+# What small models of a type need beside SIZES and MOE.
+KINDS = {"stablelm": dict(hidden_size=256), "phimoe": dict(sliding_window=None), "mistral": dict(sliding_window=None),
+         "exaone4": dict(sliding_window=None, layer_types=["full_attention"] * 3),
+         "granite": dict(attention_multiplier=0.18), "granitemoe": dict(attention_multiplier=0.18),
+         "granitemoeshared": dict(attention_multiplier=0.18)}
+# Settings that a step follows, and that change what the model computes.
+FOLLOWED = [("llama", dict(attention_bias=True, mlp_bias=True, head_dim=48)), ("mistral", dict(sliding_window=40)),
+            ("starcoder2", dict(sliding_window=64)), ("qwen3", dict(head_dim=64, attention_bias=True)),
+            ("stablelm", dict(hidden_size=256, use_parallel_residual=True, use_qkv_bias=True)),
+            ("granite", dict(residual_multiplier=0.4, attention_multiplier=0.1)), ("qwen2", dict(sliding_window=8)),
+            ("glm4_moe", dict(MOE, use_qk_norm=True)), ("nemotron", dict(hidden_size=256, partial_rotary_factor=0.25)),
+            ("llama", dict(rope_parameters=dict(rope_type="yarn", factor=4.0, rope_theta=1e4,
+                                                original_max_position_embeddings=16)))]
+
+
+def check_against_own_forward(model, device):
+    """Two requests of different lengths: every step's logits are the
+    model's own after the same tokens."""
+    decoder = PagedDecoder(model, requests=2, max_length=40)
+    texts = [prompt(5, 1).tolist(), prompt(19, 2).tolist()]
+    for place, text in enumerate(texts):
+        assert decoder.add(text) == place
+        assert agree(decoder.logits[0], own_logits(model, text))
+    for _ in range(6):
+        for place, text in enumerate(texts):
+            text.append(int(decoder._last[place]))
+        decoder.step()
+        for place, text in enumerate(texts):
+            assert agree(decoder.logits[place], own_logits(model, text))
+
+
+def known(kind):
+    from transformers import CONFIG_MAPPING
+    if kind not in CONFIG_MAPPING:
+        pytest.skip(f"this Transformers has no {kind}")
+
+
+@pytest.mark.parametrize("kind", sorted(paged.MODEL_TYPES))
+def test_accepted_models_compute_their_own_forward(kind, device):
+    known(kind)
+    model = small_model(device, kind, **dict(MOE, head_dim=None if kind == "stablelm" else 32, **KINDS.get(kind, {})))
+    check_against_own_forward(model, device)
+
+
+@pytest.mark.parametrize("kind, settings", FOLLOWED)
+def test_settings_that_are_followed(kind, settings, device):
+    known(kind)
+    check_against_own_forward(small_model(device, kind, **settings), device)
+
+
+@pytest.mark.parametrize("kind, settings, message", [
+    ("mistral", dict(sliding_window=8), "sliding window of 8"), ("mixtral", dict(sliding_window=39), "window of 39"),
+    ("starcoder2", dict(sliding_window=8), "sliding window"), ("phimoe", dict(sliding_window=8), "sliding window"),
+    ("qwen3", dict(use_sliding_window=True, sliding_window=8, max_window_layers=1), "sliding window"),
+    ("granite", dict(embedding_multiplier=12.0), "embedding_multiplier"),
+    ("granite", dict(logits_scaling=8.0), "logits_scaling"), ("granitemoe", dict(logits_scaling=8.0), "logits_scaling"),
+    ("hyperclovax", dict(embedding_multiplier=2.0), "embedding_multiplier"), ("olmo", dict(clip_qkv=0.5), "clip_qkv"),
+    ("stablelm", dict(hidden_size=256, head_dim=None, qk_layernorm=True), "qk_layernorm"),
+    ("cohere", {}, "cohere"), ("glm", {}, "glm"), ("glm4", {}, "glm4"), ("ernie4_5", {}, "ernie4_5"),
+    ("helium", {}, "helium"), ("smollm3", {}, "smollm3"), ("bitnet", {}, "bitnet"), ("olmo2", {}, "olmo2"),
+    ("diffllama", {}, "diffllama"), ("ministral3", {}, "ministral3"), ("hunyuan_v1_dense", {}, "hunyuan"),
+    ("llama", dict(rope_parameters=dict(rope_type="dynamic", factor=2.0, rope_theta=1e4)), "do not depend"),
+])
+def test_models_computed_otherwise_are_refused(kind, settings, message, device):
+    """Configurations as Transformers makes them, in models of their own."""
+    known(kind)
+    model = small_model(device, kind, **dict(dict(MOE, head_dim=32), **settings))
+    with pytest.raises(ValueError, match=message):
+        PagedDecoder(model, requests=1, max_length=40)
