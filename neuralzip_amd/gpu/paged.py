@@ -165,14 +165,18 @@ class PagedDecoder:
 
     def finish(self, *places):
         """Ends requests: their pages and places are free again."""
+        for place in places:
+            if not 0 <= place < self.requests or not self._taken[place]:
+                raise ValueError(f"Place {place} holds no request.")
+        if len(set(places)) < len(places):
+            raise ValueError("A place is named twice.")
         done = torch.zeros(self.requests, dtype=torch.bool, device=self.device)
         for place in places:
-            if not self._taken[place]:
-                raise ValueError(f"Place {place} holds no request.")
             done[place] = True
-            self._taken[place] = False
         self.tables.release(done)
         self._live.masked_fill_(done, 0)
+        for place in places:
+            self._taken[place] = False
 
     # ------------------------------------------------------------------ steps
 

@@ -143,3 +143,23 @@ def test_models_computed_otherwise_are_refused(kind, settings, message, device):
     model = small_model(device, kind, **dict(dict(MOE, head_dim=32), **settings))
     with pytest.raises(ValueError, match=message):
         PagedDecoder(model, requests=1, max_length=40)
+
+
+def state(decoder):
+    return (decoder.tables.lengths.tolist(), decoder.tables.n_free.tolist(), decoder._live.tolist(),
+            list(decoder._taken))
+
+
+@pytest.mark.parametrize("places", [(0, 0), (0, 2), (2, 0), (0, -3), (0, 3), (0, 1, 0)])
+def test_a_refused_finish_changes_nothing(device, places):
+    """Places named twice, free ones and ones that do not exist."""
+    decoder = PagedDecoder(small_model(device), requests=3, max_length=40)
+    decoder.add(prompt(20)), decoder.add(prompt(5))
+    before = state(decoder)
+    with pytest.raises(ValueError, match="holds no request|named twice"):
+        decoder.finish(*places)
+    assert state(decoder) == before
+    decoder.step()
+    decoder.finish(0, 1)
+    assert state(decoder) == ([0, 0, 0], [9], [0, 0, 0], [False] * 3)
+    decoder.finish()
