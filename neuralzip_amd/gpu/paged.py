@@ -65,8 +65,9 @@ class PagedDecoder:
 
     `repetition`, `frequency` and `presence` are adjust_logits' penalties,
     for all requests. With `grammar`, `masks` (int32, requests x ceil(vocab /
-    32), all bits set at first) holds the tokens that each request may answer
-    with next; it may be written between steps."""
+    32)) holds the tokens that each request may answer with next; it may be
+    written between steps. All bits of a free place are set, at first and when
+    its request ends."""
 
     def __init__(self, model, *, requests, max_length, page_size=16, num_pages=None, repetition=1.0, frequency=0.0,
                  presence=0.0, grammar=False):
@@ -130,13 +131,19 @@ class PagedDecoder:
     # --------------------------------------------------------------- requests
 
     @torch.no_grad()
-    def add(self, ids):
+    def add(self, ids, mask=None):
         """Takes in a prompt (1-D token ids), picks its first answer token
-        and returns the request's place."""
+        and returns the request's place. `mask` (with `grammar`): the place's
+        row of `masks` from the first answer token on."""
         ids = torch.as_tensor(ids, dtype=torch.int64)
         if ids.dim() != 1 or not 0 < ids.shape[0] <= self.max_length or int(ids.min()) < 0 \
                 or int(ids.max()) >= self.vocab:
             raise ValueError(f"A prompt is a vector of 1 to {self.max_length} token ids below {self.vocab}.")
+        if mask is not None:
+            if self.masks is None:
+                raise ValueError("A mask needs grammar=True.")
+            if not torch.is_tensor(mask) or mask.dtype != torch.int32 or mask.shape != self.masks.shape[1:]:
+                raise ValueError(f"A mask is an int32 vector of {self.masks.shape[1]} words.")
         ids, n = ids.to(self.device), ids.shape[0]
         if all(self._taken):
             raise RuntimeError("All requests' places are taken.")
@@ -154,6 +161,8 @@ class PagedDecoder:
         except Exception:
             self.tables.release(new > 0)   # a prompt that fails leaves no pages behind
             raise
+        if mask is not None:
+            self.masks[place] = mask.to(self.device)
         self._history[place, :n] = ids.int()
         self._prompts[place] = n
         self._live[place] = 1
@@ -175,6 +184,8 @@ class PagedDecoder:
             done[place] = True
         self.tables.release(done)
         self._live.masked_fill_(done, 0)
+        if self.masks is not None:
+            self.masks.masked_fill_(done[:, None], -1)
         for place in places:
             self._taken[place] = False
 

@@ -163,3 +163,48 @@ def test_a_refused_finish_changes_nothing(device, places):
     decoder.finish(0, 1)
     assert state(decoder) == ([0, 0, 0], [9], [0, 0, 0], [False] * 3)
     decoder.finish()
+
+
+def only(*tokens):
+    """Mask words that allow these tokens."""
+    words = [0] * -(-VOCAB // 32)
+    for t in tokens:
+        words[t // 32] |= 1 << t % 32
+    return torch.tensor([w - (1 << 32) if w >> 31 else w for w in words], dtype=torch.int32)
+
+
+def test_a_place_used_again_has_no_grammar(device):
+    """A request's mask ends with it, in a place used again as in a new one;
+    a mask given to add() holds for the first answer token and after it."""
+    model, text = small_model(device), prompt(9)
+    free = int(own_logits(model, text).argmax())
+    decoder = PagedDecoder(model, requests=2, max_length=40, grammar=True)
+    other = (free + 31) % VOCAB
+    place = decoder.add(text, mask=only(other, 7))
+    assert int(decoder._last[place]) in (other, 7)
+    decoder.masks[place] = only(5).to(device)
+    decoder.step()
+    assert int(decoder._last[place]) == 5
+    decoder.finish(place)
+    assert decoder.add(text) == place and int(decoder._last[place]) == free
+    assert (decoder.masks == -1).all()
+    # written before the place is taken: also for the first token
+    decoder.masks[1] = only(other).to(device)
+    assert decoder.add(text) == 1 and int(decoder._last[1]) == other
+    decoder.finish(0, 1)
+    # through generate()
+    decoder.masks[0] = only(11).to(device)
+    assert decoder.generate([text], 3) == [[11, 11, 11]]
+    assert decoder.generate([text], 1) == [[free]]
+
+
+def test_wrong_masks_are_refused(device):
+    decoder = PagedDecoder(small_model(device), requests=1, max_length=40, grammar=True)
+    before = state(decoder)
+    for bad in (only(1)[:-1], only(1).long(), only(1)[None], [1] * 7):
+        with pytest.raises(ValueError, match="mask"):
+            decoder.add(prompt(4), mask=bad)
+    assert state(decoder) == before
+    plain = PagedDecoder(decoder.model, requests=1, max_length=40)
+    with pytest.raises(ValueError, match="grammar"):
+        plain.add(prompt(4), mask=only(1))
