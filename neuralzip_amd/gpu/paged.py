@@ -158,18 +158,20 @@ class PagedDecoder:
             for layer, prompt in enumerate(out.past_key_values.layers):
                 k, v = (t[0].transpose(0, 1) for t in (prompt.keys, prompt.values))
                 self._store(k, k, v, step.positions, step.slots, *self.cache[layer])
-        except Exception:
+            if mask is not None:
+                self.masks[place] = mask.to(self.device)
+            self._history[place, :n] = ids.int()
+            self._prompts[place] = n
+            rows = torch.full((1,), place, dtype=torch.int32, device=self.device)
+            contexts = torch.full((1,), n, dtype=torch.int32, device=self.device)
+            self._pick(out.logits[0, -1:], rows, contexts)
+        except BaseException:
             self.tables.release(new > 0)   # a prompt that fails leaves no pages behind
+            if mask is not None:
+                self.masks[place] = -1
             raise
-        if mask is not None:
-            self.masks[place] = mask.to(self.device)
-        self._history[place, :n] = ids.int()
-        self._prompts[place] = n
         self._live[place] = 1
         self._taken[place] = True
-        rows = torch.full((1,), place, dtype=torch.int32, device=self.device)
-        contexts = torch.full((1,), n, dtype=torch.int32, device=self.device)
-        self._pick(out.logits[0, -1:], rows, contexts)
         return place
 
     def finish(self, *places):
@@ -284,15 +286,19 @@ class PagedDecoder:
             raise ValueError("Prompts and answers must fit max_length.")
         if len(prompts) > self._taken.count(False):
             raise RuntimeError("There are more prompts than free places.")
-        places = [self.add(p) for p in prompts]
-        tokens = [self._last[:self.requests].clone()]
-        for i in range(new_tokens - 1):
-            if capture and i == 2 and self._graph is None:
-                self.capture()
-            tokens.append(self.step().clone())
-        lengths = self.tables.lengths[places].tolist()
-        answers = torch.stack(tokens, 1)[places].tolist()
-        self.finish(*places)
+        places = []
+        try:
+            for p in prompts:
+                places.append(self.add(p))
+            tokens = [self._last[:self.requests].clone()]
+            for i in range(new_tokens - 1):
+                if capture and i == 2 and self._graph is None:
+                    self.capture()
+                tokens.append(self.step().clone())
+            lengths = self.tables.lengths[places].tolist()
+            answers = torch.stack(tokens, 1)[places].tolist()
+        finally:
+            self.finish(*places)
         if lengths != [len(p) + new_tokens - 1 for p in prompts]:
             raise RuntimeError("The pages ran out before all requests had their tokens.")
         return answers

@@ -208,3 +208,40 @@ def test_wrong_masks_are_refused(device):
     plain = PagedDecoder(decoder.model, requests=1, max_length=40)
     with pytest.raises(ValueError, match="grammar"):
         plain.add(prompt(4), mask=only(1))
+
+
+def failing(*args, **kwargs):
+    raise ArithmeticError("on purpose")
+
+
+def test_a_prompt_that_fails_late_leaves_nothing_behind(device, monkeypatch):
+    """The first pick fails, after the prompt's keys are stored."""
+    model = small_model(device)
+    decoder = PagedDecoder(model, requests=2, max_length=40, repetition=1.2, grammar=True)
+    decoder.add(prompt(5))
+    before, masks = state(decoder), decoder.masks.clone()
+    with monkeypatch.context() as patch:
+        patch.setattr(decoder, "_pick", failing)
+        with pytest.raises(ArithmeticError):
+            decoder.add(prompt(20), mask=only(3))
+    assert state(decoder) == before and torch.equal(decoder.masks, masks)
+    assert decoder.add(prompt(20)) == 1
+
+
+@pytest.mark.parametrize("where", ["second prompt", "step", "wrong id"])
+def test_a_generate_that_fails_leaves_nothing_behind(device, monkeypatch, where):
+    """Its requests end; one that was there before goes on."""
+    model = small_model(device)
+    decoder = PagedDecoder(model, requests=3, max_length=64, num_pages=6)
+    held = decoder.add(prompt(20))
+    before = state(decoder)
+    texts = [prompt(33), prompt(17) if where == "second prompt" else prompt(3)]
+    if where == "wrong id":
+        texts[1] = torch.tensor([VOCAB])
+    with monkeypatch.context() as patch:
+        if where == "step":
+            patch.setattr(decoder, "step", failing)
+        with pytest.raises(ArithmeticError if where == "step" else ValueError if where == "wrong id" else RuntimeError):
+            decoder.generate(texts, 2)
+    assert state(decoder) == before
+    assert len(decoder.generate([prompt(33)], 2)[0]) == 2 and decoder.tables.lengths[held] == 21
