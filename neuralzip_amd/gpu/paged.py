@@ -116,6 +116,7 @@ class PagedDecoder:
         self._live = filled(0, torch.int32)           # 1: the request gets a token in a step
         # row `requests` of what is written by request takes what a step's unused rows write
         self._last = torch.zeros(requests + 1, dtype=torch.int64, device=self.device)
+        self._answers = torch.full((requests,), -1, dtype=torch.int64, device=self.device)   # of the last step
         self._history = torch.zeros((requests + 1, max_length + 1), dtype=torch.int32, device=self.device)
         self._prompts = filled(0, torch.int32)
         self._penalties = {}
@@ -233,6 +234,7 @@ class PagedDecoder:
                     hidden = hidden[0]
         logits = self.model.lm_head(body.norm(hidden))[0]
         self._pick(logits, step.requests, step.contexts)
+        torch.where(step.starts.diff() > 0, self._last[:self.requests], -1, out=self._answers)
 
     def _rows(self, requests):
         return torch.where(requests < 0, self.requests, requests).long()
@@ -259,13 +261,13 @@ class PagedDecoder:
     @torch.no_grad()
     def step(self):
         """One new token for every request; returns the tokens (int64, by
-        place; those of free places mean nothing). Requests at max_length, or
-        for which no page is free, stay as they are."""
+        place). Requests at max_length, or for which no page is free, stay as
+        they are: -1, as in free places."""
         if self._graph is not None:
             self._graph.replay()
         else:
             self._run()
-        return self._last[:self.requests]
+        return self._answers
 
     @torch.no_grad()
     def capture(self):

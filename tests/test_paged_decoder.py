@@ -245,3 +245,16 @@ def test_a_generate_that_fails_leaves_nothing_behind(device, monkeypatch, where)
             decoder.generate(texts, 2)
     assert state(decoder) == before
     assert len(decoder.generate([prompt(33)], 2)[0]) == 2 and decoder.tables.lengths[held] == 21
+
+
+def test_steps_say_which_requests_got_no_token(device):
+    """-1 at max_length, without a free page and in free places."""
+    decoder = PagedDecoder(small_model(device), requests=4, max_length=24, num_pages=4)
+    full, starved, fine = decoder.add(prompt(22, 1)), decoder.add(prompt(16, 2)), decoder.add(prompt(3, 3))
+    for got_full in (True, True, False, False):
+        tokens = decoder.step().tolist()
+        assert (tokens[full] == -1) != got_full and tokens[starved] == -1 and tokens[3] == -1
+        assert 0 <= tokens[fine] == int(decoder._last[fine])
+    decoder.finish(full)      # its pages let the other go on
+    tokens = decoder.step().tolist()
+    assert tokens[full] == -1 and 0 <= tokens[starved] == int(decoder._last[starved])
