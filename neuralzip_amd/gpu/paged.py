@@ -192,6 +192,12 @@ class PagedDecoder:
         for place in places:
             self._taken[place] = False
 
+    @property
+    def tokens(self):
+        """The last token of every request's answer, the one that add()
+        picked among them (a new int64 tensor, by place)."""
+        return self._last[:self.requests].clone()
+
     # ------------------------------------------------------------------ steps
 
     def _attend(self, layer, attention, hidden, *args, **kwargs):
@@ -260,14 +266,14 @@ class PagedDecoder:
 
     @torch.no_grad()
     def step(self):
-        """One new token for every request; returns the tokens (int64, by
-        place). Requests at max_length, or for which no page is free, stay as
+        """One new token for every request; returns the tokens (a new int64
+        tensor, by place). Requests at max_length, or for which no page is free, stay as
         they are: -1, as in free places."""
         if self._graph is not None:
             self._graph.replay()
         else:
             self._run()
-        return self._answers
+        return self._answers.clone()
 
     @torch.no_grad()
     def capture(self):
@@ -292,11 +298,11 @@ class PagedDecoder:
         try:
             for p in prompts:
                 places.append(self.add(p))
-            tokens = [self._last[:self.requests].clone()]
+            tokens = [self.tokens]
             for i in range(new_tokens - 1):
                 if capture and i == 2 and self._graph is None:
                     self.capture()
-                tokens.append(self.step().clone())
+                tokens.append(self.step())
             lengths = self.tables.lengths[places].tolist()
             answers = torch.stack(tokens, 1)[places].tolist()
         finally:

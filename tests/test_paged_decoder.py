@@ -258,3 +258,21 @@ def test_steps_say_which_requests_got_no_token(device):
     decoder.finish(full)      # its pages let the other go on
     tokens = decoder.step().tolist()
     assert tokens[full] == -1 and 0 <= tokens[starved] == int(decoder._last[starved])
+
+
+def test_steps_return_tensors_of_their_own(device):
+    """What step() returned stays; `tokens` has a prompt's first answer token too."""
+    model, text = small_model(device), prompt(6)
+    decoder = PagedDecoder(model, requests=2, max_length=40)
+    place = decoder.add(text)
+    answer = [int(decoder.tokens[place])]
+    assert answer[0] == int(own_logits(model, text).argmax())
+    kept, seen = [], []
+    for _ in range(4):
+        kept.append(decoder.step())
+        seen.append(kept[-1].tolist())
+        assert int(decoder.tokens[place]) == seen[-1][place]
+    first = decoder.tokens
+    decoder.add(prompt(7))
+    decoder.step()
+    assert [t.tolist() for t in kept] == seen and first[place] == seen[-1][place]
