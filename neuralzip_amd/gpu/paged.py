@@ -240,7 +240,7 @@ class PagedDecoder:
                     hidden = hidden[0]
         logits = self.model.lm_head(body.norm(hidden))[0]
         self._pick(logits, step.requests, step.contexts)
-        torch.where(step.starts.diff() > 0, self._last[:self.requests], -1, out=self._answers)
+        self._answers.copy_(torch.where(step.starts.diff() > 0, self._last[:self.requests], -1))
 
     def _rows(self, requests):
         return torch.where(requests < 0, self.requests, requests).long()
