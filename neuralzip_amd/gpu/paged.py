@@ -125,8 +125,10 @@ class PagedDecoder:
                                    presence=filled(presence))
         self.masks = torch.full((requests, (self.vocab + 31) // 32), -1, dtype=torch.int32,
                                 device=self.device) if grammar else None
-        self.logits = None                            # of the last step, in token order, as adjusted
-        self._graph = None
+        # of the last step, in token order, or of the prompt taken in since, as
+        # adjusted; a step replayed from a graph writes the last one's anew
+        self.logits = None
+        self._graph = self._graph_logits = None
         self._taken = [False] * requests
 
     # --------------------------------------------------------------- requests
@@ -271,6 +273,7 @@ class PagedDecoder:
         they are: -1, as in free places."""
         if self._graph is not None:
             self._graph.replay()
+            self.logits = self._graph_logits
         else:
             self._run()
         return self._answers.clone()
@@ -280,10 +283,11 @@ class PagedDecoder:
         """Captures the step in a HIP graph, which step() replays from then
         on. A step should have run eagerly before."""
         runtime = getattr(self.model, RUNTIME_ATTRIBUTE, None)
-        graph = torch.cuda.CUDAGraph()
+        graph, before = torch.cuda.CUDAGraph(), self.logits
         with runtime.graph_capture() if runtime is not None else contextlib.nullcontext(), torch.cuda.graph(graph):
             self._run()
-        self._graph = graph
+        # (nothing has run yet: the logits are the last step's still)
+        self._graph, self._graph_logits, self.logits = graph, self.logits, before
 
     def generate(self, prompts, new_tokens, *, capture=False):
         """`new_tokens` greedy tokens for each prompt (as many prompts as

@@ -276,3 +276,67 @@ def test_steps_return_tensors_of_their_own(device):
     decoder.add(prompt(7))
     decoder.step()
     assert [t.tolist() for t in kept] == seen and first[place] == seen[-1][place]
+
+
+def captured(decoder, device, monkeypatch):
+    """decoder.capture(); on the CPU a graph's stand-in: capturing runs
+    nothing, and a replay writes the memory that was there at the capture
+    and no attribute."""
+    if device != "cpu":
+        return decoder.capture()
+    run, memory = decoder._run, torch.full((decoder.requests, VOCAB), float("nan"))
+
+    class Graph:
+        def replay(self):
+            before = decoder.logits
+            run()
+            memory.copy_(decoder.logits)
+            decoder.logits = before
+    with monkeypatch.context() as patch:
+        patch.setattr(torch.cuda, "CUDAGraph", Graph)
+        patch.setattr(torch.cuda, "graph", lambda graph: contextlib.nullcontext())
+        patch.setattr(decoder, "_run", lambda: setattr(decoder, "logits", memory))
+        decoder.capture()
+
+
+def test_logits_are_the_last_steps_from_a_graph_too(device, monkeypatch):
+    model = small_model(device)
+    decoder = PagedDecoder(model, requests=2, max_length=40, repetition=1.3)
+    plain = PagedDecoder(model, requests=2, max_length=40, repetition=1.3)
+    for d in (decoder, plain):
+        d.add(prompt(6)), d.step()
+    before = decoder.logits.clone()
+    captured(decoder, device, monkeypatch)
+    assert torch.equal(decoder.logits, before)     # nothing has run yet
+    for i in range(6):
+        if i == 2:
+            assert decoder.add(prompt(9)) == plain.add(prompt(9)) == 1
+            assert decoder.logits.shape == (1, VOCAB)
+        assert torch.equal(decoder.step(), plain.step())
+        n = 1 if i < 2 else 2
+        assert decoder.logits.shape == (2, VOCAB) and agree(decoder.logits[:n], plain.logits[:n])
+        assert torch.equal(decoder.tokens, plain.tokens)
+
+
+@pytest.mark.parametrize("adjusted", ["penalties", "grammar"])
+def test_captured_steps_with_penalties_and_grammar(device, monkeypatch, adjusted):
+    """Replays give the eager steps' tokens, with requests that come and go
+    between them and masks written between them."""
+    model = small_model(device)
+    how = dict(repetition=1.4, frequency=0.3, presence=0.2) if adjusted == "penalties" else dict(grammar=True)
+    decoder, plain = (PagedDecoder(model, requests=3, max_length=30, **how) for _ in range(2))
+    for d in (decoder, plain):
+        d.add(prompt(6, 1)), d.add(prompt(20, 2)), d.step()
+    captured(decoder, device, monkeypatch)
+    for i in range(14):
+        for d in (decoder, plain):
+            if i == 3:
+                d.finish(0)
+            if i == 5:
+                assert d.add(prompt(4, 3)) == 0
+            if i in (1, 6) and adjusted == "grammar":
+                d.masks[i % 2] = only(*range(i, VOCAB, 7)).to(device)
+        got = decoder.step()
+        assert torch.equal(got, plain.step()) and torch.equal(decoder.tables.lengths, plain.tables.lengths)
+        if adjusted == "grammar" and i >= 6 and got[0] >= 0:
+            assert got[0] % 7 == 6
