@@ -218,13 +218,18 @@ class PagedDecoder:
         """Attention over the pages while a step runs."""
         def forward(layer, attention):
             return lambda hidden_states, *args, **kwargs: self._attend(layer, attention, hidden_states, *args, **kwargs)
+        # (some modules may have a forward of their own already, as wrapped ones do)
+        own = [attention.__dict__.get("forward") for attention in self._attentions]
         for layer, attention in enumerate(self._attentions):
             attention.forward = forward(layer, attention)
         try:
             yield
         finally:
-            for attention in self._attentions:
-                del attention.forward
+            for attention, before in zip(self._attentions, own):
+                if before is None:
+                    del attention.forward
+                else:
+                    attention.forward = before
 
     def _run(self):
         """One step, all of it on the device."""

@@ -340,3 +340,31 @@ def test_captured_steps_with_penalties_and_grammar(device, monkeypatch, adjusted
         assert torch.equal(got, plain.step()) and torch.equal(decoder.tables.lengths, plain.tables.lengths)
         if adjusted == "grammar" and i >= 6 and got[0] >= 0:
             assert got[0] % 7 == 6
+
+
+@pytest.mark.parametrize("fails", [False, True])
+def test_forwards_of_the_attention_modules_own_are_put_back(device, monkeypatch, fails):
+    """A forward that another library set on a module is there again after a
+    step, also one that fails, and none is left where there was none."""
+    model = small_model(device)
+    calls = []
+    attention = model.model.layers[1].self_attn
+    original = attention.forward
+
+    def wrapped(*args, **kwargs):
+        calls.append(1)
+        return original(*args, **kwargs)
+    attention.forward = wrapped
+    decoder = PagedDecoder(model, requests=1, max_length=40)
+    decoder.add(prompt(5))
+    if fails:
+        monkeypatch.setattr(paged.serving, "paged_attention", failing)
+        with pytest.raises(ArithmeticError):
+            decoder.step()
+    else:
+        decoder.step()
+    assert attention.forward is wrapped
+    assert all("forward" not in layer.self_attn.__dict__ for layer in model.model.layers if layer.self_attn is not attention)
+    del calls[:]
+    own_logits(model, prompt(3))
+    assert calls == [1]
