@@ -92,7 +92,8 @@ class PagedDecoder:
         self.heads = model.config.num_attention_heads
         self.requests, self.max_length, self.vocab = requests, max_length, model.config.vocab_size
         width = -(-max_length // page_size)
-        self.tables = serving.PageTables(requests, width, page_size, num_pages or requests * width, device=self.device)
+        self.tables = serving.PageTables(requests, width, page_size, requests * width if num_pages is None else num_pages,
+                                         device=self.device)
         # one allocation for all layers: (layers, keys and values, pages, heads, places, elements)
         self.cache = torch.zeros((len(self.layers), 2, self.tables.num_pages, self.kv_heads, page_size, self.dim),
                                  dtype=dtype, device=self.device)

@@ -368,3 +368,8 @@ def test_forwards_of_the_attention_modules_own_are_put_back(device, monkeypatch,
     del calls[:]
     own_logits(model, prompt(3))
     assert calls == [1]
+
+
+def test_no_pages_are_refused(device):
+    with pytest.raises(ValueError, match="pages"):
+        PagedDecoder(small_model(device), requests=1, max_length=40, num_pages=0)
