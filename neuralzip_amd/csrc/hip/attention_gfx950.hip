@@ -187,8 +187,9 @@ using f32x4 = vec<float, 4>;
 // that small ones keep their bits (2^-24 is fp16's least). 16-bit types take
 // a weight as head(p), cut off, and the rest, rounded: one rounding to 8 or 11
 // bits would err more than everything else before the result's own rounding,
-// and matrix instructions are not what bounds the kernel. The rest is kept
-// from being 0, so that an infinite value stays infinite in both products.
+// and matrix instructions are not what bounds the kernel. Beside a head the
+// rest is kept from being 0, so that an infinite value stays infinite in both
+// products; a weight too small for a head is all rest, and may be 0.
 template <typename T> struct Piece;
 
 template <> struct Piece<bf16_t> {
@@ -481,7 +482,10 @@ void nz_attention_kernel(nz_attention_args a) {
                 for (uint32_t k = 0; k < S::kRun; ++k) {
                     const float p = S::kRun == 8 ? score[k / 4][k % 4] : score[w][k];
                     p_hi[k] = P::head(p);
-                    p_lo[k] = static_cast<T>(fmaxf(p - static_cast<float>(p_hi[k]), P::kLeast));
+                    // the larger of the rest (no larger than the head, unless that is 0) and kLeast; without
+                    // a head the rest itself
+                    const float head = static_cast<float>(p_hi[k]);
+                    p_lo[k] = static_cast<T>(__builtin_amdgcn_fmed3f(p - head, head, P::kLeast));
                 }
 #pragma unroll
                 for (uint32_t s = 0; s < S::kValueSteps; ++s)
