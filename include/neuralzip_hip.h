@@ -642,11 +642,13 @@ typedef struct nz_attention_item {
 /* Cuts rows' contexts into items of about equal length, on the device:
  * n_rows contexts (negative ones count as 0), requests[row] their requests
  * (NULL: row i is request i). Let n be n_rows, rounded up to a multiple of
- * target (target for none): `items` has room for n + target. There are at
- * most n items, as short as that allows but of at least 128 keys (512 from
- * contexts of 8192 on; except for a row's last); or at most n + target, where
- * the longest would else be more than half longer than the n-th part of all
- * keys and than half their target-th part. The rest are marked unused.
+ * target (target for none): `items` has room for n + target. No item is
+ * longer than a length L, the shortest multiple of 32 keys, from 128 on (a
+ * sixteenth of the longest context, up to 512), for which n items suffice; or
+ * n + target items, where L would else be more than half longer than the n-th
+ * part of all keys and than half their target-th part. A row has as few items
+ * as L allows, of equal length in whole 32 keys but for its last: more than
+ * half of L where there are several. The rest are marked unused.
  * `counters` has room for as many entries times `parts`, kv_heads * ceil(heads
  * / kv_heads / 16). The plan serves the attention of every layer of a step. */
 int nz_attention_plan(const int32_t* contexts, const int32_t* requests, uint32_t n_rows, uint32_t target,

@@ -16,11 +16,13 @@ namespace {
 // ------------------------------------------------------------------- plan
 
 constexpr uint32_t kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
-// Items start at multiples of kTile keys, and are cut no shorter than gives
-// each wavefront of a workgroup one such tile, or, up to kLeastLong, than a
-// sixteenth of the longest context: more items than that take longer to join
-// than they save (one row over 8 heads of 8000 keys 13.2 us with items of
-// 512 keys and 14.6 of 256; of 2001 keys 11.1 of 512 and 8.8 of 128).
+// Items start at multiples of kTile keys. The length that they may have is no
+// shorter than gives each wavefront of a workgroup one such tile, or, up to
+// kLeastLong, than a sixteenth of the longest context: more items than that
+// take longer to join than they save (one row over 8 heads of 8000 keys 13.2
+// us with items of 512 keys and 14.6 of 256; of 2001 keys 11.1 of 512 and 8.8
+// of 128). A row is then cut into equal parts, which may be little more than
+// half as long.
 constexpr uint32_t kTile = 32, kLeastItem = 128, kLeastLong = 512;
 
 struct PlanLds {

@@ -53,3 +53,37 @@ def test_attention_passes_on_infinite_values_of_full_weight():
         plan = serving.AttentionPlan(ints([3]), heads=1, kv_heads=1)
         out = serving.paged_attention(q, keys, values, ints([[0]]), plan, scale=1.0)[0, 0]
         assert out[:3].tolist() == [float("inf"), float("-inf"), float("inf")] and not out[3:].any()
+
+
+@pytest.mark.parametrize("heads, kv_heads", [(32, 8), (8, 1), (64, 2)])
+@pytest.mark.parametrize("contexts", [[0], [128], [129], [257], [2001], [8191], [8192], [8193], [100_000], [0, 0, 5000],
+                                      [129] * 40, [200] * 1500, [100_000, 7] * 40, list(range(1, 8192, 128)),
+                                      [2 ** 31 - 1, 5], [30, 400, 50, 9000] * 300])
+def test_plans_keep_their_bounds(contexts, heads, kv_heads):
+    """The longest item, the number of items and the even cut of rows, as
+    nz_attention_plan's declaration has them."""
+    plan = serving.AttentionPlan(ints(contexts), heads=heads, kv_heads=kv_heads)
+    target = 256 // (kv_heads * -(-(heads // kv_heads) // 16))
+    n, keys, longest = -(-len(contexts) // target) * target, sum(contexts), max(contexts)
+    least = min(max(-(-(-(-longest // 32)) // 16), 4), 16)
+
+    def shortest(limit):
+        """In 32 keys; items get fewer as they get longer."""
+        low, high = least, max(least, -(-longest // 32))
+        while low < high:
+            middle = (low + high) // 2
+            if sum(max(-(-c // (32 * middle)), 1) for c in contexts) <= limit:
+                high = middle
+            else:
+                low = middle + 1
+        return low
+    length = 32 * shortest(n)
+    if length > 32 * least and 2 * length * n > 3 * keys and 2 * length * target > keys:
+        n, length = n + target, 32 * shortest(n + target)
+    items = [item for item in plan.items.tolist() if item[0] >= 0]
+    assert len(contexts) <= len(items) <= n <= plan.capacity
+    for row, context in enumerate(contexts):
+        sizes = [item[3] - item[2] for item in items if item[0] == row]
+        assert sum(sizes) == context and len(sizes) <= max(-(-context // length), 1)
+        assert len(set(sizes[:-1])) <= 1 and all(0 < sizes[-1] <= s <= length for s in sizes[:-1])
+        assert all(s % 32 == 0 and 2 * s > length for s in sizes[:-1]) and sizes[-1] <= length
