@@ -14,8 +14,10 @@ one forward, around the weights that the runtime decodes.
 
 Every call launches gfx950 kernels through the C ABI (nz_pages_*,
 nz_rotary_store, nz_attention_*, nz_adjust_logits) on the current stream, or
-on `stream`, where its tensors must be ready; nothing synchronises, and
-lengths, tables and plans never leave the device, so that a step can be
+on `stream`, where its tensors must be ready. They may be let go after the
+call: they are recorded for `stream`. Results are that stream's, and who uses
+them on another one waits for it and records them there. Nothing synchronises,
+and lengths, tables and plans never leave the device, so that a step can be
 captured in a HIP graph and replayed while the requests grow. The operators
 serve: tensors that need a gradient are refused while gradients are on.
 
@@ -55,6 +57,13 @@ def _call(function, device, args, stream):
     rc = function(args, _stream_handle(device, stream))
     if rc:
         _native.check(rc)
+
+
+def _keep(stream, *tensors):
+    """The tensors' memory is not given away before `stream` is done with them."""
+    for t in tensors:
+        if t is not None:
+            t.record_stream(stream)
 
 
 def _refuse_gradients(*tensors):
@@ -191,6 +200,8 @@ class PageTables:
                                          self.requests, self.max_pages, self.page_size, self.num_pages, max_tokens,
                                          bool(advance))
         _call(_native.lib().nz_pages_extend, self.device, args, stream)
+        if stream is not None:
+            _keep(stream, new_tokens, out.slots, *self._state)
         return out
 
     def release(self, done, *, advance=True, stream=None):
@@ -205,6 +216,8 @@ class PageTables:
                                           out.n_free.data_ptr(), self.requests, self.max_pages, self.page_size,
                                           self.num_pages, bool(advance), 0)
         _call(_native.lib().nz_pages_release, self.device, args, stream)
+        if stream is not None:
+            _keep(stream, done, *self._state)
         return out
 
 
@@ -292,6 +305,9 @@ class Rotary:
             kv_heads, dim, self.rotary_dim, self.interleaved, page_size, pages, self._positions, kind, weight_type,
             self.eps)
         _call(_native.lib().nz_rotary_store, self._device, args, stream)
+        if stream is not None:
+            _keep(stream, q, k, v, positions, slots, key_cache, value_cache, out, self.cos, self.sin, self.q_weight,
+                  self.k_weight)
         return out
 
 
@@ -332,6 +348,8 @@ class AttentionPlan:
                                              _stream_handle(self.device, stream))
         if rc:
             _native.check(rc)
+        if stream is not None:
+            _keep(stream, contexts, requests, self.items)
         return self
 
     def _partials(self, head_dim, handle, stream):
@@ -389,6 +407,8 @@ def paged_attention(q, key_cache, value_cache, tables, plan, *, scale=None, out=
     rc = _native.lib().nz_attention(args, handle)
     if rc:
         _native.check(rc)
+    if stream is not None:
+        _keep(stream, q, key_cache, value_cache, tables, out)
     return out
 
 
@@ -458,4 +478,7 @@ def adjust_logits(logits, *, history=None, lengths=None, prompt_lengths=None, re
         mask_rows_ptr, logits.stride(0), out.stride(0), history_row, rows, vocab, capacity, n_bias, n_masks,
         _TYPES[logits.dtype], id_bytes, 0)
     _call(_native.lib().nz_adjust_logits, logits.device, args, stream)
+    if stream is not None:
+        _keep(stream, logits, history, lengths, prompt_lengths, repetition, frequency, presence, *(bias or ()), masks,
+              mask_rows, out)
     return out
