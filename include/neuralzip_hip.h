@@ -685,7 +685,10 @@ uint64_t nz_attention_partials(uint32_t n_items, uint32_t heads, uint32_t head_d
 /* out[row] = softmax(scale * q[row] . keys) values, over the row's context in
  * its request's pages; head h reads key-value head h / (heads / kv_heads). A
  * row without keys gives zeros. Keys whose page or request is not in range
- * count as masked. head_dim is a multiple of 16, at most 256; strides and
+ * count as masked, and so do those whose score is -infinity. Values are summed
+ * in 32 bits before the division by the weights' sum: the largest one times
+ * the context must be below 3e38. fp16 weights are held in multiples of 2^-39
+ * of the largest. head_dim is a multiple of 16, at most 256; strides and
  * addresses are multiples of 16 bytes. Items and counters are taken as
  * nz_attention_plan wrote them, for the same heads. Calls with one plan must
  * not overlap: they share its counters, which each call leaves as it found
@@ -722,7 +725,8 @@ typedef struct nz_logits_args {
  * (once) if it is in the history after the prompt; plus the row's bias for
  * it (its last entry counts); -infinity where the row's mask has no bit (bit
  * v % 32 of word v / 32; a mask outside n_masks masks nothing). In 32 bits,
- * rounded once. Ids outside the vocabulary are ignored. */
+ * rounded once. Ids outside the vocabulary are ignored. There are at most
+ * 65535 rows. */
 int nz_adjust_logits(const nz_logits_args* args, void* stream);
 
 #ifdef __cplusplus

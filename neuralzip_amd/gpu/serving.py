@@ -371,9 +371,10 @@ def paged_attention(q, key_cache, value_cache, tables, plan, *, scale=None, out=
     pages (`tables`, int32 (requests, max_pages)) of the caches (pages,
     kv_heads, page size, head_dim). Query head h reads key-value head
     h // (heads / kv_heads). `scale` is head_dim ** -0.5 by default. A row
-    without keys gives zeros; keys of pages outside the caches count as
-    masked. Sums and softmax in 32 bits, in an order that only the plan
-    decides. head_dim is a multiple of 16 up to 256; strides may be any that
+    without keys gives zeros; keys of pages outside the caches, and keys whose
+    score is -infinity, count as masked. Sums and softmax in 32 bits, in an
+    order that only the plan decides; values are summed before the division,
+    so the largest one times the context must be below 3e38. head_dim is a multiple of 16 up to 256; strides may be any that
     keep heads, tokens and pages on 16-byte boundaries."""
     if torch.is_grad_enabled():
         _refuse_gradients(q, key_cache, value_cache)
@@ -428,7 +429,7 @@ def adjust_logits(logits, *, history=None, lengths=None, prompt_lengths=None, re
     and a token's last one counts. masks: int32 (any number, ceil(vocab /
     32)), token v's bit is bit v % 32 of word v // 32; mask_rows: int32 per
     row, the row's mask, -1 for none (row i has mask i by default). In 32
-    bits, rounded once. `out` may be logits itself."""
+    bits, rounded once. At most 65535 rows. `out` may be logits itself."""
     if torch.is_grad_enabled():
         _refuse_gradients(logits)
     if logits.dim() != 2 or logits.dtype not in _TYPES or not logits.is_cuda or logits.stride(1) != 1:

@@ -55,6 +55,19 @@ def test_attention_passes_on_infinite_values_of_full_weight():
         assert out[:3].tolist() == [float("inf"), float("-inf"), float("inf")] and not out[3:].any()
 
 
+def test_attention_of_scores_that_are_minus_infinity():
+    """Such keys have no weight, as masked ones; a row of nothing else gives zeros."""
+    for dtype in (torch.float16, torch.bfloat16, torch.float32):
+        keys = torch.zeros(2, 1, 16, 64, dtype=dtype, device=DEVICE)
+        values = torch.ones(2, 1, 16, 64, dtype=dtype, device=DEVICE)
+        keys[0, 0, :, 0], keys[1, 0, 1:, 0], values[1, 0, 0] = float("-inf"), float("-inf"), 3.0
+        q = torch.zeros(2, 1, 64, dtype=dtype, device=DEVICE)
+        q[..., 0] = 1.0
+        plan = serving.AttentionPlan(ints([16, 9]), heads=1, kv_heads=1)
+        out = serving.paged_attention(q, keys, values, ints([[0], [1]]), plan)
+        assert not out[0].any() and (out[1] == 3).all()
+
+
 @pytest.mark.parametrize("heads, kv_heads", [(32, 8), (8, 1), (64, 2)])
 @pytest.mark.parametrize("contexts", [[0], [128], [129], [257], [2001], [8191], [8192], [8193], [100_000], [0, 0, 5000],
                                       [129] * 40, [200] * 1500, [100_000, 7] * 40, list(range(1, 8192, 128)),

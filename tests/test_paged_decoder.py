@@ -373,3 +373,24 @@ def test_forwards_of_the_attention_modules_own_are_put_back(device, monkeypatch,
 def test_no_pages_are_refused(device):
     with pytest.raises(ValueError, match="pages"):
         PagedDecoder(small_model(device), requests=1, max_length=40, num_pages=0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["qwen3", "mixtral"])
+def test_compressed_models_answer_as_they_are(kind):
+    """Head norms, and experts whose weights are not the runtime's, beside
+    Linears that are decoded on the fly: the same tokens, eagerly and, without
+    experts, captured."""
+    from neuralzip_amd.gpu.inference import NeuralZipRuntime, export_model_for_gpu
+    from neuralzip_amd.setup import NeuralZipSetup
+    model = small_model("cuda:0", kind, **dict(MOE, head_dim=32, **KINDS.get(kind, {}))).to(torch.bfloat16)
+    texts, how = [prompt(3, 1), prompt(25, 2)], dict(requests=2, max_length=60, page_size=32)
+    want = PagedDecoder(model, **how).generate(texts, 20)
+    setup = NeuralZipSetup(chunk_size=16384).build(model)
+    runtime = NeuralZipRuntime.attach(model, export_model_for_gpu(model, setup), device="cuda:0")
+    decoder = PagedDecoder(model, **how)
+    assert decoder.generate(texts, 20) == want
+    if kind == "qwen3":       # (experts' forwards are not captured here)
+        assert decoder.generate(texts, 20, capture=True) == want
+    del decoder
+    assert runtime is not None
