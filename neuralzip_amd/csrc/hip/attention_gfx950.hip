@@ -307,7 +307,7 @@ struct Shape {
 // matrix instructions could do with it, so they may have idle columns and
 // multiply by split weights. 64 rows of 100 to 16384 keys, 64 heads over 8 of
 // 128 fp16 elements (2.16 GB), take 370 to 394 us by the rows' order, 5.5 to
-// 5.8 TB/s; 32 rows of up to 8191 keys, 32 heads over 8 in bf16 (488 MB), 93
+// 5.8 TB/s; 32 rows of up to 8191 keys, 32 heads over 8 in bf16 (488 MB), 96
 // us; one row of 2001 keys 8.7 us, of which starting takes 2.7 and the join
 // of the items 2.7.
 // Scores are computed transposed (keys are rows, heads columns), so that a

@@ -200,9 +200,10 @@ constexpr uint32_t kRotaryThreads = 256;
 // lane's runs lie at the same place of each, so that the group's accesses are
 // whole stretches. Pairs (i, i + rotary_dim / 2) are then in one lane, in x
 // and y; neighbouring pairs are inside a run. Bound by memory: 8191 tokens of
-// 64 bf16 heads over 8, normed (340 MB), take 67 us, 5.1 TB/s, with streaming
-// stores and 72 with ordinary ones, which gain nothing for the attention that
-// reads the results (a layer of 32 tokens over 500 keys 17.6 us with either).
+// 64 bf16 heads over 8, normed (340 MB), take 64 to 67 us, 5.1 to 5.3 TB/s,
+// with streaming stores and 72 with ordinary ones, which gain nothing for the
+// attention that reads the results (a layer of 32 tokens over 500 keys 17.6 us
+// with either).
 template <typename T, uint32_t LANES>
 __global__ __launch_bounds__(kRotaryThreads) void nz_rotary_kernel(nz_rotary_args a) {
     constexpr uint32_t kRun = run_of<T>(), kRuns = 8 / kRun;   // of x and of y
@@ -338,10 +339,10 @@ __device__ __forceinline__ void for_history(const ID* ids, uint32_t length, cons
 // and stores the logits. Integer LDS atomics only: the order of arrival does
 // not show. Every chunk's workgroup reads the row's whole history, out of the
 // L2. Bound by memory, once the history is short against the vocabulary: 32
-// rows of 128256 fp32 logits with everything on (33 MB) take 9.7 us, one row of
-// 151936 bf16 logits 4.0; the first were 12.8 us with chunks of 2048, 11.3 of
+// rows of 128256 fp32 logits with everything on (33 MB) take 9.6 us, one row of
+// 151936 bf16 logits 4.1; the first were 12.8 us with chunks of 2048, 11.3 of
 // 4096 and 10.6 of 8192 tokens (64 rows with up to 8000 ids 27, 21 and 18, and
-// 16 with ids read 16 bytes at a time).
+// 16 with ids read 16 bytes at a time, which costs short histories 0.1 to 0.5).
 // VECTOR: logits and out lie alike on 16-byte boundaries.
 template <typename T, bool VECTOR>
 __global__ __launch_bounds__(kLogitsThreads) void nz_logits_kernel(nz_logits_args a) {
