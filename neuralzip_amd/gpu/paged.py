@@ -21,6 +21,7 @@ forwards keep Transformers' cache, neuralzip/gpu/inference.py:476-509).
 import contextlib
 
 import torch
+from transformers import DynamicCache
 
 from neuralzip_amd.gpu import serving
 from neuralzip_amd.gpu.inference import RUNTIME_ATTRIBUTE
@@ -158,7 +159,8 @@ class PagedDecoder:
         if int(step.status[place]) != serving.PAGES_OK:
             raise RuntimeError("There are not enough free pages for the prompt.")
         try:
-            out = self.model(input_ids=ids[None], use_cache=True)
+            # (a cache of its own: one that the model makes may keep a window only)
+            out = self.model(input_ids=ids[None], past_key_values=DynamicCache(), use_cache=True)
             for layer, prompt in enumerate(out.past_key_values.layers):
                 k, v = (t[0].transpose(0, 1) for t in (prompt.keys, prompt.values))
                 self._store(k, k, v, step.positions, step.slots, *self.cache[layer])

@@ -394,3 +394,17 @@ def test_compressed_models_answer_as_they_are(kind):
         assert decoder.generate(texts, 20, capture=True) == want
     del decoder
     assert runtime is not None
+
+
+@pytest.mark.parametrize("n", [39, 40])
+def test_prompts_as_long_as_the_window(device, n):
+    """A window of max_length tokens hides nothing, whatever the model's own
+    cache keeps."""
+    model = small_model(device, "mistral", sliding_window=40)
+    decoder = PagedDecoder(model, requests=1, max_length=40)
+    text = prompt(n)
+    assert decoder.add(text) == 0 and agree(decoder.logits[0], own_logits(model, text))
+    if n < 40:
+        first = int(decoder.tokens[0])
+        decoder.step()
+        assert agree(decoder.logits[0], own_logits(model, text.tolist() + [first]))
