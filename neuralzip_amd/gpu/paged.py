@@ -292,10 +292,12 @@ class PagedDecoder:
         on. A step should have run eagerly before."""
         runtime = getattr(self.model, RUNTIME_ATTRIBUTE, None)
         graph, before = torch.cuda.CUDAGraph(), self.logits
-        with runtime.graph_capture() if runtime is not None else contextlib.nullcontext(), torch.cuda.graph(graph):
-            self._run()
-        # (nothing has run yet: the logits are the last step's still)
-        self._graph, self._graph_logits, self.logits = graph, self.logits, before
+        try:
+            with runtime.graph_capture() if runtime is not None else contextlib.nullcontext(), torch.cuda.graph(graph):
+                self._run()
+            self._graph, self._graph_logits = graph, self.logits
+        finally:
+            self.logits = before   # nothing has run yet: the last step's still
 
     def generate(self, prompts, new_tokens, *, capture=False):
         """`new_tokens` greedy tokens for each prompt (as many prompts as

@@ -408,3 +408,21 @@ def test_prompts_as_long_as_the_window(device, n):
         first = int(decoder.tokens[0])
         decoder.step()
         assert agree(decoder.logits[0], own_logits(model, text.tolist() + [first]))
+
+
+def test_a_capture_that_fails_keeps_the_logits(device, monkeypatch):
+    decoder = PagedDecoder(small_model(device), requests=1, max_length=40)
+    decoder.add(prompt(4))
+    before = decoder.logits
+
+    def run():
+        decoder.logits = None
+        failing()
+    with monkeypatch.context() as patch:
+        patch.setattr(torch.cuda, "CUDAGraph", object)
+        patch.setattr(torch.cuda, "graph", lambda graph: contextlib.nullcontext())
+        patch.setattr(decoder, "_run", run)
+        with pytest.raises(ArithmeticError):
+            decoder.capture()
+    assert decoder.logits is before and decoder._graph is None
+    decoder.step()
