@@ -24,7 +24,7 @@
 extern "C" {
 #endif
 
-#define NZ_ABI_VERSION 13
+#define NZ_ABI_VERSION 14
 
 enum nz_status {
     NZ_OK = 0,
@@ -587,6 +587,28 @@ typedef struct nz_pages_release_args {
  * free_pages above *n_free is still written. */
 int nz_pages_release(const nz_pages_release_args* args, void* stream);
 
+typedef struct nz_pages_trim_args {
+    const int32_t* lengths;      /* n_requests                               */
+    const int32_t* keep;         /* n_requests: tokens that stay             */
+    const int32_t* tables;       /* n_requests x max_pages                   */
+    int32_t* free_pages;         /* n_pages                                  */
+    const int32_t* n_free;
+    int32_t* lengths_after;      /* n_requests (out)                         */
+    int32_t* n_free_after;       /* 1 (out)                                  */
+    uint32_t n_requests;
+    uint32_t max_pages;
+    uint32_t page_size;
+    uint32_t n_pages;
+    uint32_t advance;
+    uint32_t reserved;           /* 0 */
+} nz_pages_trim_args;
+
+/* Shortens requests to their first keep[r] tokens (a negative number counts
+ * as 0; requests that are no longer stay as they are) and puts the pages past
+ * those back onto the stack, in request order and table order, as
+ * nz_pages_release does. */
+int nz_pages_trim(const nz_pages_trim_args* args, void* stream);
+
 typedef struct nz_rotary_args {
     const void* q;               /* tokens x heads x head_dim                */
     const void* k;               /* tokens x kv_heads x head_dim             */
@@ -695,6 +717,101 @@ uint64_t nz_attention_partials(uint32_t n_items, uint32_t heads, uint32_t head_d
  * them. n_items * heads * head_dim is below 2^30. */
 int nz_attention(const nz_attention_args* args, void* stream);
 
+/* What nz_shared_attention takes at once: columns (rows that see the same
+ * keys, times the query heads of one key-value head) of an item, rows and
+ * groups of a plan. */
+#define NZ_SHARED_COLUMNS 32
+#define NZ_SHARED_MAX_ROWS 2048
+#define NZ_SHARED_MAX_GROUPS 1024
+
+/* One workgroup's share of nz_shared_attention: the keys begin .. end - 1 of
+ * some rows. */
+typedef struct nz_shared_item {
+    int32_t member;              /* its first row's place in `order`         */
+    int32_t rows;                /* 0: none                                  */
+    int32_t request;             /* whose table lists the keys               */
+    int32_t begin;
+    int32_t end;
+    int32_t keys;                /* of all items, in 1024                    */
+    int32_t reserved[2];
+} nz_shared_item;
+
+/* Where a row's sums are found: items group_first, group_first + group_step,
+ * ... (group_count of them) and own_first, own_first + 1, ... (own_count), and
+ * the row's place among the item's rows. */
+typedef struct nz_shared_row {
+    int32_t group_first, group_step, group_count, group_place;
+    int32_t own_first, own_count, own_place;
+    int32_t context;
+} nz_shared_row;
+
+typedef struct nz_shared_plan_args {
+    const int32_t* contexts;     /* n_rows: keys that a row sees             */
+    const int32_t* requests;     /* n_rows, or NULL: row i is request i      */
+    const int32_t* groups;       /* n_requests: a request's group, -1 none   */
+    const int32_t* shared;       /* n_groups: keys that its requests share   */
+    nz_shared_item* items;       /* n_items (out)                            */
+    nz_shared_row* rows;         /* n_rows (out)                             */
+    int32_t* order;              /* 2 * n_rows (out)                         */
+    uint32_t* counters;          /* n_rows * kv_heads * ceil(heads / kv_heads / NZ_SHARED_COLUMNS) (out) */
+    uint32_t n_rows;
+    uint32_t n_requests;
+    uint32_t n_groups;
+    uint32_t n_items;            /* nz_shared_items(...) at least            */
+    uint32_t heads;
+    uint32_t kv_heads;
+    uint32_t target;             /* items wanted                             */
+    uint32_t reserved;           /* 0 */
+} nz_shared_plan_args;
+
+/* Items that a plan needs room for; 0 for numbers that no plan takes. */
+uint32_t nz_shared_items(uint32_t n_rows, uint32_t n_groups, uint32_t heads, uint32_t kv_heads, uint32_t target);
+
+/* Cuts the keys of n_rows rows into items of about equal length, on the
+ * device, so that keys that several rows see are read once for as many rows
+ * as make NZ_SHARED_COLUMNS columns: the first shared[g] keys of the requests
+ * of group g, which must be at the same pages (their table rows begin with the
+ * same ones), and the other keys of neighbouring rows of one request. Negative
+ * contexts and numbers count as 0; a request outside n_requests has no keys,
+ * and a group outside n_groups is none. At most NZ_SHARED_MAX_ROWS rows and
+ * NZ_SHARED_MAX_GROUPS groups. */
+int nz_shared_plan(const nz_shared_plan_args* args, void* stream);
+
+typedef struct nz_shared_attention_args {
+    const void* q;               /* n_rows x heads x head_dim                */
+    const void* key_cache;
+    const void* value_cache;
+    void* out;                   /* n_rows x heads x head_dim                */
+    const int32_t* tables;       /* n_requests x max_pages                   */
+    const nz_shared_item* items; /* the plan's                               */
+    const nz_shared_row* rows;
+    const int32_t* order;
+    uint32_t* counters;
+    float* partials;             /* nz_shared_partials(...) words            */
+    int64_t q_row, q_head, out_row, out_head;
+    int64_t key_page, key_head, key_slot, value_page, value_head, value_slot;
+    uint32_t n_rows;
+    uint32_t n_items;
+    uint32_t heads;
+    uint32_t kv_heads;
+    uint32_t head_dim;
+    uint32_t n_requests;
+    uint32_t max_pages;
+    uint32_t page_size;
+    uint32_t n_pages;
+    uint32_t type;
+    float scale;
+    uint32_t reserved;           /* 0 */
+} nz_shared_attention_args;
+
+/* 32-bit words of scratch that nz_shared_attention needs for a plan of n_items. */
+uint64_t nz_shared_partials(uint32_t n_items, uint32_t heads, uint32_t kv_heads, uint32_t head_dim);
+
+/* nz_attention's results, with a plan of nz_shared_plan for as many rows and
+ * requests and the same heads. Calls with one plan must not overlap.
+ * nz_shared_partials(...) is below 2^30 + 2^24. */
+int nz_shared_attention(const nz_shared_attention_args* args, void* stream);
+
 typedef struct nz_logits_args {
     const void* logits;          /* rows x vocab                             */
     void* out;                   /* rows x vocab (may be logits itself)      */
@@ -728,6 +845,115 @@ typedef struct nz_logits_args {
  * rounded once. Ids outside the vocabulary are ignored. There are at most
  * 65535 rows. */
 int nz_adjust_logits(const nz_logits_args* args, void* stream);
+
+typedef struct nz_verify_args {
+    const void* logits;          /* n_rows x vocab                           */
+    const float* draft_probs;    /* n_rows x vocab, or NULL: drafts are certain */
+    const int64_t* tokens;       /* n_rows: the token that a row was computed from */
+    const int32_t* starts;       /* n_requests + 1: first row of each        */
+    const double* accept;        /* n_rows: numbers from [0, 1)              */
+    const double* sample;        /* n_requests: numbers from [0, 1)          */
+    const float* temperature;    /* n_requests, or NULL: 1                   */
+    int32_t* accepted;           /* n_requests (out)                         */
+    int64_t* next;               /* n_requests (out)                         */
+    void* scratch;               /* nz_verify_scratch(...) bytes             */
+    int64_t logits_row, draft_row;
+    uint32_t n_rows;
+    uint32_t n_requests;
+    uint32_t vocab;
+    uint32_t type;               /* of the logits                            */
+} nz_verify_args;
+
+/* Tokens of a row that a workgroup takes. */
+#define NZ_VERIFY_CHUNK 4096
+
+/* Bytes of scratch of a call of nz_verify_drafts. */
+uint64_t nz_verify_scratch(uint32_t n_rows, uint32_t n_requests, uint32_t vocab);
+
+/* Checks drafted tokens against the model's probabilities and picks the token
+ * after the last one kept. Request r's rows are starts[r] .. starts[r + 1] -
+ * 1; row j's draft is the token of row j + 1, if that is the request's too.
+ * With p = softmax(logits[j] / temperature[r]) -- certainty of the first of
+ * the largest logits where the temperature is not above 0 -- and q =
+ * draft_probs[j], or certainty of the draft, a request's drafts are accepted
+ * while accept[j] * q(draft) < p(draft). accepted[r] counts them. next[r] is
+ * picked by sample[r] from the row of the first one refused, with weights
+ * max(p - q, 0) (or p, should none be positive), or else from p in the
+ * request's last row: the first token at which the sum of the weights so far
+ * exceeds sample[r] times all of them, or the last one with a weight. A token
+ * outside the vocabulary is no draft: it is refused, and the next token picked
+ * from p. next is -1 for a request without rows, which accepts nothing, and
+ * where no logit is above -infinity. In 64 bits. NaN counts as a logit of
+ * -infinity, and a draft probability of NaN leaves nothing of p. At most 65535
+ * rows and requests and 2^22 tokens. */
+int nz_verify_drafts(const nz_verify_args* args, void* stream);
+
+enum nz_route_scoring { NZ_ROUTE_SOFTMAX = 0, NZ_ROUTE_SIGMOID = 1 };
+enum nz_expert_activation { NZ_EXPERT_SILU = 0, NZ_EXPERT_GELU = 1 };
+
+/* Experts of a layer, choices of a token, a router's hidden size, and tokens
+ * of one pass over the experts' weights, at most. */
+#define NZ_EXPERT_MAX 1024
+#define NZ_ROUTE_MAX_TOP 32
+#define NZ_ROUTE_MAX_HIDDEN 16384
+#define NZ_EXPERT_TOKENS 64
+
+typedef struct nz_route_args {
+    const void* x;               /* tokens x hidden                          */
+    const void* weight;          /* experts x hidden                         */
+    const float* bias;           /* experts, or NULL                         */
+    int32_t* ids;                /* tokens x top_k (out)                     */
+    float* weights;              /* tokens x top_k (out)                     */
+    int64_t x_row;
+    uint32_t tokens;
+    uint32_t hidden;
+    uint32_t experts;
+    uint32_t top_k;
+    uint32_t type;               /* of x                                     */
+    uint32_t weight_type;        /* `type` or NZ_FP32                        */
+    uint32_t scoring;            /* enum nz_route_scoring                    */
+    uint32_t normalize;          /* 1: a token's weights sum to `scale`      */
+    float scale;
+    uint32_t reserved;           /* 0 */
+} nz_route_args;
+
+/* Each token's top_k experts, the best first: by x . weight[e], or by its
+ * sigmoid plus bias[e], the lower expert first where two are equal; NaN is
+ * never before another. Their weights are scale times the softmax over all
+ * experts, or the sigmoids (without the bias), divided by their sum if
+ * `normalize` (0 if that is 0). In 64 bits, weights rounded once. hidden is a
+ * multiple of 8; the weight is dense and on a 16-byte boundary. */
+int nz_route_experts(const nz_route_args* args, void* stream);
+
+typedef struct nz_expert_args {
+    const void* x;               /* tokens x hidden                          */
+    const void* ids;             /* tokens x top_k, of id_bytes each         */
+    const float* weights;        /* tokens x top_k                           */
+    const void* gate_up;         /* experts x 2 * inter x hidden: gate rows, then up rows */
+    const void* down;            /* experts x hidden x inter                 */
+    void* out;                   /* tokens x hidden                          */
+    void* scratch;               /* nz_expert_scratch(...) bytes             */
+    int64_t x_row, out_row, gate_expert, gate_row, down_expert, down_row;
+    uint32_t tokens;
+    uint32_t hidden;
+    uint32_t inter;
+    uint32_t experts;
+    uint32_t top_k;
+    uint32_t type;               /* of x, gate_up, down and out              */
+    uint32_t id_bytes;           /* 4 or 8                                   */
+    uint32_t activation;         /* enum nz_expert_activation                */
+} nz_expert_args;
+
+/* Bytes of scratch of a call of nz_expert_mlp; calls on one stream may share it. */
+uint64_t nz_expert_scratch(uint32_t tokens, uint32_t hidden, uint32_t inter, uint32_t top_k);
+
+/* out[t] = the sum over k of weights[t, k] * down[e] (act(gate[e] x[t]) *
+ * (up[e] x[t])), e = ids[t, k]; an expert outside the layer adds nothing, and
+ * one that a token has twice adds both weights. In 32 bits, activations held
+ * to 16 bits at least, rounded once; the order of the sums depends on the ids
+ * alone. hidden and inter are multiples of 8, strides and addresses multiples
+ * of 16 bytes. */
+int nz_expert_mlp(const nz_expert_args* args, void* stream);
 
 #ifdef __cplusplus
 }

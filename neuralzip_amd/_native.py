@@ -88,16 +88,24 @@ class _Totals(ctypes.Structure):
 # fraction of filling a ctypes structure and is safe between threads.
 PAGES_EXTEND = struct.Struct("=13Q6I")
 PAGES_RELEASE = struct.Struct("=7Q6I")
+PAGES_TRIM = struct.Struct("=7Q6I")
 ROTARY = struct.Struct("=12Q14q11If")
 ATTENTION = struct.Struct("=8Q10q10IfI")
 LOGITS = struct.Struct("=13Q3q8I")
+SHARED_PLAN = struct.Struct("=8Q8I")
+SHARED_ATTENTION = struct.Struct("=10Q10q10IfI")
+VERIFY = struct.Struct("=10Q2q4I")
+ROUTE = struct.Struct("=5Qq8IfI")
+EXPERTS = struct.Struct("=7Q6q8I")
 ATTENTION_ITEM = np.dtype([(name, "<i4") for name in ("row", "request", "begin", "end", "index", "count", "first",
                                                       "keys")])
 VALUE_BF16, VALUE_FP16, VALUE_FP32 = 0, 1, 2   # enum nz_value_type
+ROUTE_SCORING = {"softmax": 0, "sigmoid": 1}    # enum nz_route_scoring
+EXPERT_ACTIVATION = {"silu": 0, "gelu": 1}      # enum nz_expert_activation
 
 _lib = None
 # The C ABI version (NZ_ABI_VERSION of include/neuralzip_hip.h) these bindings follow.
-ABI_VERSION = 13
+ABI_VERSION = 14
 # Activation rows one fused matrix-vector product takes (NZ_MATVEC_MAX_BATCH).
 MATVEC_MAX_BATCH = 4
 # Weights one fused product takes (NZ_MATVEC_MAX_WEIGHTS).
@@ -156,11 +164,21 @@ def lib():
         L.nz_clusterer_destroy.restype = None
         L.nz_clusterer_assign.argtypes = [vp, vp, u64, ctypes.c_int32, vp, vp, vp]
         L.nz_clusterer_count.argtypes = [vp, ctypes.POINTER(u32)]
-        for name in ("nz_pages_extend", "nz_pages_release", "nz_rotary_store", "nz_attention", "nz_adjust_logits"):
+        for name in ("nz_pages_extend", "nz_pages_release", "nz_pages_trim", "nz_rotary_store", "nz_attention",
+                     "nz_adjust_logits", "nz_shared_plan", "nz_shared_attention", "nz_verify_drafts",
+                     "nz_route_experts", "nz_expert_mlp"):
             getattr(L, name).argtypes = [ctypes.c_char_p, vp]
         L.nz_attention_plan.argtypes = [vp, vp, u32, u32, u32, vp, vp, vp]
         L.nz_attention_partials.argtypes = [u32, u32, u32]
         L.nz_attention_partials.restype = u64
+        L.nz_shared_items.argtypes = [u32, u32, u32, u32, u32]
+        L.nz_shared_items.restype = u32
+        L.nz_shared_partials.argtypes = [u32, u32, u32, u32]
+        L.nz_shared_partials.restype = u64
+        L.nz_verify_scratch.argtypes = [u32, u32, u32]
+        L.nz_verify_scratch.restype = u64
+        L.nz_expert_scratch.argtypes = [u32, u32, u32, u32]
+        L.nz_expert_scratch.restype = u64
         _lib = L
     return _lib
 

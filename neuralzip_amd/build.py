@@ -16,7 +16,8 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 HOST_SOURCES = ("codebook.cpp", "layout.cpp", "codec.cpp", "capi.cpp", "capi_storage.cpp", "capi_serving.cpp",
                 "survey.cpp")
 DEVICE_SOURCES = ("hip/decode_gfx950.hip", "hip/matvec_gfx950.hip", "hip/serving_gfx950.hip",
-                  "hip/attention_gfx950.hip")
+                  "hip/attention_gfx950.hip", "hip/shared_attention_gfx950.hip", "hip/verify_gfx950.hip",
+                  "hip/experts_gfx950.hip")
 COMMON = ["-O3", "-std=c++17", "-fPIC", "-Wall", "-I", str(CSRC), "-I", str(ROOT / "include")]
 # host float arithmetic (the setup's clustering) is evaluated as written: no fused multiply-add
 HOST_FLAGS = ["-ffp-contract=off"]

@@ -6,7 +6,6 @@
 
 #include <algorithm>
 #include <stdint.h>
-#include <stdio.h>
 
 #include "neuralzip_hip.h"
 #include "serving_types.h"
@@ -143,33 +142,44 @@ __global__ __launch_bounds__(THREADS) void nz_pages_extend_kernel(nz_pages_exten
     }
 }
 
+// Tokens that stay of a request's `length`.
+__device__ __forceinline__ int32_t kept_of(const nz_pages_release_args& a, uint32_t r, int32_t length) {
+    return a.done[r] != 0 ? 0 : length;
+}
+
+__device__ __forceinline__ int32_t kept_of(const nz_pages_trim_args& a, uint32_t r, int32_t length) {
+    return min(max(a.keep[r], 0), length);
+}
+
 // Prefix sums over the requests of the pages they give back, then the pages,
 // each found by a search in the sums: 22131 pages of 250 of 1000 requests take
 // 3.7 us, and 20 by one workgroup alone.
-template <uint32_t THREADS>
-__global__ __launch_bounds__(THREADS) void nz_pages_release_kernel(nz_pages_release_args a) {
+template <uint32_t THREADS, typename Args>
+__device__ __forceinline__ void give_back(const Args& a) {
     __shared__ uint32_t waves[1][THREADS / 64];
-    __shared__ uint32_t first[THREADS];
+    __shared__ uint32_t first[THREADS], stays[THREADS];
     const uint32_t page = a.page_size, shift = 31 - __clz(page);
     const uint32_t stride = gridDim.x * THREADS, at = blockIdx.x * THREADS + threadIdx.x;
     uint32_t top = min(static_cast<uint32_t>(max(a.n_free[0], 0)), a.n_pages);
     for (uint32_t r0 = 0; r0 < a.n_requests; r0 += THREADS) {
         const uint32_t r = r0 + threadIdx.x;
-        const bool live = r < a.n_requests, done = live && a.done[r] != 0;
-        const int32_t length = live ? max(a.lengths[r], 0) : 0;
-        const uint32_t back = done ? min((static_cast<uint32_t>(length) + page - 1) >> shift, a.max_pages) : 0;
+        const bool live = r < a.n_requests;
+        const int32_t length = live ? max(a.lengths[r], 0) : 0, kept_tokens = live ? kept_of(a, r, length) : 0;
+        const uint32_t stay = min((static_cast<uint32_t>(kept_tokens) + page - 1) >> shift, a.max_pages);
+        const uint32_t back = min((static_cast<uint32_t>(length) + page - 1) >> shift, a.max_pages) - stay;
         uint32_t sum[1] = {back}, total[1];
         block_scan<THREADS, 1>(sum, total, waves);
         first[threadIdx.x] = sum[0] - back;
+        stays[threadIdx.x] = stay;
         if (live && blockIdx.x == 0) {
-            a.lengths_after[r] = done ? 0 : length;
-            if (a.advance && gridDim.x == 1) const_cast<int32_t*>(a.lengths)[r] = done ? 0 : length;
+            a.lengths_after[r] = kept_tokens;
+            if (a.advance && gridDim.x == 1) const_cast<int32_t*>(a.lengths)[r] = kept_tokens;
         }
         __syncthreads();
         const uint32_t kept = min(total[0], a.n_pages - top);
         for (uint32_t j = at; j < kept; j += stride) {
             const uint32_t i = owner(first, THREADS, j);
-            a.free_pages[top + j] = a.tables[static_cast<uint64_t>(r0 + i) * a.max_pages + j - first[i]];
+            a.free_pages[top + j] = a.tables[static_cast<uint64_t>(r0 + i) * a.max_pages + stays[i] + j - first[i]];
         }
         top += kept;
         __syncthreads();
@@ -179,6 +189,12 @@ __global__ __launch_bounds__(THREADS) void nz_pages_release_kernel(nz_pages_rele
         if (a.advance && gridDim.x == 1) const_cast<int32_t*>(a.n_free)[0] = static_cast<int32_t>(top);
     }
 }
+
+template <uint32_t THREADS>
+__global__ __launch_bounds__(THREADS) void nz_pages_release_kernel(nz_pages_release_args a) { give_back<THREADS>(a); }
+
+template <uint32_t THREADS>
+__global__ __launch_bounds__(THREADS) void nz_pages_trim_kernel(nz_pages_trim_args a) { give_back<THREADS>(a); }
 
 // The state after a call of several workgroups, which read the old one until
 // the last of them ends.
@@ -440,13 +456,6 @@ __global__ __launch_bounds__(kLogitsThreads) void nz_logits_kernel(nz_logits_arg
     }
 }
 
-int launched(const char* what, char* message, size_t message_size) {
-    const hipError_t rc = hipGetLastError();
-    if (rc == hipSuccess) return 0;
-    snprintf(message, message_size, "%s launch failed: %s", what, hipGetErrorString(rc));
-    return -6;
-}
-
 template <typename T>
 void launch_rotary(const nz_rotary_args& a, hipStream_t stream) {
     uint32_t lanes = 1;
@@ -497,6 +506,14 @@ extern "C" int nz_hip_pages_release(const nz_pages_release_args* args, void* str
     NZ_PAGES(nz_pages_release_kernel,
              std::min<uint64_t>(args->n_pages, static_cast<uint64_t>(args->n_requests) * args->max_pages));
     return launched("pages release", message, message_size);
+}
+
+extern "C" int nz_hip_pages_trim(const nz_pages_trim_args* args, void* stream, char* message,
+                                    size_t message_size) {
+    // no more pages come back than there are, or than the tables hold
+    NZ_PAGES(nz_pages_trim_kernel,
+             std::min<uint64_t>(args->n_pages, static_cast<uint64_t>(args->n_requests) * args->max_pages));
+    return launched("pages trim", message, message_size);
 }
 
 extern "C" int nz_hip_rotary_store(const nz_rotary_args* args, void* stream, char* message, size_t message_size) {

@@ -1,12 +1,13 @@
 // serving_types.h -- shared by the serving-step kernels: value types, their
-// loads to and stores from 32-bit floats, a search in prefix sums. Device code
-// only.
+// loads to and stores from 32-bit floats, a search in prefix sums, and the
+// launchers' error report.
 #ifndef NZ_SERVING_TYPES_H
 #define NZ_SERVING_TYPES_H
 
 #include <hip/hip_runtime.h>
 
 #include <stdint.h>
+#include <stdio.h>
 
 namespace {
 
@@ -103,6 +104,14 @@ __device__ __forceinline__ uint32_t owner(const uint32_t* first, uint32_t n, uin
         else hi = mid;
     }
     return lo;
+}
+
+// After a launch: 0, or NZ_HIP_ERROR and its message.
+inline int launched(const char* what, char* message, size_t message_size) {
+    const hipError_t rc = hipGetLastError();
+    if (rc == hipSuccess) return 0;
+    snprintf(message, message_size, "%s launch failed: %s", what, hipGetErrorString(rc));
+    return -6;
 }
 
 }  // namespace

@@ -2,19 +2,27 @@
 one forward, around the weights that the runtime decodes.
 
   PageTables       block tables and a stack of free pages on the GPU; extend()
-                   gives a step's tokens their pages, slots and positions and
-                   release() takes finished requests' pages back
+                   gives a step's tokens their pages, slots and positions,
+                   trim() takes refused drafts' pages back and release()
+                   finished requests'
   Rotary           the heads' optional RMS norm and the position rotation of
                    queries and keys, with keys and values stored into their
                    pages, in one pass
   AttentionPlan    cuts a step's contexts into items of equal work, once for
   paged_attention  all layers; attention of single tokens over the pages
+  SharedPlan       the same for requests that begin with the same pages and for
+                   several rows of one request: shared keys are read once
+  route_experts    a mixture-of-experts layer for a few tokens: the router's
+  expert_mlp       choice, and the chosen experts' gated products
   adjust_logits    repetition, frequency and presence penalties, biases and
                    grammar masks, in one pass
+  verify_drafts    drafted tokens against the model's probabilities, from given
+                   random numbers, and the token after them (plain sampling
+                   where there are none)
 
 Every call launches gfx950 kernels through the C ABI (nz_pages_*,
-nz_rotary_store, nz_attention_*, nz_adjust_logits) on the current stream, or
-on `stream`, where its tensors must be ready. They may be let go after the
+nz_rotary_store, nz_attention_*, nz_shared_*, nz_route_experts, nz_expert_mlp,
+nz_adjust_logits, nz_verify_drafts) on the current stream, or on `stream`, where its tensors must be ready. They may be let go after the
 call: they are recorded for `stream`. Results are that stream's, and who uses
 them on another one waits for it and records them there. Nothing synchronises,
 and lengths, tables and plans never leave the device, so that a step can be
@@ -35,6 +43,9 @@ _TYPES = {torch.bfloat16: _native.VALUE_BF16, torch.float16: _native.VALUE_FP16,
 ATTENTION_WORKGROUPS = 256
 # Query heads of one workgroup (the columns of a matrix instruction).
 _HEADS = 16
+# The same for shared keys: workgroups, and columns (rows times query heads).
+SHARED_WORKGROUPS = 512
+_COLUMNS = 32
 # PageTables.extend's status of a request (enum nz_pages_status).
 PAGES_OK, PAGES_TOO_LONG, PAGES_NO_ROOM, PAGES_NO_PAGE = range(4)
 
@@ -220,6 +231,25 @@ class PageTables:
             _keep(stream, done, *self._state)
         return out
 
+    def trim(self, keep, *, advance=True, stream=None):
+        """Shortens the requests to their first `keep` (int32, one per
+        request) tokens and puts the pages past those back onto the free
+        stack, as after a verification that refused drafts; returns the state
+        after it. Requests that are no longer than that stay as they are, a
+        negative number counts as 0. Without `advance` lengths and n_free
+        stay."""
+        _check_vector("keep", keep, torch.int32, self.requests, self._index)
+        with _on(stream):
+            out = Released(self.requests, self.device)
+        lengths, tables, free, n_free = self._pointers
+        args = _native.PAGES_TRIM.pack(lengths, keep.data_ptr(), tables, free, n_free, out.lengths.data_ptr(),
+                                       out.n_free.data_ptr(), self.requests, self.max_pages, self.page_size,
+                                       self.num_pages, bool(advance), 0)
+        _call(_native.lib().nz_pages_trim, self.device, args, stream)
+        if stream is not None:
+            _keep(stream, keep, *self._state)
+        return out
+
 
 class Rotary:
     """Rotation by the angles whose cosines and sines are given, float32
@@ -335,6 +365,7 @@ class AttentionPlan:
         items, self._counters = words.split((8 * self.capacity, self.capacity * self._parts))
         self.items = items.view(self.capacity, 8)
         self._pointers = items.data_ptr(), self._counters.data_ptr()
+        self._format, self._function = _native.ATTENTION, _native.lib().nz_attention
         self._stream, self._scratch = _stream_handle(self.device, stream), {}
         self.update(contexts, requests=requests, stream=stream)
 
@@ -356,7 +387,7 @@ class AttentionPlan:
         """Address of the scratch for calls of `head_dim` on one stream."""
         scratch = self._scratch.get((handle, head_dim))
         if scratch is None:
-            words = _native.lib().nz_attention_partials(self.capacity, self.heads, head_dim)
+            words = self._words(head_dim)
             with _on(stream):
                 scratch = torch.empty(words, dtype=torch.float32, device=self.device)
                 if handle != self._stream:   # the plan's memory must outlive what runs there
@@ -364,10 +395,83 @@ class AttentionPlan:
             self._scratch[handle, head_dim] = scratch
         return scratch.data_ptr()
 
+    def _words(self, head_dim):
+        return _native.lib().nz_attention_partials(self.capacity, self.heads, head_dim)
+
+
+class SharedPlan(AttentionPlan):
+    """AttentionPlan for rows that see the same keys, which are then read
+    once for as many rows as make 32 query heads of a key-value head:
+
+    neighbouring rows of one request, as a step with drafted tokens has them;
+    and the first shared[g] keys of all requests of group g. `groups` (int32,
+    one per request: per row of the tables) gives a request's group, -1 for
+    none, `shared` (int32, one per group) the keys. The requests of a group
+    must have the same pages in their tables for these.
+
+    Rows see their contexts' keys, as with an AttentionPlan, and the results
+    are the same up to the order of the sums. At most 2048 rows and 1024
+    groups."""
+
+    def __init__(self, contexts, *, heads, kv_heads, requests=None, groups=None, shared=None, stream=None):
+        if kv_heads < 1 or heads < 1 or heads % kv_heads:
+            raise ValueError("heads must be a positive multiple of kv_heads.")
+        if contexts.dim() != 1 or contexts.dtype != torch.int32 or not contexts.is_cuda:
+            raise ValueError("contexts must be an int32 vector on the GPU.")
+        self.rows, self.heads, self.kv_heads = contexts.shape[0], heads, kv_heads
+        self.device, self._index = contexts.device, contexts.get_device()
+        if (groups is None) != (shared is None):
+            raise ValueError("groups and shared go together.")
+        self._groups = None
+        if groups is not None:
+            if groups.dim() != 1 or shared.dim() != 1:
+                raise ValueError("groups and shared are vectors.")
+            self._groups = groups.shape[0], shared.shape[0]
+        n_groups = self._groups[1] if self._groups else 0
+        parts = kv_heads * -(-(heads // kv_heads) // _COLUMNS)
+        self._target = max(1, SHARED_WORKGROUPS // parts)
+        self.capacity = _native.lib().nz_shared_items(self.rows, n_groups, heads, kv_heads, self._target)
+        if self.capacity == 0:
+            raise ValueError("A SharedPlan takes at most 2048 rows and 1024 groups.")
+        with _on(stream):
+            words = torch.empty(8 * self.capacity + self.rows * (10 + parts), dtype=torch.int32, device=self.device)
+        items, rows, order, self._counters = words.split((8 * self.capacity, 8 * self.rows, 2 * self.rows,
+                                                          self.rows * parts))
+        self.items = items.view(self.capacity, 8)
+        self._pointers = items.data_ptr(), rows.data_ptr(), order.data_ptr(), self._counters.data_ptr()
+        self._format, self._function = _native.SHARED_ATTENTION, _native.lib().nz_shared_attention
+        self._stream, self._scratch = _stream_handle(self.device, stream), {}
+        self.update(contexts, requests=requests, groups=groups, shared=shared, stream=stream)
+
+    def update(self, contexts, *, requests=None, groups=None, shared=None, stream=None):
+        """Plans the same number of rows (and requests and groups) anew."""
+        _check_vector("contexts", contexts, torch.int32, self.rows, self._index)
+        if requests is not None:
+            _check_vector("requests", requests, torch.int32, self.rows, self._index)
+        if (groups is None) != (self._groups is None) or (shared is None) != (groups is None):
+            raise ValueError("groups and shared are given as when the plan was made.")
+        n_requests, n_groups = self._groups or (0x7FFFFFFF, 0)
+        if groups is not None:
+            _check_vector("groups", groups, torch.int32, n_requests, self._index)
+            _check_vector("shared", shared, torch.int32, n_groups, self._index)
+        args = _native.SHARED_PLAN.pack(
+            contexts.data_ptr(), requests.data_ptr() if requests is not None else 0,
+            groups.data_ptr() if groups is not None else 0, shared.data_ptr() if shared is not None else 0,
+            *self._pointers, self.rows, n_requests, n_groups, self.capacity, self.heads, self.kv_heads, self._target, 0)
+        rc = _native.lib().nz_shared_plan(args, _stream_handle(self.device, stream))
+        if rc:
+            _native.check(rc)
+        if stream is not None:
+            _keep(stream, contexts, requests, groups, shared, self.items)
+        return self
+
+    def _words(self, head_dim):
+        return _native.lib().nz_shared_partials(self.capacity, self.heads, self.kv_heads, head_dim)
+
 
 def paged_attention(q, key_cache, value_cache, tables, plan, *, scale=None, out=None, stream=None):
     """softmax(scale q.K) V for every row of q (rows, heads, head_dim), over
-    the plan's context of its request: the keys and values at the request's
+    the context of its request in the plan (AttentionPlan or SharedPlan): the keys and values at the request's
     pages (`tables`, int32 (requests, max_pages)) of the caches (pages,
     kv_heads, page size, head_dim). Query head h reads key-value head
     h // (heads / kv_heads). `scale` is head_dim ** -0.5 by default. A row
@@ -401,11 +505,11 @@ def paged_attention(q, key_cache, value_cache, tables, plan, *, scale=None, out=
     if q2 != 1 or o2 != 1:
         raise ValueError("A head's elements must be contiguous.")
     handle = _stream_handle(plan.device, stream)
-    args = _native.ATTENTION.pack(
+    args = plan._format.pack(
         q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), out.data_ptr(), tables.data_ptr(),
         *plan._pointers, plan._partials(dim, handle, stream), q0, q1, o0, o1, *pool, rows, plan.capacity, heads,
         plan.kv_heads, dim, *table_shape, page_size, pages, kind, dim ** -0.5 if scale is None else scale, 0)
-    rc = _native.lib().nz_attention(args, handle)
+    rc = plan._function(args, handle)
     if rc:
         _native.check(rc)
     if stream is not None:
@@ -482,4 +586,152 @@ def adjust_logits(logits, *, history=None, lengths=None, prompt_lengths=None, re
     if stream is not None:
         _keep(stream, logits, history, lengths, prompt_lengths, repetition, frequency, presence, *(bias or ()), masks,
               mask_rows, out)
+    return out
+
+
+def verify_drafts(logits, tokens, starts, accept, sample, *, draft_probs=None, temperature=None, stream=None):
+    """Checks drafted tokens against the model's probabilities and picks the
+    token after the last one kept: (accepted, next), int32 and int64, one
+    per request.
+
+    logits (rows, vocab), in bfloat16, float16 or float32, are of a step whose
+    request r has the rows starts[r] .. starts[r + 1] - 1 (int32, requests + 1,
+    as Step.starts); tokens (int64) holds the tokens that the rows were
+    computed from: after a request's first row, its drafts. With p =
+    softmax(logits[j] / temperature) and q the probabilities that the draft was
+    drawn from (draft_probs[j], float32, rows x vocab; without them the draft
+    is certain), the draft of row j, in row j + 1, is accepted if those before
+    it were and accept[j] * q(draft) < p(draft). next is picked by the
+    request's `sample` from the row of the first draft refused, with weights
+    max(p - q, 0), or else from p in its last row: the first token at which the
+    sum of the weights exceeds sample times all of them. Answers made so are
+    distributed as the model's own. Without drafts this samples.
+
+    accept (rows) and sample (requests) are float64 numbers from [0, 1).
+    temperature: float32 per request; 0 or less takes the largest logit, the
+    first of equals; without it 1. A token outside the vocabulary is no draft:
+    it is refused and the next one picked from p. next is -1 for a request
+    without rows, and where no logit is above -inf. In 64 bits; NaN counts as
+    -inf. At most 65535 rows and requests and 2**22 tokens."""
+    if torch.is_grad_enabled():
+        _refuse_gradients(logits, draft_probs)
+    if logits.dim() != 2 or logits.dtype not in _TYPES or not logits.is_cuda or logits.stride(1) != 1:
+        raise ValueError("logits must be (rows, vocab) in bfloat16, float16 or float32 on the GPU, rows contiguous.")
+    (rows, vocab), index = logits.shape, logits.get_device()
+    if starts.dim() != 1 or starts.shape[0] < 1:
+        raise ValueError("starts must be a vector of one entry more than there are requests.")
+    requests = starts.shape[0] - 1
+    draft_ptr = draft_row = 0
+    if draft_probs is not None:
+        if draft_probs.shape != logits.shape or draft_probs.dtype is not torch.float32 \
+                or draft_probs.get_device() != index or draft_probs.stride(1) != 1:
+            raise ValueError("draft_probs must be float32 (rows, vocab) on the logits' device, rows contiguous.")
+        draft_ptr, draft_row = draft_probs.data_ptr(), draft_probs.stride(0)
+    lib = _native.lib()
+    with _on(stream):
+        accepted = torch.empty(requests, dtype=torch.int32, device=logits.device)
+        following = torch.empty(requests, dtype=torch.int64, device=logits.device)
+        scratch = torch.empty(lib.nz_verify_scratch(rows, requests, vocab), dtype=torch.uint8, device=logits.device)
+    args = _native.VERIFY.pack(
+        logits.data_ptr(), draft_ptr, _pointer("tokens", tokens, torch.int64, rows, index),
+        _pointer("starts", starts, torch.int32, requests + 1, index),
+        _pointer("accept", accept, torch.float64, rows, index),
+        _pointer("sample", sample, torch.float64, requests, index),
+        _pointer("temperature", temperature, torch.float32, requests, index), accepted.data_ptr(),
+        following.data_ptr(), scratch.data_ptr(), logits.stride(0), draft_row, rows, requests, vocab,
+        _TYPES[logits.dtype])
+    _call(lib.nz_verify_drafts, logits.device, args, stream)
+    if stream is not None:
+        _keep(stream, logits, tokens, starts, accept, sample, draft_probs, temperature)
+    return accepted, following
+
+
+def route_experts(x, weight, top_k, *, scoring="softmax", normalize=True, bias=None, scale=1.0, stream=None):
+    """The experts of each token: (ids, weights), int32 and float32 (tokens,
+    top_k), the best expert first.
+
+    The scores are x (tokens, hidden) times the rows of weight (experts,
+    hidden; in x's dtype or float32). With `scoring` "softmax" the largest are
+    chosen and weighted by their softmax over all experts; with "sigmoid"
+    those of the largest sigmoid plus `bias` (float32, experts), weighted by
+    the sigmoid. `normalize` divides a token's weights by their sum; `scale`
+    multiplies them. Of equal experts the lower one is first, and NaN is never
+    before another. In 64 bits, rounded once. hidden is a multiple of 8 up to
+    16384; at most 1024 experts, 32 of them chosen."""
+    if torch.is_grad_enabled():
+        _refuse_gradients(x, weight, bias)
+    if x.dim() != 2 or x.dtype not in _TYPES or x.stride(1) != 1 or weight.dim() != 2 \
+            or weight.shape[1] != x.shape[1]:
+        raise ValueError("x must be (tokens, hidden), rows contiguous, and weight (experts, hidden).")
+    if weight.dtype not in (x.dtype, torch.float32) or not weight.is_contiguous() or weight.get_device() != x.get_device():
+        raise ValueError("weight must be contiguous, in x's dtype or float32, on x's device.")
+    if scoring not in _native.ROUTE_SCORING:
+        raise ValueError(f"scoring is one of {', '.join(_native.ROUTE_SCORING)}.")
+    (tokens, hidden), experts = x.shape, weight.shape[0]
+    if not 1 <= top_k <= min(experts, 32):
+        raise ValueError("top_k must be from 1 to 32 and the experts.")
+    bias_ptr = _pointer("bias", bias, torch.float32, experts, x.get_device())
+    with _on(stream):
+        ids = torch.empty((tokens, top_k), dtype=torch.int32, device=x.device)
+        weights = torch.empty((tokens, top_k), dtype=torch.float32, device=x.device)
+    args = _native.ROUTE.pack(x.data_ptr(), weight.data_ptr(), bias_ptr, ids.data_ptr(), weights.data_ptr(),
+                              x.stride(0), tokens, hidden, experts, top_k, _TYPES[x.dtype], _TYPES[weight.dtype],
+                              _native.ROUTE_SCORING[scoring], bool(normalize), scale, 0)
+    _call(_native.lib().nz_route_experts, x.device, args, stream)
+    if stream is not None:
+        _keep(stream, x, weight, bias)
+    return ids, weights
+
+
+def expert_mlp(x, ids, weights, gate_up, down, *, activation="silu", out=None, stream=None):
+    """The sum over a token's experts e of its weight times down[e]
+    (act(gate[e] x) * (up[e] x)), like x (tokens, hidden).
+
+    ids (int32 or int64) and weights (float32), (tokens, top_k), are as
+    route_experts gives them; gate_up (experts, 2 * inter, hidden) holds each
+    expert's gate rows and then its up rows, down is (experts, hidden, inter),
+    both in x's dtype. `activation` is "silu" or "gelu" (with erf). An expert
+    outside the layer adds nothing, and one that a token has twice adds both
+    weights. In 32 bits, rounded once, in an order that only the ids decide.
+    hidden and inter are multiples of 8; any strides whose rows lie on 16-byte
+    boundaries. Made for a few tokens: the experts' weights are read once for
+    every 64."""
+    if torch.is_grad_enabled():
+        _refuse_gradients(x, weights, gate_up, down)
+    dtype, index = x.dtype, x.get_device()
+    if x.dim() != 2 or dtype not in _TYPES or gate_up.dim() != 3 or down.dim() != 3:
+        raise ValueError("x must be (tokens, hidden), gate_up (experts, 2 * inter, hidden) and down (experts, hidden, "
+                         "inter).")
+    (tokens, hidden), (experts, _, inter) = x.shape, down.shape
+    if gate_up.shape != (experts, 2 * inter, hidden) or down.shape[1] != hidden:
+        raise ValueError(f"gate_up {tuple(gate_up.shape)} and down {tuple(down.shape)} do not fit one another or "
+                         f"x {tuple(x.shape)}.")
+    if gate_up.dtype is not dtype or down.dtype is not dtype or gate_up.get_device() != index \
+            or down.get_device() != index:
+        raise ValueError("The experts' weights must have x's dtype and device.")
+    if x.stride(1) != 1 or gate_up.stride(2) != 1 or down.stride(2) != 1:
+        raise ValueError("Rows must be contiguous.")
+    if ids.dim() != 2 or ids.shape[0] != tokens or ids.dtype not in (torch.int32, torch.int64) \
+            or ids.get_device() != index or not ids.is_contiguous():
+        raise ValueError("ids must be contiguous int32 or int64 (tokens, top_k) on x's device.")
+    if weights.shape != ids.shape or weights.dtype is not torch.float32 or weights.get_device() != index \
+            or not weights.is_contiguous():
+        raise ValueError("weights must be contiguous float32 like ids, on x's device.")
+    if activation not in _native.EXPERT_ACTIVATION:
+        raise ValueError(f"activation is one of {', '.join(_native.EXPERT_ACTIVATION)}.")
+    top_k, lib = ids.shape[1], _native.lib()
+    if out is None:
+        out = _like(x, stream)
+    elif out.shape != x.shape or out.dtype is not dtype or out.get_device() != index or out.stride(1) != 1:
+        raise ValueError("`out` must be like x, rows contiguous.")
+    with _on(stream):
+        scratch = torch.empty(lib.nz_expert_scratch(tokens, hidden, inter, top_k), dtype=torch.uint8, device=x.device)
+    args = _native.EXPERTS.pack(
+        x.data_ptr(), ids.data_ptr(), weights.data_ptr(), gate_up.data_ptr(), down.data_ptr(), out.data_ptr(),
+        scratch.data_ptr(), x.stride(0), out.stride(0), gate_up.stride(0), gate_up.stride(1), down.stride(0),
+        down.stride(1), tokens, hidden, inter, experts, top_k, _TYPES[dtype], ids.element_size(),
+        _native.EXPERT_ACTIVATION[activation])
+    _call(lib.nz_expert_mlp, x.device, args, stream)
+    if stream is not None:
+        _keep(stream, x, ids, weights, gate_up, down, out)
     return out
