@@ -864,8 +864,9 @@ typedef struct nz_verify_args {
     uint32_t type;               /* of the logits                            */
 } nz_verify_args;
 
-/* Tokens of a row that a workgroup takes. */
+/* Tokens of a row that a workgroup takes, and tokens of a row at most. */
 #define NZ_VERIFY_CHUNK 4096
+#define NZ_VERIFY_MAX_VOCAB (1 << 22)
 
 /* Bytes of scratch of a call of nz_verify_drafts. */
 uint64_t nz_verify_scratch(uint32_t n_rows, uint32_t n_requests, uint32_t vocab);
@@ -885,17 +886,16 @@ uint64_t nz_verify_scratch(uint32_t n_rows, uint32_t n_requests, uint32_t vocab)
  * from p. next is -1 for a request without rows, which accepts nothing, and
  * where no logit is above -infinity. In 64 bits. NaN counts as a logit of
  * -infinity, and a draft probability of NaN leaves nothing of p. At most 65535
- * rows and requests and 2^22 tokens. */
+ * rows and requests and NZ_VERIFY_MAX_VOCAB tokens. */
 int nz_verify_drafts(const nz_verify_args* args, void* stream);
 
 enum nz_route_scoring { NZ_ROUTE_SOFTMAX = 0, NZ_ROUTE_SIGMOID = 1 };
 enum nz_expert_activation { NZ_EXPERT_SILU = 0, NZ_EXPERT_GELU = 1 };
 
-/* Experts of a layer, choices of a token, a router's hidden size, and tokens
- * of one pass over the experts' weights, at most. */
+/* Experts of a layer, choices of a token, and tokens of one pass over the
+ * experts' weights, at most. */
 #define NZ_EXPERT_MAX 1024
 #define NZ_ROUTE_MAX_TOP 32
-#define NZ_ROUTE_MAX_HIDDEN 16384
 #define NZ_EXPERT_TOKENS 64
 
 typedef struct nz_route_args {
@@ -904,6 +904,7 @@ typedef struct nz_route_args {
     const float* bias;           /* experts, or NULL                         */
     int32_t* ids;                /* tokens x top_k (out)                     */
     float* weights;              /* tokens x top_k (out)                     */
+    void* scratch;               /* tokens x experts 64-bit numbers          */
     int64_t x_row;
     uint32_t tokens;
     uint32_t hidden;
@@ -922,7 +923,8 @@ typedef struct nz_route_args {
  * never before another. Their weights are scale times the softmax over all
  * experts, or the sigmoids (without the bias), divided by their sum if
  * `normalize` (0 if that is 0). In 64 bits, weights rounded once. hidden is a
- * multiple of 8; the weight is dense and on a 16-byte boundary. */
+ * multiple of 8; the weight is dense and on a 16-byte boundary. At most 65535
+ * tokens. */
 int nz_route_experts(const nz_route_args* args, void* stream);
 
 typedef struct nz_expert_args {

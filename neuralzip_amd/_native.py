@@ -95,7 +95,7 @@ LOGITS = struct.Struct("=13Q3q8I")
 SHARED_PLAN = struct.Struct("=8Q8I")
 SHARED_ATTENTION = struct.Struct("=10Q10q10IfI")
 VERIFY = struct.Struct("=10Q2q4I")
-ROUTE = struct.Struct("=5Qq8IfI")
+ROUTE = struct.Struct("=6Qq8IfI")
 EXPERTS = struct.Struct("=7Q6q8I")
 ATTENTION_ITEM = np.dtype([(name, "<i4") for name in ("row", "request", "begin", "end", "index", "count", "first",
                                                       "keys")])

@@ -274,7 +274,7 @@ uint64_t nz_verify_scratch(uint32_t n_rows, uint32_t n_requests, uint32_t vocab)
 int nz_verify_drafts(const nz_verify_args* args, void* stream) {
     return run(args, stream, nz_hip_verify_drafts, [](const nz_verify_args& a) {
         type_size(a.type);
-        if (a.n_rows > 65535 || a.n_requests > 65535 || a.vocab == 0 || a.vocab > 1u << 22)
+        if (a.n_rows > 65535 || a.n_requests > 65535 || a.vocab == 0 || a.vocab > NZ_VERIFY_MAX_VOCAB)
             refuse("There must be at most 65535 rows and requests, and 1 to 2^22 tokens.");
         if (a.n_requests == 0) return true;
         if (!a.starts || !a.sample || !a.accepted || !a.next ||
@@ -293,13 +293,14 @@ int nz_route_experts(const nz_route_args* args, void* stream) {
         if (a.scoring > NZ_ROUTE_SIGMOID || a.normalize > 1 || a.reserved)
             refuse("scoring is an nz_route_scoring, normalize 0 or 1 and reserved 0.");
         check_hidden(a.hidden, "hidden must be a positive multiple of 8.");
-        if (a.hidden > NZ_ROUTE_MAX_HIDDEN || a.experts > NZ_EXPERT_MAX || a.tokens > kMaxGrid)
+        if (a.hidden > 1u << 24 || a.experts > NZ_EXPERT_MAX || a.tokens > 65535)
             refuse("Too many experts or tokens, or too long rows.");
         if (a.top_k == 0 || a.top_k > NZ_ROUTE_MAX_TOP || a.top_k > a.experts)
             refuse("top_k must be from 1 to NZ_ROUTE_MAX_TOP and the experts.");
         if (a.tokens == 0) return true;
-        if (!a.x || !a.weight || !a.ids || !a.weights) refuse("Null router argument.");
+        if (!a.x || !a.weight || !a.ids || !a.weights || !a.scratch) refuse("Null router argument.");
         check_alignment(4, a.weight, 0);
+        if (reinterpret_cast<uintptr_t>(a.scratch) % 8) refuse("The scratch must be on an 8-byte boundary.");
         return false;
     });
 }

@@ -17,7 +17,7 @@ namespace {
 
 // ------------------------------------------------------------------ router
 
-constexpr uint32_t kRouteThreads = 1024, kRouteWaves = kRouteThreads / 64;
+constexpr uint32_t kScoreThreads = 256, kScoreWaves = kScoreThreads / 64;
 
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
@@ -25,72 +25,84 @@ __device__ __forceinline__ double wave_sum(double v) {
     return v;
 }
 
-// One token: its products with every expert's row, summed in 64 bits so that
-// the choice does not depend on their order, then each expert's place among
-// them by counting those before it.
-template <typename T, typename W>
-__global__ __launch_bounds__(kRouteThreads) void nz_route_kernel(nz_route_args a) {
-    constexpr uint32_t kRun = run_of<W>();
-    __shared__ double score[NZ_EXPERT_MAX], chance[NZ_EXPERT_MAX];
-    __shared__ double sums[kRouteWaves], tops[kRouteWaves];
-    extern __shared__ __align__(16) float x[];
-    const uint32_t token = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const T* src = static_cast<const T*>(a.x) + static_cast<int64_t>(token) * a.x_row;
-    for (uint32_t d = threadIdx.x; d < a.hidden; d += kRouteThreads) x[d] = to_float(src[d]);
-    __syncthreads();
-    for (uint32_t e = wave; e < a.experts; e += kRouteWaves) {
-        const W* row = static_cast<const W*>(a.weight) + static_cast<uint64_t>(e) * a.hidden;
-        double sum = 0.0;
-        for (uint32_t d = lane * kRun; d < a.hidden; d += 64 * kRun) {
-            const vec<W, kRun> w = *reinterpret_cast<const vec<W, kRun>*>(row + d);
+// Eight neighbouring elements, wherever they lie in memory.
+template <typename T>
+__device__ __forceinline__ void load_eight(const T* src, float (&x)[8]) {
+    T raw[8];
+    __builtin_memcpy(raw, src, sizeof raw);
 #pragma unroll
-            for (uint32_t i = 0; i < kRun; ++i)
-                sum = fma(static_cast<double>(to_float(static_cast<W>(w[i]))), static_cast<double>(x[d + i]), sum);
-        }
-        sum = wave_sum(sum);
-        if (lane == 0) score[e] = sum;
+    for (uint32_t i = 0; i < 8; ++i) x[i] = to_float(raw[i]);
+}
+
+// Tokens' products with the experts' rows, a wavefront each, summed in 64 bits
+// so that the choice does not depend on their order. (Both steps in one
+// workgroup per token took 22 us for one token of 2048 elements and 128
+// experts, which one compute unit multiplied.)
+template <typename T, typename W>
+__global__ __launch_bounds__(kScoreThreads) void nz_route_scores_kernel(nz_route_args a) {
+    const uint32_t token = blockIdx.y, lane = threadIdx.x & 63, e = blockIdx.x * kScoreWaves + (threadIdx.x >> 6);
+    if (e >= a.experts) return;
+    const T* src = static_cast<const T*>(a.x) + static_cast<int64_t>(token) * a.x_row;
+    const W* row = static_cast<const W*>(a.weight) + static_cast<uint64_t>(e) * a.hidden;
+    double sums[2] = {};
+#pragma unroll 4
+    for (uint32_t d = lane * 8; d < a.hidden; d += 512) {
+        float x[8], w[8];
+        load_eight(src + d, x);
+        load_runs(row + d, run_of<W>(), w);
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) sums[i % 2] = fma(static_cast<double>(w[i]), static_cast<double>(x[i]), sums[i % 2]);
     }
-    __syncthreads();
+    const double sum = wave_sum(sums[0] + sums[1]);
+    if (lane == 0) static_cast<double*>(a.scratch)[static_cast<uint64_t>(token) * a.experts + e] = sum;
+}
+
+// One token's choice, a thread per expert: its place is the number of those
+// before it.
+__global__ __launch_bounds__(NZ_EXPERT_MAX) void nz_route_choice_kernel(nz_route_args a) {
+    constexpr uint32_t kMaxWaves = NZ_EXPERT_MAX / 64;
+    __shared__ double ranks[NZ_EXPERT_MAX], sums[kMaxWaves], tops[kMaxWaves], picked[NZ_ROUTE_MAX_TOP];
+    const uint32_t token = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     // (threads past the experts take part in the sums)
     const uint32_t e = threadIdx.x;
-    double mine = e < a.experts ? score[e] : -INFINITY;
+    double mine = -INFINITY;
+    if (e < a.experts) mine = static_cast<const double*>(a.scratch)[static_cast<uint64_t>(token) * a.experts + e];
+    const double bias = a.bias != nullptr && e < a.experts ? static_cast<double>(a.bias[e]) : 0.0;
     if (mine != mine) mine = -INFINITY;
-    double top = mine;
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d <<= 1) top = fmax(top, __shfl_xor(top, d));
-    if (lane == 0) tops[wave] = top;
-    __syncthreads();
-#pragma unroll
-    for (uint32_t w = 0; w < kRouteWaves; ++w) top = fmax(top, tops[w]);
-    double share;
+    double share, rank;
     if (a.scoring == NZ_ROUTE_SIGMOID) {
         share = 1.0 / (1.0 + exp(-mine));
+        rank = share + bias;
     } else {
-        share = mine == top ? 1.0 : exp(mine - top);   // (infinite scores are equal)
-        const double sum = wave_sum(e < a.experts ? share : 0.0);
-        if (lane == 0) sums[wave] = sum;
-        __syncthreads();
-        double all = 0.0;
+        rank = mine + bias;
+        double top = mine;
 #pragma unroll
-        for (uint32_t w = 0; w < kRouteWaves; ++w) all += sums[w];
-        share /= all;
+        for (uint32_t d = 1; d < 64; d <<= 1) top = fmax(top, __shfl_xor(top, d));
+        if (lane == 0) tops[wave] = top;
+        __syncthreads();
+        for (uint32_t w = 0; w < waves; ++w) top = fmax(top, tops[w]);
+        share = mine == top ? 1.0 : exp(mine - top);   // (infinite scores are equal)
+        if (!a.normalize) {   // the chosen ones' sum divides them otherwise
+            const double sum = wave_sum(e < a.experts ? share : 0.0);
+            if (lane == 0) sums[wave] = sum;
+            __syncthreads();
+            double all = 0.0;
+            for (uint32_t w = 0; w < waves; ++w) all += sums[w];
+            share /= all;
+        }
     }
-    double rank = a.scoring == NZ_ROUTE_SIGMOID ? share : mine;
-    if (a.bias != nullptr && e < a.experts) rank += static_cast<double>(a.bias[e]);
     if (rank != rank) rank = -INFINITY;
+    if (e < a.experts) ranks[e] = rank;
     __syncthreads();
-    if (e < a.experts) score[e] = rank, chance[e] = share;
-    __syncthreads();
-    int32_t* const ids = a.ids + static_cast<uint64_t>(token) * a.top_k;
-    __shared__ double picked[NZ_ROUTE_MAX_TOP];
     if (e < a.experts) {
         uint32_t before = 0;
+#pragma unroll 8
         for (uint32_t j = 0; j < a.experts; ++j) {
-            const double other = score[j];
+            const double other = ranks[j];
             before += other > rank || (other == rank && j < e);
         }
         if (before < a.top_k) {
-            ids[before] = static_cast<int32_t>(e);
+            a.ids[static_cast<uint64_t>(token) * a.top_k + before] = static_cast<int32_t>(e);
             picked[before] = share;
         }
     }
@@ -113,16 +125,27 @@ constexpr uint32_t kTokens = NZ_EXPERT_TOKENS, kBlocks = kTokens / 16;
 constexpr uint32_t kUpThreads = 256, kUpWaves = kUpThreads / 64;
 constexpr uint32_t kDownThreads = 512, kDownWaves = kDownThreads / 64;
 // Elements of the outputs that a workgroup makes for its tokens.
-constexpr uint32_t kRows = 16;
+constexpr uint32_t kRows = 16, kDownRows = 32;
+// Pieces of a weight's row that a lane asks for before it multiplies any: a
+// wavefront's are neighbours, whole lines of the memory.
+constexpr uint32_t kBatch = 4;
+// Workgroups that share a part of the outputs, at most.
+constexpr uint32_t kMaxSplits = 8;
 
 // Which of a pass's tokens chose each expert, and the experts that any did, in
-// rising order.
+// rising order. In a workgroup's dynamic LDS, as long as the layer needs.
 struct Choice {
-    unsigned long long tokens[NZ_EXPERT_MAX];   // by expert, a bit per token
-    uint32_t active[NZ_EXPERT_MAX];
+    unsigned long long* tokens;   // by expert, a bit per token
+    uint32_t* active;
+    int32_t* ids;                 // tokens x top_k, -1: none
     uint32_t n_active;
-    uint32_t waves[kDownWaves];
-    int32_t ids[kTokens * NZ_ROUTE_MAX_TOP];    // -1: none
+
+    static __host__ __device__ uint32_t bytes(uint32_t experts, uint32_t choices) {
+        return (12 * experts + 4 * choices + 15) / 16 * 16;
+    }
+    __device__ Choice(unsigned char* lds, uint32_t experts)
+        : tokens(reinterpret_cast<unsigned long long*>(lds)), active(reinterpret_cast<uint32_t*>(lds + 8 * experts)),
+          ids(reinterpret_cast<int32_t*>(lds + 12 * experts)), n_active(0) {}
 };
 
 __device__ __forceinline__ int64_t id_at(const nz_expert_args& a, uint64_t i) {
@@ -131,32 +154,33 @@ __device__ __forceinline__ int64_t id_at(const nz_expert_args& a, uint64_t i) {
 
 template <uint32_t THREADS>
 __device__ __forceinline__ void choose(const nz_expert_args& a, uint32_t token0, uint32_t tokens, Choice& c) {
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ uint32_t waves[THREADS / 64];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = tokens * a.top_k;
+    const uint64_t first = static_cast<uint64_t>(token0) * a.top_k;
+    uint64_t id = threadIdx.x < n ? static_cast<uint64_t>(id_at(a, first + threadIdx.x)) : 0;
     for (uint32_t e = threadIdx.x; e < a.experts; e += THREADS) c.tokens[e] = 0;
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < tokens * a.top_k; i += THREADS) {
-        const uint64_t e = static_cast<uint64_t>(id_at(a, static_cast<uint64_t>(token0) * a.top_k + i));
-        if (e < a.experts) atomicOr(&c.tokens[e], 1ull << i / a.top_k);
-        c.ids[i] = e < a.experts ? static_cast<int32_t>(e) : -1;
+    for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+        if (i != threadIdx.x) id = static_cast<uint64_t>(id_at(a, first + i));
+        if (id < a.experts) atomicOr(&c.tokens[id], 1ull << i / a.top_k);
+        c.ids[i] = id < a.experts ? static_cast<int32_t>(id) : -1;
     }
     __syncthreads();
-    uint32_t before = 0;
     for (uint32_t e0 = 0; e0 < a.experts; e0 += THREADS) {
         const uint32_t e = e0 + threadIdx.x;
         const bool live = e < a.experts && c.tokens[e] != 0;
         const uint64_t bits = __ballot(live);
-        if (lane == 0) c.waves[wave] = __popcll(bits);
+        if (lane == 0) waves[wave] = __popcll(bits);
         __syncthreads();
-        uint32_t at = before;
+        uint32_t at = c.n_active;
+#pragma unroll
         for (uint32_t w = 0; w < THREADS / 64; ++w) {
-            if (w < wave) at += c.waves[w];
-            before += c.waves[w];
+            if (w < wave) at += waves[w];
+            c.n_active += waves[w];
         }
         if (live) c.active[at + __popcll(bits & ((1ull << lane) - 1))] = e;
         __syncthreads();
     }
-    if (threadIdx.x == 0) c.n_active = before;
-    __syncthreads();
 }
 
 // The place of an expert among a token's choices (the first, if it is there twice).
@@ -184,62 +208,73 @@ __device__ __forceinline__ float activate(uint32_t kind, float x) {
 
 // The gated activations of one expert's tokens, for kRows of its inner
 // elements: act(gate x) * (up x), in 32 bits. Weight rows are the rows of the
-// matrix instructions and tokens their columns; the wavefronts share the depth.
-template <typename T>
+// matrix instructions and tokens their columns, in up to NB blocks; the
+// wavefronts share the depth.
+template <typename T, uint32_t NB>
 __global__ __launch_bounds__(kUpThreads) void nz_expert_up_kernel(nz_expert_args a, float* __restrict__ acts,
                                                                   uint32_t* __restrict__ counters, uint32_t n_counters) {
     using P = Piece<T>;
     using piece = typename P::type;
     constexpr uint32_t kDepth = 4 * P::kRun;
-    __shared__ Choice choice;
+    extern __shared__ __align__(16) unsigned char lds[];
     __shared__ uint32_t list[kTokens];
-    __shared__ float sums[kUpWaves][2][kTokens][kRows + 1];
+    __shared__ float sums[kUpWaves][2][16 * NB][kRows + 1];
     const uint32_t lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0)
         for (uint32_t i = threadIdx.x; i < n_counters; i += kUpThreads) counters[i] = 0;
     const uint32_t token0 = blockIdx.z * kTokens, tokens = min(kTokens, a.tokens - token0);
+    Choice choice(lds, a.experts);
     choose<kUpThreads>(a, token0, tokens, choice);
     if (blockIdx.y >= choice.n_active) return;
     const uint32_t expert = choice.active[blockIdx.y];
     const uint64_t mask = choice.tokens[expert];
-    const uint32_t count = __popcll(mask), blocks = (count + 15) / 16;
+    const uint32_t count = __popcll(mask), blocks = __builtin_amdgcn_readfirstlane((count + 15) / 16);
     if (threadIdx.x < 64 && mask >> threadIdx.x & 1) list[__popcll(mask & ((1ull << threadIdx.x) - 1))] = threadIdx.x;
     __syncthreads();
     const uint32_t row0 = blockIdx.x * kRows, row = min(row0 + col, a.inter - 1);
     const T* const gate = static_cast<const T*>(a.gate_up) + expert * a.gate_expert + row * a.gate_row;
     const T* const up = gate + a.inter * a.gate_row;
-    const T* x[kBlocks];
+    const T* x[NB];
 #pragma unroll
-    for (uint32_t b = 0; b < kBlocks; ++b)
-        x[b] = static_cast<const T*>(a.x) + (token0 + (b * 16 + col < count ? list[b * 16 + col] : list[0])) * a.x_row;
-    f32x4 sum[2][kBlocks] = {};
-#pragma unroll 4
-    for (uint32_t d0 = wave * kDepth; d0 < a.hidden; d0 += kUpWaves * kDepth) {
-        const uint32_t d = d0 + quad * P::kRun;
-        piece g = {}, u = {};
-        if (d < a.hidden) {
-            g = *reinterpret_cast<const piece*>(gate + d);
-            u = *reinterpret_cast<const piece*>(up + d);
-        }
+    for (uint32_t b = 0; b < NB; ++b)
+        x[b] = static_cast<const T*>(a.x) + (token0 + list[b * 16 + col < count ? b * 16 + col : 0]) * a.x_row;
+    f32x4 sum[2][NB] = {};
+    for (uint32_t d0 = wave * kBatch * kDepth; d0 < a.hidden; d0 += kUpWaves * kBatch * kDepth) {
+        piece g[kBatch], u[kBatch], y[NB][kBatch];
 #pragma unroll
-        for (uint32_t b = 0; b < kBlocks; ++b) {
-            if (b < blocks) {
-                piece y = {};
-                if (d < a.hidden && b * 16 + col < count) y = *reinterpret_cast<const piece*>(x[b] + d);
-                sum[0][b] = P::mma(g, y, sum[0][b]);
-                sum[1][b] = P::mma(u, y, sum[1][b]);
+        for (uint32_t j = 0; j < kBatch; ++j) {
+            const uint32_t d = d0 + j * kDepth + quad * P::kRun;
+            g[j] = u[j] = piece{};
+            if (d < a.hidden) {
+                g[j] = *reinterpret_cast<const piece*>(gate + d);
+                u[j] = *reinterpret_cast<const piece*>(up + d);
             }
         }
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+            for (uint32_t j = 0; j < kBatch; ++j) {
+                const uint32_t d = d0 + j * kDepth + quad * P::kRun;
+                y[b][j] = piece{};
+                if (d < a.hidden && b * 16 + col < count) y[b][j] = *reinterpret_cast<const piece*>(x[b] + d);
+            }
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b)
+            if (NB == 1 || b < blocks)
+#pragma unroll
+                for (uint32_t j = 0; j < kBatch; ++j) {
+                    sum[0][b] = P::mma(g[j], y[b][j], sum[0][b]);
+                    sum[1][b] = P::mma(u[j], y[b][j], sum[1][b]);
+                }
     }
 #pragma unroll
-    for (uint32_t b = 0; b < kBlocks; ++b)
-        if (b < blocks)
+    for (uint32_t b = 0; b < NB; ++b)
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                sums[wave][0][b * 16 + col][4 * quad + i] = sum[0][b][i];
-                sums[wave][1][b * 16 + col][4 * quad + i] = sum[1][b][i];
-            }
+        for (uint32_t i = 0; i < 4; ++i) {
+            sums[wave][0][b * 16 + col][4 * quad + i] = sum[0][b][i];
+            sums[wave][1][b * 16 + col][4 * quad + i] = sum[1][b][i];
+        }
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < count * kRows; i += kUpThreads) {
         const uint32_t c = i / kRows, r = i % kRows;
@@ -284,82 +319,104 @@ __device__ __forceinline__ int split(const float (&x)[Piece<T>::kRun], typename 
     return lift;
 }
 
-// kRows elements of the outputs: over the chosen experts and their inner
+// kDownRows elements of the outputs: over the chosen experts and their inner
 // elements, each wavefront a share of them in a row, with the tokens that
 // chose an expert as columns; the columns of an expert are added to their
 // tokens' sums, times the weights, when it ends. `splits` workgroups share the
 // experts; the last to arrive adds their sums in order.
-template <typename T>
+template <typename T, uint32_t NB>
 __global__ __launch_bounds__(kDownThreads) void nz_expert_down_kernel(nz_expert_args a, const float* __restrict__ acts,
                                                                       float* __restrict__ partials,
                                                                       uint32_t* __restrict__ counters, uint32_t splits) {
     using P = Piece<T>;
     using piece = typename P::type;
-    constexpr uint32_t kDepth = 4 * P::kRun;
-    __shared__ Choice choice;
-    __shared__ __align__(16) float sums[kDownWaves][kTokens][kRows];
+    constexpr uint32_t kDepth = 4 * P::kRun, kTiles = kDownRows / 16;
+    constexpr bool kLifted = std::is_same<T, _Float16>::value;
+    extern __shared__ __align__(16) unsigned char lds[];
+    __shared__ __align__(16) float sums[kDownWaves][16 * NB][kDownRows];
     __shared__ uint32_t list[kDownWaves][kTokens];
     __shared__ uint32_t last;
     const uint32_t lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t token0 = blockIdx.z * kTokens, tokens = min(kTokens, a.tokens - token0);
-    for (uint32_t i = threadIdx.x; i < kDownWaves * kTokens * kRows; i += kDownThreads) (&sums[0][0][0])[i] = 0.0f;
+    for (uint32_t i = threadIdx.x; i < kDownWaves * 16 * NB * kDownRows; i += kDownThreads) (&sums[0][0][0])[i] = 0.0f;
+    Choice choice(lds, a.experts);
     choose<kDownThreads>(a, token0, tokens, choice);
-    const uint32_t row0 = blockIdx.x * kRows, row = min(row0 + col, a.hidden - 1);
-    const uint32_t steps = (a.inter + kDepth - 1) / kDepth;
+    const uint32_t row0 = blockIdx.x * kDownRows;
+    const uint32_t steps = (a.inter + kBatch * kDepth - 1) / (kBatch * kDepth);
     const uint64_t all = static_cast<uint64_t>(choice.n_active) * steps;
     const uint32_t shares = splits * kDownWaves, mine = blockIdx.y * kDownWaves + wave;
     uint64_t at = all * mine / shares;
     const uint64_t until = all * (mine + 1) / shares;
     while (at < until) {
-        const uint32_t n = static_cast<uint32_t>(at / steps), expert = choice.active[n];
-        const uint32_t s0 = static_cast<uint32_t>(at % steps);
+        const uint32_t n = static_cast<uint32_t>(at / steps);
+        const uint32_t expert = __builtin_amdgcn_readfirstlane(choice.active[n]), s0 = static_cast<uint32_t>(at % steps);
         const uint32_t s1 = static_cast<uint32_t>(min(static_cast<uint64_t>(steps), s0 + (until - at)));
         const uint64_t mask = choice.tokens[expert];
-        const uint32_t count = __popcll(mask), blocks = (count + 15) / 16;
+        const uint32_t count = __popcll(mask), blocks = __builtin_amdgcn_readfirstlane((count + 15) / 16);
         if (mask >> lane & 1) list[wave][__popcll(mask & ((1ull << lane) - 1))] = lane;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        const T* const down = static_cast<const T*>(a.down) + expert * a.down_expert + row * a.down_row;
-        const float* x[kBlocks];
-        uint32_t token[kBlocks];
+        const T* down[kTiles];
 #pragma unroll
-        for (uint32_t b = 0; b < kBlocks; ++b) {
+        for (uint32_t t = 0; t < kTiles; ++t)
+            down[t] = static_cast<const T*>(a.down) + expert * a.down_expert + min(row0 + 16 * t + col, a.hidden - 1) * a.down_row;
+        const float* x[NB];
+        uint32_t token[NB];
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b) {
             token[b] = b * 16 + col < count ? list[wave][b * 16 + col] : 0;
             x[b] = acts;
             if (b * 16 + col < count)
                 x[b] += (static_cast<uint64_t>(token0 + token[b]) * a.top_k + place_of(a, choice, token[b], expert)) * a.inter;
         }
-        f32x4 sum[kBlocks] = {};
-#pragma unroll 2
+        f32x4 sum[kTiles][NB] = {};
         for (uint32_t s = s0; s < s1; ++s) {
-            const uint32_t d = s * kDepth + quad * P::kRun;
-            piece w = {};
-            if (d < a.inter) w = *reinterpret_cast<const piece*>(down + d);
+            piece w[kTiles][kBatch];
 #pragma unroll
-            for (uint32_t b = 0; b < kBlocks; ++b) {
-                if (b < blocks) {
-                    float y[P::kRun] = {};
-                    if (d < a.inter && b * 16 + col < count) load_floats<P::kRun>(x[b] + d, y);
-                    piece hi, lo;
-                    const int lift = split<T>(y, hi, lo);
-                    f32x4 part = std::is_same<T, _Float16>::value ? f32x4{} : sum[b];
-                    part = P::mma(w, hi, part);
-                    if (sizeof(T) == 2) part = P::mma(w, lo, part);
-                    if (std::is_same<T, _Float16>::value) {
+            for (uint32_t t = 0; t < kTiles; ++t)
 #pragma unroll
-                        for (uint32_t i = 0; i < 4; ++i) sum[b][i] += __builtin_amdgcn_ldexpf(part[i], lift);
-                    } else {
-                        sum[b] = part;
+                for (uint32_t j = 0; j < kBatch; ++j) {
+                    const uint32_t d = (s * kBatch + j) * kDepth + quad * P::kRun;
+                    w[t][j] = piece{};
+                    if (d < a.inter) w[t][j] = *reinterpret_cast<const piece*>(down[t] + d);
+                }
+#pragma unroll
+            for (uint32_t b = 0; b < NB; ++b)
+                if (NB == 1 || b < blocks) {
+                    float y[kBatch][P::kRun] = {};
+#pragma unroll
+                    for (uint32_t j = 0; j < kBatch; ++j) {
+                        const uint32_t d = (s * kBatch + j) * kDepth + quad * P::kRun;
+                        if (d < a.inter && b * 16 + col < count) load_floats<P::kRun>(x[b] + d, y[j]);
+                    }
+#pragma unroll
+                    for (uint32_t j = 0; j < kBatch; ++j) {
+                        piece hi, lo;
+                        const int lift = split<T>(y[j], hi, lo);
+#pragma unroll
+                        for (uint32_t t = 0; t < kTiles; ++t) {
+                            f32x4 part = kLifted ? f32x4{} : sum[t][b];
+                            part = P::mma(w[t][j], hi, part);
+                            if (sizeof(T) == 2) part = P::mma(w[t][j], lo, part);
+                            if (kLifted) {
+#pragma unroll
+                                for (uint32_t i = 0; i < 4; ++i) sum[t][b][i] += __builtin_amdgcn_ldexpf(part[i], lift);
+                            } else {
+                                sum[t][b] = part;
+                            }
+                        }
                     }
                 }
-            }
         }
 #pragma unroll
-        for (uint32_t b = 0; b < kBlocks; ++b) {
+        for (uint32_t b = 0; b < NB; ++b) {
             if (b * 16 + col < count) {
                 const float weight = weight_of(a, choice, token0, token[b], expert);
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) sums[wave][token[b]][4 * quad + i] += weight * sum[b][i];
+                for (uint32_t t = 0; t < kTiles; ++t) {
+                    f32x4* const to = reinterpret_cast<f32x4*>(&sums[wave][token[b]][16 * t + 4 * quad]);
+                    *to += weight * sum[t][b];
+                }
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the list's reads
@@ -369,14 +426,17 @@ __global__ __launch_bounds__(kDownThreads) void nz_expert_down_kernel(nz_expert_
     T* const out = static_cast<T*>(a.out);
     const uint64_t plane = static_cast<uint64_t>(a.tokens) * a.hidden;
     const rsrc_t scratch = device_buffer(partials);
-    for (uint32_t i = threadIdx.x; i < tokens * kRows / 4; i += kDownThreads) {
-        const uint32_t t = i / (kRows / 4), r = i % (kRows / 4) * 4;
+    const auto place = [&](uint32_t split, uint32_t t, uint32_t r) {
+        return 4 * static_cast<uint32_t>(split * plane + (token0 + t) * static_cast<uint64_t>(a.hidden) + row0 + r);
+    };
+    for (uint32_t i = threadIdx.x; i < tokens * kDownRows / 4; i += kDownThreads) {
+        const uint32_t t = i / (kDownRows / 4), r = i % (kDownRows / 4) * 4;
         if (row0 + r >= a.hidden) continue;
         f32x4 sum = {};
 #pragma unroll
         for (uint32_t w = 0; w < kDownWaves; ++w) sum += *reinterpret_cast<const f32x4*>(&sums[w][t][r]);
         if (splits == 1) store_row(out + (token0 + t) * a.out_row + row0 + r, sum, 1.0f);
-        else put_four(scratch, 4 * static_cast<uint32_t>(blockIdx.y * plane + (token0 + t) * static_cast<uint64_t>(a.hidden) + row0 + r), sum);
+        else put_four(scratch, place(blockIdx.y, t, r), sum);
     }
     if (splits == 1) return;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wavefront's stores have arrived
@@ -386,42 +446,57 @@ __global__ __launch_bounds__(kDownThreads) void nz_expert_down_kernel(nz_expert_
                                       __HIP_MEMORY_SCOPE_AGENT) + 1 == splits;
     __syncthreads();
     if (!last) return;
-    for (uint32_t i = threadIdx.x; i < tokens * kRows / 4; i += kDownThreads) {
-        const uint32_t t = i / (kRows / 4), r = i % (kRows / 4) * 4;
+    for (uint32_t i = threadIdx.x; i < tokens * kDownRows / 4; i += kDownThreads) {
+        const uint32_t t = i / (kDownRows / 4), r = i % (kDownRows / 4) * 4;
         if (row0 + r >= a.hidden) continue;
-        f32x4 sum = {};
-        for (uint32_t k = 0; k < splits; ++k)
-            sum += get_four(scratch, 4 * static_cast<uint32_t>(k * plane + (token0 + t) * static_cast<uint64_t>(a.hidden) + row0 + r));
+        f32x4 part[kMaxSplits], sum = {};
+#pragma unroll
+        for (uint32_t k = 0; k < kMaxSplits; ++k) part[k] = get_four(scratch, place(min(k, splits - 1), t, r));
+#pragma unroll
+        for (uint32_t k = 0; k < kMaxSplits; ++k)
+            if (k < splits) sum += part[k];
         store_row(out + (token0 + t) * a.out_row + row0 + r, sum, 1.0f);
     }
 }
 
+uint32_t down_groups(uint32_t hidden) { return (hidden + kDownRows - 1) / kDownRows; }
+
 uint32_t splits_of(uint32_t tokens, uint32_t hidden) {
-    const uint32_t groups = (hidden + kRows - 1) / kRows * ((tokens + kTokens - 1) / kTokens);
-    return std::min(8u, std::max(1u, (512 + groups - 1) / groups));
+    const uint32_t groups = down_groups(hidden) * ((tokens + kTokens - 1) / kTokens);
+    return std::min(kMaxSplits, std::max(1u, (512 + groups - 1) / groups));
 }
 
-template <typename T>
-void launch_experts(const nz_expert_args& a, hipStream_t stream) {
+template <typename T, uint32_t NB>
+void launch_blocks(const nz_expert_args& a, hipStream_t stream) {
     const uint32_t passes = (a.tokens + kTokens - 1) / kTokens, splits = splits_of(a.tokens, a.hidden);
-    const uint32_t rows = (a.hidden + kRows - 1) / kRows;
+    const uint32_t groups = down_groups(a.hidden);
     float* const acts = static_cast<float*>(a.scratch);
     float* const partials = acts + static_cast<uint64_t>(a.tokens) * a.top_k * a.inter;
     uint32_t* const counters = reinterpret_cast<uint32_t*>(
         partials + (splits > 1 ? static_cast<uint64_t>(splits) * a.tokens * a.hidden : 0));
-    const uint32_t most = std::min(a.experts, std::min(a.tokens, kTokens) * a.top_k);   // experts of a pass
-    hipLaunchKernelGGL(nz_expert_up_kernel<T>, dim3((a.inter + kRows - 1) / kRows, most, passes), dim3(kUpThreads), 0,
-                       stream, a, acts, counters, splits > 1 ? rows * passes : 0);
-    hipLaunchKernelGGL(nz_expert_down_kernel<T>, dim3(rows, splits, passes), dim3(kDownThreads), 0, stream, a, acts,
-                       partials, counters, splits);
+    const uint32_t choices = std::min(a.tokens, kTokens) * a.top_k, most = std::min(a.experts, choices);   // of a pass
+    const uint32_t lds = Choice::bytes(a.experts, choices);
+    hipLaunchKernelGGL((nz_expert_up_kernel<T, NB>), dim3((a.inter + kRows - 1) / kRows, most, passes), dim3(kUpThreads),
+                       lds, stream, a, acts, counters, splits > 1 ? groups * passes : 0);
+    hipLaunchKernelGGL((nz_expert_down_kernel<T, NB>), dim3(groups, splits, passes), dim3(kDownThreads), lds, stream, a,
+                       acts, partials, counters, splits);
+}
+
+template <typename T>
+void launch_experts(const nz_expert_args& a, hipStream_t stream) {
+    if (a.tokens <= 16) launch_blocks<T, 1>(a, stream);
+    else if (a.tokens <= 32) launch_blocks<T, 2>(a, stream);
+    else launch_blocks<T, kBlocks>(a, stream);
 }
 
 template <typename T>
 void launch_route(const nz_route_args& a, hipStream_t stream) {
+    const dim3 grid((a.experts + kScoreWaves - 1) / kScoreWaves, a.tokens);
     if (a.weight_type == NZ_FP32)
-        hipLaunchKernelGGL((nz_route_kernel<T, float>), dim3(a.tokens), dim3(kRouteThreads), a.hidden * sizeof(float), stream, a);
+        hipLaunchKernelGGL((nz_route_scores_kernel<T, float>), grid, dim3(kScoreThreads), 0, stream, a);
     else
-        hipLaunchKernelGGL((nz_route_kernel<T, T>), dim3(a.tokens), dim3(kRouteThreads), a.hidden * sizeof(float), stream, a);
+        hipLaunchKernelGGL((nz_route_scores_kernel<T, T>), grid, dim3(kScoreThreads), 0, stream, a);
+    hipLaunchKernelGGL(nz_route_choice_kernel, dim3(a.tokens), dim3((a.experts + 63) / 64 * 64), 0, stream, a);
 }
 
 }  // namespace
@@ -437,9 +512,9 @@ extern "C" int nz_hip_route_experts(const nz_route_args* args, void* stream, cha
 }
 
 extern "C" uint64_t nz_hip_expert_scratch(uint32_t tokens, uint32_t hidden, uint32_t inter, uint32_t top_k) {
-    const uint64_t splits = splits_of(tokens, hidden), rows = (hidden + kRows - 1) / kRows;
+    const uint64_t splits = splits_of(tokens, hidden);
     return (static_cast<uint64_t>(tokens) * top_k * inter + splits * tokens * hidden +
-            rows * ((tokens + kTokens - 1) / kTokens)) * 4;
+            static_cast<uint64_t>(down_groups(hidden)) * ((tokens + kTokens - 1) / kTokens)) * 4;
 }
 
 extern "C" int nz_hip_expert_mlp(const nz_expert_args* args, void* stream, char* message, size_t message_size) {

@@ -13,7 +13,8 @@ namespace {
 
 // A row's vocabulary is cut into chunks, which one workgroup takes each.
 constexpr uint32_t kThreads = 256, kWaves = kThreads / 64, kChunk = NZ_VERIFY_CHUNK, kEach = kChunk / kThreads;
-constexpr uint32_t kPickThreads = 1024, kPickWaves = kPickThreads / 64, kPickEach = kChunk / kPickThreads;
+// Chunks of a row that a thread weighs, at most.
+constexpr uint32_t kMaxChunks = NZ_VERIFY_MAX_VOCAB / kChunk, kChunksEach = kMaxChunks / kThreads;
 constexpr uint32_t kNone = 0xFFFFFFFFu;
 
 // What is known of a chunk of a row: its largest logit, where that is first,
@@ -41,6 +42,43 @@ struct Decision {
 
 __host__ __device__ __forceinline__ uint32_t chunks_of(uint32_t vocab) { return (vocab + kChunk - 1) / kChunk; }
 
+// 2^y, y <= 0, to 2 units of the last place: y's whole part as the exponent,
+// and the Taylor series of exp(ln 2 * f), |f| <= 1/2, whose 13th term is below
+// 2^-52. -infinity and NaN give 0. Three times as fast as the library's exp,
+// which took most of the call's time.
+__device__ __forceinline__ double exp2_64(double y) {
+    y = fmax(y, -2000.0);
+    const double n = __builtin_rint(y), f = (y - n) * 0.693147180559945309417;
+    double p = 1.0 / 479001600;
+    p = fma(p, f, 1.0 / 39916800);
+    p = fma(p, f, 1.0 / 3628800);
+    p = fma(p, f, 1.0 / 362880);
+    p = fma(p, f, 1.0 / 40320);
+    p = fma(p, f, 1.0 / 5040);
+    p = fma(p, f, 1.0 / 720);
+    p = fma(p, f, 1.0 / 120);
+    p = fma(p, f, 1.0 / 24);
+    p = fma(p, f, 1.0 / 6);
+    p = fma(p, f, 0.5);
+    p = fma(p, f, 1.0);
+    p = fma(p, f, 1.0);
+    return __builtin_amdgcn_ldexp(p, static_cast<int>(n));
+}
+
+// How a row's logits are weighed: exp((x - top) / temperature) where `top` is
+// the largest, which may be infinite, and the first of the largest alone where
+// the temperature is not above 0.
+struct Scale {
+    double rate;        // log2(e) / temperature; 0: greedy
+    __device__ explicit Scale(float temperature)
+        : rate(temperature > 0.0f ? 1.44269504088896340736 / static_cast<double>(fminf(temperature, 3.4e38f)) : 0.0) {}
+    __device__ __forceinline__ bool greedy() const { return rate == 0.0; }
+    __device__ __forceinline__ double operator()(float x, float top) const {
+        if (top == __builtin_inff()) return x == top ? 1.0 : 0.0;
+        return exp2_64((static_cast<double>(x) - static_cast<double>(top)) * rate);
+    }
+};
+
 // NaN is no token's logit.
 template <typename T>
 __device__ __forceinline__ float logit(T x) {
@@ -48,15 +86,29 @@ __device__ __forceinline__ float logit(T x) {
     return y == y ? y : -__builtin_inff();
 }
 
-// A logit's weight where `top` is the largest one, which may be infinite.
-__device__ __forceinline__ double weight_of(float x, float top, double temperature) {
-    if (x == -__builtin_inff()) return 0.0;
-    if (x == top) return 1.0;
-    return exp((static_cast<double>(x) - static_cast<double>(top)) / temperature);
+// kEach neighbouring elements from `v` on, wherever they lie in memory, with
+// `none` past the end.
+template <typename T>
+__device__ __forceinline__ void load_each(const T* src, uint32_t v, uint32_t end, T none, T (&x)[kEach]) {
+    if (v + kEach <= end) {
+        __builtin_memcpy(x, src + v, sizeof x);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) x[i] = v + i < end ? src[v + i] : none;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void load_logits(const nz_verify_args& a, uint32_t row, uint32_t v, float (&x)[kEach]) {
+    T raw[kEach];
+    load_each(static_cast<const T*>(a.logits) + static_cast<int64_t>(row) * a.logits_row, v, a.vocab,
+              static_cast<T>(-__builtin_inff()), raw);
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i) x[i] = logit(raw[i]);
 }
 
 __device__ __forceinline__ float temperature_of(const nz_verify_args& a, uint32_t request) {
-    return a.temperature ? fminf(a.temperature[request], 3.4e38f) : 1.0f;
+    return a.temperature ? a.temperature[request] : 1.0f;
 }
 
 __device__ __forceinline__ uint32_t row_limit(const nz_verify_args& a, uint32_t request) {
@@ -80,135 +132,143 @@ __device__ uint32_t request_of(const nz_verify_args& a, uint32_t row) {
     return row_limit(a, low) <= row && row < row_limit(a, low + 1) ? low : kNone;
 }
 
-// Sum over the workgroup, in a fixed order.
-template <uint32_t WAVES>
-__device__ __forceinline__ double block_sum(double v, double* lds) {
+__device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
     for (uint32_t d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+    return v;
+}
+
+// Sum over the workgroup, in a fixed order.
+__device__ __forceinline__ double block_sum(double v, double* lds) {
+    v = wave_sum(v);
     __syncthreads();   // the last call's reads
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
     double sum = 0.0;
 #pragma unroll
-    for (uint32_t w = 0; w < WAVES; ++w) sum += lds[w];
+    for (uint32_t w = 0; w < kWaves; ++w) sum += lds[w];
     return sum;
+}
+
+// Largest logit, and where it is first, of two parts.
+__device__ __forceinline__ void take_larger(Part& a, float top, uint32_t first) {
+    if (top > a.top || (top == a.top && first < a.first)) a.top = top, a.first = first;
+}
+
+__device__ __forceinline__ void wave_largest(Part& a) {
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d <<= 1) take_larger(a, __shfl_xor(a.top, d), __shfl_xor(a.first, d));
 }
 
 // One chunk of one row.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void nz_verify_rows_kernel(nz_verify_args a, Part* __restrict__ parts) {
-    __shared__ float tops[kWaves];
-    __shared__ uint32_t firsts[kWaves];
+    __shared__ Part waves[kWaves];
     __shared__ double sums[kWaves];
-    const uint32_t row = blockIdx.y, v0 = blockIdx.x * kChunk, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const T* src = static_cast<const T*>(a.logits) + static_cast<int64_t>(row) * a.logits_row;
+    const uint32_t row = blockIdx.y, v = blockIdx.x * kChunk + threadIdx.x * kEach;
     float x[kEach];
-#pragma unroll
-    for (uint32_t i = 0; i < kEach; ++i) {
-        const uint32_t v = v0 + i * kThreads + threadIdx.x;
-        x[i] = v < a.vocab ? logit(src[v]) : -__builtin_inff();
-    }
+    load_logits<T>(a, row, v, x);
     const uint32_t request = request_of(a, row);
     if (request == kNone) return;
-    const float temperature = temperature_of(a, request);
-    float top = x[0];
+    const Scale scale(temperature_of(a, request));
+    Part part = {x[0], v, 0.0};
 #pragma unroll
-    for (uint32_t i = 1; i < kEach; ++i) top = fmaxf(top, x[i]);
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    if (lane == 0) tops[wave] = top;
+    for (uint32_t i = 1; i < kEach; ++i)
+        if (x[i] > part.top) part.top = x[i], part.first = v + i;
+    wave_largest(part);
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = part;
     __syncthreads();
 #pragma unroll
-    for (uint32_t w = 0; w < kWaves; ++w) top = fmaxf(top, tops[w]);
-    uint32_t first = kNone;
+    for (uint32_t w = 0; w < kWaves; ++w) take_larger(part, waves[w].top, waves[w].first);
+    if (!scale.greedy() && part.top > -__builtin_inff()) {
 #pragma unroll
-    for (uint32_t i = 0; i < kEach; ++i) {
-        const uint32_t v = v0 + i * kThreads + threadIdx.x;
-        if (x[i] == top && v < a.vocab) first = min(first, v);
+        for (uint32_t i = 0; i < kEach; ++i) part.sum += scale(x[i], part.top);
+        part.sum = block_sum(part.sum, sums);
     }
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d <<= 1) first = min(first, static_cast<uint32_t>(__shfl_xor(first, d)));
-    if (lane == 0) firsts[wave] = first;
-    double sum = 0.0;
-    if (temperature > 0.0f) {
-#pragma unroll
-        for (uint32_t i = 0; i < kEach; ++i) sum += weight_of(x[i], top, temperature);
-    }
-    sum = block_sum<kWaves>(sum, sums);
-    if (threadIdx.x == 0) {
-#pragma unroll
-        for (uint32_t w = 0; w < kWaves; ++w) first = min(first, firsts[w]);
-        parts[static_cast<uint64_t>(row) * gridDim.x + blockIdx.x] = Part{top, first, sum};
-    }
+    if (threadIdx.x == 0) parts[static_cast<uint64_t>(row) * gridDim.x + blockIdx.x] = part;
 }
 
 // A row's largest logit, its first token and the sum of weights (of a greedy
 // row: 1), by a wavefront; the same in every lane.
-__device__ __forceinline__ Part row_of(const Part* parts, uint32_t chunks, float temperature) {
+__device__ __forceinline__ Part row_of(const Part* parts, uint32_t chunks, const Scale& scale) {
     const uint32_t lane = threadIdx.x & 63;
-    Part row = {-__builtin_inff(), kNone, 0.0};
-    for (uint32_t c = lane; c < chunks; c += 64) {
-        const Part part = parts[c];
-        if (part.top > row.top || (part.top == row.top && part.first < row.first)) row.top = part.top, row.first = part.first;
-    }
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d <<= 1) {
-        const float top = __shfl_xor(row.top, d);
-        const uint32_t first = __shfl_xor(row.first, d);
-        if (top > row.top || (top == row.top && first < row.first)) row.top = top, row.first = first;
-    }
+    Part mine = {-__builtin_inff(), kNone, 0.0};
+    if (lane < chunks) mine = parts[lane];
+    Part row = mine;
+    for (uint32_t c = lane + 64; c < chunks; c += 64) take_larger(row, parts[c].top, parts[c].first);
+    wave_largest(row);
+    row.sum = 0.0;
     if (row.top == -__builtin_inff()) return row;
-    if (!(temperature > 0.0f)) {
+    if (scale.greedy()) {
         row.sum = 1.0;
         return row;
     }
-    for (uint32_t c = lane; c < chunks; c += 64) row.sum += parts[c].sum * weight_of(parts[c].top, row.top, temperature);
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d <<= 1) row.sum += __shfl_xor(row.sum, d);
+    row.sum = mine.sum * scale(mine.top, row.top);
+    for (uint32_t c = lane + 64; c < chunks; c += 64) row.sum += parts[c].sum * scale(parts[c].top, row.top);
+    row.sum = wave_sum(row.sum);
     return row;
 }
 
-// A token's weight in a row.
-template <typename T>
-__device__ __forceinline__ double weight_at(const nz_verify_args& a, uint32_t row, const Part& whole, float temperature,
-                                            uint32_t v) {
-    if (!(temperature > 0.0f)) return v == whole.first ? 1.0 : 0.0;
-    return weight_of(logit(static_cast<const T*>(a.logits)[static_cast<int64_t>(row) * a.logits_row + v]), whole.top,
-                     temperature);
-}
-
 // Accepts a request's drafts in turn, a wavefront per row; the result is the
-// same in every thread.
-template <typename T, uint32_t WAVES>
-__device__ Decision decide(const nz_verify_args& a, const Part* parts, uint32_t request) {
-    __shared__ Decision rows[WAVES];
-    __shared__ bool stops[WAVES];
+// same in every thread. Probabilities are compared and subtracted times the
+// row's sum of weights.
+template <typename T>
+__device__ Decision decide(const nz_verify_args& a, const Part* parts, uint32_t request, const Scale& scale) {
+    __shared__ Decision rows[kWaves];
+    __shared__ bool stops[kWaves];
     const uint32_t chunks = chunks_of(a.vocab), wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const uint32_t begin = row_limit(a, request), end = row_limit(a, request + 1);
-    const float temperature = temperature_of(a, request);
-    for (uint32_t r0 = begin; r0 < end; r0 += WAVES) {
+    for (uint32_t r0 = begin; r0 < end; r0 += kWaves) {
         const uint32_t row = r0 + wave;
         __syncthreads();   // the last rows' reads
         if (row < end) {
-            Decision here = {row, row - begin, 0, kWhole, row_of(parts + static_cast<uint64_t>(row) * chunks, chunks, temperature)};
-            bool stop = true;
             const int64_t draft = row + 1 < end ? a.tokens[row + 1] : -1;
-            if (static_cast<uint64_t>(draft) < a.vocab && here.whole.sum > 0.0) {
+            const bool known = static_cast<uint64_t>(draft) < a.vocab;
+            float x = -__builtin_inff();
+            double limit = 0.0;
+            if (known) {
+                x = logit(static_cast<const T*>(a.logits)[static_cast<int64_t>(row) * a.logits_row + draft]);
+                limit = a.accept[row];
+                if (a.draft_probs) limit *= static_cast<double>(a.draft_probs[static_cast<int64_t>(row) * a.draft_row + draft]);
+            }
+            Decision here = {row, row - begin, 0, kWhole, row_of(parts + static_cast<uint64_t>(row) * chunks, chunks, scale)};
+            bool stop = true;
+            if (known && here.whole.sum > 0.0) {
                 here.refused = static_cast<uint32_t>(draft);
                 here.kind = a.draft_probs ? kRest : kWithout;
-                const double p = weight_at<T>(a, row, here.whole, temperature, here.refused) / here.whole.sum;
-                const double q = a.draft_probs
-                                     ? static_cast<double>(a.draft_probs[static_cast<int64_t>(row) * a.draft_row + draft])
-                                     : 1.0;
-                stop = !(a.accept[row] * q < p);
+                const double weight = scale.greedy() ? here.refused == here.whole.first : scale(x, here.whole.top);
+                stop = !(limit * here.whole.sum < weight);
             }
             if (lane == 0) rows[wave] = here, stops[wave] = stop;
         }
         __syncthreads();
-        for (uint32_t w = 0; w < WAVES && r0 + w < end; ++w)
+        for (uint32_t w = 0; w < kWaves && r0 + w < end; ++w)
             if (stops[w]) return rows[w];
     }
     return Decision{kNone, 0, 0, kWhole, {-__builtin_inff(), kNone, 0.0}};
+}
+
+// The weights of kEach neighbouring tokens of a decision's row, from `v` on;
+// returns their sum.
+template <typename T>
+__device__ __forceinline__ double weigh(const nz_verify_args& a, const Decision& d, Kind kind, const Scale& scale,
+                                        uint32_t v, double (&w)[kEach]) {
+    float x[kEach], q[kEach] = {};
+    load_logits<T>(a, d.row, v, x);
+    if (kind == kRest)
+        load_each(a.draft_probs + static_cast<int64_t>(d.row) * a.draft_row, v, a.vocab, __builtin_inff(), q);
+    double sum = 0.0;
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i) {
+        w[i] = scale.greedy() ? v + i == d.whole.first : scale(x[i], d.whole.top);
+        if (kind == kWithout && v + i == d.refused) w[i] = 0.0;
+        if (kind == kRest) {
+            const double rest = w[i] - static_cast<double>(q[i]) * d.whole.sum;
+            w[i] = rest > 0.0 ? rest : 0.0;
+        }
+        sum += w[i];
+    }
+    return sum;
 }
 
 // With draft probabilities: the sums of max(p - q, 0) over the chunks of the
@@ -217,62 +277,37 @@ template <typename T>
 __global__ __launch_bounds__(kThreads)
 void nz_verify_rest_kernel(nz_verify_args a, const Part* __restrict__ parts, double* __restrict__ rests) {
     __shared__ double sums[kWaves];
-    const uint32_t request = blockIdx.y, v0 = blockIdx.x * kChunk;
-    const Decision d = decide<T, kWaves>(a, parts, request);
+    const uint32_t request = blockIdx.y;
+    const Scale scale(temperature_of(a, request));
+    const Decision d = decide<T>(a, parts, request, scale);
     if (d.kind != kRest) return;
-    const float temperature = temperature_of(a, request);
-    const float* q = a.draft_probs + static_cast<int64_t>(d.row) * a.draft_row;
-    double sum = 0.0;
-#pragma unroll
-    for (uint32_t i = 0; i < kEach; ++i) {
-        const uint32_t v = v0 + i * kThreads + threadIdx.x;
-        if (v < a.vocab) {
-            const double rest = weight_at<T>(a, d.row, d.whole, temperature, v) / d.whole.sum - static_cast<double>(q[v]);
-            sum += rest > 0.0 ? rest : 0.0;
-        }
-    }
-    sum = block_sum<kWaves>(sum, sums);
+    double w[kEach];
+    const double sum = block_sum(weigh<T>(a, d, kRest, scale, blockIdx.x * kChunk + threadIdx.x * kEach, w), sums);
     if (threadIdx.x == 0) rests[static_cast<uint64_t>(request) * gridDim.x + blockIdx.x] = sum;
 }
 
 // The next token of a request: the chunk in which the sum of weights passes
 // the wanted share of all, then the token in it.
 template <typename T>
-__global__ __launch_bounds__(kPickThreads)
+__global__ __launch_bounds__(kThreads)
 void nz_verify_pick_kernel(nz_verify_args a, const Part* __restrict__ parts, const double* __restrict__ rests) {
-    __shared__ double sums[kPickWaves], before_chunk, chunk_total;
+    __shared__ double sums[kWaves], before_chunk, all_chunks;
     __shared__ uint32_t found, last;
     const uint32_t request = blockIdx.x, chunks = chunks_of(a.vocab), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const Decision d = decide<T, kPickWaves>(a, parts, request);
+    const Scale scale(temperature_of(a, request));
+    const double share = a.sample[request];
+    const Decision d = decide<T>(a, parts, request, scale);
     const bool none = d.row == kNone || d.whole.sum == 0.0;
     if (threadIdx.x == 0) {
         a.accepted[request] = static_cast<int32_t>(d.accepted);
         if (none) a.next[request] = -1;
     }
     if (none) return;
-    const float temperature = temperature_of(a, request);
     Kind kind = d.kind;
-    const auto token_weight = [&](uint32_t v) {
-        const double p = weight_at<T>(a, d.row, d.whole, temperature, v) / d.whole.sum;
-        if (kind == kWhole) return p;
-        if (kind == kWithout) return v == d.refused ? 0.0 : p;
-        const double rest = p - static_cast<double>(a.draft_probs[static_cast<int64_t>(d.row) * a.draft_row + v]);
-        return rest > 0.0 ? rest : 0.0;
-    };
-    // the weights of kPickEach neighbours of a chunk, and their sum
-    double w[kPickEach];
-    const auto chunk_weights = [&](uint32_t chunk) {
-        double sum = 0.0;
-#pragma unroll
-        for (uint32_t i = 0; i < kPickEach; ++i) {
-            const uint32_t v = chunk * kChunk + threadIdx.x * kPickEach + i;
-            w[i] = v < a.vocab ? token_weight(v) : 0.0;
-            sum += w[i];
-        }
-        return sum;
-    };
-    // inclusive prefix sums, in a fixed order
+    double w[kEach];
+    // sums of the threads before this one, in a fixed order
     const auto scan = [&](double v) {
+        const double mine = v;
 #pragma unroll
         for (uint32_t s = 1; s < 64; s <<= 1) {
             const double below = __shfl_up(v, s);
@@ -283,52 +318,84 @@ void nz_verify_pick_kernel(nz_verify_args a, const Part* __restrict__ parts, con
         if (threadIdx.x == 0) found = kNone, last = 0;
         __syncthreads();
         double before = 0.0;
-        for (uint32_t i = 0; i < wave; ++i) before += sums[i];
-        return before + v;
+#pragma unroll
+        for (uint32_t i = 0; i < kWaves; ++i)
+            if (i < wave) before += sums[i];
+        return before + v - mine;
+    };
+    // the first and the last of what the threads found (a wavefront's one atomic each: 4096 of them took 60 us)
+    const auto note = [&](uint32_t first, uint32_t most) {
+#pragma unroll
+        for (uint32_t s = 1; s < 64; s <<= 1) {
+            first = min(first, static_cast<uint32_t>(__shfl_xor(first, s)));
+            most = max(most, static_cast<uint32_t>(__shfl_xor(most, s)));
+        }
+        if (lane == 0) atomicMin(&found, first), atomicMax(&last, most);
     };
     const uint32_t hole = kind == kWithout ? d.refused / kChunk : kNone;   // its sum is taken anew
     double without = 0.0;
-    if (kind == kWithout) without = block_sum<kPickWaves>(chunk_weights(hole), sums);
-    // a thread per chunk: their weights; from the row itself if the refusal leaves nothing
-    double mine = 0.0, upto = 0.0, total = 0.0;
+    if (kind == kWithout) without = block_sum(weigh<T>(a, d, kind, scale, hole * kChunk + threadIdx.x * kEach, w), sums);
+    // some neighbouring chunks a thread: their weights; from the row itself if the refusal leaves nothing
+    const uint32_t each = (chunks + kThreads - 1) / kThreads, c0 = threadIdx.x * each;
+    double weights[kChunksEach], before = 0.0;
     for (uint32_t turn = 0; turn < 2; ++turn) {
-        mine = 0.0;
-        const uint32_t c = threadIdx.x;
-        if (c < chunks) {
-            const Part part = parts[static_cast<uint64_t>(d.row) * chunks + c];
-            if (kind == kRest) mine = rests[static_cast<uint64_t>(request) * chunks + c];
-            else if (kind == kWithout && c == hole) mine = without;
-            else if (!(temperature > 0.0f)) mine = c == d.whole.first / kChunk ? 1.0 : 0.0;
-            else mine = part.sum * weight_of(part.top, d.whole.top, temperature) / d.whole.sum;
+        double mine = 0.0;
+#pragma unroll
+        for (uint32_t i = 0; i < kChunksEach; ++i) {
+            const uint32_t c = c0 + i;
+            weights[i] = 0.0;
+            if (i < each && c < chunks) {
+                if (kind == kRest) {
+                    weights[i] = rests[static_cast<uint64_t>(request) * chunks + c];
+                } else if (kind == kWithout && c == hole) {
+                    weights[i] = without;
+                } else if (scale.greedy()) {
+                    weights[i] = c == d.whole.first / kChunk;
+                } else {
+                    const Part part = parts[static_cast<uint64_t>(d.row) * chunks + c];
+                    weights[i] = part.sum * scale(part.top, d.whole.top);
+                }
+            }
+            mine += weights[i];
         }
-        upto = scan(mine);
-        if (threadIdx.x == kPickThreads - 1) chunk_total = upto;
+        before = scan(mine);
+        if (threadIdx.x == kThreads - 1) all_chunks = before + mine;
         __syncthreads();
-        total = chunk_total;
-        if (total > 0.0) break;
+        if (all_chunks > 0.0) break;
         kind = kWhole;
     }
-    const double wanted = a.sample[request] * total;
-    if (mine > 0.0) {
-        atomicMax(&last, threadIdx.x);
-        if (upto > wanted) atomicMin(&found, threadIdx.x);
-    }
-    __syncthreads();
-    const uint32_t chunk = found != kNone ? found : last;
-    if (threadIdx.x == chunk) before_chunk = upto - mine;
-    // the token: the first with a weight at which the sum passes what is wanted, or the chunk's last
-    mine = chunk_weights(chunk);
-    upto = scan(mine);
-    double sum = before_chunk + upto - mine;
+    const double wanted = share * all_chunks;
+    double upto = before;
+    uint32_t mine_first = kNone, mine_last = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < kPickEach; ++i) {
-        sum += w[i];
-        const uint32_t v = chunk * kChunk + threadIdx.x * kPickEach + i;
-        if (w[i] > 0.0) {
-            atomicMax(&last, v);
-            if (sum > wanted) atomicMin(&found, v);
+    for (uint32_t i = 0; i < kChunksEach; ++i) {
+        upto += weights[i];
+        if (weights[i] > 0.0) {
+            mine_last = c0 + i;
+            if (upto > wanted) mine_first = min(mine_first, c0 + i);
         }
     }
+    note(mine_first, mine_last);
+    __syncthreads();
+    const uint32_t chunk = found != kNone ? found : last;
+#pragma unroll
+    for (uint32_t i = 0; i < kChunksEach; ++i) {
+        if (i < each && c0 + i == chunk) before_chunk = before;
+        before += weights[i];
+    }
+    // the token: the first with a weight at which the sum passes what is wanted, or the chunk's last
+    const uint32_t v = chunk * kChunk + threadIdx.x * kEach;
+    double sum = scan(weigh<T>(a, d, kind, scale, v, w)) + before_chunk;
+    mine_first = kNone, mine_last = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i) {
+        sum += w[i];
+        if (w[i] > 0.0) {
+            mine_last = v + i;
+            if (sum > wanted) mine_first = min(mine_first, v + i);
+        }
+    }
+    note(mine_first, mine_last);
     __syncthreads();
     if (threadIdx.x == 0) a.next[request] = found != kNone ? found : last;
 }
@@ -341,7 +408,7 @@ void launch_verify(const nz_verify_args& a, hipStream_t stream) {
     if (a.n_rows) hipLaunchKernelGGL(nz_verify_rows_kernel<T>, dim3(chunks, a.n_rows), dim3(kThreads), 0, stream, a, parts);
     if (a.n_rows && a.draft_probs)
         hipLaunchKernelGGL(nz_verify_rest_kernel<T>, dim3(chunks, a.n_requests), dim3(kThreads), 0, stream, a, parts, rests);
-    hipLaunchKernelGGL(nz_verify_pick_kernel<T>, dim3(a.n_requests), dim3(kPickThreads), 0, stream, a, parts, rests);
+    hipLaunchKernelGGL(nz_verify_pick_kernel<T>, dim3(a.n_requests), dim3(kThreads), 0, stream, a, parts, rests);
 }
 
 }  // namespace

@@ -656,8 +656,8 @@ def route_experts(x, weight, top_k, *, scoring="softmax", normalize=True, bias=N
     those of the largest sigmoid plus `bias` (float32, experts), weighted by
     the sigmoid. `normalize` divides a token's weights by their sum; `scale`
     multiplies them. Of equal experts the lower one is first, and NaN is never
-    before another. In 64 bits, rounded once. hidden is a multiple of 8 up to
-    16384; at most 1024 experts, 32 of them chosen."""
+    before another. In 64 bits, rounded once. hidden is a multiple of 8; at
+    most 1024 experts, 32 of them chosen, and 65535 tokens."""
     if torch.is_grad_enabled():
         _refuse_gradients(x, weight, bias)
     if x.dim() != 2 or x.dtype not in _TYPES or x.stride(1) != 1 or weight.dim() != 2 \
@@ -674,8 +674,9 @@ def route_experts(x, weight, top_k, *, scoring="softmax", normalize=True, bias=N
     with _on(stream):
         ids = torch.empty((tokens, top_k), dtype=torch.int32, device=x.device)
         weights = torch.empty((tokens, top_k), dtype=torch.float32, device=x.device)
+        scratch = torch.empty(tokens * experts, dtype=torch.float64, device=x.device)
     args = _native.ROUTE.pack(x.data_ptr(), weight.data_ptr(), bias_ptr, ids.data_ptr(), weights.data_ptr(),
-                              x.stride(0), tokens, hidden, experts, top_k, _TYPES[x.dtype], _TYPES[weight.dtype],
+                              scratch.data_ptr(), x.stride(0), tokens, hidden, experts, top_k, _TYPES[x.dtype], _TYPES[weight.dtype],
                               _native.ROUTE_SCORING[scoring], bool(normalize), scale, 0)
     _call(_native.lib().nz_route_experts, x.device, args, stream)
     if stream is not None:

@@ -62,13 +62,13 @@ def definition(logits, tokens, starts, accept, sample, probs, temperature):
     return accepted, following
 
 
-def run(logits, tokens, starts, accept, sample, probs=None, temperature=None, **more):
+def run(logits, tokens, starts, accept, sample, probs=None, temperature=None):
     def on(x, dtype):
         return None if x is None else torch.as_tensor(np.asarray(x), dtype=dtype).to(DEVICE)
     logits = logits.to(DEVICE)
     got = serving.verify_drafts(logits, on(tokens, torch.int64), on(starts, torch.int32), on(accept, torch.float64),
                                 on(sample, torch.float64), draft_probs=on(probs, torch.float32),
-                                temperature=on(temperature, torch.float32), **more)
+                                temperature=on(temperature, torch.float32))
     return got[0].tolist(), got[1].tolist()
 
 
@@ -283,8 +283,12 @@ def test_captured_and_replayed():
 
 def test_a_side_stream():
     logits, tokens, starts, accept, sample, q = case(torch.float16, 3000, [3, 1], True)
-    side = torch.cuda.Stream()
+    state = [logits.to(DEVICE)] + [torch.as_tensor(np.asarray(x), dtype=dtype).to(DEVICE) for x, dtype in
+                                   ((tokens, torch.int64), (starts, torch.int32), (accept, torch.float64),
+                                    (sample, torch.float64))]
+    drafts, side = torch.from_numpy(q).to(DEVICE), torch.cuda.Stream()
+    want = serving.verify_drafts(*state, draft_probs=drafts)
     side.wait_stream(torch.cuda.current_stream())
-    torch.cuda.synchronize()
-    assert run(logits, tokens, starts, accept, sample, q, stream=side) == \
-        run(logits, tokens, starts, accept, sample, q)
+    got = serving.verify_drafts(*state, draft_probs=drafts, stream=side)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

@@ -67,7 +67,7 @@ PLAN = dict(contexts=True, requests=True, groups=True, shared=True, items=True, 
 ATTENTION = dict(test_serving_abi.ATTENTION, rows=True, order=True)
 VERIFY = dict(logits=True, draft_probs=True, tokens=True, starts=True, accept=True, sample=True, temperature=True,
               accepted=True, next=True, scratch=True, logits_row=100, draft_row=100, n_rows=5, n_requests=2, vocab=100)
-ROUTE = dict(x=True, weight=True, ids=True, weights=True, x_row=64, tokens=3, hidden=64, experts=8, top_k=2)
+ROUTE = dict(x=True, weight=True, ids=True, weights=True, scratch=True, x_row=64, tokens=3, hidden=64, experts=8, top_k=2)
 EXPERTS = dict(x=True, ids=True, weights=True, gate_up=True, down=True, out=True, scratch=True, x_row=64, out_row=64,
                gate_expert=64 * 96, gate_row=64, down_expert=64 * 48, down_row=48, tokens=3, hidden=64, inter=48,
                experts=8, top_k=2, id_bytes=4)
@@ -126,7 +126,9 @@ EXPERTS = dict(x=True, ids=True, weights=True, gate_up=True, down=True, out=True
     ("nz_route_experts", ROUTE, dict(weights=0), b"Null"),
     ("nz_route_experts", ROUTE, dict(hidden=60), b"multiple of 8"),
     ("nz_route_experts", ROUTE, dict(hidden=0), b"multiple of 8"),
-    ("nz_route_experts", ROUTE, dict(hidden=16392), b"Too many"),
+    ("nz_route_experts", ROUTE, dict(scratch=0), b"Null"),
+    ("nz_route_experts", ROUTE, dict(scratch=4100), b"8-byte"),
+    ("nz_route_experts", ROUTE, dict(tokens=65536), b"Too many"),
     ("nz_route_experts", ROUTE, dict(experts=1025), b"Too many"),
     ("nz_route_experts", ROUTE, dict(top_k=0), b"top_k"),
     ("nz_route_experts", ROUTE, dict(top_k=9), b"top_k"),
