@@ -13,12 +13,14 @@ namespace {
 
 // A row's vocabulary is cut into chunks, which one workgroup takes each.
 constexpr uint32_t kThreads = 256, kWaves = kThreads / 64, kChunk = NZ_VERIFY_CHUNK, kEach = kChunk / kThreads;
+// Of workgroups that decide on a request's drafts, a wavefront per row.
+constexpr uint32_t kPickThreads = 512, kPickWaves = kPickThreads / 64, kPickEach = kChunk / kPickThreads;
 // Chunks of a row that a thread weighs, at most.
-constexpr uint32_t kMaxChunks = NZ_VERIFY_MAX_VOCAB / kChunk, kChunksEach = kMaxChunks / kThreads;
+constexpr uint32_t kMaxChunks = NZ_VERIFY_MAX_VOCAB / kChunk, kChunksEach = kMaxChunks / kPickThreads;
 constexpr uint32_t kNone = 0xFFFFFFFFu;
 
-// What is known of a chunk of a row: its largest logit, where that is first,
-// and the sum of the weights exp((x - top) / temperature).
+// What is known of a chunk of a row: its largest logit, where that is first (of
+// a greedy row), and the sum of the weights exp((x - top) / temperature).
 struct Part {
     float top;
     uint32_t first;
@@ -38,44 +40,75 @@ struct Decision {
     uint32_t refused;
     Kind kind;
     Part whole;         // of the row
+    double weight;      // of the draft
 };
 
 __host__ __device__ __forceinline__ uint32_t chunks_of(uint32_t vocab) { return (vocab + kChunk - 1) / kChunk; }
 
-// 2^y, y <= 0, to 2 units of the last place: y's whole part as the exponent,
-// and the Taylor series of exp(ln 2 * f), |f| <= 1/2, whose 13th term is below
-// 2^-52. -infinity and NaN give 0. Three times as fast as the library's exp,
-// which took most of the call's time.
-__device__ __forceinline__ double exp2_64(double y) {
-    y = fmax(y, -2000.0);
-    const double n = __builtin_rint(y), f = (y - n) * 0.693147180559945309417;
-    double p = 1.0 / 479001600;
-    p = fma(p, f, 1.0 / 39916800);
-    p = fma(p, f, 1.0 / 3628800);
-    p = fma(p, f, 1.0 / 362880);
-    p = fma(p, f, 1.0 / 40320);
-    p = fma(p, f, 1.0 / 5040);
-    p = fma(p, f, 1.0 / 720);
-    p = fma(p, f, 1.0 / 120);
-    p = fma(p, f, 1.0 / 24);
-    p = fma(p, f, 1.0 / 6);
-    p = fma(p, f, 0.5);
-    p = fma(p, f, 1.0);
-    p = fma(p, f, 1.0);
-    return __builtin_amdgcn_ldexp(p, static_cast<int>(n));
-}
+// Weights are held times 2^60, so that the smallest that 64 bits hold beside a
+// largest of 1 are normal numbers.
+constexpr double kUnit = 0x1p60;
+constexpr double kReach = 1074.0;    // its log2
 
 // How a row's logits are weighed: exp((x - top) / temperature) where `top` is
-// the largest, which may be infinite, and the first of the largest alone where
-// the temperature is not above 0.
+// the largest, and the first of the largest alone where the temperature is not
+// above 0.
 struct Scale {
     double rate;        // log2(e) / temperature; 0: greedy
-    __device__ explicit Scale(float temperature)
-        : rate(temperature > 0.0f ? 1.44269504088896340736 / static_cast<double>(fminf(temperature, 3.4e38f)) : 0.0) {}
+    // The Taylor series of 2^f, (ln 2)^k / k!, kept in scalar registers (as
+    // literals each takes two moves into vector registers).
+    static constexpr uint32_t kTerms = 13;
+    double series[kTerms];
+
+    __device__ __forceinline__ explicit Scale(float temperature)
+        : rate(temperature > 0.0f ? 1.44269504088896340736 / static_cast<double>(fminf(temperature, 3.4e38f)) : 0.0) {
+        double term = kUnit;
+#pragma unroll
+        for (uint32_t k = 0; k < kTerms; ++k) {
+            series[k] = term;
+            term = term * 0.693147180559945309417 / (k + 1);
+            asm("" : "+s"(series[k]));
+        }
+    }
     __device__ __forceinline__ bool greedy() const { return rate == 0.0; }
+    // What logits have to be above for a weight: nothing below it rounds to one, and the series' exponents stay
+    // inside 64 bits, whichever way this is rounded.
+    __device__ __forceinline__ float floor_of(float top) const {
+        const float reach = static_cast<float>(fmin(kReach / rate, 3e38));
+        const float below = top - fmaxf(fabsf(top) * 0x1p-23f, 0x1p-149f);   // the next number, or the one after
+        return fminf(top - reach + fabsf(top) * 0x1p-22f, below);
+    }
+    // 2^y, y = (x - top) rate <= 0, to 2 units of the last place: y's whole
+    // part, the low bits of a sum with 1.5 * 2^52, as the exponent, and the
+    // series for the rest, |f| <= 1/2, whose next term is below 2^-52. The
+    // library's exp takes four times as long, and most of the call's time was
+    // spent in it.
+    __device__ __forceinline__ double finite(float x, float top, float floor) const {
+        const double y = (static_cast<double>(x) - static_cast<double>(top)) * rate;
+        const double shifted = y + 0x1.8p52, f = y - (shifted - 0x1.8p52);
+        double p = series[kTerms - 1];
+#pragma unroll
+        for (uint32_t k = kTerms - 1; k-- > 0;) p = fma(p, f, series[k]);
+        vec<uint32_t, 2> bits = __builtin_bit_cast(vec<uint32_t, 2>, p);
+        bits.y += __builtin_bit_cast(vec<uint32_t, 2>, shifted).x << 20;
+        return x > floor ? __builtin_bit_cast(double, bits) : 0.0;
+    }
+    // the weights of some logits (NaN has none)
+    template <uint32_t N>
+    __device__ __forceinline__ void weigh(const float (&x)[N], float top, double (&w)[N]) const {
+        if (top == __builtin_inff()) {
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i) w[i] = x[i] == top ? kUnit : 0.0;
+        } else {
+            const float floor = floor_of(top);
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i) w[i] = finite(x[i], top, floor);
+        }
+    }
     __device__ __forceinline__ double operator()(float x, float top) const {
-        if (top == __builtin_inff()) return x == top ? 1.0 : 0.0;
-        return exp2_64((static_cast<double>(x) - static_cast<double>(top)) * rate);
+        double w[1];
+        weigh({x}, top, w);
+        return w[0];
     }
 };
 
@@ -86,25 +119,42 @@ __device__ __forceinline__ float logit(T x) {
     return y == y ? y : -__builtin_inff();
 }
 
-// kEach neighbouring elements from `v` on, wherever they lie in memory, with
+// Largest of a wavefront's values, NaN aside; the same in every lane.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_max(float v) {
+    const int low = __float_as_int(-__builtin_inff());
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(low, __float_as_int(v), CTRL, ROWS, 0xF, false)));
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+    v = dpp_max<0x111, 0xF>(v);
+    v = dpp_max<0x112, 0xF>(v);
+    v = dpp_max<0x114, 0xF>(v);
+    v = dpp_max<0x118, 0xF>(v);
+    v = dpp_max<0x142, 0xA>(v);
+    v = dpp_max<0x143, 0xC>(v);
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
+// Neighbouring elements from `v` on, wherever they lie in memory, with
 // `none` past the end.
-template <typename T>
-__device__ __forceinline__ void load_each(const T* src, uint32_t v, uint32_t end, T none, T (&x)[kEach]) {
-    if (v + kEach <= end) {
+template <uint32_t N, typename T>
+__device__ __forceinline__ void load_each(const T* src, uint32_t v, uint32_t end, T none, T (&x)[N]) {
+    if (v + N <= end) {
         __builtin_memcpy(x, src + v, sizeof x);
     } else {
 #pragma unroll
-        for (uint32_t i = 0; i < kEach; ++i) x[i] = v + i < end ? src[v + i] : none;
+        for (uint32_t i = 0; i < N; ++i) x[i] = v + i < end ? src[v + i] : none;
     }
 }
 
-template <typename T>
-__device__ __forceinline__ void load_logits(const nz_verify_args& a, uint32_t row, uint32_t v, float (&x)[kEach]) {
-    T raw[kEach];
+template <typename T, uint32_t N>
+__device__ __forceinline__ void load_logits(const nz_verify_args& a, uint32_t row, uint32_t v, float (&x)[N]) {
+    T raw[N];
     load_each(static_cast<const T*>(a.logits) + static_cast<int64_t>(row) * a.logits_row, v, a.vocab,
               static_cast<T>(-__builtin_inff()), raw);
 #pragma unroll
-    for (uint32_t i = 0; i < kEach; ++i) x[i] = logit(raw[i]);
+    for (uint32_t i = 0; i < N; ++i) x[i] = logit(raw[i]);
 }
 
 __device__ __forceinline__ float temperature_of(const nz_verify_args& a, uint32_t request) {
@@ -115,21 +165,27 @@ __device__ __forceinline__ uint32_t row_limit(const nz_verify_args& a, uint32_t 
     return min(static_cast<uint32_t>(max(a.starts[request], 0)), a.n_rows);
 }
 
-// The request whose rows hold `row` (kNone: none does), by a wavefront: the
-// last start that is no larger, 64 of them read at a time.
-__device__ uint32_t request_of(const nz_verify_args& a, uint32_t row) {
+// The request whose rows hold `row` (kNone: none does) and its temperature, by
+// a wavefront: 64 requests at a time, all of what is needed of them read at
+// once, after a search among every 64th start where there are more.
+__device__ __forceinline__ uint32_t request_of(const nz_verify_args& a, uint32_t row, float& temperature) {
     const uint32_t lane = threadIdx.x & 63;
-    uint32_t low = 0, count = a.n_requests;   // of starts that may be the one
-    while (count > 1) {
+    uint32_t low = 0, count = a.n_requests;
+    while (count > 64) {
         const uint32_t step = (count + 63) / 64, at = lane * step;
-        const bool below = at < count && row_limit(a, low + at) <= row;
-        const uint64_t bits = __ballot(below);
+        const uint64_t bits = __ballot(at < count && row_limit(a, low + at) <= row);
         if (bits == 0) return kNone;
         const uint32_t last = 63 - __builtin_clzll(bits);
         low += last * step;
         count = min(step, count - last * step);
     }
-    return row_limit(a, low) <= row && row < row_limit(a, low + 1) ? low : kNone;
+    const uint32_t request = low + min(lane, count - 1);
+    const uint32_t begin = row_limit(a, request), end = row_limit(a, request + 1);
+    const float mine = temperature_of(a, request);
+    const uint64_t bits = __ballot(lane < count && begin <= row && row < end);
+    if (bits == 0) return kNone;
+    temperature = __shfl(mine, __builtin_ctzll(bits));
+    return low + __builtin_ctzll(bits);
 }
 
 __device__ __forceinline__ double wave_sum(double v) {
@@ -139,6 +195,7 @@ __device__ __forceinline__ double wave_sum(double v) {
 }
 
 // Sum over the workgroup, in a fixed order.
+template <uint32_t WAVES>
 __device__ __forceinline__ double block_sum(double v, double* lds) {
     v = wave_sum(v);
     __syncthreads();   // the last call's reads
@@ -146,7 +203,7 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {
     __syncthreads();
     double sum = 0.0;
 #pragma unroll
-    for (uint32_t w = 0; w < kWaves; ++w) sum += lds[w];
+    for (uint32_t w = 0; w < WAVES; ++w) sum += lds[w];
     return sum;
 }
 
@@ -160,30 +217,51 @@ __device__ __forceinline__ void wave_largest(Part& a) {
     for (uint32_t d = 1; d < 64; d <<= 1) take_larger(a, __shfl_xor(a.top, d), __shfl_xor(a.first, d));
 }
 
-// One chunk of one row.
+// One chunk of one row. Bound by the vector units: some 20 instructions of 64
+// bits a logit.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void nz_verify_rows_kernel(nz_verify_args a, Part* __restrict__ parts) {
-    __shared__ Part waves[kWaves];
+    __shared__ float tops[kWaves];
+    __shared__ uint32_t firsts[kWaves];
     __shared__ double sums[kWaves];
     const uint32_t row = blockIdx.y, v = blockIdx.x * kChunk + threadIdx.x * kEach;
-    float x[kEach];
-    load_logits<T>(a, row, v, x);
-    const uint32_t request = request_of(a, row);
-    if (request == kNone) return;
-    const Scale scale(temperature_of(a, request));
-    Part part = {x[0], v, 0.0};
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    T raw[kEach];
+    load_each(static_cast<const T*>(a.logits) + static_cast<int64_t>(row) * a.logits_row, v, a.vocab,
+              static_cast<T>(-__builtin_inff()), raw);
+    float temperature;
+    if (request_of(a, row, temperature) == kNone) return;
+    const Scale scale(temperature);
+    float x[kEach], top = -__builtin_inff();
 #pragma unroll
-    for (uint32_t i = 1; i < kEach; ++i)
-        if (x[i] > part.top) part.top = x[i], part.first = v + i;
-    wave_largest(part);
-    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = part;
+    for (uint32_t i = 0; i < kEach; ++i) {
+        x[i] = to_float(raw[i]);
+        top = fmaxf(top, x[i]);
+    }
+    top = wave_max(top);
+    if (lane == 0) tops[wave] = top;
     __syncthreads();
 #pragma unroll
-    for (uint32_t w = 0; w < kWaves; ++w) take_larger(part, waves[w].top, waves[w].first);
-    if (!scale.greedy() && part.top > -__builtin_inff()) {
+    for (uint32_t w = 0; w < kWaves; ++w) top = fmaxf(top, tops[w]);
+    Part part = {top, kNone, 0.0};
+    if (scale.greedy()) {
 #pragma unroll
-        for (uint32_t i = 0; i < kEach; ++i) part.sum += scale(x[i], part.top);
-        part.sum = block_sum(part.sum, sums);
+        for (uint32_t i = kEach; i-- > 0;)
+            if (x[i] == top && v + i < a.vocab) part.first = v + i;
+        // (lanes hold rising tokens)
+        const uint64_t bits = __ballot(part.first != kNone);
+        if (lane == 0) firsts[wave] = kNone;
+        if (bits != 0 && lane == __builtin_ctzll(bits)) firsts[wave] = part.first;
+        __syncthreads();
+        part.first = kNone;
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; ++w) part.first = min(part.first, firsts[w]);
+    } else if (top > -__builtin_inff()) {
+        double w[kEach];
+        scale.weigh(x, top, w);
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) part.sum += w[i];
+        part.sum = block_sum<kWaves>(part.sum, sums);
     }
     if (threadIdx.x == 0) parts[static_cast<uint64_t>(row) * gridDim.x + blockIdx.x] = part;
 }
@@ -203,8 +281,8 @@ __device__ __forceinline__ Part row_of(const Part* parts, uint32_t chunks, const
         row.sum = 1.0;
         return row;
     }
-    row.sum = mine.sum * scale(mine.top, row.top);
-    for (uint32_t c = lane + 64; c < chunks; c += 64) row.sum += parts[c].sum * scale(parts[c].top, row.top);
+    row.sum = mine.sum * (scale(mine.top, row.top) / kUnit);
+    for (uint32_t c = lane + 64; c < chunks; c += 64) row.sum += parts[c].sum * (scale(parts[c].top, row.top) / kUnit);
     row.sum = wave_sum(row.sum);
     return row;
 }
@@ -212,13 +290,13 @@ __device__ __forceinline__ Part row_of(const Part* parts, uint32_t chunks, const
 // Accepts a request's drafts in turn, a wavefront per row; the result is the
 // same in every thread. Probabilities are compared and subtracted times the
 // row's sum of weights.
-template <typename T>
+template <typename T, uint32_t WAVES>
 __device__ Decision decide(const nz_verify_args& a, const Part* parts, uint32_t request, const Scale& scale) {
-    __shared__ Decision rows[kWaves];
-    __shared__ bool stops[kWaves];
+    __shared__ Decision rows[WAVES];
+    __shared__ bool stops[WAVES];
     const uint32_t chunks = chunks_of(a.vocab), wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const uint32_t begin = row_limit(a, request), end = row_limit(a, request + 1);
-    for (uint32_t r0 = begin; r0 < end; r0 += kWaves) {
+    for (uint32_t r0 = begin; r0 < end; r0 += WAVES) {
         const uint32_t row = r0 + wave;
         __syncthreads();   // the last rows' reads
         if (row < end) {
@@ -231,36 +309,37 @@ __device__ Decision decide(const nz_verify_args& a, const Part* parts, uint32_t 
                 limit = a.accept[row];
                 if (a.draft_probs) limit *= static_cast<double>(a.draft_probs[static_cast<int64_t>(row) * a.draft_row + draft]);
             }
-            Decision here = {row, row - begin, 0, kWhole, row_of(parts + static_cast<uint64_t>(row) * chunks, chunks, scale)};
+            Decision here = {row, row - begin, 0, kWhole, row_of(parts + static_cast<uint64_t>(row) * chunks, chunks, scale), 0.0};
             bool stop = true;
             if (known && here.whole.sum > 0.0) {
                 here.refused = static_cast<uint32_t>(draft);
                 here.kind = a.draft_probs ? kRest : kWithout;
-                const double weight = scale.greedy() ? here.refused == here.whole.first : scale(x, here.whole.top);
-                stop = !(limit * here.whole.sum < weight);
+                here.weight = scale.greedy() ? here.refused == here.whole.first : scale(x, here.whole.top);
+                stop = !(limit * here.whole.sum < here.weight);
             }
             if (lane == 0) rows[wave] = here, stops[wave] = stop;
         }
         __syncthreads();
-        for (uint32_t w = 0; w < kWaves && r0 + w < end; ++w)
+        for (uint32_t w = 0; w < WAVES && r0 + w < end; ++w)
             if (stops[w]) return rows[w];
     }
-    return Decision{kNone, 0, 0, kWhole, {-__builtin_inff(), kNone, 0.0}};
+    return Decision{kNone, 0, 0, kWhole, {-__builtin_inff(), kNone, 0.0}, 0.0};
 }
 
-// The weights of kEach neighbouring tokens of a decision's row, from `v` on;
+// The weights of neighbouring tokens of a decision's row, from `v` on;
 // returns their sum.
-template <typename T>
+template <typename T, uint32_t N>
 __device__ __forceinline__ double weigh(const nz_verify_args& a, const Decision& d, Kind kind, const Scale& scale,
-                                        uint32_t v, double (&w)[kEach]) {
-    float x[kEach], q[kEach] = {};
+                                        uint32_t v, double (&w)[N]) {
+    float x[N], q[N] = {};
     load_logits<T>(a, d.row, v, x);
     if (kind == kRest)
         load_each(a.draft_probs + static_cast<int64_t>(d.row) * a.draft_row, v, a.vocab, __builtin_inff(), q);
+    if (!scale.greedy()) scale.weigh(x, d.whole.top, w);
     double sum = 0.0;
 #pragma unroll
-    for (uint32_t i = 0; i < kEach; ++i) {
-        w[i] = scale.greedy() ? v + i == d.whole.first : scale(x[i], d.whole.top);
+    for (uint32_t i = 0; i < N; ++i) {
+        if (scale.greedy()) w[i] = v + i == d.whole.first;
         if (kind == kWithout && v + i == d.refused) w[i] = 0.0;
         if (kind == kRest) {
             const double rest = w[i] - static_cast<double>(q[i]) * d.whole.sum;
@@ -271,32 +350,44 @@ __device__ __forceinline__ double weigh(const nz_verify_args& a, const Decision&
     return sum;
 }
 
-// With draft probabilities: the sums of max(p - q, 0) over the chunks of the
-// row that a request's next token is picked from.
+// With draft probabilities, the decisions are made first.
+template <typename T>
+__global__ __launch_bounds__(kPickThreads)
+void nz_verify_decide_kernel(nz_verify_args a, const Part* __restrict__ parts, Decision* __restrict__ decisions) {
+    const uint32_t request = blockIdx.x;
+    const Scale scale(temperature_of(a, request));
+    const Decision d = decide<T, kPickWaves>(a, parts, request, scale);
+    if (threadIdx.x == 0) decisions[request] = d;
+}
+
+// Then the sums of max(p - q, 0) over the chunks of the row that a request's
+// next token is picked from. (When its workgroups decided each for itself, it
+// took 17 us of 65 for 48 requests of 128256 tokens.)
 template <typename T>
 __global__ __launch_bounds__(kThreads)
-void nz_verify_rest_kernel(nz_verify_args a, const Part* __restrict__ parts, double* __restrict__ rests) {
+void nz_verify_rest_kernel(nz_verify_args a, const Decision* __restrict__ decisions, double* __restrict__ rests) {
     __shared__ double sums[kWaves];
     const uint32_t request = blockIdx.y;
-    const Scale scale(temperature_of(a, request));
-    const Decision d = decide<T>(a, parts, request, scale);
+    const Decision d = decisions[request];
     if (d.kind != kRest) return;
+    const Scale scale(temperature_of(a, request));
     double w[kEach];
-    const double sum = block_sum(weigh<T>(a, d, kRest, scale, blockIdx.x * kChunk + threadIdx.x * kEach, w), sums);
+    const double sum = block_sum<kWaves>(weigh<T>(a, d, kRest, scale, blockIdx.x * kChunk + threadIdx.x * kEach, w), sums);
     if (threadIdx.x == 0) rests[static_cast<uint64_t>(request) * gridDim.x + blockIdx.x] = sum;
 }
 
 // The next token of a request: the chunk in which the sum of weights passes
 // the wanted share of all, then the token in it.
 template <typename T>
-__global__ __launch_bounds__(kThreads)
-void nz_verify_pick_kernel(nz_verify_args a, const Part* __restrict__ parts, const double* __restrict__ rests) {
-    __shared__ double sums[kWaves], before_chunk, all_chunks;
+__global__ __launch_bounds__(kPickThreads)
+void nz_verify_pick_kernel(nz_verify_args a, const Part* __restrict__ parts, const Decision* __restrict__ decisions,
+                           const double* __restrict__ rests) {
+    __shared__ double sums[kPickWaves], before_chunk, all_chunks;
     __shared__ uint32_t found, last;
     const uint32_t request = blockIdx.x, chunks = chunks_of(a.vocab), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Scale scale(temperature_of(a, request));
     const double share = a.sample[request];
-    const Decision d = decide<T>(a, parts, request, scale);
+    const Decision d = decisions ? decisions[request] : decide<T, kPickWaves>(a, parts, request, scale);
     const bool none = d.row == kNone || d.whole.sum == 0.0;
     if (threadIdx.x == 0) {
         a.accepted[request] = static_cast<int32_t>(d.accepted);
@@ -304,7 +395,7 @@ void nz_verify_pick_kernel(nz_verify_args a, const Part* __restrict__ parts, con
     }
     if (none) return;
     Kind kind = d.kind;
-    double w[kEach];
+    double w[kPickEach];
     // sums of the threads before this one, in a fixed order
     const auto scan = [&](double v) {
         const double mine = v;
@@ -319,9 +410,14 @@ void nz_verify_pick_kernel(nz_verify_args a, const Part* __restrict__ parts, con
         __syncthreads();
         double before = 0.0;
 #pragma unroll
-        for (uint32_t i = 0; i < kWaves; ++i)
+        for (uint32_t i = 0; i < kPickWaves; ++i)
             if (i < wave) before += sums[i];
         return before + v - mine;
+    };
+    const auto chunk_weight = [&](uint32_t c) -> double {
+        if (scale.greedy()) return c == d.whole.first / kChunk;
+        const Part part = parts[static_cast<uint64_t>(d.row) * chunks + c];
+        return part.sum * (scale(part.top, d.whole.top) / kUnit);
     };
     // the first and the last of what the threads found (a wavefront's one atomic each: 4096 of them took 60 us)
     const auto note = [&](uint32_t first, uint32_t most) {
@@ -332,11 +428,17 @@ void nz_verify_pick_kernel(nz_verify_args a, const Part* __restrict__ parts, con
         }
         if (lane == 0) atomicMin(&found, first), atomicMax(&last, most);
     };
-    const uint32_t hole = kind == kWithout ? d.refused / kChunk : kNone;   // its sum is taken anew
+    // without the draft refused: its chunk's sum less its weight, or, where that would cancel, anew
+    const uint32_t hole = kind == kWithout ? d.refused / kChunk : kNone;
     double without = 0.0;
-    if (kind == kWithout) without = block_sum(weigh<T>(a, d, kind, scale, hole * kChunk + threadIdx.x * kEach, w), sums);
+    if (kind == kWithout) {
+        const double all = chunk_weight(hole), less = all - d.weight;
+        without = 2.0 * less >= all
+                      ? less
+                      : block_sum<kPickWaves>(weigh<T>(a, d, kind, scale, hole * kChunk + threadIdx.x * kPickEach, w), sums);
+    }
     // some neighbouring chunks a thread: their weights; from the row itself if the refusal leaves nothing
-    const uint32_t each = (chunks + kThreads - 1) / kThreads, c0 = threadIdx.x * each;
+    const uint32_t each = (chunks + kPickThreads - 1) / kPickThreads, c0 = threadIdx.x * each;
     double weights[kChunksEach], before = 0.0;
     for (uint32_t turn = 0; turn < 2; ++turn) {
         double mine = 0.0;
@@ -349,17 +451,14 @@ void nz_verify_pick_kernel(nz_verify_args a, const Part* __restrict__ parts, con
                     weights[i] = rests[static_cast<uint64_t>(request) * chunks + c];
                 } else if (kind == kWithout && c == hole) {
                     weights[i] = without;
-                } else if (scale.greedy()) {
-                    weights[i] = c == d.whole.first / kChunk;
                 } else {
-                    const Part part = parts[static_cast<uint64_t>(d.row) * chunks + c];
-                    weights[i] = part.sum * scale(part.top, d.whole.top);
+                    weights[i] = chunk_weight(c);
                 }
             }
             mine += weights[i];
         }
         before = scan(mine);
-        if (threadIdx.x == kThreads - 1) all_chunks = before + mine;
+        if (threadIdx.x == kPickThreads - 1) all_chunks = before + mine;
         __syncthreads();
         if (all_chunks > 0.0) break;
         kind = kWhole;
@@ -384,11 +483,11 @@ void nz_verify_pick_kernel(nz_verify_args a, const Part* __restrict__ parts, con
         before += weights[i];
     }
     // the token: the first with a weight at which the sum passes what is wanted, or the chunk's last
-    const uint32_t v = chunk * kChunk + threadIdx.x * kEach;
+    const uint32_t v = chunk * kChunk + threadIdx.x * kPickEach;
     double sum = scan(weigh<T>(a, d, kind, scale, v, w)) + before_chunk;
     mine_first = kNone, mine_last = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < kEach; ++i) {
+    for (uint32_t i = 0; i < kPickEach; ++i) {
         sum += w[i];
         if (w[i] > 0.0) {
             mine_last = v + i;
@@ -404,11 +503,16 @@ template <typename T>
 void launch_verify(const nz_verify_args& a, hipStream_t stream) {
     const uint32_t chunks = chunks_of(a.vocab);
     Part* const parts = static_cast<Part*>(a.scratch);
-    double* const rests = reinterpret_cast<double*>(parts + static_cast<uint64_t>(a.n_rows) * chunks);
+    Decision* const decisions = reinterpret_cast<Decision*>(parts + static_cast<uint64_t>(a.n_rows) * chunks);
+    double* const rests = reinterpret_cast<double*>(decisions + a.n_requests);
+    const bool decided = a.draft_probs && a.n_rows;
     if (a.n_rows) hipLaunchKernelGGL(nz_verify_rows_kernel<T>, dim3(chunks, a.n_rows), dim3(kThreads), 0, stream, a, parts);
-    if (a.n_rows && a.draft_probs)
-        hipLaunchKernelGGL(nz_verify_rest_kernel<T>, dim3(chunks, a.n_requests), dim3(kThreads), 0, stream, a, parts, rests);
-    hipLaunchKernelGGL(nz_verify_pick_kernel<T>, dim3(a.n_requests), dim3(kThreads), 0, stream, a, parts, rests);
+    if (decided) {
+        hipLaunchKernelGGL(nz_verify_decide_kernel<T>, dim3(a.n_requests), dim3(kPickThreads), 0, stream, a, parts, decisions);
+        hipLaunchKernelGGL(nz_verify_rest_kernel<T>, dim3(chunks, a.n_requests), dim3(kThreads), 0, stream, a, decisions, rests);
+    }
+    hipLaunchKernelGGL(nz_verify_pick_kernel<T>, dim3(a.n_requests), dim3(kPickThreads), 0, stream, a, parts,
+                       decided ? decisions : nullptr, rests);
 }
 
 }  // namespace
@@ -416,7 +520,9 @@ void launch_verify(const nz_verify_args& a, hipStream_t stream) {
 // The callers (capi_serving.cpp) have checked the arguments.
 
 extern "C" uint64_t nz_hip_verify_scratch(uint32_t n_rows, uint32_t n_requests, uint32_t vocab) {
-    return (static_cast<uint64_t>(n_rows) * sizeof(Part) + static_cast<uint64_t>(n_requests) * 8) * chunks_of(vocab);
+    static_assert(sizeof(Part) == 16 && sizeof(Decision) % 8 == 0, "scratch of 8-byte numbers");
+    return static_cast<uint64_t>(n_rows) * chunks_of(vocab) * sizeof(Part) +
+           n_requests * (sizeof(Decision) + static_cast<uint64_t>(chunks_of(vocab)) * sizeof(double));
 }
 
 extern "C" int nz_hip_verify_drafts(const nz_verify_args* args, void* stream, char* message, size_t message_size) {
