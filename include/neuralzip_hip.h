@@ -736,13 +736,15 @@ typedef struct nz_shared_item {
     int32_t reserved[2];
 } nz_shared_item;
 
-/* Where a row's sums are found: items group_first, group_first + group_step,
- * ... (group_count of them) and own_first, own_first + 1, ... (own_count), and
- * the row's place among the item's rows. */
+/* Where a row's sums are found: in items group_first, group_first +
+ * group_step, ... (group_count of them), own_first, own_first + 1, ...
+ * (own_count) and tail_first, ... (tail_count), and the row's places among the
+ * rows of the first (the low 8 bits) and the second. */
 typedef struct nz_shared_row {
-    int32_t group_first, group_step, group_count, group_place;
-    int32_t own_first, own_count, own_place;
-    int32_t context;
+    int32_t group_first, group_step, group_count;
+    int32_t own_first, own_count;
+    int32_t tail_first, tail_count;
+    int32_t places;
 } nz_shared_row;
 
 typedef struct nz_shared_plan_args {
@@ -753,7 +755,6 @@ typedef struct nz_shared_plan_args {
     nz_shared_item* items;       /* n_items (out)                            */
     nz_shared_row* rows;         /* n_rows (out)                             */
     int32_t* order;              /* 2 * n_rows (out)                         */
-    uint32_t* counters;          /* n_rows * kv_heads * ceil(heads / kv_heads / NZ_SHARED_COLUMNS) (out) */
     uint32_t n_rows;
     uint32_t n_requests;
     uint32_t n_groups;
@@ -771,10 +772,11 @@ uint32_t nz_shared_items(uint32_t n_rows, uint32_t n_groups, uint32_t heads, uin
  * device, so that keys that several rows see are read once for as many rows
  * as make NZ_SHARED_COLUMNS columns: the first shared[g] keys of the requests
  * of group g, which must be at the same pages (their table rows begin with the
- * same ones), and the other keys of neighbouring rows of one request. Negative
- * contexts and numbers count as 0; a request outside n_requests has no keys,
- * and a group outside n_groups is none. At most NZ_SHARED_MAX_ROWS rows and
- * NZ_SHARED_MAX_GROUPS groups. */
+ * same ones), for rows that see as many; and of the other keys those that all
+ * of as many neighbouring rows of one request see. What a row sees past these
+ * is read for it alone. Negative contexts and numbers count as 0; a request
+ * outside n_requests has no keys, and a group outside n_groups is none. At
+ * most NZ_SHARED_MAX_ROWS rows and NZ_SHARED_MAX_GROUPS groups. */
 int nz_shared_plan(const nz_shared_plan_args* args, void* stream);
 
 typedef struct nz_shared_attention_args {
@@ -786,7 +788,6 @@ typedef struct nz_shared_attention_args {
     const nz_shared_item* items; /* the plan's                               */
     const nz_shared_row* rows;
     const int32_t* order;
-    uint32_t* counters;
     float* partials;             /* nz_shared_partials(...) words            */
     int64_t q_row, q_head, out_row, out_head;
     int64_t key_page, key_head, key_slot, value_page, value_head, value_slot;
@@ -808,8 +809,8 @@ typedef struct nz_shared_attention_args {
 uint64_t nz_shared_partials(uint32_t n_items, uint32_t heads, uint32_t kv_heads, uint32_t head_dim);
 
 /* nz_attention's results, with a plan of nz_shared_plan for as many rows and
- * requests and the same heads. Calls with one plan must not overlap.
- * nz_shared_partials(...) is below 2^30 + 2^24. */
+ * requests and the same heads. Calls with one plan may overlap if each has
+ * partials of its own. */
 int nz_shared_attention(const nz_shared_attention_args* args, void* stream);
 
 typedef struct nz_logits_args {

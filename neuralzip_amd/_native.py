@@ -92,8 +92,8 @@ PAGES_TRIM = struct.Struct("=7Q6I")
 ROTARY = struct.Struct("=12Q14q11If")
 ATTENTION = struct.Struct("=8Q10q10IfI")
 LOGITS = struct.Struct("=13Q3q8I")
-SHARED_PLAN = struct.Struct("=8Q8I")
-SHARED_ATTENTION = struct.Struct("=10Q10q10IfI")
+SHARED_PLAN = struct.Struct("=7Q8I")
+SHARED_ATTENTION = struct.Struct("=9Q10q10IfI")
 VERIFY = struct.Struct("=10Q2q4I")
 ROUTE = struct.Struct("=6Qq8IfI")
 EXPERTS = struct.Struct("=7Q6q8I")

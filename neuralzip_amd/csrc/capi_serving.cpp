@@ -215,7 +215,7 @@ int nz_shared_plan(const nz_shared_plan_args* args, void* stream) {
                    "NZ_SHARED_MAX_ROWS and NZ_SHARED_MAX_GROUPS.");
         if (a.n_items < items) refuse("The plan has room for fewer items than nz_shared_items.");
         if (a.n_items > kMaxGrid || a.n_requests > kMaxGrid) refuse("Items and requests must be below 2^31.");
-        if (!a.items || (a.n_rows && (!a.contexts || !a.rows || !a.order || !a.counters)) ||
+        if (!a.items || (a.n_rows && (!a.contexts || !a.rows || !a.order)) ||
             (a.n_groups && (!a.groups || !a.shared)))
             refuse("Null shared plan argument.");
         return false;
@@ -235,7 +235,7 @@ int nz_shared_attention(const nz_shared_attention_args* args, void* stream) {
         if (a.reserved) refuse("reserved is 0.");
         if (a.n_rows == 0) return true;
         if (!a.q || !a.key_cache || !a.value_cache || !a.out || !a.tables || !a.items || !a.rows || !a.order ||
-            !a.counters || !a.partials)
+            !a.partials)
             refuse("Null attention argument.");
         check_pages(a.n_requests, a.max_pages, a.page_size, a.n_pages);
         if (a.n_pages == 0 || a.n_requests == 0) refuse("There must be pages and requests.");
@@ -247,7 +247,7 @@ int nz_shared_attention(const nz_shared_attention_args* args, void* stream) {
         if (a.n_rows > NZ_SHARED_MAX_ROWS) refuse("Too many rows in one call.");
         if (a.n_items < a.n_rows) refuse("The plan has fewer items than rows.");
         if (a.heads > kMaxGrid || a.n_items > kMaxGrid ||
-            a.n_items * shared_width(a.heads, a.kv_heads) > (1ull << 30) / a.head_dim)
+            a.n_items * shared_width(a.heads, a.kv_heads) > kMaxGrid)
             refuse("Too many items and heads in one call.");
         return false;
     });

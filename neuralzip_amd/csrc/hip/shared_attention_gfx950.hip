@@ -23,18 +23,17 @@ constexpr uint32_t kMaxRows = NZ_SHARED_MAX_ROWS, kMaxGroups = NZ_SHARED_MAX_GRO
 // for each wavefront of a workgroup.
 constexpr uint32_t kTile = 32, kLeastItem = 128;
 
-// Tiles are numbered group by group, then row by row; their keys are cut alike
-// within a group.
 struct PlanLds {
     uint32_t waves[kPlanWaves], counts[kPlanWaves];
     uint64_t keys[kPlanWaves];
-    int32_t context[kMaxRows], request[kMaxRows], group[kMaxRows];
-    uint32_t start[kMaxRows];                 // of the run of rows of one request
+    int32_t request[kMaxRows], group[kMaxRows];
+    uint32_t context[kMaxRows];
+    uint32_t start[kMaxRows];                 // of the run of rows that are read together
     uint32_t rank[kMaxRows];                  // among the rows of its group
-    uint32_t own_first[kMaxRows + 1];         // first item of the tile that begins at a row
+    uint32_t own[kMaxRows + 1];               // keys, then first item, of the tile that begins at a row (0: none does)
+    uint32_t tail[kMaxRows + 1];              // the same of what a row alone sees
     uint32_t members[kMaxGroups], base[kMaxGroups], shared[kMaxGroups];
     int32_t least[kMaxGroups], most[kMaxGroups];   // requests of its rows
-    uint32_t longest[kMaxGroups];             // context of them
     uint32_t group_first[kMaxGroups + 1];     // a group's first item
     uint32_t order[kMaxRows];                 // rows by group
 };
@@ -59,40 +58,39 @@ __device__ __forceinline__ uint32_t plan_scan(uint32_t v, uint32_t& total, PlanL
 // Items of `keys` keys when none is longer than `share`.
 __device__ __forceinline__ uint32_t cuts(uint32_t keys, uint32_t share) { return (keys + share - 1) / share; }
 
-// One workgroup. Groups of which several requests have rows are read by tiles
-// of as many rows as fit kColumns columns; then each request's rows in such
-// tiles, from where the group's keys end. Latency bound.
+// One workgroup. Three kinds of items: the shared keys of groups of which
+// several requests have rows, for tiles of as many rows as fit kColumns
+// columns; the other keys that all of a tile of neighbouring rows of one
+// request see; and what a row sees past those of its tile. So every row of an
+// item sees all of its keys. Latency bound.
 __global__ __launch_bounds__(kPlanThreads) void nz_shared_plan_kernel(nz_shared_plan_args a) {
     __shared__ PlanLds lds;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = a.n_rows;
     const uint32_t heads = a.heads / a.kv_heads, tile_rows = heads <= kColumns ? kColumns / heads : 1;
-    const uint32_t parts = a.kv_heads * ((heads + kColumns - 1) / kColumns);
 
     for (uint32_t g = threadIdx.x; g < a.n_groups; g += kPlanThreads) {
         lds.shared[g] = static_cast<uint32_t>(max(a.shared[g], 0));
         lds.members[g] = 0;
         lds.least[g] = 0x7FFFFFFF;
         lds.most[g] = -1;
-        lds.longest[g] = 0;
     }
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < n; i += kPlanThreads) {
         const int32_t request = a.requests ? a.requests[i] : static_cast<int32_t>(i);
         const bool known = static_cast<uint32_t>(request) < a.n_requests;
+        const uint32_t context = known ? static_cast<uint32_t>(max(a.contexts[i], 0)) : 0;
         int32_t group = known && a.n_groups ? a.groups[request] : -1;
-        if (static_cast<uint32_t>(group) >= a.n_groups || lds.shared[group] == 0) group = -1;
-        lds.context[i] = known ? max(a.contexts[i], 0) : 0;
+        // a row that sees less than its group shares is read by itself
+        if (static_cast<uint32_t>(group) >= a.n_groups || lds.shared[group] == 0 || lds.shared[group] > context) group = -1;
+        lds.context[i] = context;
         lds.request[i] = known ? request : -1;
         lds.group[i] = group;
         if (group >= 0) {
             atomicMin(&lds.least[group], request);
             atomicMax(&lds.most[group], request);
-            atomicMax(&lds.longest[group], static_cast<uint32_t>(lds.context[i]));
         }
     }
     __syncthreads();
-    for (uint32_t g = threadIdx.x; g < a.n_groups; g += kPlanThreads)
-        lds.shared[g] = min(lds.shared[g], lds.longest[g]);
     // Rows' places in their groups, in row order: by one wavefront, 64 rows at a time.
     if (wave == 0 && a.n_groups) {
         for (uint32_t i0 = 0; i0 < n; i0 += 64) {
@@ -122,72 +120,79 @@ __global__ __launch_bounds__(kPlanThreads) void nz_shared_plan_kernel(nz_shared_
         placed += total;
     }
     __syncthreads();
-    uint64_t keys = 0;
-    uint32_t longest = 0, tiles = 0;
     for (uint32_t i = threadIdx.x; i < n; i += kPlanThreads) {
         const int32_t group = lds.group[i];
         if (group >= 0) lds.order[lds.base[group] + lds.rank[i]] = i;
     }
-    // runs of rows of one request
+    // runs of rows of one request, all of them in its group or none
     uint32_t runs_before = 0;
     for (uint32_t i0 = 0; i0 < n; i0 += kPlanThreads) {
         const uint32_t i = i0 + threadIdx.x;
-        const bool begins_run = i < n && (i == 0 || lds.request[i] < 0 || lds.request[i - 1] != lds.request[i]);
+        const bool begins_run = i < n && (i == 0 || lds.request[i] < 0 || lds.request[i - 1] != lds.request[i] ||
+                                          lds.group[i - 1] != lds.group[i]);
         uint32_t total;
         const uint32_t upto = plan_scan(begins_run, total, lds);
         if (i < n) lds.start[i] = runs_before + upto - 1;   // the run's number, for now
-        if (begins_run) lds.own_first[runs_before + upto - 1] = i;
+        if (begins_run) lds.own[runs_before + upto - 1] = i;
         runs_before += total;
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n; i += kPlanThreads) lds.start[i] = lds.own_first[lds.start[i]];
+    for (uint32_t i = threadIdx.x; i < n; i += kPlanThreads) lds.start[i] = lds.own[lds.start[i]];
     __syncthreads();
-    // Keys of the tile of its request's rows that begins at row i (0: no tile).
-    const auto own_keys = [&](uint32_t i) -> uint32_t {
-        if ((i - lds.start[i]) % tile_rows) return 0;
-        uint32_t most = 0;
-        for (uint32_t j = i; j < min(i + tile_rows, n) && lds.start[j] == lds.start[i]; ++j)
-            most = max(most, static_cast<uint32_t>(lds.context[j]));
-        const uint32_t from = lds.group[i] >= 0 ? lds.shared[lds.group[i]] : 0;
-        return most > from ? most - from : 0;
+    // The tile of its request's rows that a row is in: its first row, rows, and where the keys begin and end that
+    // all of them see.
+    struct Tile {
+        uint32_t first, rows, begin, end;
     };
-    const auto begins = [&](uint32_t i) { return (i - lds.start[i]) % tile_rows == 0; };
+    const auto tile_of = [&](uint32_t i) {
+        const uint32_t start = lds.start[i];
+        Tile t = {i - (i - start) % tile_rows, 0, 0, 0xFFFFFFFFu};
+        while (t.rows < tile_rows && t.first + t.rows < n && lds.start[t.first + t.rows] == start)
+            t.end = min(t.end, lds.context[t.first + t.rows++]);
+        t.begin = lds.group[i] >= 0 ? lds.shared[lds.group[i]] : 0;
+        return t;
+    };
+    uint64_t keys = 0;
+    uint32_t longest = 0, pieces = 0;
     for (uint32_t i = threadIdx.x; i < n; i += kPlanThreads) {
-        const uint32_t own = own_keys(i);
-        lds.own_first[i] = own;
-        keys += own;
-        longest = max(longest, own);
-        tiles += begins(i);
+        const Tile t = tile_of(i);
+        const uint32_t own = t.first == i ? t.end - t.begin : 0, tail = lds.context[i] - t.end;
+        lds.own[i] = own;
+        lds.tail[i] = tail;
+        keys += own + tail;
+        longest = max(longest, max(own, tail));
+        // (a row without any keys is an item too)
+        pieces += (own > 0) + (tail > 0 || lds.context[i] == 0);
     }
     for (uint32_t g = threadIdx.x; g < a.n_groups; g += kPlanThreads) {
         const uint32_t count = cuts(lds.members[g], tile_rows);
         if (count) longest = max(longest, lds.shared[g]);
         keys += static_cast<uint64_t>(count) * lds.shared[g];
-        tiles += count;
+        pieces += count;
     }
 #pragma unroll
     for (uint32_t d = 1; d < 64; d <<= 1) {
         keys += __shfl_xor(keys, d);
         longest = max(longest, static_cast<uint32_t>(__shfl_xor(longest, d)));
-        tiles += __shfl_xor(tiles, d);
+        pieces += __shfl_xor(pieces, d);
     }
-    if (lane == 0) lds.keys[wave] = keys, lds.waves[wave] = longest, lds.counts[wave] = tiles;
+    if (lane == 0) lds.keys[wave] = keys, lds.waves[wave] = longest, lds.counts[wave] = pieces;
     __syncthreads();
-    keys = 0, tiles = 0;
+    keys = 0, pieces = 0;
 #pragma unroll
     for (uint32_t w = 0; w < kPlanWaves; ++w) {
         keys += lds.keys[w];
         longest = max(longest, lds.waves[w]);
-        tiles += lds.counts[w];
+        pieces += lds.counts[w];
     }
     __syncthreads();
     // The shortest length of items, in tiles of keys, that gives few enough.
-    const uint32_t limit = min(cuts(max(a.target, tiles), a.target) * a.target, a.n_items);
+    const uint32_t limit = min(cuts(max(a.target, pieces), a.target) * a.target, a.n_items);
     uint32_t lo = kLeastItem / kTile, hi = max((longest + kTile - 1) / kTile, lo);
     const auto count_items = [&](uint32_t share) {   // a wavefront's sum
         uint32_t sum = 0;
         for (uint32_t i = lane; i < n; i += 64)
-            if (begins(i)) sum += max(cuts(lds.own_first[i], share), lds.group[i] < 0 ? 1u : 0u);
+            sum += cuts(lds.own[i], share) + max(cuts(lds.tail[i], share), lds.context[i] == 0 ? 1u : 0u);
         for (uint32_t g = lane; g < a.n_groups; g += 64)
             sum += cuts(lds.members[g], tile_rows) * cuts(lds.shared[g], share);
         return last_lane(wave_scan(sum));
@@ -206,17 +211,18 @@ __global__ __launch_bounds__(kPlanThreads) void nz_shared_plan_kernel(nz_shared_
         if (few) hi = min(below, hi);
     }
     const uint32_t share = lo * kTile;
-    // a tile's items are of equal length, in whole kTile keys
+    // items are of equal length, in whole kTile keys
     const auto each_of = [&](uint32_t length) {
         const uint32_t count = max(cuts(length, share), 1u);
         return max((cuts(length, count) + kTile - 1) / kTile * kTile, kTile);
     };
+    const auto items_of = [&](uint32_t length) { return cuts(length, each_of(length)); };
     __syncthreads();
-    // first items: the groups', then the tiles of requests' rows
+    // first items, kind by kind
     uint32_t first = 0;
     for (uint32_t g0 = 0; g0 < a.n_groups; g0 += kPlanThreads) {
         const uint32_t g = g0 + threadIdx.x;
-        const uint32_t count = g < a.n_groups ? cuts(lds.members[g], tile_rows) * cuts(lds.shared[g], each_of(lds.shared[g])) : 0;
+        const uint32_t count = g < a.n_groups ? cuts(lds.members[g], tile_rows) * items_of(lds.shared[g]) : 0;
         uint32_t total;
         const uint32_t upto = plan_scan(count, total, lds);
         if (g < a.n_groups) lds.group_first[g] = first + upto - count;
@@ -224,35 +230,30 @@ __global__ __launch_bounds__(kPlanThreads) void nz_shared_plan_kernel(nz_shared_
     }
     const uint32_t grouped = first;
     for (uint32_t i0 = 0; i0 < n; i0 += kPlanThreads) {
-        const uint32_t i = i0 + threadIdx.x;
-        uint32_t count = 0;
-        if (i < n && begins(i)) {
-            count = cuts(lds.own_first[i], each_of(lds.own_first[i]));
-            if (count == 0 && lds.group[i] < 0) count = 1;   // rows without keys are written too
-        }
+        const uint32_t i = i0 + threadIdx.x, count = i < n ? items_of(lds.own[i]) : 0;
         uint32_t total;
         const uint32_t upto = plan_scan(count, total, lds);
-        if (i < n) lds.own_first[i] = first + upto - count;
+        if (i < n) lds.own[i] = first + upto - count;
         first += total;
     }
-    if (threadIdx.x == 0) lds.own_first[n] = first, lds.group_first[a.n_groups] = grouped;
+    const uint32_t owned = first;
+    for (uint32_t i0 = 0; i0 < n; i0 += kPlanThreads) {
+        const uint32_t i = i0 + threadIdx.x;
+        const uint32_t count = i < n ? max(items_of(lds.tail[i]), lds.context[i] == 0 ? 1u : 0u) : 0;
+        uint32_t total;
+        const uint32_t upto = plan_scan(count, total, lds);
+        if (i < n) lds.tail[i] = first + upto - count;
+        first += total;
+    }
+    if (threadIdx.x == 0) lds.group_first[a.n_groups] = grouped, lds.own[n] = owned, lds.tail[n] = first;
     __syncthreads();
     const int32_t total_keys = static_cast<int32_t>(min<uint64_t>((keys + 1023) / 1024, 0x7FFFFFFFu));
-    // the items of the groups: parts of the keys, and within them tiles of rows, so that those that read the
-    // same keys are neighbours
     for (uint32_t j = threadIdx.x; j < first; j += kPlanThreads) {
         nz_shared_item item;
         if (j < grouped) {
-            uint32_t g = 0;
-            {   // the last group that begins at or before j (groups without items begin where the next one does)
-                uint32_t low = 0, high = a.n_groups;
-                while (high - low > 1) {
-                    const uint32_t mid = (low + high) >> 1;
-                    if (lds.group_first[mid] <= j) low = mid;
-                    else high = mid;
-                }
-                g = low;
-            }
+            // parts of the keys, and within them tiles of rows, so that those that read the same keys are neighbours
+            // (groups without items begin where the next one does)
+            const uint32_t g = owner(lds.group_first, a.n_groups, j);
             const uint32_t count = cuts(lds.members[g], tile_rows), k = j - lds.group_first[g];
             const uint32_t tile = k % count, part = k / count, each = each_of(lds.shared[g]);
             item.member = static_cast<int32_t>(lds.base[g] + tile * tile_rows);
@@ -260,17 +261,24 @@ __global__ __launch_bounds__(kPlanThreads) void nz_shared_plan_kernel(nz_shared_
             item.request = lds.request[lds.order[lds.base[g]]];
             item.begin = static_cast<int32_t>(part * each);
             item.end = static_cast<int32_t>(min(lds.shared[g], (part + 1) * each));
-        } else {
-            const uint32_t i = owner(lds.own_first, n, j);
-            const uint32_t from = lds.group[i] >= 0 ? lds.shared[lds.group[i]] : 0, own = own_keys(i);
-            const uint32_t each = each_of(own), part = j - lds.own_first[i];
-            uint32_t rows = 1;
-            while (rows < tile_rows && i + rows < n && lds.start[i + rows] == lds.start[i]) ++rows;
+        } else if (j < owned) {
+            const uint32_t i = owner(lds.own, n, j);
+            const Tile t = tile_of(i);
+            const uint32_t each = each_of(t.end - t.begin), part = j - lds.own[i];
             item.member = static_cast<int32_t>(n + i);
-            item.rows = static_cast<int32_t>(rows);
+            item.rows = static_cast<int32_t>(t.rows);
             item.request = lds.request[i];
-            item.begin = static_cast<int32_t>(from + part * each);
-            item.end = static_cast<int32_t>(from + min(own, (part + 1) * each));
+            item.begin = static_cast<int32_t>(t.begin + part * each);
+            item.end = static_cast<int32_t>(min(t.end, t.begin + (part + 1) * each));
+        } else {
+            const uint32_t i = owner(lds.tail, n, j);
+            const Tile t = tile_of(i);
+            const uint32_t each = each_of(lds.context[i] - t.end), part = j - lds.tail[i];
+            item.member = static_cast<int32_t>(n + i);
+            item.rows = 1;
+            item.request = lds.request[i];
+            item.begin = static_cast<int32_t>(t.end + part * each);
+            item.end = static_cast<int32_t>(min(lds.context[i], t.end + (part + 1) * each));
         }
         item.keys = total_keys;
         item.reserved[0] = item.reserved[1] = 0;
@@ -280,25 +288,25 @@ __global__ __launch_bounds__(kPlanThreads) void nz_shared_plan_kernel(nz_shared_
     for (uint32_t j = first + threadIdx.x; j < a.n_items; j += kPlanThreads) a.items[j] = none;
     for (uint32_t i = threadIdx.x; i < n; i += kPlanThreads) {
         const int32_t g = lds.group[i];
+        const Tile t = tile_of(i);
         nz_shared_row row = {};
+        uint32_t place = 0;
         if (g >= 0) {
-            const uint32_t count = cuts(lds.members[g], tile_rows);
             row.group_first = static_cast<int32_t>(lds.group_first[g] + lds.rank[i] / tile_rows);
-            row.group_step = static_cast<int32_t>(count);
-            row.group_count = static_cast<int32_t>(cuts(lds.shared[g], each_of(lds.shared[g])));
-            row.group_place = static_cast<int32_t>(lds.rank[i] % tile_rows);
+            row.group_step = static_cast<int32_t>(cuts(lds.members[g], tile_rows));
+            row.group_count = static_cast<int32_t>(items_of(lds.shared[g]));
+            place = lds.rank[i] % tile_rows;
             a.order[lds.base[g] + lds.rank[i]] = static_cast<int32_t>(i);
         }
-        const uint32_t place = (i - lds.start[i]) % tile_rows, tile = i - place;
-        row.own_first = static_cast<int32_t>(lds.own_first[tile]);
-        // (rows inside a tile begin none: their first item is the next tile's)
-        row.own_count = static_cast<int32_t>(lds.own_first[tile + 1] - lds.own_first[tile]);
-        row.own_place = static_cast<int32_t>(place);
-        row.context = lds.context[i];
+        // (a row that begins no tile has no items there: its first is the next one's)
+        row.own_first = static_cast<int32_t>(lds.own[t.first]);
+        row.own_count = static_cast<int32_t>(lds.own[t.first + 1] - lds.own[t.first]);
+        row.tail_first = static_cast<int32_t>(lds.tail[i]);
+        row.tail_count = static_cast<int32_t>(lds.tail[i + 1] - lds.tail[i]);
+        row.places = static_cast<int32_t>(place | (i - t.first) << 8);
         a.rows[i] = row;
         a.order[n + i] = static_cast<int32_t>(i);
     }
-    for (uint64_t i = threadIdx.x; i < static_cast<uint64_t>(n) * parts; i += kPlanThreads) a.counters[i] = 0;
 }
 
 // -------------------------------------------------------------- attention
@@ -309,9 +317,8 @@ constexpr uint32_t kBlocks = kColumns / 16;
 
 // One item: the softmax of up to kColumns columns -- rows that see the same
 // keys, times the query heads of one key-value head -- over the keys begin ..
-// end - 1, tile by tile with a running maximum and sum per column, each over
-// the keys below its row's context (see nz_attention_kernel, whose product
-// layout this has, for a tile of one row).
+// end - 1, tile by tile with a running maximum and sum per column (see
+// nz_attention_kernel, whose product layout this has).
 template <typename T, uint32_t DP, bool FULL>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 128 && sizeof(T) == 2 ? 2 : 1)))
 void nz_shared_attention_kernel(nz_shared_attention_args a) {
@@ -321,7 +328,8 @@ void nz_shared_attention_kernel(nz_shared_attention_args a) {
     using value_run = vec<T, S::kValueRun>;
     __shared__ float lds_m[kWaves][kColumns], lds_l[kWaves][kColumns];
     __shared__ __align__(16) float lds_o[kWaves][kColumns][DP + 4];
-    __shared__ uint32_t ended[kColumns], n_ended;
+    __shared__ nz_shared_row rows[kColumns];   // of the item
+    __shared__ uint32_t numbers[kColumns];
 
     const uint32_t group = a.heads / a.kv_heads, blocks = (group + kColumns - 1) / kColumns;
     const uint32_t turn = blockIdx.x / kXcds, unit = turn / blocks * kXcds + blockIdx.x % kXcds, block = turn % blocks;
@@ -333,7 +341,16 @@ void nz_shared_attention_kernel(nz_shared_attention_args a) {
     const uint32_t head0 = kv_head * group + block * kColumns;
     const uint32_t heads = min(kColumns, (kv_head + 1) * group - head0);   // of a row
     const uint32_t columns = static_cast<uint32_t>(item.rows) * heads;
-    const int32_t* const members = a.order + item.member;
+    // A request's rows are neighbours; a group's are listed.
+    const uint32_t member = static_cast<uint32_t>(item.member);
+    const auto row_at = [&](uint32_t i) {
+        return member >= a.n_rows ? member - a.n_rows + i : static_cast<uint32_t>(a.order[member + i]);
+    };
+    if (threadIdx.x < static_cast<uint32_t>(item.rows)) {
+        const uint32_t row = row_at(threadIdx.x);
+        numbers[threadIdx.x] = row;
+        rows[threadIdx.x] = a.rows[row];
+    }
     const uint32_t lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t shift = 31 - __clz(a.page_size), place_mask = a.page_size - 1;
@@ -346,30 +363,6 @@ void nz_shared_attention_kernel(nz_shared_attention_args a) {
 
     auto run_tiles = [&](auto width) {
         constexpr uint32_t NT = decltype(width)::value;
-        piece q[NT][S::kKeySteps];
-        uint32_t limit[NT], lowest = end;   // keys that a column sees
-#pragma unroll
-        for (uint32_t b = 0; b < NT; ++b) {
-            const uint32_t c = b * 16 + col;
-            const bool used = c < columns;
-            const uint32_t row = used ? static_cast<uint32_t>(members[c / heads]) : 0;
-            limit[b] = used ? min(static_cast<uint32_t>(max(a.rows[row].context, 0)), end) : 0;
-            if (used) lowest = min(lowest, limit[b]);
-            const T* src = static_cast<const T*>(a.q) + row * a.q_row + (head0 + c % heads) * a.q_head;
-#pragma unroll
-            for (uint32_t s = 0; s < S::kKeySteps; ++s) {
-                const uint32_t d = s * 4 * S::kRun + quad * S::kRun;
-                q[b][s] = piece{};
-                if (used && (FULL || d < a.head_dim)) q[b][s] = *reinterpret_cast<const piece*>(src + d);
-            }
-        }
-#pragma unroll
-        for (uint32_t d = 1; d < 16; d <<= 1) lowest = min(lowest, static_cast<uint32_t>(__shfl_xor(lowest, d)));
-        f32x4 o[NT][S::kValueSteps][S::kValueRun] = {};
-        float m[NT], l[NT];
-#pragma unroll
-        for (uint32_t b = 0; b < NT; ++b) m[b] = -__builtin_inff(), l[b] = 0.0f;
-
         // The pages of a tile's runs of 16 keys (a run lies in one page), a
         // tile ahead of the keys, and keys a tile ahead of their products.
         // Past the end, and where there is no page, page 0 is read and
@@ -401,11 +394,28 @@ void nz_shared_attention_kernel(nz_shared_attention_args a) {
         uint32_t t0 = static_cast<uint32_t>(item.begin) / 16 * 16 + wave * S::kKeys;
         const uint32_t begin = static_cast<uint32_t>(item.begin);
         int32_t page[S::kHalves], next[S::kHalves];
-        if (t0 < end) {
-            entries(t0, page);
-            load_keys(t0, page);
-            entries(t0 + kStep, next);
+        piece q[NT][S::kKeySteps];
+#pragma unroll
+        for (uint32_t b = 0; b < NT; ++b) {
+            const uint32_t c = b * 16 + col;
+            const bool used = c < columns;
+            const uint32_t row = used ? row_at(c / heads) : 0;
+            const T* src = static_cast<const T*>(a.q) + row * a.q_row + (head0 + c % heads) * a.q_head;
+#pragma unroll
+            for (uint32_t s = 0; s < S::kKeySteps; ++s) {
+                const uint32_t d = s * 4 * S::kRun + quad * S::kRun;
+                q[b][s] = piece{};
+                if (used && (FULL || d < a.head_dim)) q[b][s] = *reinterpret_cast<const piece*>(src + d);
+            }
         }
+        entries(t0, page);
+        load_keys(t0, page);
+        entries(t0 + kStep, next);
+        f32x4 o[NT][S::kValueSteps][S::kValueRun] = {};
+        float m[NT], l[NT];
+#pragma unroll
+        for (uint32_t b = 0; b < NT; ++b) m[b] = -__builtin_inff(), l[b] = 0.0f;
+
         for (; t0 < end; t0 += kStep) {
             const T* values[S::kHalves];
             bool valid[S::kHalves];
@@ -440,11 +450,9 @@ void nz_shared_attention_kernel(nz_shared_attention_args a) {
 #pragma unroll
                     for (uint32_t i = 0; i < 4; ++i) {
                         const uint32_t t = t0 + 16 * h + 4 * quad + i;
-                        score[b][h][i] = valid[h] && t >= begin && t < limit[b] ? acc[i] * scale : -__builtin_inff();
+                        score[b][h][i] = valid[h] && t >= begin && t < end ? acc[i] * scale : -__builtin_inff();
                     }
                 }
-            // every column of the item sees every key of the tile
-            const bool even = t0 >= begin && t0 + S::kKeys <= lowest && valid[0] && valid[S::kHalves - 1];
             if (t0 + kStep < end) {
                 load_keys(t0 + kStep, next);
 #pragma unroll
@@ -485,62 +493,36 @@ void nz_shared_attention_kernel(nz_shared_attention_args a) {
                     p_lo[k] = static_cast<T>(__builtin_amdgcn_fmed3f(p - head, head, P::kLeast));
                 }
             };
-            if (even) {
+            // Values of keys outside the item may be anything, NaN among it.
+            if (t0 < begin || t0 + S::kKeys > end || !valid[0] || !valid[S::kHalves - 1]) {
 #pragma unroll
-                for (uint32_t w = 0; w < S::kGroups; ++w) {
-                    piece p_hi[NT], p_lo[NT];
-#pragma unroll
-                    for (uint32_t b = 0; b < NT; ++b) weights(b, w, p_hi[b], p_lo[b]);
+                for (uint32_t w = 0; w < S::kGroups; ++w)
 #pragma unroll
                     for (uint32_t s = 0; s < S::kValueSteps; ++s)
 #pragma unroll
-                        for (uint32_t e = 0; e < S::kValueRun; ++e) {
-                            piece x;
-#pragma unroll
-                            for (uint32_t k = 0; k < S::kRun; ++k) x[k] = v[w][s][k][e];
-#pragma unroll
-                            for (uint32_t b = 0; b < NT; ++b) {
-                                o[b][s][e] = P::mma(x, p_hi[b], o[b][s][e]);
-                                if (S::kRun == 8) o[b][s][e] = P::mma(x, p_lo[b], o[b][s][e]);
-                            }
+                        for (uint32_t k = 0; k < S::kRun; ++k) {
+                            const uint32_t h = S::kRun == 8 ? k / 4 : w, t = t0 + 16 * h + 4 * quad + k % 4;
+                            if (!valid[h] || t < begin || t >= end) v[w][s][k] = value_run{};
                         }
-                }
-            } else {
-                // Some columns see fewer of these keys than others, and the
-                // values of keys that they don't see may be anything, NaN
-                // among it: the columns of each limit in turn, with the
-                // values past it as zeros.
+            }
 #pragma unroll
-                for (uint32_t b = 0; b < NT; ++b) {
-                    uint64_t left = __ballot(b * 16 + col < columns);
-                    while (left) {
-                        const uint32_t seen = static_cast<uint32_t>(
-                            __builtin_amdgcn_readlane(static_cast<int>(limit[b]), __builtin_ctzll(left)));
-                        const bool mine = limit[b] == seen;
-                        left &= ~__ballot(mine);
+            for (uint32_t w = 0; w < S::kGroups; ++w) {
+                piece p_hi[NT], p_lo[NT];
 #pragma unroll
-                        for (uint32_t w = 0; w < S::kGroups; ++w) {
-                            piece p_hi, p_lo;
-                            weights(b, w, p_hi, p_lo);
+                for (uint32_t b = 0; b < NT; ++b) weights(b, w, p_hi[b], p_lo[b]);
 #pragma unroll
-                            for (uint32_t s = 0; s < S::kValueSteps; ++s)
+                for (uint32_t s = 0; s < S::kValueSteps; ++s)
 #pragma unroll
-                                for (uint32_t e = 0; e < S::kValueRun; ++e) {
-                                    piece x;
+                    for (uint32_t e = 0; e < S::kValueRun; ++e) {
+                        piece x;
 #pragma unroll
-                                    for (uint32_t k = 0; k < S::kRun; ++k) {
-                                        const uint32_t h = S::kRun == 8 ? k / 4 : w;
-                                        const uint32_t t = t0 + 16 * h + 4 * quad + k % 4;
-                                        x[k] = valid[h] && t >= begin && t < seen ? v[w][s][k][e] : T{};
-                                    }
-                                    f32x4 sum = P::mma(x, p_hi, o[b][s][e]);
-                                    if (S::kRun == 8) sum = P::mma(x, p_lo, sum);
+                        for (uint32_t k = 0; k < S::kRun; ++k) x[k] = v[w][s][k][e];
 #pragma unroll
-                                    for (uint32_t i = 0; i < 4; ++i) o[b][s][e][i] = mine ? sum[i] : o[b][s][e][i];
-                                }
+                        for (uint32_t b = 0; b < NT; ++b) {
+                            o[b][s][e] = P::mma(x, p_hi[b], o[b][s][e]);
+                            if (S::kRun == 8) o[b][s][e] = P::mma(x, p_lo[b], o[b][s][e]);
                         }
                     }
-                }
             }
         }
 #pragma unroll
@@ -569,13 +551,9 @@ void nz_shared_attention_kernel(nz_shared_attention_args a) {
     // The item's sums over its wavefronts: rows of one item are done, of the
     // others they are parts, unnormalised and with their maximum and weight.
     const uint32_t quads = a.head_dim / 4;   // runs of 4 elements of a head
-    const uint32_t width = parts * kColumns;   // an item's slots
-    const auto slot_of = [&](uint32_t which_item, uint32_t column) {
-        return which_item * width + part * kColumns + column;
-    };
-    float* const part_o = a.partials;
-    float* const part_ml = a.partials + static_cast<uint64_t>(a.n_items) * width * a.head_dim;
-    const rsrc_t all_o = device_buffer(part_o), all_ml = device_buffer(part_ml);
+    const uint64_t slot0 = (static_cast<uint64_t>(which) * parts + part) * kColumns;
+    float* const part_o = a.partials + slot0 * a.head_dim;
+    float* const part_ml = a.partials + static_cast<uint64_t>(a.n_items) * parts * kColumns * a.head_dim + 2 * slot0;
     T* const out = static_cast<T*>(a.out);
     for (uint32_t i = threadIdx.x; i < columns * quads; i += kThreads) {
         const uint32_t c = i / quads, d = i % quads * 4;
@@ -591,99 +569,94 @@ void nz_shared_attention_kernel(nz_shared_attention_args a) {
             weight += share * lds_l[w][c];
             sum += share * *reinterpret_cast<const f32x4*>(&lds_o[w][c][d]);
         }
-        const uint32_t row = static_cast<uint32_t>(members[c / heads]);
-        if (a.rows[row].group_count + a.rows[row].own_count == 1) {
-            store_row(out + row * a.out_row + (head0 + c % heads) * a.out_head + d, sum, weight);
+        const nz_shared_row& r = rows[c / heads];
+        if (r.group_count + r.own_count + r.tail_count == 1) {
+            store_row(out + numbers[c / heads] * a.out_row + (head0 + c % heads) * a.out_head + d, sum, weight);
         } else {
-            const uint32_t slot = slot_of(which, c);
-            if (d == 0) put_pair(all_ml, 8 * slot, top, weight);
-            put_four(all_o, 4 * (slot * a.head_dim + d), sum);
+            if (d == 0) *reinterpret_cast<vec<float, 2>*>(part_ml + 2 * c) = vec<float, 2>{top, weight};
+            *reinterpret_cast<f32x4*>(part_o + c * a.head_dim + d) = sum;
         }
     }
-    // The last of a row's items to arrive joins them all, in their order.
-    if (threadIdx.x == 0) n_ended = 0;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wavefront's stores have arrived
-    __syncthreads();
-    if (threadIdx.x < static_cast<uint32_t>(item.rows)) {
-        const uint32_t row = static_cast<uint32_t>(members[threadIdx.x]);
-        const uint32_t count = static_cast<uint32_t>(a.rows[row].group_count + a.rows[row].own_count);
-        if (count > 1) {
-            uint32_t* const counter = a.counters + static_cast<uint64_t>(row) * parts + part;
-            if (__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == count) {
-                ended[atomicAdd(&n_ended, 1u)] = row;
-                *counter = 0;   // for the next call
-            }
-        }
-    }
-    __syncthreads();
-    // A run of 4 elements of a head: its items kBatch at a time, which are in
-    // flight together and summed from their own maximum, then the batches in
-    // their order. So the result is the same whether one thread takes them all
-    // or, where a single row ended, one thread each batch.
-    constexpr uint32_t kBatch = 8;
-    const uint32_t row_runs = heads * quads, runs = n_ended * row_runs;
-    if (runs == 0) return;
+}
+
+// The rows of several items: their parts, joined in order. A workgroup takes
+// one row's query heads of a key-value head; each run of 4 elements of a head
+// is joined by `subs` threads, each over a share of the items, kBatch of them
+// in flight at a time.
+constexpr uint32_t kJoinThreads = 512;
+
+template <typename T>
+__global__ __launch_bounds__(kJoinThreads) void nz_shared_join_kernel(nz_shared_attention_args a) {
     struct Sums {
         f32x4 sum;
         float top, weight;
+        uint32_t pad[2];
     };
-    const auto batch_of = [&](const nz_shared_row& r, uint32_t k, uint32_t h, uint32_t d) {
-        const uint32_t groups = static_cast<uint32_t>(r.group_count), n = groups + static_cast<uint32_t>(r.own_count);
-        vec<float, 2> ml[kBatch];
-        f32x4 x[kBatch];
+    __shared__ Sums all[kJoinThreads];
+    const uint32_t row = blockIdx.y, part = blockIdx.x;
+    const nz_shared_row r = a.rows[row];
+    const uint32_t groups = static_cast<uint32_t>(r.group_count), own = groups + static_cast<uint32_t>(r.own_count);
+    const uint32_t n = own + static_cast<uint32_t>(r.tail_count);
+    if (n <= 1) return;
+    const uint32_t group = a.heads / a.kv_heads, blocks = (group + kColumns - 1) / kColumns, parts = a.kv_heads * blocks;
+    const uint32_t kv_head = part / blocks, head0 = kv_head * group + part % blocks * kColumns;
+    const uint32_t heads = min(kColumns, (kv_head + 1) * group - head0), quads = a.head_dim / 4;
+    const float* const part_ml = a.partials + static_cast<uint64_t>(a.n_items) * parts * kColumns * a.head_dim;
+    const uint32_t runs = heads * quads, subs = max(kJoinThreads / runs, 1u);
+    T* const out = static_cast<T*>(a.out) + row * a.out_row + head0 * a.out_head;
+    for (uint32_t i = threadIdx.x; i < runs * subs; i += kJoinThreads) {
+        const uint32_t run = i % runs, sub = i / runs, h = run / quads, d = run % quads * 4;
+        const uint32_t k0 = sub * n / subs, k1 = (sub + 1) * n / subs;
+        Sums s = {{}, -__builtin_inff(), 0.0f, {}};
+        constexpr uint32_t kBatch = 16;
+        for (uint32_t k = k0; k < k1; k += kBatch) {
+            vec<float, 2> ml[kBatch];
+            f32x4 x[kBatch];
 #pragma unroll
-        for (uint32_t j = 0; j < kBatch; ++j) {
-            const uint32_t at = min(k + j, n - 1);
-            const uint32_t from = at < groups ? r.group_first + at * r.group_step : r.own_first + (at - groups);
-            const uint32_t place = static_cast<uint32_t>(at < groups ? r.group_place : r.own_place);
-            const uint32_t slot = slot_of(from, place * heads + h);
-            ml[j] = get_pair(all_ml, 8 * slot);
-            x[j] = get_four(all_o, 4 * (slot * a.head_dim + d));
-        }
-        Sums s = {{}, -__builtin_inff(), 0.0f};
+            for (uint32_t j = 0; j < kBatch; ++j) {
+                const uint32_t at = min(k + j, k1 - 1);
+                const uint32_t from = at < groups ? r.group_first + at * r.group_step
+                                      : at < own  ? r.own_first + (at - groups)
+                                                  : r.tail_first + (at - own);
+                const uint32_t place = at < groups ? r.places & 0xFF : at < own ? r.places >> 8 : 0;
+                const uint64_t slot = (static_cast<uint64_t>(from) * parts + part) * kColumns + place * heads + h;
+                ml[j] = *reinterpret_cast<const vec<float, 2>*>(part_ml + 2 * slot);
+                x[j] = *reinterpret_cast<const f32x4*>(a.partials + slot * a.head_dim + d);
+            }
+            float higher = s.top;
 #pragma unroll
-        for (uint32_t j = 0; j < kBatch; ++j) s.top = fmaxf(s.top, ml[j].x);
-        const float base = finite_base(s.top);
+            for (uint32_t j = 0; j < kBatch; ++j) higher = fmaxf(higher, ml[j].x);
+            const float base = finite_base(higher), fade = __builtin_amdgcn_exp2f(s.top - base);
+            s.top = higher;
+            s.weight *= fade;
+            s.sum *= fade;
 #pragma unroll
-        for (uint32_t j = 0; j < kBatch; ++j) {
-            const float share = __builtin_amdgcn_exp2f(ml[j].x - base);
-            if (k + j < n) {
-                s.weight += share * ml[j].y;
-                s.sum += share * x[j];
+            for (uint32_t j = 0; j < kBatch; ++j) {
+                const float share = __builtin_amdgcn_exp2f(ml[j].x - base);
+                if (k + j < k1) {
+                    s.weight += share * ml[j].y;
+                    s.sum += share * x[j];
+                }
             }
         }
-        return s;
-    };
-    const auto join = [](Sums& s, const Sums& more) {
-        const float top = fmaxf(s.top, more.top), base = finite_base(top);
-        const float fade = __builtin_amdgcn_exp2f(s.top - base), share = __builtin_amdgcn_exp2f(more.top - base);
-        s.sum = fade * s.sum + share * more.sum;
-        s.weight = fade * s.weight + share * more.weight;
-        s.top = top;
-    };
-    const nz_shared_row first = a.rows[ended[0]];
-    const uint32_t batches = (static_cast<uint32_t>(first.group_count + first.own_count) + kBatch - 1) / kBatch;
-    // (the wavefronts' sums have been read)
-    if (n_ended == 1 && batches > 1 && 2 * runs <= kThreads && runs * batches * sizeof(Sums) <= sizeof(lds_o)) {
-        Sums* const all = reinterpret_cast<Sums*>(&lds_o[0][0][0]);
-        for (uint32_t i = threadIdx.x; i < runs * batches; i += kThreads)
-            all[i] = batch_of(first, i / runs * kBatch, i % runs / quads, i % quads * 4);
-        __syncthreads();
-        if (threadIdx.x < runs) {
-            Sums s = all[threadIdx.x];
-            for (uint32_t k = 1; k < batches; ++k) join(s, all[k * runs + threadIdx.x]);
-            store_row(out + ended[0] * a.out_row + (head0 + threadIdx.x / quads) * a.out_head + threadIdx.x % quads * 4, s.sum,
-                      s.weight);
-        }
-        return;
+        if (subs == 1) store_row(out + h * a.out_head + d, s.sum, s.weight);
+        else all[i] = s;
     }
-    for (uint32_t i = threadIdx.x; i < runs; i += kThreads) {
-        const uint32_t row = ended[i / row_runs], h = i % row_runs / quads, d = i % quads * 4;
-        const nz_shared_row r = a.rows[row];
-        const uint32_t n = static_cast<uint32_t>(r.group_count + r.own_count);
-        Sums s = batch_of(r, 0, h, d);
-        for (uint32_t k = kBatch; k < n; k += kBatch) join(s, batch_of(r, k, h, d));
-        store_row(out + row * a.out_row + (head0 + h) * a.out_head + d, s.sum, s.weight);
+    if (subs == 1) return;
+    __syncthreads();
+    if (threadIdx.x < runs) {
+        const uint32_t h = threadIdx.x / quads, d = threadIdx.x % quads * 4;
+        float top = -__builtin_inff(), weight = 0.0f;
+        for (uint32_t sub = 0; sub < subs; ++sub) top = fmaxf(top, all[sub * runs + threadIdx.x].top);
+        const float base = finite_base(top);
+        f32x4 sum = {};
+        for (uint32_t sub = 0; sub < subs; ++sub) {
+            const Sums& s = all[sub * runs + threadIdx.x];
+            const float share = __builtin_amdgcn_exp2f(s.top - base);
+            weight += share * s.weight;
+            sum += share * s.sum;
+        }
+        store_row(out + h * a.out_head + d, sum, weight);
     }
 }
 
@@ -702,6 +675,8 @@ void launch_shared(const nz_shared_attention_args& a, hipStream_t stream) {
     else if (a.head_dim <= 64) launch_dim<T, 64>(a, grid, stream);
     else if (a.head_dim <= 128) launch_dim<T, 128>(a, grid, stream);
     else launch_dim<T, 256>(a, grid, stream);
+    const uint32_t parts = a.kv_heads * ((group + kColumns - 1) / kColumns);
+    hipLaunchKernelGGL(nz_shared_join_kernel<T>, dim3(parts, a.n_rows), dim3(kJoinThreads), 0, stream, a);
 }
 
 }  // namespace

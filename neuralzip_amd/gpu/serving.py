@@ -44,7 +44,7 @@ ATTENTION_WORKGROUPS = 256
 # Query heads of one workgroup (the columns of a matrix instruction).
 _HEADS = 16
 # The same for shared keys: workgroups, and columns (rows times query heads).
-SHARED_WORKGROUPS = 512
+SHARED_WORKGROUPS = int(__import__("os").environ.get("SW", 512))
 _COLUMNS = 32
 # PageTables.extend's status of a request (enum nz_pages_status).
 PAGES_OK, PAGES_TOO_LONG, PAGES_NO_ROOM, PAGES_NO_PAGE = range(4)
@@ -403,8 +403,9 @@ class SharedPlan(AttentionPlan):
     """AttentionPlan for rows that see the same keys, which are then read
     once for as many rows as make 32 query heads of a key-value head:
 
-    neighbouring rows of one request, as a step with drafted tokens has them;
-    and the first shared[g] keys of all requests of group g. `groups` (int32,
+    neighbouring rows of one request, as a step with drafted tokens has them,
+    as far as the shortest of their contexts; and the first shared[g] keys of
+    all requests of group g, for rows whose contexts are that long. `groups` (int32,
     one per request: per row of the tables) gives a request's group, -1 for
     none, `shared` (int32, one per group) the keys. The requests of a group
     must have the same pages in their tables for these.
@@ -434,11 +435,10 @@ class SharedPlan(AttentionPlan):
         if self.capacity == 0:
             raise ValueError("A SharedPlan takes at most 2048 rows and 1024 groups.")
         with _on(stream):
-            words = torch.empty(8 * self.capacity + self.rows * (10 + parts), dtype=torch.int32, device=self.device)
-        items, rows, order, self._counters = words.split((8 * self.capacity, 8 * self.rows, 2 * self.rows,
-                                                          self.rows * parts))
+            words = torch.empty(8 * self.capacity + 10 * self.rows, dtype=torch.int32, device=self.device)
+        items, rows, self.order = words.split((8 * self.capacity, 8 * self.rows, 2 * self.rows))
         self.items = items.view(self.capacity, 8)
-        self._pointers = items.data_ptr(), rows.data_ptr(), order.data_ptr(), self._counters.data_ptr()
+        self._pointers = items.data_ptr(), rows.data_ptr(), self.order.data_ptr()
         self._format, self._function = _native.SHARED_ATTENTION, _native.lib().nz_shared_attention
         self._stream, self._scratch = _stream_handle(self.device, stream), {}
         self.update(contexts, requests=requests, groups=groups, shared=shared, stream=stream)

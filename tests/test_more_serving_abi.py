@@ -49,9 +49,10 @@ def test_floats_and_constants_are_the_header_s():
                         ("NZ_EXPERT_SILU", _native.EXPERT_ACTIVATION["silu"]),
                         ("NZ_EXPERT_GELU", _native.EXPERT_ACTIVATION["gelu"])):
         assert f"{name} = {value}" in text
-    # a shared plan's attention takes what the other's does, with two arrays more
+    # a shared plan's attention takes what the other's does, with the plan's arrays
     mine, other = ([f for f, _ in fields(n)] for n in ("nz_shared_attention_args", "nz_attention_args"))
-    assert [f for f in mine if f not in ("rows", "order")] == other and mine.index("rows") == other.index("items") + 1
+    assert [f for f in mine if f not in ("rows", "order")] == [f for f in other if f != "counters"]
+    assert mine[mine.index("items"):][:4] == ["items", "rows", "order", "partials"]
 
 
 def packed(name, **values):
@@ -62,9 +63,9 @@ def packed(name, **values):
 
 TRIM = dict(lengths=True, keep=True, tables=True, free_pages=True, n_free=True, lengths_after=True, n_free_after=True,
             n_requests=4, max_pages=8, page_size=16, n_pages=32)
-PLAN = dict(contexts=True, requests=True, groups=True, shared=True, items=True, rows=True, order=True, counters=True,
+PLAN = dict(contexts=True, requests=True, groups=True, shared=True, items=True, rows=True, order=True,
             n_rows=10, n_requests=4, n_groups=2, n_items=32, heads=8, kv_heads=2, target=16)
-ATTENTION = dict(test_serving_abi.ATTENTION, rows=True, order=True)
+ATTENTION = {k: v for k, v in dict(test_serving_abi.ATTENTION, rows=True, order=True).items() if k != "counters"}
 VERIFY = dict(logits=True, draft_probs=True, tokens=True, starts=True, accept=True, sample=True, temperature=True,
               accepted=True, next=True, scratch=True, logits_row=100, draft_row=100, n_rows=5, n_requests=2, vocab=100)
 ROUTE = dict(x=True, weight=True, ids=True, weights=True, scratch=True, x_row=64, tokens=3, hidden=64, experts=8, top_k=2)
@@ -84,7 +85,6 @@ EXPERTS = dict(x=True, ids=True, weights=True, gate_up=True, down=True, out=True
     ("nz_shared_plan", PLAN, dict(items=0), b"Null"),
     ("nz_shared_plan", PLAN, dict(rows=0), b"Null"),
     ("nz_shared_plan", PLAN, dict(order=0), b"Null"),
-    ("nz_shared_plan", PLAN, dict(counters=0), b"Null"),
     ("nz_shared_plan", PLAN, dict(groups=0), b"Null"),
     ("nz_shared_plan", PLAN, dict(shared=0), b"Null"),
     ("nz_shared_plan", PLAN, dict(heads=3), b"multiple of kv_heads"),
@@ -104,7 +104,7 @@ EXPERTS = dict(x=True, ids=True, weights=True, gate_up=True, down=True, out=True
     ("nz_shared_attention", ATTENTION, dict(head_dim=272), b"head_dim"),
     ("nz_shared_attention", ATTENTION, dict(n_requests=0), b"pages and requests"),
     ("nz_shared_attention", ATTENTION, dict(n_items=1), b"fewer items"),
-    ("nz_shared_attention", ATTENTION, dict(n_items=1 << 20), b"Too many"),
+    ("nz_shared_attention", ATTENTION, dict(n_items=1 << 26), b"Too many"),
     ("nz_shared_attention", ATTENTION, dict(n_rows=2049, n_items=4096), b"Too many"),
     ("nz_shared_attention", ATTENTION, dict(key_slot=3), b"16 bytes"),
     ("nz_shared_attention", ATTENTION, dict(type=3), b"value type"),
