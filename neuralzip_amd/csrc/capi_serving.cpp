@@ -203,7 +203,8 @@ uint32_t nz_shared_items(uint32_t n_rows, uint32_t n_groups, uint32_t heads, uin
     const uint32_t tile_rows = std::max(1u, NZ_SHARED_COLUMNS / (heads / kv_heads));
     // a tile per row, and those of the groups
     const uint32_t tiles = n_rows + (n_groups ? std::min(n_rows, n_groups + n_rows / tile_rows) : 0);
-    return (std::max(tiles, target) + target - 1) / target * target;
+    const uint32_t items = (std::max(tiles, target) + target - 1) / target * target;
+    return n_groups ? items + items / 2 : items;
 }
 
 int nz_shared_plan(const nz_shared_plan_args* args, void* stream) {

@@ -72,10 +72,14 @@ __device__ __forceinline__ V fetch(const T* src) {
     return PAST ? __builtin_nontemporal_load(p) : *p;
 }
 
-// Largest of a column's values over the four lanes that hold it.
+// Largest of a column's values over the four lanes that hold it: those 16 and
+// 32 lanes away come by exchanges of rows of lanes.
 __device__ __forceinline__ float column_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
+    const uint32_t x = __float_as_uint(v);
+    const auto near = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    const uint32_t y = __float_as_uint(fmaxf(__uint_as_float(near[0]), __uint_as_float(near[1])));
+    const auto far = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+    return fmaxf(__uint_as_float(far[0]), __uint_as_float(far[1]));
 }
 
 __device__ __forceinline__ float column_sum(float v) {

@@ -22,6 +22,11 @@ constexpr uint32_t kMaxRows = NZ_SHARED_MAX_ROWS, kMaxGroups = NZ_SHARED_MAX_GRO
 // Items start at multiples of kTile keys and are no shorter than one such tile
 // for each wavefront of a workgroup.
 constexpr uint32_t kTile = 32, kLeastItem = 128;
+// Keys of a group, which its other items read too, take about half as long as
+// a row's own, which come from memory. (32 requests behind 8176 keys: 48 us
+// against 51 with items of one length and no more of them; 64 over three
+// prefixes of 16384 keys: 275 against 315.)
+constexpr uint32_t kGroupLength = 2;
 
 struct PlanLds {
     uint32_t waves[kPlanWaves], counts[kPlanWaves];
@@ -186,15 +191,17 @@ __global__ __launch_bounds__(kPlanThreads) void nz_shared_plan_kernel(nz_shared_
         pieces += lds.counts[w];
     }
     __syncthreads();
-    // The shortest length of items, in tiles of keys, that gives few enough.
-    const uint32_t limit = min(cuts(max(a.target, pieces), a.target) * a.target, a.n_items);
+    // The shortest length of items, in tiles of keys, that gives few enough: half more of them where there are
+    // groups, whose items are up to kGroupLength times as long as the others.
+    const uint32_t whole_rounds = cuts(max(a.target, pieces), a.target) * a.target;
+    const uint32_t limit = min(a.n_groups ? whole_rounds + whole_rounds / 2 : whole_rounds, a.n_items);
     uint32_t lo = kLeastItem / kTile, hi = max((longest + kTile - 1) / kTile, lo);
     const auto count_items = [&](uint32_t share) {   // a wavefront's sum
         uint32_t sum = 0;
         for (uint32_t i = lane; i < n; i += 64)
             sum += cuts(lds.own[i], share) + max(cuts(lds.tail[i], share), lds.context[i] == 0 ? 1u : 0u);
         for (uint32_t g = lane; g < a.n_groups; g += 64)
-            sum += cuts(lds.members[g], tile_rows) * cuts(lds.shared[g], share);
+            sum += cuts(lds.members[g], tile_rows) * cuts(lds.shared[g], kGroupLength * share);
         return last_lane(wave_scan(sum));
     };
     while (lo < hi) {
@@ -212,17 +219,19 @@ __global__ __launch_bounds__(kPlanThreads) void nz_shared_plan_kernel(nz_shared_
     }
     const uint32_t share = lo * kTile;
     // items are of equal length, in whole kTile keys
-    const auto each_of = [&](uint32_t length) {
-        const uint32_t count = max(cuts(length, share), 1u);
+    const auto each_of = [&](uint32_t length, uint32_t most) {
+        const uint32_t count = max(cuts(length, most), 1u);
         return max((cuts(length, count) + kTile - 1) / kTile * kTile, kTile);
     };
-    const auto items_of = [&](uint32_t length) { return cuts(length, each_of(length)); };
+    const auto items_of = [&](uint32_t length) { return cuts(length, each_of(length, share)); };
+    const auto group_each = [&](uint32_t g) { return each_of(lds.shared[g], kGroupLength * share); };
+    const auto group_items = [&](uint32_t g) { return cuts(lds.shared[g], group_each(g)); };
     __syncthreads();
     // first items, kind by kind
     uint32_t first = 0;
     for (uint32_t g0 = 0; g0 < a.n_groups; g0 += kPlanThreads) {
         const uint32_t g = g0 + threadIdx.x;
-        const uint32_t count = g < a.n_groups ? cuts(lds.members[g], tile_rows) * items_of(lds.shared[g]) : 0;
+        const uint32_t count = g < a.n_groups ? cuts(lds.members[g], tile_rows) * group_items(g) : 0;
         uint32_t total;
         const uint32_t upto = plan_scan(count, total, lds);
         if (g < a.n_groups) lds.group_first[g] = first + upto - count;
@@ -255,7 +264,7 @@ __global__ __launch_bounds__(kPlanThreads) void nz_shared_plan_kernel(nz_shared_
             // (groups without items begin where the next one does)
             const uint32_t g = owner(lds.group_first, a.n_groups, j);
             const uint32_t count = cuts(lds.members[g], tile_rows), k = j - lds.group_first[g];
-            const uint32_t tile = k % count, part = k / count, each = each_of(lds.shared[g]);
+            const uint32_t tile = k % count, part = k / count, each = group_each(g);
             item.member = static_cast<int32_t>(lds.base[g] + tile * tile_rows);
             item.rows = static_cast<int32_t>(min(tile_rows, lds.members[g] - tile * tile_rows));
             item.request = lds.request[lds.order[lds.base[g]]];
@@ -264,7 +273,7 @@ __global__ __launch_bounds__(kPlanThreads) void nz_shared_plan_kernel(nz_shared_
         } else if (j < owned) {
             const uint32_t i = owner(lds.own, n, j);
             const Tile t = tile_of(i);
-            const uint32_t each = each_of(t.end - t.begin), part = j - lds.own[i];
+            const uint32_t each = each_of(t.end - t.begin, share), part = j - lds.own[i];
             item.member = static_cast<int32_t>(n + i);
             item.rows = static_cast<int32_t>(t.rows);
             item.request = lds.request[i];
@@ -273,7 +282,7 @@ __global__ __launch_bounds__(kPlanThreads) void nz_shared_plan_kernel(nz_shared_
         } else {
             const uint32_t i = owner(lds.tail, n, j);
             const Tile t = tile_of(i);
-            const uint32_t each = each_of(lds.context[i] - t.end), part = j - lds.tail[i];
+            const uint32_t each = each_of(lds.context[i] - t.end, share), part = j - lds.tail[i];
             item.member = static_cast<int32_t>(n + i);
             item.rows = 1;
             item.request = lds.request[i];
@@ -294,7 +303,7 @@ __global__ __launch_bounds__(kPlanThreads) void nz_shared_plan_kernel(nz_shared_
         if (g >= 0) {
             row.group_first = static_cast<int32_t>(lds.group_first[g] + lds.rank[i] / tile_rows);
             row.group_step = static_cast<int32_t>(cuts(lds.members[g], tile_rows));
-            row.group_count = static_cast<int32_t>(items_of(lds.shared[g]));
+            row.group_count = static_cast<int32_t>(group_items(g));
             place = lds.rank[i] % tile_rows;
             a.order[lds.base[g] + lds.rank[i]] = static_cast<int32_t>(i);
         }

@@ -44,7 +44,7 @@ ATTENTION_WORKGROUPS = 256
 # Query heads of one workgroup (the columns of a matrix instruction).
 _HEADS = 16
 # The same for shared keys: workgroups, and columns (rows times query heads).
-SHARED_WORKGROUPS = int(__import__("os").environ.get("SW", 512))
+SHARED_WORKGROUPS = 512
 _COLUMNS = 32
 # PageTables.extend's status of a request (enum nz_pages_status).
 PAGES_OK, PAGES_TOO_LONG, PAGES_NO_ROOM, PAGES_NO_PAGE = range(4)

@@ -175,7 +175,7 @@ def test_sizes_of_plans_and_scratch():
     lib = _native.lib()
     assert lib.nz_shared_items(1, 0, 32, 8, 64) == 64 and lib.nz_shared_items(0, 0, 32, 8, 64) == 64
     assert lib.nz_shared_items(65, 0, 32, 8, 64) == 128
-    assert lib.nz_shared_items(64, 3, 32, 8, 64) == 128     # 64 rows' tiles and at most 3 + 8 of the groups
+    assert lib.nz_shared_items(64, 3, 32, 8, 64) == 192     # 64 rows' tiles, at most 3 + 8 of the groups, and half more
     for wrong in ((2049, 0, 8, 2, 1), (1, 1025, 8, 2, 1), (1, 0, 0, 1, 1), (1, 0, 8, 0, 1), (1, 0, 7, 2, 1),
                   (1, 0, 8, 2, 0)):
         assert lib.nz_shared_items(*wrong) == 0
