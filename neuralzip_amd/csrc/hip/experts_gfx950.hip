@@ -240,8 +240,9 @@ __global__ __launch_bounds__(kUpThreads) void nz_expert_up_kernel(nz_expert_args
     for (uint32_t b = 0; b < NB; ++b)
         x[b] = static_cast<const T*>(a.x) + (token0 + list[b * 16 + col < count ? b * 16 + col : 0]) * a.x_row;
     f32x4 sum[2][NB] = {};
-    for (uint32_t d0 = wave * kBatch * kDepth; d0 < a.hidden; d0 += kUpWaves * kBatch * kDepth) {
-        piece g[kBatch], u[kBatch], y[NB][kBatch];
+    // weights are asked for a batch ahead
+    piece g[kBatch], u[kBatch];
+    const auto fetch_weights = [&](uint32_t d0) {
 #pragma unroll
         for (uint32_t j = 0; j < kBatch; ++j) {
             const uint32_t d = d0 + j * kDepth + quad * P::kRun;
@@ -251,6 +252,13 @@ __global__ __launch_bounds__(kUpThreads) void nz_expert_up_kernel(nz_expert_args
                 u[j] = *reinterpret_cast<const piece*>(up + d);
             }
         }
+    };
+    constexpr uint32_t kStep = kUpWaves * kBatch * kDepth;
+    fetch_weights(wave * kBatch * kDepth);
+    for (uint32_t d0 = wave * kBatch * kDepth; d0 < a.hidden; d0 += kStep) {
+        piece y[NB][kBatch], g_now[kBatch], u_now[kBatch];
+#pragma unroll
+        for (uint32_t j = 0; j < kBatch; ++j) g_now[j] = g[j], u_now[j] = u[j];
 #pragma unroll
         for (uint32_t b = 0; b < NB; ++b)
 #pragma unroll
@@ -259,13 +267,14 @@ __global__ __launch_bounds__(kUpThreads) void nz_expert_up_kernel(nz_expert_args
                 y[b][j] = piece{};
                 if (d < a.hidden && b * 16 + col < count) y[b][j] = *reinterpret_cast<const piece*>(x[b] + d);
             }
+        fetch_weights(d0 + kStep);
 #pragma unroll
         for (uint32_t b = 0; b < NB; ++b)
             if (NB == 1 || b < blocks)
 #pragma unroll
                 for (uint32_t j = 0; j < kBatch; ++j) {
-                    sum[0][b] = P::mma(g[j], y[b][j], sum[0][b]);
-                    sum[1][b] = P::mma(u[j], y[b][j], sum[1][b]);
+                    sum[0][b] = P::mma(g_now[j], y[b][j], sum[0][b]);
+                    sum[1][b] = P::mma(u_now[j], y[b][j], sum[1][b]);
                 }
     }
 #pragma unroll
@@ -344,14 +353,13 @@ __global__ __launch_bounds__(kDownThreads) void nz_expert_down_kernel(nz_expert_
     choose<kDownThreads>(a, token0, tokens, choice);
     const uint32_t row0 = blockIdx.x * kDownRows;
     const uint32_t steps = (a.inter + kBatch * kDepth - 1) / (kBatch * kDepth);
-    const uint64_t all = static_cast<uint64_t>(choice.n_active) * steps;
-    const uint32_t shares = splits * kDownWaves, mine = blockIdx.y * kDownWaves + wave;
-    uint64_t at = all * mine / shares;
-    const uint64_t until = all * (mine + 1) / shares;
+    const uint32_t all = choice.n_active * steps, shares = splits * kDownWaves, mine = blockIdx.y * kDownWaves + wave;
+    const uint32_t each = all / shares, more = all % shares;
+    uint32_t at = mine * each + min(mine, more);
+    const uint32_t until = at + each + (mine < more);
     while (at < until) {
-        const uint32_t n = static_cast<uint32_t>(at / steps);
-        const uint32_t expert = __builtin_amdgcn_readfirstlane(choice.active[n]), s0 = static_cast<uint32_t>(at % steps);
-        const uint32_t s1 = static_cast<uint32_t>(min(static_cast<uint64_t>(steps), s0 + (until - at)));
+        const uint32_t n = at / steps, s0 = at - n * steps, s1 = min(steps, s0 + (until - at));
+        const uint32_t expert = __builtin_amdgcn_readfirstlane(choice.active[n]);
         const uint64_t mask = choice.tokens[expert];
         const uint32_t count = __popcll(mask), blocks = __builtin_amdgcn_readfirstlane((count + 15) / 16);
         if (mask >> lane & 1) list[wave][__popcll(mask & ((1ull << lane) - 1))] = lane;
@@ -370,16 +378,25 @@ __global__ __launch_bounds__(kDownThreads) void nz_expert_down_kernel(nz_expert_
                 x[b] += (static_cast<uint64_t>(token0 + token[b]) * a.top_k + place_of(a, choice, token[b], expert)) * a.inter;
         }
         f32x4 sum[kTiles][NB] = {};
-        for (uint32_t s = s0; s < s1; ++s) {
-            piece w[kTiles][kBatch];
+        piece next[kTiles][kBatch];   // weights, asked for a batch ahead
+        const auto fetch_weights = [&](uint32_t s) {
 #pragma unroll
             for (uint32_t t = 0; t < kTiles; ++t)
 #pragma unroll
                 for (uint32_t j = 0; j < kBatch; ++j) {
                     const uint32_t d = (s * kBatch + j) * kDepth + quad * P::kRun;
-                    w[t][j] = piece{};
-                    if (d < a.inter) w[t][j] = *reinterpret_cast<const piece*>(down[t] + d);
+                    next[t][j] = piece{};
+                    if (s < s1 && d < a.inter) next[t][j] = *reinterpret_cast<const piece*>(down[t] + d);
                 }
+        };
+        fetch_weights(s0);
+        for (uint32_t s = s0; s < s1; ++s) {
+            piece w[kTiles][kBatch];
+#pragma unroll
+            for (uint32_t t = 0; t < kTiles; ++t)
+#pragma unroll
+                for (uint32_t j = 0; j < kBatch; ++j) w[t][j] = next[t][j];
+            fetch_weights(s + 1);
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b)
                 if (NB == 1 || b < blocks) {
@@ -461,9 +478,20 @@ __global__ __launch_bounds__(kDownThreads) void nz_expert_down_kernel(nz_expert_
 
 uint32_t down_groups(uint32_t hidden) { return (hidden + kDownRows - 1) / kDownRows; }
 
+// Workgroups that share a part of the outputs: the fewest for which the rounds
+// of one workgroup a compute unit (its registers leave room for no second) are
+// at most a tenth longer than for the best number. (16 experts of 1096 x 520
+// fp32 elements: 23 us with 8, the last 24 of 280 workgroups alone, and 18 with
+// 7.)
 uint32_t splits_of(uint32_t tokens, uint32_t hidden) {
+    constexpr uint32_t kUnits = 256;
     const uint32_t groups = down_groups(hidden) * ((tokens + kTokens - 1) / kTokens);
-    return std::min(kMaxSplits, std::max(1u, (512 + groups - 1) / groups));
+    const auto rounds = [&](uint32_t splits) { return (groups * splits + kUnits - 1) / kUnits / static_cast<double>(splits); };
+    double best = rounds(1);
+    for (uint32_t s = 2; s <= kMaxSplits; ++s) best = std::min(best, rounds(s));
+    uint32_t splits = 1;
+    while (rounds(splits) > 1.1 * best) ++splits;
+    return splits;
 }
 
 template <typename T, uint32_t NB>
