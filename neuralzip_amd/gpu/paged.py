@@ -1,5 +1,6 @@
-"""Greedy decoding of many requests with lengths of their own over a paged
-key-value cache, on a Transformers decoder model, compressed or not.
+"""Decoding of many requests with lengths of their own over a paged key-value
+cache, on a Transformers decoder model, compressed or not: greedily, or sampled
+at a temperature, with tokens drafted by the caller, behind shared prefixes.
 
 PagedDecoder runs every new token of a step through the operators of
 neuralzip_amd.gpu.serving: PageTables gives the tokens their pages, Rotary
@@ -10,6 +11,13 @@ hooks decode the weights as in any forward. Prompts run through the model's
 own forward, one at a time, and their keys and values are then stored into
 the request's pages. A step never asks the device for anything, so that it
 can be captured in a HIP graph (capture()) and replayed while requests grow.
+
+Requests may begin with a prefix (add_prefix()), whose pages they share and
+whose keys a step reads once for all of them. With `drafts`, a step takes that
+many drafted tokens per request along, and verify_drafts keeps those that the
+model would have answered; trim() takes the others' pages back. With `experts`,
+a step's mixture-of-experts layers run through expert_mlp, which a graph can
+hold, in place of the model's own.
 
 Models are Llama-like, of the types in MODEL_TYPES:
 model.model.{embed_tokens, layers, norm, rotary_emb} and model.lm_head, layers
@@ -22,6 +30,7 @@ import contextlib
 
 import torch
 from transformers import DynamicCache
+from transformers.activations import ACT2FN
 
 from neuralzip_amd.gpu import serving
 from neuralzip_amd.gpu.inference import RUNTIME_ATTRIBUTE
@@ -59,20 +68,51 @@ def _check_model(config, max_length):
                          f"less than max_length.")
 
 
+def _expert_modules(model, dtype):
+    """The experts of a model's MoE layers, which expert_mlp computes: stacked
+    weights gate_up_proj (experts, 2 * inter, hidden) and down_proj (experts,
+    hidden, inter), SiLU and no bias."""
+    found = [m for m in model.modules() if torch.is_tensor(getattr(m, "gate_up_proj", None))
+             and torch.is_tensor(getattr(m, "down_proj", None))]
+    if not found:
+        raise ValueError("experts=True needs a model with mixture-of-experts layers.")
+    for m in found:
+        up, down = m.gate_up_proj, m.down_proj
+        if up.dim() != 3 or down.dim() != 3 or up.shape != (down.shape[0], 2 * down.shape[2], down.shape[1]) \
+                or up.dtype != dtype or down.dtype != dtype or up.shape[2] % 8 or down.shape[2] % 8 or up.shape[0] > 1024 \
+                or not isinstance(getattr(m, "act_fn", None), (torch.nn.SiLU, type(ACT2FN["silu"]))) \
+                or {name for name, _ in m.named_parameters()} != {"gate_up_proj", "down_proj"}:
+            raise ValueError(f"expert_mlp does not compute {type(m).__name__}: it needs stacked weights of one type, sizes "
+                             f"of a multiple of 8, SiLU and no bias.")
+    return found
+
+
 class PagedDecoder:
     """`requests` places for requests of at most `max_length` tokens, prompt
     and answer together, on pages of `page_size` tokens: `num_pages` of them
-    for all requests, or enough for all at full length.
+    for all requests and prefixes, or enough for all at full length.
 
     `repetition`, `frequency` and `presence` are adjust_logits' penalties,
     for all requests. With `grammar`, `masks` (int32, requests x ceil(vocab /
     32)) holds the tokens that each request may answer with next; it may be
     written between steps. All bits of a free place are set, at first and when
-    its request ends."""
+    its request ends.
+
+    `temperature`: answers are sampled at it (0 or None: the likeliest token).
+    `drafts`: drafted tokens that a request may bring to a step, at most;
+    requests * (drafts + 1) is at most 2048. `prefixes`: places for prefixes of
+    up to max_length tokens; requests and prefixes are then at most 2048 and
+    1024. `experts`: steps run the experts of MoE layers by expert_mlp."""
 
     def __init__(self, model, *, requests, max_length, page_size=16, num_pages=None, repetition=1.0, frequency=0.0,
-                 presence=0.0, grammar=False):
+                 presence=0.0, grammar=False, temperature=None, drafts=0, prefixes=0, experts=False):
         _check_model(model.config, max_length)
+        if drafts < 0 or prefixes < 0:
+            raise ValueError("drafts and prefixes must not be negative.")
+        if drafts and grammar:
+            raise ValueError("A mask holds for the next token only: drafts and a grammar do not go together.")
+        if (drafts or prefixes) and (requests * (drafts + 1) > 2048 or prefixes > 1024):
+            raise ValueError("requests * (drafts + 1) must be at most 2048 and prefixes at most 1024.")
         body = model.model
         self.model, self.layers = model, list(body.layers)
         self._attentions = [layer.self_attn for layer in self.layers]
@@ -92,9 +132,12 @@ class PagedDecoder:
         self.kv_heads = model.config.num_key_value_heads
         self.heads = model.config.num_attention_heads
         self.requests, self.max_length, self.vocab = requests, max_length, model.config.vocab_size
-        width = -(-max_length // page_size)
-        self.tables = serving.PageTables(requests, width, page_size, requests * width if num_pages is None else num_pages,
+        self._drafts_most, self.temperature = drafts, 0.0 if temperature is None else float(temperature)
+        width, rows = -(-max_length // page_size), requests + prefixes
+        # prefixes have the table rows behind the requests'
+        self.tables = serving.PageTables(rows, width, page_size, rows * width if num_pages is None else num_pages,
                                          device=self.device)
+        self._experts = _expert_modules(model, embedding.dtype) if experts else []
         # one allocation for all layers: (layers, keys and values, pages, heads, places, elements)
         self.cache = torch.zeros((len(self.layers), 2, self.tables.num_pages, self.kv_heads, page_size, self.dim),
                                  dtype=dtype, device=self.device)
@@ -113,12 +156,30 @@ class PagedDecoder:
 
         def filled(value, dtype=torch.float32):
             return torch.full((requests,), value, dtype=dtype, device=self.device)
-        self._step = serving.Step(requests, requests, self.device)
-        self._plan = serving.AttentionPlan(filled(0, torch.int32), heads=self.heads, kv_heads=self.kv_heads)
-        self._live = filled(0, torch.int32)           # 1: the request gets a token in a step
+        tokens = requests * (drafts + 1)
+        self._step = serving.Step(rows, tokens, self.device)
+        none = torch.zeros(tokens, dtype=torch.int32, device=self.device)
+        # the prefix that each request begins with (-1: none), and their lengths in whole pages
+        self._prefix_of = [-1] * requests
+        self._groups = {}
+        if prefixes:
+            self._groups = dict(groups=torch.full((rows,), -1, dtype=torch.int32, device=self.device),
+                                shared=torch.zeros(prefixes, dtype=torch.int32, device=self.device))
+        if drafts or prefixes:
+            self._plan = serving.SharedPlan(none, heads=self.heads, kv_heads=self.kv_heads, requests=none, **self._groups)
+        else:
+            self._plan = serving.AttentionPlan(none, heads=self.heads, kv_heads=self.kv_heads)
+        self._prefixes = [None] * prefixes            # their token ids
+        self._live = torch.zeros(rows, dtype=torch.int32, device=self.device)   # 1: the request gets a token in a step
         # row `requests` of what is written by request takes what a step's unused rows write
         self._last = torch.zeros(requests + 1, dtype=torch.int64, device=self.device)
-        self._answers = torch.full((requests,), -1, dtype=torch.int64, device=self.device)   # of the last step
+        # of the last step, and what it was given
+        self._answers = torch.full((requests, drafts + 1) if drafts else (requests,), -1, dtype=torch.int64,
+                                   device=self.device)
+        self._drafted = torch.full((requests, drafts), -1, dtype=torch.int64, device=self.device)
+        self._accept = torch.zeros(tokens, dtype=torch.float64, device=self.device)
+        self._sample = torch.zeros(requests, dtype=torch.float64, device=self.device)
+        self._temperatures = filled(self.temperature)
         self._history = torch.zeros((requests + 1, max_length + 1), dtype=torch.int32, device=self.device)
         self._prompts = filled(0, torch.int32)
         self._penalties = {}
@@ -135,47 +196,130 @@ class PagedDecoder:
 
     # --------------------------------------------------------------- requests
 
+    def _checked(self, ids, before=0):
+        """Token ids of a prompt or a prefix, behind `before` others, on the CPU."""
+        ids = torch.as_tensor(ids, dtype=torch.int64)
+        if ids.dim() != 1 or not 0 < ids.shape[0] <= self.max_length - before or int(ids.min()) < 0 \
+                or int(ids.max()) >= self.vocab:
+            raise ValueError(f"A prompt is a vector of 1 to {self.max_length - before} token ids below {self.vocab}.")
+        return ids
+
+    def _take_in(self, row, ids, cache, known):
+        """Gives table row `row` pages for its tokens past the first ones it
+        has, runs the model over `ids`, which follow the `known` tokens of
+        `cache`, and stores all keys and values that the row has no page for
+        yet; returns the logits. A row that fails is left as it was."""
+        new = torch.zeros(self.tables.requests, dtype=torch.int32, device=self.device)
+        held = int(self.tables.lengths[row])
+        n = known + ids.shape[0] - held
+        new[row] = n
+        step = self.tables.extend(new, n)
+        if int(step.status[row]) != serving.PAGES_OK:
+            raise RuntimeError("There are not enough free pages for the prompt.")
+        try:
+            out = self.model(input_ids=ids[None], past_key_values=cache, use_cache=True)
+            for layer, prompt in enumerate(out.past_key_values.layers):
+                k, v = (t[0, :, held:].transpose(0, 1) for t in (prompt.keys, prompt.values))
+                self._store(k, k, v, step.positions, step.slots, *self.cache[layer])
+        except BaseException:
+            self._give_back(row, held)   # a prompt that fails leaves no pages behind
+            raise
+        return out.logits
+
+    def _give_back(self, row, held):
+        """Takes a row's pages back, but for its first `held` tokens' (whole
+        pages that it shares), and empties it."""
+        if held:
+            first = held // self.tables.page_size
+            own = self.tables.tables[row, first:].clone()
+            self.tables.tables[row, :own.shape[0]] = own
+            self.tables.lengths[row] -= held
+        done = torch.zeros(self.tables.requests, dtype=torch.bool, device=self.device)
+        done[row] = True
+        self.tables.release(done)
+
     @torch.no_grad()
-    def add(self, ids, mask=None):
+    def add_prefix(self, ids):
+        """Takes in a prefix (1-D token ids) that requests may begin with
+        and returns its number."""
+        ids = self._checked(ids)
+        if None not in self._prefixes:
+            raise RuntimeError("All prefixes' places are taken.")
+        number = self._prefixes.index(None)
+        self._take_in(self.requests + number, ids.to(self.device), DynamicCache(), 0)
+        self._groups["shared"][number] = ids.shape[0] // self.tables.page_size * self.tables.page_size
+        self._prefixes[number] = ids.to(self.device)
+        return number
+
+    def drop_prefix(self, number):
+        """Ends a prefix that no request begins with any more."""
+        if not 0 <= number < len(self._prefixes) or self._prefixes[number] is None:
+            raise ValueError(f"There is no prefix {number}.")
+        if number in self._prefix_of:
+            raise ValueError(f"Requests begin with prefix {number}.")
+        self._give_back(self.requests + number, 0)
+        self._prefixes[number] = None
+
+    def _prefix_cache(self, number):
+        """A prefix's keys and values, out of its pages, as the model's cache."""
+        cache, n, page = DynamicCache(), self._prefixes[number].shape[0], self.tables.page_size
+        pages = self.tables.tables[self.requests + number, :-(-n // page)].long()
+        for layer in range(len(self.layers)):
+            keys, values = (t[pages].transpose(0, 1).reshape(self.kv_heads, -1, self.dim)[None, :, :n]
+                            for t in self.cache[layer])
+            cache.update(keys, values, layer)
+        return cache
+
+    @torch.no_grad()
+    def add(self, ids, mask=None, prefix=None):
         """Takes in a prompt (1-D token ids), picks its first answer token
         and returns the request's place. `mask` (with `grammar`): the place's
-        row of `masks` from the first answer token on."""
-        ids = torch.as_tensor(ids, dtype=torch.int64)
-        if ids.dim() != 1 or not 0 < ids.shape[0] <= self.max_length or int(ids.min()) < 0 \
-                or int(ids.max()) >= self.vocab:
-            raise ValueError(f"A prompt is a vector of 1 to {self.max_length} token ids below {self.vocab}.")
+        row of `masks` from the first answer token on. `prefix`: the number of
+        a prefix that the prompt follows."""
+        if prefix is not None and (not 0 <= prefix < len(self._prefixes) or self._prefixes[prefix] is None):
+            raise ValueError(f"There is no prefix {prefix}.")
+        before = 0 if prefix is None else self._prefixes[prefix].shape[0]
+        ids = self._checked(ids, before)
         if mask is not None:
             if self.masks is None:
                 raise ValueError("A mask needs grammar=True.")
             if not torch.is_tensor(mask) or mask.dtype != torch.int32 or mask.shape != self.masks.shape[1:]:
                 raise ValueError(f"A mask is an int32 vector of {self.masks.shape[1]} words.")
-        ids, n = ids.to(self.device), ids.shape[0]
+        ids = ids.to(self.device)
         if all(self._taken):
             raise RuntimeError("All requests' places are taken.")
         place = self._taken.index(False)
-        new = torch.zeros(self.requests, dtype=torch.int32, device=self.device)
-        new[place] = n
-        step = self.tables.extend(new, n)
-        if int(step.status[place]) != serving.PAGES_OK:
-            raise RuntimeError("There are not enough free pages for the prompt.")
+        held = 0 if prefix is None else before // self.tables.page_size * self.tables.page_size
+        if held:
+            pages = held // self.tables.page_size
+            self.tables.tables[place, :pages] = self.tables.tables[self.requests + prefix, :pages]
+            self.tables.lengths[place] = held
+        # (a cache of its own: one that the model makes may keep a window only)
         try:
-            # (a cache of its own: one that the model makes may keep a window only)
-            out = self.model(input_ids=ids[None], past_key_values=DynamicCache(), use_cache=True)
-            for layer, prompt in enumerate(out.past_key_values.layers):
-                k, v = (t[0].transpose(0, 1) for t in (prompt.keys, prompt.values))
-                self._store(k, k, v, step.positions, step.slots, *self.cache[layer])
+            logits = self._take_in(place, ids, DynamicCache() if prefix is None else self._prefix_cache(prefix), before)
+        except BaseException:
+            self.tables.lengths[place] = 0
+            raise
+        try:
             if mask is not None:
                 self.masks[place] = mask.to(self.device)
-            self._history[place, :n] = ids.int()
+            n = before + ids.shape[0]
+            if before:
+                self._history[place, :before] = self._prefixes[prefix].int()
+            self._history[place, before:n] = ids.int()
             self._prompts[place] = n
             rows = torch.full((1,), place, dtype=torch.int32, device=self.device)
             contexts = torch.full((1,), n, dtype=torch.int32, device=self.device)
-            self._pick(out.logits[0, -1:], rows, contexts)
+            self._numbers(None)
+            self._pick(logits[0, -1:], rows, contexts)
         except BaseException:
-            self.tables.release(new > 0)   # a prompt that fails leaves no pages behind
+            self._give_back(place, held)   # a prompt that fails leaves no pages behind
             if mask is not None:
                 self.masks[place] = -1
             raise
+        if prefix is not None:
+            self._groups["groups"][place] = prefix
+            self._prefix_of[place] = prefix
         self._live[place] = 1
         self._taken[place] = True
         return place
@@ -187,13 +331,20 @@ class PagedDecoder:
                 raise ValueError(f"Place {place} holds no request.")
         if len(set(places)) < len(places):
             raise ValueError("A place is named twice.")
-        done = torch.zeros(self.requests, dtype=torch.bool, device=self.device)
+        done = torch.zeros(self.tables.requests, dtype=torch.bool, device=self.device)
         for place in places:
-            done[place] = True
+            prefix = self._prefix_of[place]
+            if prefix < 0:
+                done[place] = True
+            else:
+                page = self.tables.page_size
+                self._give_back(place, self._prefixes[prefix].shape[0] // page * page)
+                self._groups["groups"][place] = -1
+                self._prefix_of[place] = -1
+            self._live[place] = 0
+            if self.masks is not None:
+                self.masks[place] = -1
         self.tables.release(done)
-        self._live.masked_fill_(done, 0)
-        if self.masks is not None:
-            self.masks.masked_fill_(done[:, None], -1)
         for place in places:
             self._taken[place] = False
 
@@ -218,47 +369,89 @@ class PagedDecoder:
 
     @contextlib.contextmanager
     def _paged(self):
-        """Attention over the pages while a step runs."""
+        """Attention over the pages while a step runs, and the experts' products."""
         def forward(layer, attention):
             return lambda hidden_states, *args, **kwargs: self._attend(layer, attention, hidden_states, *args, **kwargs)
+
+        def mlp(experts):
+            return lambda hidden, index, weights: serving.expert_mlp(
+                hidden, index.contiguous(), weights.float().contiguous(), experts.gate_up_proj, experts.down_proj)
+        modules = self._attentions + self._experts
         # (some modules may have a forward of their own already, as wrapped ones do)
-        own = [attention.__dict__.get("forward") for attention in self._attentions]
+        own = [module.__dict__.get("forward") for module in modules]
         for layer, attention in enumerate(self._attentions):
             attention.forward = forward(layer, attention)
+        for experts in self._experts:
+            experts.forward = mlp(experts)
         try:
             yield
         finally:
-            for attention, before in zip(self._attentions, own):
+            for module, before in zip(modules, own):
                 if before is None:
-                    del attention.forward
+                    del module.forward
                 else:
-                    attention.forward = before
+                    module.forward = before
 
     def _run(self):
         """One step, all of it on the device."""
         # pages may reach past max_length; the rotary tables and the histories do not
-        asked = torch.where(self.tables.lengths < self.max_length, self._live, 0)
-        self.tables.extend(asked, self.requests, out=self._step)
+        room = self.max_length - self.tables.lengths
+        asked = torch.where(room > 0, self._live if not self._drafts_most else
+                            self._live * room.clamp(max=self._drafts_most + 1), 0)
+        self.tables.extend(asked, self._step.max_tokens, out=self._step)
         step = self._step
-        self._plan.update(step.contexts, requests=step.requests)
+        self._plan.update(step.contexts, requests=step.requests, **self._groups)
         body, rows = self.model.model, self._rows(step.requests)
-        hidden = body.embed_tokens(self._last[rows])[None]
+        fed = self._last[rows]
+        if self._drafts_most:
+            drafted = torch.cat((self._last[:-1, None], self._drafted), 1)
+            at = torch.arange(step.max_tokens, device=self.device) - step.starts[rows].long()
+            fed = torch.where(step.requests < 0, 0, drafted[rows.clamp(max=self.requests - 1),
+                                                            at.clamp(0, self._drafts_most)])
+        # (a draft that is no token is fed as one, and refused)
+        hidden = body.embed_tokens(fed.clamp(0, self.vocab - 1) if self._drafts_most else fed)[None]
         with self._paged():
             for layer in self.layers:
                 hidden = layer(hidden)
                 if isinstance(hidden, tuple):
                     hidden = hidden[0]
         logits = self.model.lm_head(body.norm(hidden))[0]
+        if self._drafts_most:
+            self._keep(logits, rows, fed)
+            return
         self._pick(logits, step.requests, step.contexts)
-        self._answers.copy_(torch.where(step.starts.diff() > 0, self._last[:self.requests], -1))
+        some = step.starts[:self.requests + 1].diff() > 0
+        self._answers.copy_(torch.where(some, self._last[:self.requests], -1))
+
+    def _keep(self, logits, rows, fed):
+        """Verifies a step's drafts, takes back what was stored for those
+        refused, and notes the answers."""
+        step, n = self._step, self.requests
+        # a row's history is what was fed up to it
+        self._history[rows, torch.where(step.requests < 0, 0, step.positions).long()] = fed.int()
+        logits = self._adjusted(logits, rows, step.requests, step.contexts)
+        self.logits = logits
+        starts = step.starts[:n + 1]
+        accepted, following = serving.verify_drafts(logits, fed, starts, self._accept, self._sample,
+                                                    temperature=self._temperatures)
+        count, following = starts.diff(), following.clamp(min=0)
+        kept = torch.where(count > 0, step.lengths[:n] - count + accepted + 1, step.lengths[:n])
+        self.tables.trim(torch.cat((kept, step.lengths[n:])))
+        some = count > 0
+        self._last[:n] = torch.where(some, following, self._last[:n])
+        owner = torch.where(some, torch.arange(n, device=self.device), n)   # (row n takes what is not to be written)
+        self._history[owner, torch.where(some, kept, 0).long()] = following.int()
+        place = torch.arange(self._drafts_most + 1, device=self.device)
+        drafted = torch.cat((self._drafted, following[:, None]), 1)
+        answers = torch.where(place < accepted[:, None], drafted, -1)
+        answers = torch.where(place == accepted[:, None], following[:, None], answers)
+        self._answers.copy_(torch.where(some[:, None], answers, -1))
 
     def _rows(self, requests):
         return torch.where(requests < 0, self.requests, requests).long()
 
-    def _pick(self, logits, requests, contexts):
-        """Adjusts the logits of tokens that make their requests `contexts`
-        long, and notes the likeliest next ones."""
-        rows = self._rows(requests)
+    def _adjusted(self, logits, rows, requests, contexts):
+        """The logits of rows of `requests` (-1: none) that make them `contexts` long."""
         adjust = {}
         if self._penalties:
             inside = rows.clamp(max=self.requests - 1)
@@ -266,19 +459,60 @@ class PagedDecoder:
                           lengths=contexts, prompt_lengths=self._prompts[inside])
         if self.masks is not None:
             adjust.update(masks=self.masks, mask_rows=requests)
-        if adjust:
-            logits = serving.adjust_logits(logits, **adjust)
-        self.logits = logits
-        best = logits.argmax(-1)
+        return serving.adjust_logits(logits, **adjust) if adjust else logits
+
+    def _pick(self, logits, requests, contexts):
+        """Adjusts the logits of tokens that make their requests `contexts`
+        long, one a request, and notes the likeliest next ones, or samples
+        them."""
+        rows = self._rows(requests)
+        self.logits = logits = self._adjusted(logits, rows, requests, contexts)
+        if self.temperature > 0:
+            # every row for itself, with its request's number
+            one = torch.arange(rows.shape[0] + 1, dtype=torch.int32, device=self.device)
+            at = rows.clamp(max=self.requests - 1)
+            _, best = serving.verify_drafts(logits, rows, one, self._accept[:rows.shape[0]], self._sample[at],
+                                            temperature=self._temperatures[at])
+            best = best.clamp(min=0)
+        else:
+            best = logits.argmax(-1)
         self._last.index_copy_(0, rows, best)
         place = rows * self._history.shape[1] + contexts.long()
         self._history.view(-1).index_copy_(0, place, best.int())
 
+    def _numbers(self, numbers):
+        """Takes the step's random numbers, or draws them."""
+        if numbers is None:
+            if self.temperature > 0:
+                self._accept.uniform_()
+                self._sample.uniform_()
+            return
+        for t, given in zip((self._accept, self._sample), numbers):
+            if given.shape != t.shape or given.dtype != t.dtype:
+                raise ValueError(f"numbers are float64 vectors of {self._accept.shape[0]} and {self.requests}.")
+        for t, given in zip((self._accept, self._sample), numbers):
+            t.copy_(given)
+
     @torch.no_grad()
-    def step(self):
-        """One new token for every request; returns the tokens (a new int64
-        tensor, by place). Requests at max_length, or for which no page is free, stay as
-        they are: -1, as in free places."""
+    def step(self, drafts=None, *, numbers=None):
+        """New tokens for every request; returns the tokens (a new int64
+        tensor): one by place, or, with `drafts`, up to drafts + 1 by place,
+        those accepted and the one after them, then -1. Requests at max_length,
+        or for which no page is free, stay as they are: -1, as in free places.
+
+        drafts (with the decoder's `drafts`): int64 (requests, drafts), by
+        place, what a request's text is taken to go on with, -1 for none; the
+        tokens after a -1 are not used. numbers: (accept, sample), float64 from
+        [0, 1), requests * (drafts + 1) and requests of them, in place of
+        torch's own."""
+        if drafts is not None:
+            if not torch.is_tensor(drafts) or drafts.shape != self._drafted.shape or drafts.dtype != torch.int64 \
+                    or not self._drafts_most:
+                raise ValueError(f"drafts are int64 ({self.requests}, {self._drafts_most}).")
+            self._drafted.copy_(drafts)
+        else:
+            self._drafted.fill_(-1)
+        self._numbers(numbers)
         if self._graph is not None:
             self._graph.replay()
             self.logits = self._graph_logits
@@ -300,10 +534,12 @@ class PagedDecoder:
             self.logits = before   # nothing has run yet: the last step's still
 
     def generate(self, prompts, new_tokens, *, capture=False):
-        """`new_tokens` greedy tokens for each prompt (as many prompts as
+        """`new_tokens` tokens for each prompt (as many prompts as
         there are free places); lists of token ids. `capture` replays the
         steps after the second from a HIP graph. Raises where the pages did
         not suffice for all."""
+        if self._drafts_most:
+            raise ValueError("generate() takes one token a step: it needs a decoder without drafts.")
         if new_tokens < 1 or any(len(p) + new_tokens - 1 > self.max_length for p in prompts):
             raise ValueError("Prompts and answers must fit max_length.")
         if len(prompts) > self._taken.count(False):
