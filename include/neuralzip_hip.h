@@ -919,8 +919,8 @@ typedef struct nz_route_args {
     uint32_t reserved;           /* 0 */
 } nz_route_args;
 
-/* Each token's top_k experts, the best first: by x . weight[e], or by its
- * sigmoid plus bias[e], the lower expert first where two are equal; NaN is
+/* Each token's top_k experts, the best first: by x . weight[e] or its
+ * sigmoid, plus bias[e], the lower expert first where two are equal; NaN is
  * never before another. Their weights are scale times the softmax over all
  * experts, or the sigmoids (without the bias), divided by their sum if
  * `normalize` (0 if that is 0). In 64 bits, weights rounded once. hidden is a

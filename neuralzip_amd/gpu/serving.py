@@ -653,10 +653,11 @@ def route_experts(x, weight, top_k, *, scoring="softmax", normalize=True, bias=N
     The scores are x (tokens, hidden) times the rows of weight (experts,
     hidden; in x's dtype or float32). With `scoring` "softmax" the largest are
     chosen and weighted by their softmax over all experts; with "sigmoid"
-    those of the largest sigmoid plus `bias` (float32, experts), weighted by
-    the sigmoid. `normalize` divides a token's weights by their sum; `scale`
-    multiplies them. Of equal experts the lower one is first, and NaN is never
-    before another. In 64 bits, rounded once. hidden is a multiple of 8; at
+    those of the largest sigmoid, weighted by it. `bias` (float32, experts) is
+    added to what is compared, not to the weights. `normalize` divides a
+    token's weights by their sum; `scale` multiplies them. Of equal experts the
+    lower one is first, and NaN is never before another. In 64 bits, rounded
+    once. hidden is a multiple of 8; at
     most 1024 experts, 32 of them chosen, and 65535 tokens."""
     if torch.is_grad_enabled():
         _refuse_gradients(x, weight, bias)

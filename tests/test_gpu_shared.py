@@ -226,6 +226,48 @@ def test_a_captured_plan_follows_its_contexts():
         assert torch.equal(out, serving.paged_attention(q, keys, values, tables, eager))
 
 
+def test_plans_of_no_rows_and_no_groups():
+    none = ints([])
+    plan = serving.SharedPlan(none, heads=4, kv_heads=2, requests=none)
+    q, caches = randn(0, 4, 64), [randn(3, 2, 16, 64) for _ in range(2)]
+    assert serving.paged_attention(q, *caches, ints([[0, 1]]), plan).shape == (0, 4, 64)
+    q = randn(2, 4, 64, seed=1)
+    one = serving.SharedPlan(ints([20, 9]), heads=4, kv_heads=2, groups=ints([-1, 7]), shared=none)
+    two = serving.AttentionPlan(ints([20, 9]), heads=4, kv_heads=2)
+    tables = ints([[0, 1], [2, 0]])
+    got, want = (serving.paged_attention(q, *caches, tables, plan) for plan in (one, two))
+    assert (got - want).abs().max() <= 2.0 ** -18 * caches[1].abs().max()
+
+
+@pytest.mark.parametrize("change, message", [
+    (dict(contexts=[3, 4, 5]), "contexts"), (dict(requests=[0]), "requests"), (dict(groups=[0]), "groups"),
+    (dict(shared=[1, 2]), "shared"), (dict(groups=None, shared=None), "as when the plan was made")])
+def test_updates_of_other_sizes_are_refused(change, message):
+    given = dict(contexts=[3, 4], requests=[0, 1], groups=[0, 0], shared=[2])
+    plan = serving.SharedPlan(**{k: ints(v) for k, v in given.items()}, heads=2, kv_heads=1)
+    with pytest.raises(ValueError, match=message):
+        plan.update(**{k: None if v is None else ints(v) for k, v in dict(given, **change).items()})
+
+
+def test_refusals_that_need_the_device():
+    with pytest.raises(ValueError, match="2048 rows"):
+        serving.SharedPlan(ints([1] * 2049), heads=2, kv_heads=1)
+    with pytest.raises(ValueError, match="go together"):
+        serving.SharedPlan(ints([1]), heads=2, kv_heads=1, groups=ints([0]))
+    with pytest.raises(ValueError, match="vectors"):
+        serving.SharedPlan(ints([1]), heads=2, kv_heads=1, groups=ints([[0]]), shared=ints([1]))
+    plan = serving.SharedPlan(ints([1, 2]), heads=2, kv_heads=1)
+    q, caches, tables = randn(2, 2, 64), [randn(3, 1, 16, 64) for _ in range(2)], ints([[0], [1]])
+    with pytest.raises(ValueError, match="q must be"):
+        serving.paged_attention(randn(3, 2, 64), *caches, tables, plan)
+    with pytest.raises(ValueError, match="Caches must"):
+        serving.paged_attention(q, caches[0], caches[1][:2], tables, plan)
+    with pytest.raises(ValueError, match="tables must"):
+        serving.paged_attention(q, *caches, tables.long(), plan)
+    with pytest.raises(ValueError, match="no backward"):
+        serving.paged_attention(q.clone().requires_grad_(), *caches, tables, plan)
+
+
 def test_a_side_stream():
     q, keys, values, tables, _, contexts, of, groups = shared_case(torch.bfloat16, 8, 2, 64, 16, MIXED)
     extra = dict(groups=ints(groups), shared=ints([48, 80, 32]))

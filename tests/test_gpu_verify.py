@@ -292,3 +292,21 @@ def test_a_side_stream():
     got = serving.verify_drafts(*state, draft_probs=drafts, stream=side)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("change, message", [
+    (dict(logits=torch.zeros(4, 10)), "logits"),
+    (dict(tokens="short"), "tokens"), (dict(accept="float"), "accept"), (dict(sample="short"), "sample"),
+    (dict(starts="long"), "starts"), (dict(draft_probs="half"), "draft_probs"), (dict(temperature="short"), "temperature")])
+def test_refusals_that_need_the_device(change, message):
+    f64 = torch.float64
+    state = dict(logits=torch.zeros(4, 10, device=DEVICE), tokens=torch.zeros(4, dtype=torch.int64, device=DEVICE),
+                 starts=torch.tensor([0, 2, 4], dtype=torch.int32, device=DEVICE),
+                 accept=torch.zeros(4, dtype=f64, device=DEVICE), sample=torch.zeros(2, dtype=f64, device=DEVICE),
+                 draft_probs=torch.zeros(4, 10, device=DEVICE), temperature=torch.ones(2, device=DEVICE))
+    for name, how in change.items():
+        t = state[name]
+        state[name] = how if torch.is_tensor(how) else \
+            {"short": t[:-1], "float": t.float(), "long": t.long(), "half": t.half()}[how]
+    with pytest.raises(ValueError, match=message):
+        serving.verify_drafts(**state)
