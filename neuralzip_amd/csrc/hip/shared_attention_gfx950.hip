@@ -617,7 +617,7 @@ __global__ __launch_bounds__(kJoinThreads) void nz_shared_join_kernel(nz_shared_
         const uint32_t run = i % runs, sub = i / runs, h = run / quads, d = run % quads * 4;
         const uint32_t k0 = sub * n / subs, k1 = (sub + 1) * n / subs;
         Sums s = {{}, -__builtin_inff(), 0.0f, {}};
-        constexpr uint32_t kBatch = 16;
+        constexpr uint32_t kBatch = 8;
         for (uint32_t k = k0; k < k1; k += kBatch) {
             vec<float, 2> ml[kBatch];
             f32x4 x[kBatch];
