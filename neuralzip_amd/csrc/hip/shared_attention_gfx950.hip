@@ -196,13 +196,14 @@ __global__ __launch_bounds__(kPlanThreads) void nz_shared_plan_kernel(nz_shared_
     const uint32_t whole_rounds = cuts(max(a.target, pieces), a.target) * a.target;
     const uint32_t limit = min(a.n_groups ? whole_rounds + whole_rounds / 2 : whole_rounds, a.n_items);
     uint32_t lo = kLeastItem / kTile, hi = max((longest + kTile - 1) / kTile, lo);
-    const auto count_items = [&](uint32_t share) {   // a wavefront's sum
-        uint32_t sum = 0;
+    const auto group_share = [](uint32_t share) { return share < 1u << 30 ? kGroupLength * share : share; };
+    const auto count_items = [&](uint32_t share) {   // a wavefront's sum, or as much as is too many
+        uint64_t sum = 0;
         for (uint32_t i = lane; i < n; i += 64)
             sum += cuts(lds.own[i], share) + max(cuts(lds.tail[i], share), lds.context[i] == 0 ? 1u : 0u);
         for (uint32_t g = lane; g < a.n_groups; g += 64)
-            sum += cuts(lds.members[g], tile_rows) * cuts(lds.shared[g], kGroupLength * share);
-        return last_lane(wave_scan(sum));
+            sum += static_cast<uint64_t>(cuts(lds.members[g], tile_rows)) * cuts(lds.shared[g], group_share(share));
+        return last_lane(wave_scan(static_cast<uint32_t>(min<uint64_t>(sum, 1u << 25))));
     };
     while (lo < hi) {
         const uint32_t step = (hi - lo + kPlanWaves) / (kPlanWaves + 1);
@@ -224,7 +225,7 @@ __global__ __launch_bounds__(kPlanThreads) void nz_shared_plan_kernel(nz_shared_
         return max((cuts(length, count) + kTile - 1) / kTile * kTile, kTile);
     };
     const auto items_of = [&](uint32_t length) { return cuts(length, each_of(length, share)); };
-    const auto group_each = [&](uint32_t g) { return each_of(lds.shared[g], kGroupLength * share); };
+    const auto group_each = [&](uint32_t g) { return each_of(lds.shared[g], group_share(share)); };
     const auto group_items = [&](uint32_t g) { return cuts(lds.shared[g], group_each(g)); };
     __syncthreads();
     // first items, kind by kind

@@ -157,6 +157,21 @@ def test_plans_cover_every_row_and_key_once():
                 assert row[:n] == [1] * n
 
 
+@pytest.mark.parametrize("rows, shared", [(2, None), (2048, None), (2, 2 ** 31 - 1), (2048, 2 ** 31 - 1), (300, 2 ** 30 + 5)])
+def test_plans_of_the_longest_contexts(rows, shared):
+    """Counts of items and ends of keys stay inside 32 bits. (Only planned.)"""
+    extra = dict(groups=ints([0] * rows), shared=ints([shared])) if shared else {}
+    plan = serving.SharedPlan(ints([2 ** 31 - 1] * rows), heads=8, kv_heads=8, **extra)
+    order, seen = plan.order.tolist(), [[] for _ in range(rows)]
+    for member, n, _, begin, end, _, _, _ in plan.items.tolist():
+        for row in order[member:member + n]:
+            seen[row].append((begin, end))
+    for items in seen:
+        items.sort()
+        assert items[0][0] == 0 and items[-1][1] == 2 ** 31 - 1
+        assert all(a[1] == b[0] for a, b in zip(items, items[1:]))
+
+
 def test_what_is_not_finite_stays_where_it_is_seen():
     """A key that one row sees and its neighbour does not may have any value."""
     q, keys, values, tables, host, contexts, of, _ = shared_case(torch.bfloat16, 4, 1, 64, 16, [(-1, 0, 45, 4)] * 2)
