@@ -11,8 +11,9 @@
  *     thread-local message from nz_last_error();
  *   - host functions are re-entrant; nz_decode_launch, nz_matvec_launch,
  *     nz_matvec_reduce, nz_matvec_rows and the serving-step operators
- *     (nz_pages_*, nz_rotary_store, nz_attention_*, nz_adjust_logits) are
- *     asynchronous and ordered on the given HIP stream.
+ *     (nz_pages_*, nz_rotary_store, nz_attention_*, nz_shared_*,
+ *     nz_adjust_logits, nz_verify_drafts, nz_route_experts, nz_expert_mlp)
+ *     are asynchronous and ordered on the given HIP stream.
  */
 #ifndef NEURALZIP_HIP_H
 #define NEURALZIP_HIP_H
@@ -503,8 +504,9 @@ int nz_clusterer_count(const nz_clusterer* clusterer, uint32_t* n_clusters);
 
 /* One step of many requests whose lengths differ, around the decoded
  * weights: pages for the step's tokens, rotation of queries and keys with
- * the store into the pages, attention over them, and the logits'
- * adjustments. No counterpart in the reference, whose forwards keep
+ * the store into the pages, attention over them (shared prefixes read once),
+ * mixture-of-experts layers, the logits' adjustments and the verification of
+ * drafted tokens. No counterpart in the reference, whose forwards keep
  * Transformers' own cache and attention (gpu/inference.py:476-509).
  *
  * The key-value cache of a layer is two arrays (keys, values) of n_pages

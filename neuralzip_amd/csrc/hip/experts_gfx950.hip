@@ -37,7 +37,8 @@ __device__ __forceinline__ void load_eight(const T* src, float (&x)[8]) {
 // Tokens' products with the experts' rows, a wavefront each, summed in 64 bits
 // so that the choice does not depend on their order. (Both steps in one
 // workgroup per token took 22 us for one token of 2048 elements and 128
-// experts, which one compute unit multiplied.)
+// experts, which one compute unit multiplied; this 4.6, the latency of one
+// row, and as much for 32 tokens of 4096 elements and 8.)
 template <typename T, typename W>
 __global__ __launch_bounds__(kScoreThreads) void nz_route_scores_kernel(nz_route_args a) {
     const uint32_t token = blockIdx.y, lane = threadIdx.x & 63, e = blockIdx.x * kScoreWaves + (threadIdx.x >> 6);
@@ -207,7 +208,11 @@ __device__ __forceinline__ float activate(uint32_t kind, float x) {
 // The gated activations of one expert's tokens, for kRows of its inner
 // elements: act(gate x) * (up x), in 32 bits. Weight rows are the rows of the
 // matrix instructions and tokens their columns, in up to NB blocks; the
-// wavefronts share the depth.
+// wavefronts share the depth. Bound by the weights' way from memory: 8 experts
+// of 14336 x 4096 bf16 elements for 32 tokens in 366 us (5.1 TB/s); 8 of 768 x
+// 2048 for one token in 13.6 (3.7), of which some 3.5 go by before the choice
+// is known. (With batches of 8 pieces that layer took 40.9 us instead of 36.6,
+// with registers for four wavefronts a SIMD the wide one 654 instead of 546.)
 template <typename T, uint32_t NB>
 __global__ __launch_bounds__(kUpThreads) void nz_expert_up_kernel(nz_expert_args a, float* __restrict__ acts,
                                                                   uint32_t* __restrict__ counters, uint32_t n_counters) {
@@ -330,7 +335,9 @@ __device__ __forceinline__ int split(const float (&x)[Piece<T>::kRun], typename 
 // elements, each wavefront a share of them in a row, with the tokens that
 // chose an expert as columns; the columns of an expert are added to their
 // tokens' sums, times the weights, when it ends. `splits` workgroups share the
-// experts; the last to arrive adds their sums in order.
+// experts; the last to arrive adds their sums in order. Bound by the weights'
+// way from memory and, for few tokens, by the latencies of the choice and of
+// the last sums: 212 us (4.4 TB/s) and 12.0 us for the layers above.
 template <typename T, uint32_t NB>
 __global__ __launch_bounds__(kDownThreads) void nz_expert_down_kernel(nz_expert_args a, const float* __restrict__ acts,
                                                                       float* __restrict__ partials,
