@@ -342,7 +342,9 @@ constexpr uint32_t kBlocks = kColumns / 16;
 // 252 us (without its rows' own keys) with the wavefronts sharing tiles and
 // taking a block of columns each, 271 to 282 with keys passed through LDS and
 // 327 with values; leaving out the rescaling where no maximum rose, the masks
-// inside items, and items of groups and rows in turn changed nothing.
+// inside items, and items of groups and rows in turn changed nothing. Three
+// workgroups a compute unit (queries in LDS, half of the sums there at a time,
+// keys asked for after the softmax) took 297, two of such ones 275.
 template <typename T, uint32_t DP, bool FULL>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 128 && sizeof(T) == 2 ? 2 : 1)))
 void nz_shared_attention_kernel(nz_shared_attention_args a) {

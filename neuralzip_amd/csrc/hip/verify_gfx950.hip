@@ -220,7 +220,7 @@ __device__ __forceinline__ void wave_largest(Part& a) {
 // One chunk of one row. Bound by the vector units, some 20 instructions of 64
 // bits a logit: 240 rows of 128256 fp32 logits in 37 us (3.3 TB/s; the units
 // are busy 63 % of the time), 104 in bf16 in 16. Several chunks a workgroup,
-// each read ahead, took as long.
+// each read ahead, took as long, as did registers for eight wavefronts a SIMD.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void nz_verify_rows_kernel(nz_verify_args a, Part* __restrict__ parts) {
     __shared__ float tops[kWaves];
