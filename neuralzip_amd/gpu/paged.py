@@ -396,8 +396,11 @@ class PagedDecoder:
         """One step, all of it on the device."""
         # pages may reach past max_length; the rotary tables and the histories do not
         room = self.max_length - self.tables.lengths
-        asked = torch.where(room > 0, self._live if not self._drafts_most else
-                            self._live * room.clamp(max=self._drafts_most + 1), 0)
+        wanted = self._live
+        if self._drafts_most:
+            given = (self._drafted >= 0).int().cumprod(1).sum(1, dtype=torch.int32)
+            wanted = wanted * torch.nn.functional.pad(given + 1, (0, self.tables.requests - self.requests)).minimum(room)
+        asked = torch.where(room > 0, wanted, 0)
         self.tables.extend(asked, self._step.max_tokens, out=self._step)
         step = self._step
         self._plan.update(step.contexts, requests=step.requests, **self._groups)
@@ -498,7 +501,8 @@ class PagedDecoder:
         """New tokens for every request; returns the tokens (a new int64
         tensor): one by place, or, with `drafts`, up to drafts + 1 by place,
         those accepted and the one after them, then -1. Requests at max_length,
-        or for which no page is free, stay as they are: -1, as in free places.
+        or without free pages for a token and their drafts, stay as they are:
+        -1, as in free places.
 
         drafts (with the decoder's `drafts`): int64 (requests, drafts), by
         place, what a request's text is taken to go on with, -1 for none; the

@@ -179,6 +179,28 @@ def test_drafts_up_to_max_length(device):
     assert (out == -1).all() and decoder.tables.lengths.tolist() == [14, 0] and torch.equal(keys, decoder.cache)
 
 
+def test_drafts_ask_for_the_pages_of_those_given(device):
+    """A request asks for room for its drafts, not for as many as it might
+    bring: without any it takes the last place of its last page."""
+    model = small_model(device)
+    text = prompt(10, 1).tolist()
+    answer = greedy(model, [text], 12)[0]
+    decoder = PagedDecoder(model, requests=2, max_length=80, drafts=4, page_size=16, num_pages=1)
+    decoder.add(text)
+    got = [int(decoder.tokens[0])]
+    for n, fits in ((4, True), (4, False), (1, False), (0, True), (0, False)):   # 10 tokens, then 15, then 16
+        drafts = torch.full((2, 4), -1)
+        drafts[0, :n] = torch.tensor(answer[len(got):len(got) + n])
+        lengths = decoder.tables.lengths.tolist()
+        out = decoder.step(drafts.to(device))[0].tolist()
+        new = answer[len(got):len(got) + n + 1] if fits else []
+        assert out == new + [-1] * (5 - len(new))
+        got += new
+        assert decoder.tables.lengths.tolist() == [lengths[0] + len(new), 0]
+        check_free_pages(decoder)
+    assert got == answer[:7]
+
+
 def test_drafts_with_penalties_see_the_drafts_before_them(device):
     model = small_model(device)
     texts = [prompt(6, 1).tolist()]
