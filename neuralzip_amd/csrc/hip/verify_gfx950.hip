@@ -46,22 +46,23 @@ struct Decision {
 __host__ __device__ __forceinline__ uint32_t chunks_of(uint32_t vocab) { return (vocab + kChunk - 1) / kChunk; }
 
 // Weights are held times 2^60, so that the smallest that 64 bits hold beside a
-// largest of 1 are normal numbers.
+// largest of 1 are normal numbers. Those of 2^-kReach and less are 0, as 64
+// bits would round them.
 constexpr double kUnit = 0x1p60;
-constexpr double kReach = 1074.0;    // its log2
+constexpr double kReach = 1075.0;
 
 // How a row's logits are weighed: exp((x - top) / temperature) where `top` is
 // the largest, and the first of the largest alone where the temperature is not
 // above 0.
 struct Scale {
-    double rate;        // log2(e) / temperature; 0: greedy
+    double rate;        // log2(e) / temperature (an infinite one: so small that every number weighs as much); 0: greedy
     // The Taylor series of 2^f, (ln 2)^k / k!, kept in scalar registers (as
     // literals each takes two moves into vector registers).
     static constexpr uint32_t kTerms = 13;
     double series[kTerms];
 
     __device__ __forceinline__ explicit Scale(float temperature)
-        : rate(temperature > 0.0f ? 1.44269504088896340736 / static_cast<double>(fminf(temperature, 3.4e38f)) : 0.0) {
+        : rate(temperature > 0.0f ? 1.44269504088896340736 / fmin(static_cast<double>(temperature), 1e300) : 0.0) {
         double term = kUnit;
 #pragma unroll
         for (uint32_t k = 0; k < kTerms; ++k) {
@@ -71,19 +72,13 @@ struct Scale {
         }
     }
     __device__ __forceinline__ bool greedy() const { return rate == 0.0; }
-    // What logits have to be above for a weight: nothing below it rounds to one, and the series' exponents stay
-    // inside 64 bits, whichever way this is rounded.
-    __device__ __forceinline__ float floor_of(float top) const {
-        const float reach = static_cast<float>(fmin(kReach / rate, 3e38));
-        const float below = top - fmaxf(fabsf(top) * 0x1p-23f, 0x1p-149f);   // the next number, or the one after
-        return fminf(top - reach + fabsf(top) * 0x1p-22f, below);
-    }
     // 2^y, y = (x - top) rate <= 0, to 2 units of the last place: y's whole
     // part, the low bits of a sum with 1.5 * 2^52, as the exponent, and the
     // series for the rest, |f| <= 1/2, whose next term is below 2^-52. The
     // library's exp takes four times as long, and most of the call's time was
-    // spent in it.
-    __device__ __forceinline__ double finite(float x, float top, float floor) const {
+    // spent in it. The cut is by y itself: past it the whole part would not
+    // stay inside the exponent, however near x is to top.
+    __device__ __forceinline__ double finite(float x, float top) const {
         const double y = (static_cast<double>(x) - static_cast<double>(top)) * rate;
         const double shifted = y + 0x1.8p52, f = y - (shifted - 0x1.8p52);
         double p = series[kTerms - 1];
@@ -91,7 +86,7 @@ struct Scale {
         for (uint32_t k = kTerms - 1; k-- > 0;) p = fma(p, f, series[k]);
         vec<uint32_t, 2> bits = __builtin_bit_cast(vec<uint32_t, 2>, p);
         bits.y += __builtin_bit_cast(vec<uint32_t, 2>, shifted).x << 20;
-        return x > floor ? __builtin_bit_cast(double, bits) : 0.0;
+        return y > -kReach ? __builtin_bit_cast(double, bits) : 0.0;
     }
     // the weights of some logits (NaN has none)
     template <uint32_t N>
@@ -100,9 +95,8 @@ struct Scale {
 #pragma unroll
             for (uint32_t i = 0; i < N; ++i) w[i] = x[i] == top ? kUnit : 0.0;
         } else {
-            const float floor = floor_of(top);
 #pragma unroll
-            for (uint32_t i = 0; i < N; ++i) w[i] = finite(x[i], top, floor);
+            for (uint32_t i = 0; i < N; ++i) w[i] = finite(x[i], top);
         }
     }
     __device__ __forceinline__ double operator()(float x, float top) const {

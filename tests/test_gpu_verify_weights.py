@@ -1,0 +1,74 @@
+"""verify_drafts where weights are at the ends of 64 bits, against the
+definition in 64 bits: logits next to one another at low temperatures, logits
+as far apart as 32 bits allow at high ones. Results are whole numbers and have
+to be equal."""
+import itertools
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_verify import check, run
+
+pytestmark = pytest.mark.gpu
+
+MOST = float(np.finfo(np.float32).max)
+# Some whose neighbour below is half of 2^-23 of them away, some of which it is
+# nearly all; negative ones, a subnormal one and those at both ends.
+TOPS = [16.0, 12.0, 1.75, 1.0, 100.0, 30.0, 1e6, 1.5e10, 3e38, -16.0, -12.0, -1e6, 1e-40, 2.0 ** -126, 0.0, MOST]
+TEMPERATURES = [1e-6, 1e-7, 1e-8, 1e-9, 1e-10, 1e-12, 1e-20, 1e-38, 1e-45, 1.0]
+
+
+def below(top, steps):
+    x = np.float32(top)
+    for _ in range(steps):
+        x = np.nextafter(x, np.float32(-np.inf))
+    return float(x)
+
+
+@pytest.mark.parametrize("top", TOPS)
+@pytest.mark.parametrize("place", [3, 5000])
+def test_logits_next_to_the_largest(top, place):
+    """The runner-up one and two steps below, in the largest one's chunk and in
+    another: as a row of its own, and behind a draft of the largest, which is
+    accepted by its number or refused by it."""
+    for steps, t in itertools.product((1, 2), TEMPERATURES):
+        row = torch.full((3, 5003), -math.inf)
+        row[:, 1], row[:, place], row[:, 2] = top, below(top, steps), below(top, 3 * steps)
+        for u in (0.0, 0.4, 0.6, 0.99):
+            check(row[:1], [0], [0, 1], [0.0], [u], temperature=[t])
+            for draft, accept in ((1, 0.4), (1, 1.0), (place, 0.0), (place, 0.9)):
+                check(row, [0, draft, 1], [0, 3], [accept, 0.3, 0.0], [u], temperature=[t])
+                q = np.zeros((3, 5003), dtype=np.float32)
+                q[:, 1], q[:, place] = 0.5, 0.25
+                check(row, [0, draft, 1], [0, 3], [accept, 0.3, 0.0], [u], q, [t])
+
+
+def test_the_last_weights_that_64_bits_hold():
+    """Behind the refusal of the largest logit (by a number that is not below
+    1) its runner-up is picked as long as it has a weight."""
+    row = torch.zeros(2, 5000)
+    for place, gap in itertools.product((7, 4999), (700.0, 744.0, 745.0, 745.5, 746.0, 2000.0, 1e30)):
+        row[:], row[:, 1], row[:, place] = -math.inf, 0.0, -gap
+        assert run(row, [0, 1], [0, 2], [1.0, 0.0], [0.5]) == ([0], [place if gap < 745.2 else 1])
+
+
+@pytest.mark.parametrize("t", [1e38, 3e38, 3.4e38, MOST])
+def test_logits_far_apart_at_high_temperatures(t):
+    rng = np.random.default_rng(1)
+    row = torch.from_numpy(rng.uniform(-3.4e38, 3.4e38, (4, 300)).astype(np.float32))
+    row[:, 7], row[:, 9], row[:, 11] = MOST, -MOST, -math.inf
+    for u in rng.random(20):
+        check(row, [0, 9, 9, 5], [0, 2, 4], [0.001, 0.0, 0.9, 0.5], [u, 1 - u], temperature=[t, t])
+    two = torch.tensor([[3e38, -3e38]])
+    share = 1 / (1 + math.exp(-6e38 / float(np.float32(t))))
+    for u in (share - 1e-5, share + 1e-5):
+        assert run(two, [0], [0, 1], [0.0], [u], temperature=[t]) == ([0], [int(u > share)])
+
+
+def test_an_infinite_temperature():
+    """Every finite logit is as likely as any other."""
+    row = torch.tensor([[3e38, -3e38, -math.inf, 0.0, math.nan, 1.0]])
+    for i, token in enumerate((0, 1, 3, 5)):
+        assert run(row, [0], [0, 1], [0.0], [i / 4 + 0.01], temperature=[math.inf]) == ([0], [token])
