@@ -246,8 +246,8 @@ __global__ __launch_bounds__(kThreads) void nz_verify_rows_kernel(nz_verify_args
             if (x[i] == top && v + i < a.vocab) part.first = v + i;
         // (lanes hold rising tokens)
         const uint64_t bits = __ballot(part.first != kNone);
-        if (lane == 0) firsts[wave] = kNone;
-        if (bits != 0 && lane == __builtin_ctzll(bits)) firsts[wave] = part.first;
+        const uint32_t first = __shfl(part.first, bits ? __builtin_ctzll(bits) : 0);
+        if (lane == 0) firsts[wave] = first;
         __syncthreads();
         part.first = kNone;
 #pragma unroll

@@ -72,3 +72,17 @@ def test_an_infinite_temperature():
     row = torch.tensor([[3e38, -3e38, -math.inf, 0.0, math.nan, 1.0]])
     for i, token in enumerate((0, 1, 3, 5)):
         assert run(row, [0], [0, 1], [0.0], [i / 4 + 0.01], temperature=[math.inf]) == ([0], [token])
+
+
+def test_the_first_of_the_largest_wherever_it_lies():
+    """Without a temperature, in every thread of a chunk, alone and with equals
+    behind it in its own wavefront, the next ones and the next chunk."""
+    for behind in (None, 1, 700, 3000, 4096):
+        row = torch.zeros(513, 9000)
+        places = [8 * i + i % 8 for i in range(513)]
+        for i, place in enumerate(places):
+            row[i, place] = 2.0
+            if behind is not None:
+                row[i, place + behind] = 2.0
+        got = run(row, [0] * 513, list(range(514)), [0.0] * 513, [0.9] * 513, temperature=[0.0] * 513)
+        assert got == ([0] * 513, places)
