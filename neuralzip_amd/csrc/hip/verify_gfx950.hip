@@ -485,7 +485,8 @@ void nz_verify_pick_kernel(nz_verify_args a, const Part* __restrict__ parts, con
     }
     // the token: the first with a weight at which the sum passes what is wanted, or the chunk's last
     const uint32_t v = chunk * kChunk + threadIdx.x * kPickEach;
-    double sum = scan(weigh<T>(a, d, kind, scale, v, w)) + before_chunk;
+    double sum = scan(weigh<T>(a, d, kind, scale, v, w));   // its barriers come before before_chunk is read
+    sum += before_chunk;
     mine_first = kNone, mine_last = 0;
 #pragma unroll
     for (uint32_t i = 0; i < kPickEach; ++i) {

@@ -86,3 +86,14 @@ def test_the_first_of_the_largest_wherever_it_lies():
                 row[i, place + behind] = 2.0
         got = run(row, [0] * 513, list(range(514)), [0.0] * 513, [0.9] * 513, temperature=[0.0] * 513)
         assert got == ([0] * 513, places)
+
+
+def test_tokens_in_every_chunk():
+    """Equal weights: the token is the number's place, in each of a row's chunks,
+    whose sums of those before another thread hands on."""
+    vocab, step = 1 << 16, 1021
+    tokens = list(range(0, vocab, step))
+    n = len(tokens)
+    row = torch.zeros(n, vocab, dtype=torch.bfloat16)
+    got = run(row, [0] * n, list(range(n + 1)), [0.0] * n, [t / vocab for t in tokens])
+    assert got == ([0] * n, tokens)
