@@ -303,7 +303,11 @@ __global__ __launch_bounds__(kUpThreads) void nz_expert_up_kernel(nz_expert_args
 // Activations as two pieces whose sum they are to 16 or 22 bits: one rounding
 // to a weight's type would err as much as the result's own. fp16 pieces are
 // those of the activations divided by 2^lift, so that neither large nor small
-// ones leave fp16's range.
+// ones leave fp16's range, whatever is infinite beside them. Beside a head the
+// rest has its sign and is kept from being 0 (which errs by at most 2^-23 of the
+// largest of the 32), so that an infinite weight or activation is infinite in
+// both products; an activation below 2^-24 of the largest is all rest, and may
+// be 0.
 template <typename T>
 __device__ __forceinline__ int split(const float (&x)[Piece<T>::kRun], typename Piece<T>::type& hi,
                                      typename Piece<T>::type& lo) {
@@ -318,15 +322,15 @@ __device__ __forceinline__ int split(const float (&x)[Piece<T>::kRun], typename 
         float most = 0.0f;
 #pragma unroll
         for (uint32_t i = 0; i < kRun; ++i) most = fmaxf(most, fabsf(x[i]));
-        most = column_max(most);
+        most = fminf(column_max(most), 0x1.fffffep127f);
         lift = __builtin_amdgcn_frexp_expf(most);
     }
 #pragma unroll
     for (uint32_t i = 0; i < kRun; ++i) {
         const float y = std::is_same<T, _Float16>::value ? __builtin_amdgcn_ldexpf(x[i], -lift) : x[i];
         hi[i] = Piece<T>::head(y);
-        const float head = static_cast<float>(hi[i]), rest = y - head;
-        lo[i] = static_cast<T>(fabsf(head) < __builtin_inff() ? rest : 0.0f);
+        const float head = static_cast<float>(hi[i]);
+        lo[i] = static_cast<T>(copysignf(__builtin_amdgcn_fmed3f(fabsf(y - head), fabsf(head), Piece<T>::kLeast), y));
     }
     return lift;
 }
