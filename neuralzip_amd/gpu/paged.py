@@ -490,10 +490,11 @@ class PagedDecoder:
                 self._accept.uniform_()
                 self._sample.uniform_()
             return
-        for t, given in zip((self._accept, self._sample), numbers):
-            if given.shape != t.shape or given.dtype != t.dtype:
-                raise ValueError(f"numbers are float64 vectors of {self._accept.shape[0]} and {self.requests}.")
-        for t, given in zip((self._accept, self._sample), numbers):
+        own, numbers = (self._accept, self._sample), tuple(numbers)
+        if len(numbers) != 2 or any(not torch.is_tensor(given) or given.shape != t.shape or given.dtype != t.dtype
+                                    for t, given in zip(own, numbers)):
+            raise ValueError(f"numbers are float64 vectors of {self._accept.shape[0]} and {self.requests}.")
+        for t, given in zip(own, numbers):
             t.copy_(given)
 
     @torch.no_grad()
