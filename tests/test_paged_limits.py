@@ -6,7 +6,7 @@ import torch
 
 import plain_more_serving
 from neuralzip_amd.gpu.paged import PagedDecoder
-from test_paged_decoder import prompt, small_model
+from test_paged_decoder import MOE, VOCAB, prompt, small_model
 
 
 @pytest.fixture(params=["cpu", pytest.param("cuda:0", marks=pytest.mark.gpu)])
@@ -33,3 +33,45 @@ def test_numbers_are_two(device, count):
     decoder.step(numbers=given[:2])
     decoder.step(numbers=list(given[:2]))
     assert decoder.tables.lengths.tolist() == [lengths[0] + 2, 0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind, more", [("llama", {}), ("qwen3_moe", dict(experts=True))])
+def test_compressed_weights_behind_prefixes_and_drafts(kind, more):
+    """bfloat16 weights decoded on the fly by the runtime: the same tokens as
+    without it, since the decode is bit-exact, eagerly and from a graph, with
+    prefixes, drafts, sampling and experts."""
+    from neuralzip_amd.gpu.inference import NeuralZipRuntime, export_model_for_gpu
+    from neuralzip_amd.setup import NeuralZipSetup
+    device = "cuda:0"
+    model = small_model(device, kind, **(dict(MOE, head_dim=32) if more else {})).bfloat16()
+
+    def answers(capture):
+        decoder = PagedDecoder(model, requests=3, max_length=100, drafts=2, prefixes=1, temperature=0.9, **more)
+        prefix = decoder.add_prefix(prompt(40, 1))
+        torch.manual_seed(2)
+        for n, seed, behind in ((3, 2, prefix), (20, 3, prefix), (9, 4, None)):
+            decoder.add(prompt(n, seed), prefix=behind)
+        out = [decoder.tokens.tolist()]
+        for turn in range(9):
+            if turn == 3 and capture:
+                decoder.capture()
+            g = torch.Generator(device=device).manual_seed(turn)
+            drafts = torch.randint(-1, VOCAB, (3, 2), generator=g, device=device)
+            drafts[0] = decoder.tokens[0]
+            # (by numbers of 0 every draft that has a chance is accepted)
+            numbers = ((0.0 if turn % 2 else 0.3) * torch.rand(9, generator=g, device=device, dtype=torch.float64),
+                       torch.rand(3, generator=g, device=device, dtype=torch.float64))
+            out.append(decoder.step(drafts, numbers=numbers).tolist())
+            if turn == 5:
+                decoder.finish(1)
+                torch.manual_seed(turn)
+                assert decoder.add(prompt(30, 5), prefix=prefix) == 1
+        return out
+    want = answers(False)
+    assert any(step[0][1] >= 0 for step in want[1:])      # some drafts were accepted
+    runtime = NeuralZipRuntime.attach(model, export_model_for_gpu(model, NeuralZipSetup(chunk_size=16384).build(model)),
+                                      device=device)
+    assert answers(False) == want
+    assert answers(True) == want
+    assert runtime is not None
