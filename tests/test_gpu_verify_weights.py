@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_verify import check, run
+from test_gpu_verify import chances, check, run
 
 pytestmark = pytest.mark.gpu
 
@@ -97,3 +97,50 @@ def test_tokens_in_every_chunk():
     row = torch.zeros(n, vocab, dtype=torch.bfloat16)
     got = run(row, [0] * n, list(range(n + 1)), [0.0] * n, [t / vocab for t in tokens])
     assert got == ([0] * n, tokens)
+
+
+def answer_shares(p, q, rest_of):
+    """How often each token is a request's first one, over a draft drawn from q
+    that is kept with probability min(1, p / q), or replaced by a token with
+    weights rest_of(draft) otherwise."""
+    share = np.zeros(len(p))
+    for d in range(len(p)):
+        kept = min(1.0, p[d] / q[d])
+        rest = rest_of(d)
+        share[d] += q[d] * kept
+        share += q[d] * (1.0 - kept) * rest / rest.sum()
+    return share
+
+
+def test_first_tokens_are_distributed_as_the_model_s():
+    """The draft is accepted below p / q and not above it, which gives its share
+    exactly; the token after a refusal is counted over n even numbers, each
+    token's share off by less than a number's, 1 / n. Rules that pick that token
+    from p, or from p without the draft, are far outside that bound."""
+    vocab, n = 8, 2000
+    rng = np.random.default_rng(3)
+    logits = torch.from_numpy(rng.standard_normal((1, vocab))).float()
+    p, q32 = chances(logits.double().numpy()[0], 1.0), chances(rng.standard_normal(vocab), 1.0).astype(np.float32)
+    q = q32.astype(np.float64)       # (its sum is 1 to within vocab * 2^-25)
+    bound = 1.0 / n + vocab * 2.0 ** -24
+    outside = np.eye(vocab)
+    for wrong in (lambda d: p, lambda d: p * (1.0 - outside[d])):
+        assert np.abs(answer_shares(p, q, wrong) - p).max() > 20 * bound
+    assert np.abs(answer_shares(p, q, lambda d: np.maximum(p - q, 0.0)) - p).max() < bound / 10
+    sample = (np.arange(n) + 0.5) / n
+    counts = {}
+    for d in range(vocab):
+        def at(accept, samples):
+            rows = 2 * len(samples)
+            return run(logits.repeat(rows, 1), [0, d] * len(samples), list(range(0, rows + 1, 2)), [accept, 0.0] * len(samples),
+                       samples, np.tile(q32, (rows, 1)))
+        limit = p[d] / q[d]
+        assert at(min(limit, 1.0) * (1 - 1e-12), [0.5])[0] == [1]
+        counts[d] = np.zeros(vocab)
+        if limit < 1.0:
+            accepted, following = at(limit * (1 + 1e-12), sample)
+            assert accepted == [0] * n
+            counts[d] = np.bincount(following, minlength=vocab).astype(np.float64)
+    assert any(c.sum() for c in counts.values())
+    share = answer_shares(p, q, lambda d: counts[d] if counts[d].sum() else np.ones(vocab))
+    assert np.abs(share - p).max() <= bound
