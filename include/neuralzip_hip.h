@@ -608,7 +608,10 @@ typedef struct nz_pages_trim_args {
 /* Shortens requests to their first keep[r] tokens (a negative number counts
  * as 0; requests that are no longer stay as they are) and puts the pages past
  * those back onto the stack, in request order and table order, as
- * nz_pages_release does. */
+ * nz_pages_release does. Both take every page of a request's length for its
+ * own: a request whose table row begins with pages that others use is trimmed
+ * to no fewer tokens than these hold, and ended by a trim to them and a length
+ * of 0, not by nz_pages_release. */
 int nz_pages_trim(const nz_pages_trim_args* args, void* stream);
 
 typedef struct nz_rotary_args {

@@ -167,7 +167,13 @@ class PageTables:
     `n_free` (the stack of unused pages and its height) are the state, on the
     device; they may be written by hand. All requests start empty and all pages
     free, the lowest on top. Calls that change one PageTables run one after
-    another, on one stream or ordered by events."""
+    another, on one stream or ordered by events.
+
+    Every page of a request's length is taken for its own: nothing here knows
+    that rows written by hand share some. A request behind shared pages is
+    trimmed to no fewer tokens than these hold, and ended by trimming it to
+    them and writing 0 into its length; release() would put the shared pages
+    onto the free stack, which may then give them to another request."""
 
     def __init__(self, requests, max_pages, page_size, num_pages, device="cuda"):
         if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
@@ -217,8 +223,8 @@ class PageTables:
 
     def release(self, done, *, advance=True, stream=None):
         """Puts the pages of the requests whose `done` (bool) is set back
-        onto the free stack and sets their lengths to 0; returns the state
-        after it. Without `advance` lengths and n_free stay."""
+        onto the free stack, shared ones too, and sets their lengths to 0;
+        returns the state after it. Without `advance` lengths and n_free stay."""
         _check_vector("done", done, torch.bool, self.requests, self._index)
         with _on(stream):
             out = Released(self.requests, self.device)
@@ -236,7 +242,8 @@ class PageTables:
         request) tokens and puts the pages past those back onto the free
         stack, as after a verification that refused drafts; returns the state
         after it. Requests that are no longer than that stay as they are, a
-        negative number counts as 0. Without `advance` lengths and n_free
+        negative number counts as 0; what is kept must include pages that
+        other requests share. Without `advance` lengths and n_free
         stay."""
         _check_vector("keep", keep, torch.int32, self.requests, self._index)
         with _on(stream):
@@ -408,7 +415,8 @@ class SharedPlan(AttentionPlan):
     all requests of group g, for rows whose contexts are that long. `groups` (int32,
     one per request: per row of the tables) gives a request's group, -1 for
     none, `shared` (int32, one per group) the keys. The requests of a group
-    must have the same pages in their tables for these.
+    must have the same pages in their tables for these, which PageTables does
+    not know of (its notes say how such requests are trimmed and ended).
 
     Rows see their contexts' keys, as with an AttentionPlan, and the results
     are the same up to the order of the sums. At most 2048 rows and 1024
