@@ -75,3 +75,46 @@ def test_compressed_weights_behind_prefixes_and_drafts(kind, more):
     assert answers(False) == want
     assert answers(True) == want
     assert runtime is not None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("requests", [1, 2, 5])
+def test_replayed_steps_of_a_long_vocabulary(requests):
+    """Replays give an eager decoder's tokens, with eager work between them."""
+    vocab = 151936
+    model = small_model("cuda:0", "llama", vocab_size=vocab)
+    pair = [PagedDecoder(model, requests=requests, max_length=60) for _ in range(2)]
+    for decoder in pair:
+        for place in range(requests):
+            decoder.add(torch.randint(3, vocab, (4 + place,), generator=torch.Generator().manual_seed(place)))
+        decoder.step(), decoder.step()
+    pair[1].capture()
+    for _ in range(12):
+        one, two = (decoder.step() for decoder in pair)
+        assert torch.equal(one, two) and torch.equal(pair[0].tokens, pair[1].tokens)
+        assert torch.equal(two, pair[1].logits.argmax(-1))
+        torch.randn(1000, 1000, device="cuda:0").sum().item()
+
+
+@pytest.mark.gpu
+def test_a_replayed_choice_of_a_long_vocabulary():
+    """The choice of a step alone, in a graph of few nodes."""
+    vocab = 151936
+    model = small_model("cuda:0", "llama", vocab_size=vocab)
+    decoder = PagedDecoder(model, requests=1, max_length=60)
+    decoder.add(prompt(5))
+    logits = torch.randn(1, vocab, device="cuda:0")
+    rows, contexts = torch.zeros(1, dtype=torch.int32, device="cuda:0"), torch.full((1,), 9, dtype=torch.int32, device="cuda:0")
+    decoder._pick(logits, rows, contexts)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        decoder._pick(logits, rows, contexts)
+    wrong = []
+    for i in range(12):
+        logits.copy_(torch.randn(1, vocab, device="cuda:0"))
+        graph.replay()
+        torch.cuda.synchronize()
+        if int(decoder.tokens[0]) != int(logits.argmax(-1)):
+            wrong.append(i)
+    assert not wrong
