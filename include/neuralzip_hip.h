@@ -13,7 +13,8 @@
  *     nz_matvec_reduce, nz_matvec_rows and the serving-step operators
  *     (nz_pages_*, nz_rotary_store, nz_attention_*, nz_shared_*,
  *     nz_adjust_logits, nz_verify_drafts, nz_route_experts, nz_expert_mlp)
- *     are asynchronous and ordered on the given HIP stream.
+ *     are asynchronous and ordered on the given HIP stream, a default one
+ *     on that of the current device, which has to be the arguments'.
  */
 #ifndef NEURALZIP_HIP_H
 #define NEURALZIP_HIP_H

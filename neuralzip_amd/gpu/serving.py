@@ -65,7 +65,17 @@ def _like(t, stream):
 def _call(function, device, args, stream):
     if device.type != "cuda":
         raise ValueError("The serving operators run on the GPU.")
-    rc = function(args, _stream_handle(device, stream))
+    _launch(function, device, args, _stream_handle(device, stream))
+
+
+def _launch(function, device, *args):
+    """Calls a launching function on the tensors' device: the handle of a
+    default stream names that of whichever device is current."""
+    if torch._C._cuda_getDevice() == device.index:
+        rc = function(*args)
+    else:
+        with torch.cuda.device(device):
+            rc = function(*args)
     if rc:
         _native.check(rc)
 
@@ -381,11 +391,9 @@ class AttentionPlan:
         _check_vector("contexts", contexts, torch.int32, self.rows, self._index)
         if requests is not None:
             _check_vector("requests", requests, torch.int32, self.rows, self._index)
-        rc = _native.lib().nz_attention_plan(contexts.data_ptr(), requests.data_ptr() if requests is not None else None,
-                                             self.rows, self._target, self._parts, *self._pointers,
-                                             _stream_handle(self.device, stream))
-        if rc:
-            _native.check(rc)
+        _launch(_native.lib().nz_attention_plan, self.device, contexts.data_ptr(),
+                requests.data_ptr() if requests is not None else None, self.rows, self._target, self._parts,
+                *self._pointers, _stream_handle(self.device, stream))
         if stream is not None:
             _keep(stream, contexts, requests, self.items)
         return self
@@ -466,9 +474,7 @@ class SharedPlan(AttentionPlan):
             contexts.data_ptr(), requests.data_ptr() if requests is not None else 0,
             groups.data_ptr() if groups is not None else 0, shared.data_ptr() if shared is not None else 0,
             *self._pointers, self.rows, n_requests, n_groups, self.capacity, self.heads, self.kv_heads, self._target, 0)
-        rc = _native.lib().nz_shared_plan(args, _stream_handle(self.device, stream))
-        if rc:
-            _native.check(rc)
+        _launch(_native.lib().nz_shared_plan, self.device, args, _stream_handle(self.device, stream))
         if stream is not None:
             _keep(stream, contexts, requests, groups, shared, self.items)
         return self
@@ -517,9 +523,7 @@ def paged_attention(q, key_cache, value_cache, tables, plan, *, scale=None, out=
         q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), out.data_ptr(), tables.data_ptr(),
         *plan._pointers, plan._partials(dim, handle, stream), q0, q1, o0, o1, *pool, rows, plan.capacity, heads,
         plan.kv_heads, dim, *table_shape, page_size, pages, kind, dim ** -0.5 if scale is None else scale, 0)
-    rc = plan._function(args, handle)
-    if rc:
-        _native.check(rc)
+    _launch(plan._function, plan.device, args, handle)
     if stream is not None:
         _keep(stream, q, key_cache, value_cache, tables, out)
     return out
