@@ -511,7 +511,7 @@ class PagedDecoder:
         place, what a request's text is taken to go on with, -1 for none; the
         tokens after a -1 are not used. numbers: (accept, sample), float64 from
         [0, 1), requests * (drafts + 1) and requests of them, in place of
-        torch's own."""
+        torch's own. A step that raises leaves all requests as they were."""
         if drafts is not None:
             if not torch.is_tensor(drafts) or drafts.shape != self._drafted.shape or drafts.dtype != torch.int64 \
                     or not self._drafts_most:
@@ -524,7 +524,16 @@ class PagedDecoder:
             self._graph.replay()
             self.logits = self._graph_logits
         else:
-            self._run()
+            pages = self.tables
+            state = pages.lengths, pages.free, pages.n_free
+            before = [t.clone() for t in state]
+            try:
+                self._run()
+            except BaseException:
+                # a step that fails changes no request (tables past the lengths mean nothing)
+                for t, old in zip(state, before):
+                    t.copy_(old)
+                raise
         return self._answers.clone()
 
     @torch.no_grad()

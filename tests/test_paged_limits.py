@@ -118,3 +118,36 @@ def test_a_replayed_choice_of_a_long_vocabulary():
         if int(decoder.tokens[0]) != int(logits.argmax(-1)):
             wrong.append(i)
     assert not wrong
+
+
+@pytest.mark.parametrize("drafts", [0, 2])
+@pytest.mark.parametrize("broken", ["layers", "lm_head"])
+def test_a_step_that_fails_changes_no_request(device, drafts, broken):
+    """Lengths and pages are those before it, and the next step's answers the
+    ones that it would have given."""
+    model = small_model(device)
+    pair = [PagedDecoder(model, requests=3, max_length=60, drafts=drafts, prefixes=1) for _ in range(2)]
+    texts = [prompt(15, 2), prompt(16, 3), prompt(5, 4)]
+    for decoder in pair:
+        prefix = decoder.add_prefix(prompt(20, 1))
+        for text in texts:
+            decoder.add(text, prefix=prefix)
+        decoder.step()
+    given = [] if not drafts else [torch.full((3, drafts), 7, device=device)]
+    module = model.model.layers[1] if broken == "layers" else model.lm_head
+    before = [t.clone() for t in pair[0].tables._state]
+
+    def fails(*args, **kwargs):
+        raise ArithmeticError("on purpose")
+    module.forward = fails
+    for _ in range(2):
+        with pytest.raises(ArithmeticError):
+            pair[0].step(*given)
+    del module.forward
+    state = pair[0].tables._state
+    assert torch.equal(state[0], before[0]) and torch.equal(state[3], before[3])
+    n = int(state[3])
+    assert sorted(state[2][:n].tolist()) == sorted(before[2][:n].tolist())
+    for _ in range(20):
+        assert torch.equal(pair[0].step(*given), pair[1].step(*given))
+        assert torch.equal(pair[0].tables.lengths, pair[1].tables.lengths)
