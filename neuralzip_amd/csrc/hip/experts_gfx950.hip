@@ -216,8 +216,8 @@ __device__ __forceinline__ float activate(uint32_t kind, float x) {
 // elements: act(gate x) * (up x), in 32 bits. Weight rows are the rows of the
 // matrix instructions and tokens their columns, in up to NB blocks; the
 // wavefronts share the depth. Bound by the weights' way from memory: 8 experts
-// of 14336 x 4096 bf16 elements for 32 tokens in 366 us (5.1 TB/s); 8 of 768 x
-// 2048 for one token in 13.6 (3.7), of which some 3.5 go by before the choice
+// of 14336 x 4096 bf16 elements for 32 tokens in 365 us (5.1 TB/s); 8 of 768 x
+// 2048 for one token in 13.4 (3.7), of which some 3.5 go by before the choice
 // is known. (With batches of 8 pieces that layer took 40.9 us instead of 36.6,
 // with registers for four wavefronts a SIMD the wide one 654 instead of 546.)
 template <typename T, uint32_t NB>
@@ -348,7 +348,9 @@ __device__ __forceinline__ int split(const float (&x)[Piece<T>::kRun], typename 
 // tokens' sums, times the weights, when it ends. `splits` workgroups share the
 // experts; the last to arrive adds their sums in order. Bound by the weights'
 // way from memory and, for few tokens, by the latencies of the choice and of
-// the last sums: 212 us (4.4 TB/s) and 12.0 us for the layers above.
+// the last sums: 211 us (4.5 TB/s) and 12.3 us for the layers above. All of it
+// is read again for every kTokens tokens: 65 tokens of the wide layer take 963 us,
+// where 64 take 652.
 template <typename T, uint32_t NB>
 __global__ __launch_bounds__(kDownThreads) void nz_expert_down_kernel(nz_expert_args a, const float* __restrict__ acts,
                                                                       float* __restrict__ partials,

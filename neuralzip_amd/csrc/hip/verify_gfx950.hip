@@ -212,7 +212,7 @@ __device__ __forceinline__ void wave_largest(Part& a) {
 }
 
 // One chunk of one row. Bound by the vector units, some 20 instructions of 64
-// bits a logit: 240 rows of 128256 fp32 logits in 37 us (3.3 TB/s; the units
+// bits a logit: 240 rows of 128256 fp32 logits in 38 us (3.3 TB/s; the units
 // are busy 63 % of the time), 104 in bf16 in 16. Several chunks a workgroup,
 // each read ahead, took as long, as did registers for eight wavefronts a SIMD.
 template <typename T>
@@ -360,7 +360,7 @@ void nz_verify_decide_kernel(nz_verify_args a, const Part* __restrict__ parts, D
 
 // Then the sums of max(p - q, 0) over the chunks of the row that a request's
 // next token is picked from. Bound by memory: 48 rows of 128256 fp32 logits and
-// as many probabilities in 11.6 us (4.2 TB/s). (When its workgroups decided
+// as many probabilities in 11.5 us (4.3 TB/s). (When its workgroups decided
 // each for itself, 17.)
 template <typename T>
 __global__ __launch_bounds__(kThreads)
@@ -377,8 +377,8 @@ void nz_verify_rest_kernel(nz_verify_args a, const Decision* __restrict__ decisi
 
 // The next token of a request: the chunk in which the sum of weights passes
 // the wanted share of all, then the token in it. Bound by latencies, the
-// decision's among them: 7.6 us for one row, 10.8 for 32 requests of up to five
-// drafts, 7.2 for 48 that are decided already.
+// decision's among them: 7.6 us for one row, 10.7 for 32 requests of up to five
+// drafts, 7.4 for 48 that are decided already.
 template <typename T>
 __global__ __launch_bounds__(kPickThreads)
 void nz_verify_pick_kernel(nz_verify_args a, const Part* __restrict__ parts, const Decision* __restrict__ decisions,

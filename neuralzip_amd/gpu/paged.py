@@ -14,10 +14,11 @@ can be captured in a HIP graph (capture()) and replayed while requests grow.
 
 Requests may begin with a prefix (add_prefix()), whose pages they share and
 whose keys a step reads once for all of them. With `drafts`, a step takes that
-many drafted tokens per request along, and verify_drafts keeps those that the
-model would have answered; trim() takes the others' pages back. With `experts`,
-a step's mixture-of-experts layers run through expert_mlp, which a graph can
-hold, in place of the model's own.
+many drafted tokens per request along, as certain ones (their drafter's
+probabilities are not asked for), and verify_drafts keeps those that the model
+would have answered; trim() takes the others' pages back. With `experts`, the
+experts of a step's mixture-of-experts layers run through expert_mlp, which a
+graph can hold, in place of the model's own.
 
 Models are Llama-like, of the types in MODEL_TYPES:
 model.model.{embed_tokens, layers, norm, rotary_emb} and model.lm_head, layers
@@ -102,7 +103,10 @@ class PagedDecoder:
     `drafts`: drafted tokens that a request may bring to a step, at most;
     requests * (drafts + 1) is at most 2048. `prefixes`: places for prefixes of
     up to max_length tokens; requests and prefixes are then at most 2048 and
-    1024. `experts`: steps run the experts of MoE layers by expert_mlp."""
+    1024. `experts`: steps run the experts of MoE layers by expert_mlp, the
+    routers as the model has them. It is made for steps of few tokens: with more
+    than some 64 of them, requests times drafts + 1, on wide experts, or some 1000
+    on small ones, the model's own forward is faster."""
 
     def __init__(self, model, *, requests, max_length, page_size=16, num_pages=None, repetition=1.0, frequency=0.0,
                  presence=0.0, grammar=False, temperature=None, drafts=0, prefixes=0, experts=False):

@@ -22,9 +22,11 @@ one forward, around the weights that the runtime decodes.
 
 Every call launches gfx950 kernels through the C ABI (nz_pages_*,
 nz_rotary_store, nz_attention_*, nz_shared_*, nz_route_experts, nz_expert_mlp,
-nz_adjust_logits, nz_verify_drafts) on the current stream, or on `stream`, where its tensors must be ready. They may be let go after the
-call: they are recorded for `stream`. Results are that stream's, and who uses
-them on another one waits for it and records them there. Nothing synchronises,
+nz_adjust_logits, nz_verify_drafts) on its tensors' device, on that one's
+current stream, or on `stream`, where its tensors must be ready. They may be
+let go after the call: they are recorded for `stream`. Results are that
+stream's, and who uses them on another one waits for it and records them
+there. Nothing synchronises,
 and lengths, tables and plans never leave the device, so that a step can be
 captured in a HIP graph and replayed while the requests grow. The operators
 serve: tensors that need a gradient are refused while gradients are on.
@@ -428,7 +430,8 @@ class SharedPlan(AttentionPlan):
 
     Rows see their contexts' keys, as with an AttentionPlan, and the results
     are the same up to the order of the sums. At most 2048 rows and 1024
-    groups."""
+    groups. Rows that share nothing, rows that see nothing and heads of 256
+    elements are faster with an AttentionPlan."""
 
     def __init__(self, contexts, *, heads, kv_heads, requests=None, groups=None, shared=None, stream=None):
         if kv_heads < 1 or heads < 1 or heads % kv_heads:
@@ -485,15 +488,16 @@ class SharedPlan(AttentionPlan):
 
 def paged_attention(q, key_cache, value_cache, tables, plan, *, scale=None, out=None, stream=None):
     """softmax(scale q.K) V for every row of q (rows, heads, head_dim), over
-    the context of its request in the plan (AttentionPlan or SharedPlan): the keys and values at the request's
-    pages (`tables`, int32 (requests, max_pages)) of the caches (pages,
-    kv_heads, page size, head_dim). Query head h reads key-value head
+    the context of its request in the plan (AttentionPlan or SharedPlan): the
+    keys and values at the request's pages (`tables`, int32 (requests,
+    max_pages)) of the caches (pages, kv_heads, page size, head_dim). Query head h reads key-value head
     h // (heads / kv_heads). `scale` is head_dim ** -0.5 by default. A row
     without keys gives zeros; keys of pages outside the caches, and keys whose
     score is -infinity, count as masked. Sums and softmax in 32 bits, in an
     order that only the plan decides; values are summed before the division,
-    so the largest one times the context must be below 3e38. head_dim is a multiple of 16 up to 256; strides may be any that
-    keep heads, tokens and pages on 16-byte boundaries."""
+    so the largest one times the context must be below 3e38. head_dim is a
+    multiple of 16 up to 256; strides may be any that keep heads, tokens and
+    pages on 16-byte boundaries."""
     if torch.is_grad_enabled():
         _refuse_gradients(q, key_cache, value_cache)
     dtype, index, shape = q.dtype, q.get_device(), q.shape
@@ -621,7 +625,7 @@ def verify_drafts(logits, tokens, starts, accept, sample, *, draft_probs=None, t
 
     accept (rows) and sample (requests) are float64 numbers from [0, 1).
     temperature: float32 per request; 0 or less takes the largest logit, the
-    first of equals; without it 1. A token outside the vocabulary is no draft:
+    first of equals; infinity makes all above -inf as likely; without it 1. A token outside the vocabulary is no draft:
     it is refused and the next one picked from p. next is -1 for a request
     without rows, and where no logit is above -inf. In 64 bits; NaN counts as
     -inf. At most 65535 rows and requests and 2**22 tokens."""
@@ -669,8 +673,8 @@ def route_experts(x, weight, top_k, *, scoring="softmax", normalize=True, bias=N
     added to what is compared, not to the weights. `normalize` divides a
     token's weights by their sum; `scale` multiplies them. Of equal experts the
     lower one is first, and NaN is never before another. In 64 bits, rounded
-    once. hidden is a multiple of 8; at
-    most 1024 experts, 32 of them chosen, and 65535 tokens."""
+    once. hidden is a multiple of 8; at most 1024 experts, 32 of them chosen,
+    and 65535 tokens."""
     if torch.is_grad_enabled():
         _refuse_gradients(x, weight, bias)
     if x.dim() != 2 or x.dtype not in _TYPES or x.stride(1) != 1 or weight.dim() != 2 \
@@ -709,7 +713,8 @@ def expert_mlp(x, ids, weights, gate_up, down, *, activation="silu", out=None, s
     weights. In 32 bits, rounded once, in an order that only the ids decide.
     hidden and inter are multiples of 8; any strides whose rows lie on 16-byte
     boundaries. Made for a few tokens: the experts' weights are read once for
-    every 64."""
+    every 64, so that products of the experts' own are faster from some 64 tokens
+    on for wide experts, and from some 1000 for small ones."""
     if torch.is_grad_enabled():
         _refuse_gradients(x, weights, gate_up, down)
     dtype, index = x.dtype, x.get_device()
