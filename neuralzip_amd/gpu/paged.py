@@ -475,8 +475,8 @@ class PagedDecoder:
         rows = self._rows(requests)
         self.logits = logits = self._adjusted(logits, rows, requests, contexts)
         # (argmax of a row of 2^17 tokens or more clears counters by a memset; as a graph's last node it has given wrong
-        # tokens from the second replay on)
-        if self.temperature > 0 or logits.is_cuda:
+        # tokens from the second replay on. Of more rows than verify_drafts takes it needs none.)
+        if self.temperature > 0 or (logits.is_cuda and logits.shape[0] <= 65535):
             # every row for itself, with its request's number
             one = torch.arange(rows.shape[0] + 1, dtype=torch.int32, device=self.device)
             at = rows.clamp(max=self.requests - 1)

@@ -151,3 +151,16 @@ def test_a_step_that_fails_changes_no_request(device, drafts, broken):
     for _ in range(20):
         assert torch.equal(pair[0].step(*given), pair[1].step(*given))
         assert torch.equal(pair[0].tables.lengths, pair[1].tables.lengths)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("requests", [65535, 65536, 70000])
+def test_greedy_choices_of_more_requests_than_one_verification_takes(requests):
+    device = "cuda:0"
+    decoder = PagedDecoder(small_model(device), requests=requests, max_length=16)
+    logits = torch.randn(requests, VOCAB, device=device)
+    logits[:, 7] = logits.amax(-1)        # two largest, or one
+    places = torch.arange(requests, dtype=torch.int32, device=device)
+    decoder._pick(logits, places, torch.full_like(places, 3))
+    assert torch.equal(decoder.tokens, (logits == logits.amax(-1, keepdim=True)).int().argmax(-1))
+    assert torch.equal(decoder._history[:requests, 3].long(), decoder.tokens)
